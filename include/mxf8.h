@@ -1,6 +1,7 @@
 /*
  * mxf8.h - C ABI of the MI355X (gfx950) FP8 hot path: dynamic e4m3 quantizers, the
- * row-wise scaled FP8 GEMM with a fused epilogue, and the FP8 flash-attention forward.
+ * row-wise scaled FP8 GEMM with a fused epilogue, and the FP8 flash-attention forward; and of
+ * what a DiT block has around them: rotary positions, gated residual norms, the 4-bit linear.
  *
  * Conventions
  *  - Every pointer is a device pointer; every size, leading dimension and stride is in
@@ -268,6 +269,97 @@ int mxf8_attn_fwd_q(const void* q, const int64_t q_strides[4], float c,
                     float* sq_out, void* out, int out_dtype, const int64_t out_strides[4],
                     int64_t B, int64_t H, int64_t Sq, int64_t Sk, int64_t D,
                     int kv_mode, hipStream_t stream);
+
+/*
+ * Rotary positions over several axes (time, height, width, ...).  No counterpart in the reference's
+ * files: the DiT's own position code (diffusers) stands between its QKV projection and attention.
+ *   pos  [n, axes] contiguous, 1 to 4 axes; pos_type 0 fp32, 1 fp64, 2 int32, 3 int64
+ *   axis_dims [axes] (host memory): channels of each axis, even; axis a has axis_dims[a] / 2 pairs, the
+ *   pairs of all axes in order, P <= 256 of them
+ *   table [n, P, 2] fp32 (written): (cos, sin) of pos[s, a] * theta^(-2 i / axis_dims[a]) for pair i of
+ *   axis a.  The angle is formed and reduced in fp64.
+ */
+int mxf8_rotary_table(const void* pos, int pos_type, int64_t n, int64_t axes, const int64_t* axis_dims,
+                      double theta, float* table, hipStream_t stream);
+
+/*
+ * Per-head RMS norm and rotation of q and k in one launch (no counterpart in the reference, as above).
+ *   q [B, Hq, S, D], k [B, Hk, S, D] of `dtype` (bf16, fp16, fp32), element strides {b, h, s, d} with
+ *   unit d stride (any alignment); Hq or Hk may be 0 (its pointers are then not read)
+ *   y = x / sqrt(mean_d(x^2) + eps) * weight with q_weight / k_weight [D] of `dtype`; NULL: y = x
+ *   pair j < P of y, channels (2 j, 2 j + 1) when `interleaved`, else (j, j + P), turns by
+ *   table[b, s, j] = (cos, sin): (u, v) = (a cos - b sin, a sin + b cos); channels >= 2 P pass through
+ *   table fp32, batch stride table_batch_stride elements (0: one table [S, P, 2] for all items)
+ *   q_out, k_out of `dtype` with strides like the inputs' (written; must not overlap them).  fp32
+ *   arithmetic, one rounding.  2 P <= D <= 4096.
+ */
+int mxf8_rotate_qk(const void* q, const int64_t q_strides[4], int64_t Hq, const void* k, const int64_t k_strides[4],
+                   int64_t Hk, int dtype, int64_t B, int64_t S, int64_t D, const float* table,
+                   int64_t table_batch_stride, int64_t P, const void* q_weight, const void* k_weight, float eps,
+                   int interleaved, void* q_out, const int64_t qo_strides[4], void* k_out,
+                   const int64_t ko_strides[4], hipStream_t stream);
+
+/* mxf8_gated_residual_norm's output y: as it is, as mxf8_quant_rows's codes, as mxf8_mxfp4_quant's */
+enum { MXF8_QUANT_NONE = 0, MXF8_QUANT_E4M3 = 1, MXF8_QUANT_MXFP4 = 2 };
+
+/*
+ * Gated residual with the norms on its two sides, and the modulation of the next branch's input (no
+ * counterpart in the reference: the DiT block's code between two branches, outside its files).  Per token:
+ *   u = branch, or with branch_weight [C]: branch / sqrt(mean(branch^2) + eps) * branch_weight
+ *   r = residual_scale * x + gate * u                                  (written, rounded once)
+ *   n = layer ? (r - mean(r)) / sqrt(var(r) + eps) : r / sqrt(mean(r^2) + eps)     (of the unrounded r)
+ *   y = n * weight * (1 + scale) + shift                               (rounded once)
+ *   x, branch [B, S, C] of `dtype` (bf16, fp16, fp32), batch and token strides given, channels contiguous,
+ *   any alignment; branch NULL: r = residual_scale * x, not written
+ *   gate, shift, scale: `spans` rows [C] per batch item, one for every S / spans tokens (batch and span
+ *   strides given); each may be NULL (gate 1, shift 0, scale 0); weight [C] or NULL (1)
+ *   r [B, S, C] contiguous; y [B, S, C] contiguous, required when quant == MXF8_QUANT_NONE, else optional
+ *   quant == MXF8_QUANT_E4M3: codes [B S, C] and fp32 scales [B S], mxf8_quant_rows(y) bit for bit
+ *   quant == MXF8_QUANT_MXFP4: codes [B S, C / 2] and scales, mxf8_mxfp4_quant(y) bit for bit; C % 32 == 0
+ * fp32 arithmetic; C <= 16384.  Outputs must not overlap inputs.
+ */
+int mxf8_gated_residual_norm(const void* x, int64_t x_batch, int64_t x_token, const void* branch, int64_t br_batch,
+                             int64_t br_token, int dtype, int64_t B, int64_t S, int64_t C, const void* gate,
+                             int64_t g_batch, int64_t g_span, const void* shift, int64_t sh_batch, int64_t sh_span,
+                             const void* scale, int64_t sc_batch, int64_t sc_span, int64_t spans,
+                             const void* branch_weight, const void* weight, int layer, float eps, float residual_scale,
+                             int quant, void* r, void* y, uint8_t* codes, void* scales, hipStream_t stream);
+
+/*
+ * Four-bit blocks (OCP MX FP4; no counterpart in the reference).  A row is cut into blocks of 32 elements;
+ * a block is 32 e2m1 codes (+-{0, 1/2, 1, 3/2, 2, 3, 4, 6}) times a power of two.
+ *   codes  [M, K / 2]: two codes a byte, the even element in the low half
+ *   scales [ceil(K / 256), M, 8] uint8: exponent + 127 of block 8 s + i of row m at [s, m, i]; 255 marks a
+ *   block with an infinity or NaN, which reads as NaN throughout; bytes of blocks past K are ignored
+ * K % 32 == 0, K <= 2^22.
+ */
+
+/* Bytes of the scales of an M x K matrix. */
+int64_t mxf8_mxfp4_scale_bytes(int64_t M, int64_t K);
+
+/*
+ * Quantizer: the power of two puts a block's largest magnitude into [3.5, 7) (2^-127 at the least), values are
+ * rounded to the nearest code, ties to the even one, and those above 6 become 6.
+ *   x [M, K] of `dtype` (bf16, fp16, fp32), row stride ldx, any alignment; codes 4-byte aligned (written),
+ *   scales (written, 127 past K)
+ */
+int mxf8_mxfp4_quant(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, uint8_t* codes, uint8_t* scales,
+                     hipStream_t stream);
+
+/* The values of codes and scales, [M, K] of `dtype`: exact in bf16 and fp32, rounded in fp16; a value past the
+ * type's range (from 2^128 on in bf16 and fp32) becomes infinite. */
+int mxf8_mxfp4_dequant(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, void* out, int dtype,
+                       hipStream_t stream);
+
+/*
+ * Linear on four-bit blocks: out[m, n] = bf16(act(sum_k a[m, k] w[n, k] + bias[n])), fp32 accumulation and
+ * activation, one rounding.
+ *   a4, sa: activations [M, K]; w4, sw: weights [N, K]; both as mxf8_mxfp4_quant writes them; codes 16-byte
+ *   and scales 8-byte aligned
+ *   bias [N] bf16 or NULL; out [M, N] bf16, row stride ld_out >= N
+ */
+int mxf8_gemm_mxfp4(const uint8_t* a4, const uint8_t* w4, const uint8_t* sa, const uint8_t* sw, const void* bias,
+                    int act, void* out, int64_t M, int64_t N, int64_t K, int64_t ld_out, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -20,11 +20,13 @@ _ops_loaded = False
 BF16, F16, F32 = 0, 1, 2
 ACT_NONE, ACT_GELU_TANH = 0, 1
 KV_AUTO, KV_STREAM = 0, 1
+QUANT_NONE, QUANT_E4M3, QUANT_MXFP4 = 0, 1, 2
 
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _I64x4 = _i64 * 4
 
 # name -> (restype, argtypes); mirrors include/mxf8.h
@@ -55,6 +57,16 @@ _SIGNATURES = {
                              _i64, _i32, _vp]),
     "mxf8_attn_fwd_q": (_i32, [_vp, _I64x4, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _f32, _vp, _vp, _i32, _I64x4, _i64,
                                _i64, _i64, _i64, _i64, _i32, _vp]),
+    "mxf8_rotary_table": (_i32, [_vp, _i32, _i64, _i64, ctypes.POINTER(_i64), _f64, _vp, _vp]),
+    "mxf8_rotate_qk": (_i32, [_vp, _I64x4, _i64, _vp, _I64x4, _i64, _i32, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp,
+                              _f32, _i32, _vp, _I64x4, _vp, _I64x4, _vp]),
+    "mxf8_gated_residual_norm": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _i64, _i64, _i64, _vp, _i64, _i64, _vp,
+                                        _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i32, _f32, _f32, _i32, _vp, _vp,
+                                        _vp, _vp, _vp]),
+    "mxf8_mxfp4_scale_bytes": (_i64, [_i64, _i64]),
+    "mxf8_mxfp4_quant": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "mxf8_mxfp4_dequant": (_i32, [_vp, _vp, _i64, _i64, _vp, _i32, _vp]),
+    "mxf8_gemm_mxfp4": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _i64, _vp]),
 }
 EXPORTS = tuple(_SIGNATURES)
 

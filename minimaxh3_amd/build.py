@@ -27,6 +27,10 @@ SOURCES = [
     ("capi.hip", "capi", []),
     ("quant.hip", "quant", []),
     ("gemm.hip", "gemm", []),
+    ("gemm_mxfp4.hip", "gemm_mxfp4", []),
+    ("mxfp4.hip", "mxfp4", []),
+    ("rotary.hip", "rotary", []),
+    ("block_norm.hip", "block_norm", []),
     ("attn.hip", "attn", []),
 ] + [
     ("attn_inst.hip", f"attn_d{d}_o{o}", [f"-DMXF8_ATTN_D={d}", f"-DMXF8_ATTN_ODT={o}"])

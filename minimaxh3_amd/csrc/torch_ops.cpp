@@ -1,5 +1,6 @@
 // The hot torch.library ops (mxf8::quant_rows, adaln_quant_rows, gemm_rowwise, lora_down,
-// attn_quant_kv, attn_fwd_q) as native kernels over the C ABI of libmxf8.  Their schemas and
+// attn_quant_kv, attn_fwd_q, rotary_table, rotate_qk, gated_residual_norm, mxfp4_quant,
+// mxfp4_dequant, gemm_mxfp4) as native kernels over the C ABI of libmxf8.  Their schemas and
 // fake kernels are declared in minimaxh3_amd/ops.py; the kernels here take the CUDA and
 // AutogradCUDA entries of the dispatcher (the device type of a ROCm GPU), where they stand in
 // for the Python kernels of the declarations.
@@ -282,6 +283,230 @@ Tensor attn_fwd_q(const Tensor& q, double c, const Tensor& k8, const Tensor& v8t
   return out;
 }
 
+// ---- rotary positions, gated residual norms, 4-bit linear -------------------------------------
+
+Tensor rotary_table(const Tensor& positions, at::IntArrayRef axis_dims, double theta) {
+  require_gfx950(positions, "rotary_table");
+  const int64_t axes = static_cast<int64_t>(axis_dims.size());
+  TORCH_CHECK_VALUE(positions.dim() >= 2 && positions.size(-1) == axes, "rotary_table: positions [..., ", axes,
+                    "] expected for ", axes, " axes, got ", positions.sizes());
+  int type;
+  switch (positions.scalar_type()) {
+    case at::kFloat: type = 0; break;
+    case at::kDouble: type = 1; break;
+    case at::kInt: type = 2; break;
+    case at::kLong: type = 3; break;
+    default: TORCH_CHECK_VALUE(false, "rotary_table: positions must be fp32, fp64, int32 or int64, got ",
+                               positions.scalar_type());
+  }
+  int64_t pairs = 0;
+  for (const int64_t d : axis_dims) {
+    TORCH_CHECK_VALUE(d > 0 && d % 2 == 0 && d <= 512, "rotary_table: axis dimensions must be even and positive, got ",
+                      axis_dims);
+    pairs += d / 2;
+  }
+  const Tensor pos = positions.contiguous();
+  std::vector<int64_t> shape(positions.sizes().begin(), positions.sizes().end() - 1);
+  shape.push_back(pairs);
+  shape.push_back(2);
+  Tensor table = empty(shape, pos, at::kFloat);
+  const c10::DeviceGuard guard(pos.device());
+  check(mxf8_rotary_table(pos.data_ptr(), type, axes ? pos.numel() / axes : 0, axes, axis_dims.data(), theta,
+                          table.data_ptr<float>(), stream_of(pos)),
+        "rotary_table");
+  return table;
+}
+
+// x with contiguous channels (a copy where they are not).
+Tensor rows_of(const Tensor& x) { return x.size(-1) > 1 && x.stride(-1) != 1 ? x.contiguous() : x; }
+
+void check_weight(const optional<Tensor>& w, int64_t n, const Tensor& x, const char* what, const char* name) {
+  if (!w) return;
+  TORCH_CHECK_VALUE(w->dim() == 1 && w->numel() == n && w->scalar_type() == x.scalar_type() && w->is_contiguous(), what,
+                    name, " must be ", n, " contiguous ", x.scalar_type(), " values, got ", w->scalar_type(), " ",
+                    w->sizes());
+  on_device(*w, x.device(), what, name);
+}
+
+std::tuple<Tensor, Tensor> rotate_qk(const Tensor& q_in, const optional<Tensor>& k_in, const Tensor& table,
+                                     const optional<Tensor>& q_weight, const optional<Tensor>& k_weight, double eps,
+                                     bool interleaved) {
+  const char* what = "rotate_qk: ";
+  require_gfx950(q_in, "rotate_qk");
+  TORCH_CHECK_VALUE(q_in.dim() == 4, what, "q must be [B, H, S, D], got ", q_in.sizes());
+  const int64_t B = q_in.size(0), Hq = q_in.size(1), S = q_in.size(2), D = q_in.size(3);
+  const at::Device dev = q_in.device();
+  dtype_code(q_in);
+  if (k_in) {
+    TORCH_CHECK_VALUE(k_in->dim() == 4 && k_in->size(0) == B && k_in->size(2) == S && k_in->size(3) == D, what,
+                      "k must be [B, Hk, S, D] with q's B, S and D, got ", k_in->sizes(), " for q ", q_in.sizes());
+    TORCH_CHECK_VALUE(k_in->scalar_type() == q_in.scalar_type(), what, "q and k must have one dtype");
+    on_device(*k_in, dev, what, "k");
+  }
+  TORCH_CHECK_VALUE(k_in || !k_weight, what, "k_weight needs k");
+  TORCH_CHECK_VALUE(table.scalar_type() == at::kFloat && table.is_contiguous() &&
+                        (table.dim() == 3 || (table.dim() == 4 && table.size(0) == B)) && table.size(-1) == 2 &&
+                        table.size(-3) == S && 2 * table.size(-2) <= D,
+                    what, "table must be contiguous fp32 [S, P, 2] or [B, S, P, 2] with 2 P <= D, got ",
+                    table.scalar_type(), " ", table.sizes(), " for q ", q_in.sizes());
+  on_device(table, dev, what, "table");
+  check_weight(q_weight, D, q_in, what, "q_weight");
+  check_weight(k_weight, D, q_in, what, "k_weight");
+  const Tensor q = rows_of(q_in), k = k_in ? rows_of(*k_in) : Tensor();
+  Tensor qo = at::empty_like(q), ko = k_in ? at::empty_like(k) : empty({0}, q, q.scalar_type());
+  if (qo.stride(3) != 1) qo = at::empty(q.sizes(), q.options());
+  if (k_in && ko.stride(3) != 1) ko = at::empty(k.sizes(), k.options());
+  const int64_t P = table.size(-2);
+  const c10::DeviceGuard guard(dev);
+  check(mxf8_rotate_qk(q.data_ptr(), q.strides().data(), Hq, k_in ? k.data_ptr() : nullptr,
+                       k_in ? k.strides().data() : nullptr, k_in ? k.size(1) : 0, dtype_code(q), B, S, D,
+                       table.data_ptr<float>(), table.dim() == 4 ? S * P * 2 : 0, P,
+                       q_weight ? q_weight->data_ptr() : nullptr, k_weight ? k_weight->data_ptr() : nullptr,
+                       static_cast<float>(eps), interleaved, qo.data_ptr(), qo.strides().data(),
+                       k_in ? ko.data_ptr() : nullptr, k_in ? ko.strides().data() : nullptr, stream_of(q)),
+        "rotate_qk");
+  return {qo, ko};
+}
+
+// Modulation rows [B, C] or [B, G, C]: their number per item, and the strides of item and row.
+struct ModRows {
+  Tensor t;
+  int64_t batch = 0, span = 0;
+  const void* ptr() const { return t.defined() ? t.data_ptr() : nullptr; }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> gated_residual_norm(
+    const Tensor& x_in, const optional<Tensor>& branch_in, const optional<Tensor>& gate, const optional<Tensor>& shift,
+    const optional<Tensor>& scale, const optional<Tensor>& branch_weight, const optional<Tensor>& weight, bool layer,
+    double eps, double residual_scale, int64_t quant, bool want_y) {
+  const char* what = "gated_residual_norm: ";
+  require_gfx950(x_in, "gated_residual_norm");
+  TORCH_CHECK_VALUE(x_in.dim() == 3, what, "x must be [B, S, C], got ", x_in.sizes());
+  const int64_t B = x_in.size(0), S = x_in.size(1), C = x_in.size(2), M = B * S;
+  const at::Device dev = x_in.device();
+  const int dt = dtype_code(x_in);
+  TORCH_CHECK_VALUE(C > 0, what, "x has no channels");
+  if (branch_in) {
+    TORCH_CHECK_VALUE(branch_in->sizes() == x_in.sizes() && branch_in->scalar_type() == x_in.scalar_type(), what,
+                      "branch must have x's shape and dtype, got ", branch_in->scalar_type(), " ", branch_in->sizes());
+    on_device(*branch_in, dev, what, "branch");
+  }
+  TORCH_CHECK_VALUE(branch_in || (!gate && !branch_weight), what, "gate and branch_weight need a branch");
+  check_weight(branch_weight, C, x_in, what, "branch_weight");
+  check_weight(weight, C, x_in, what, "weight");
+  TORCH_CHECK_VALUE(quant >= MXF8_QUANT_NONE && quant <= MXF8_QUANT_MXFP4, what, "bad quantization ", quant);
+  TORCH_CHECK_VALUE(quant != MXF8_QUANT_MXFP4 || C % 32 == 0, what, "C = ", C, " must be a multiple of 32 for mxfp4");
+  int64_t spans = 0;
+  auto rows = [&](const optional<Tensor>& t, const char* name) {
+    ModRows m;
+    if (!t) return m;
+    TORCH_CHECK_VALUE((t->dim() == 2 || t->dim() == 3) && t->size(0) == B && t->size(-1) == C &&
+                          t->scalar_type() == x_in.scalar_type(),
+                      what, name, " must be [B, C] or [B, G, C] of x's dtype, got ", t->scalar_type(), " ", t->sizes());
+    on_device(*t, dev, what, name);
+    const int64_t g = t->dim() == 3 ? t->size(1) : 1;
+    TORCH_CHECK_VALUE(spans == 0 || spans == g, what, "gate, shift and scale must have the same number of rows");
+    TORCH_CHECK_VALUE(g > 0 && S % g == 0, what, name, " has ", g, " rows per item, which do not divide S = ", S);
+    spans = g;
+    m.t = rows_of(*t);
+    m.batch = m.t.stride(0);
+    m.span = m.t.dim() == 3 ? m.t.stride(1) : 0;
+    return m;
+  };
+  const ModRows g = rows(gate, "gate"), sh = rows(shift, "shift"), sc = rows(scale, "scale");
+  const Tensor x = rows_of(x_in), br = branch_in ? rows_of(*branch_in) : Tensor();
+  Tensor r = empty(branch_in ? at::IntArrayRef{B, S, C} : at::IntArrayRef{0}, x, x.scalar_type());
+  const bool y_out = want_y || quant == MXF8_QUANT_NONE;
+  Tensor y = empty(y_out ? at::IntArrayRef{B, S, C} : at::IntArrayRef{0}, x, x.scalar_type());
+  Tensor codes, scales;
+  if (quant == MXF8_QUANT_E4M3) {
+    codes = empty({M, C}, x, kE4M3);
+    scales = empty({M, 1}, x, at::kFloat);
+  } else if (quant == MXF8_QUANT_MXFP4) {
+    codes = empty({M, C / 2}, x, at::kByte);
+    scales = empty({cdiv(C, 256), M, 8}, x, at::kByte);
+  } else {
+    codes = empty({0}, x, at::kByte);
+    scales = empty({0}, x, at::kByte);
+  }
+  const c10::DeviceGuard guard(dev);
+  check(mxf8_gated_residual_norm(x.data_ptr(), x.stride(0), x.stride(1), branch_in ? br.data_ptr() : nullptr,
+                                 branch_in ? br.stride(0) : 0, branch_in ? br.stride(1) : 0, dt, B, S, C, g.ptr(),
+                                 g.batch, g.span, sh.ptr(), sh.batch, sh.span, sc.ptr(), sc.batch, sc.span,
+                                 spans ? spans : 1, branch_weight ? branch_weight->data_ptr() : nullptr,
+                                 weight ? weight->data_ptr() : nullptr, layer, static_cast<float>(eps),
+                                 static_cast<float>(residual_scale), static_cast<int>(quant),
+                                 branch_in ? r.data_ptr() : nullptr, y_out ? y.data_ptr() : nullptr,
+                                 quant ? static_cast<uint8_t*>(codes.data_ptr()) : nullptr,
+                                 quant ? scales.data_ptr() : nullptr, stream_of(x)),
+        "gated_residual_norm");
+  return {r, y, codes, scales};
+}
+
+std::tuple<Tensor, Tensor> mxfp4_quant(const Tensor& x_in) {
+  require_gfx950(x_in, "mxfp4_quant");
+  TORCH_CHECK_VALUE(x_in.dim() == 2 && x_in.size(1) > 0 && x_in.size(1) % 32 == 0,
+                    "mxfp4_quant: x [M, K] with K a multiple of 32 expected, got ", x_in.sizes());
+  dtype_code(x_in);
+  const Tensor x = x_in.stride(1) != 1 || x_in.stride(0) < x_in.size(1) ? x_in.contiguous() : x_in;
+  const int64_t M = x.size(0), K = x.size(1);
+  Tensor codes = empty({M, K / 2}, x, at::kByte), scales = empty({cdiv(K, 256), M, 8}, x, at::kByte);
+  const c10::DeviceGuard guard(x.device());
+  check(mxf8_mxfp4_quant(x.data_ptr(), dtype_code(x), M, K, std::max(x.stride(0), K),
+                         static_cast<uint8_t*>(codes.data_ptr()), static_cast<uint8_t*>(scales.data_ptr()),
+                         stream_of(x)),
+        "mxfp4_quant");
+  return {codes, scales};
+}
+
+// Codes [R, K / 2] and scales of an R-row matrix of K columns.
+void check_mxfp4(const Tensor& codes, const Tensor& scales, const char* what, const char* name) {
+  TORCH_CHECK_VALUE(codes.dim() == 2 && codes.scalar_type() == at::kByte && codes.size(1) > 0 &&
+                        codes.size(1) % 16 == 0 && codes.is_contiguous(),
+                    what, name, " codes must be contiguous uint8 [rows, K / 2] with K a multiple of 32, got ",
+                    codes.scalar_type(), " ", codes.sizes());
+  const std::array<int64_t, 3> want = {cdiv(codes.size(1), 128), codes.size(0), 8};
+  TORCH_CHECK_VALUE(scales.sizes() == at::IntArrayRef(want) && scales.scalar_type() == at::kByte && scales.is_contiguous(),
+                    what, name, " scales must be contiguous uint8 ", at::IntArrayRef(want), ", got ", scales.scalar_type(),
+                    " ", scales.sizes());
+  on_device(scales, codes.device(), what, name);
+}
+
+Tensor mxfp4_dequant(const Tensor& codes, const Tensor& scales, at::ScalarType dtype) {
+  require_gfx950(codes, "mxfp4_dequant");
+  check_mxfp4(codes, scales, "mxfp4_dequant: ", "x");
+  Tensor out = empty({codes.size(0), 2 * codes.size(1)}, codes, dtype);
+  const c10::DeviceGuard guard(codes.device());
+  check(mxf8_mxfp4_dequant(static_cast<const uint8_t*>(codes.data_ptr()), static_cast<const uint8_t*>(scales.data_ptr()),
+                           out.size(0), out.size(1), out.data_ptr(), dtype_code(out), stream_of(codes)),
+        "mxfp4_dequant");
+  return out;
+}
+
+Tensor gemm_mxfp4(const Tensor& a4, const Tensor& w4, const Tensor& sa, const Tensor& sw, const optional<Tensor>& bias,
+                  int64_t act) {
+  const char* what = "gemm_mxfp4: ";
+  require_gfx950(a4, "gemm_mxfp4");
+  check_mxfp4(a4, sa, what, "activation");
+  check_mxfp4(w4, sw, what, "weight");
+  TORCH_CHECK_VALUE(a4.size(1) == w4.size(1), what, "activations of K = ", 2 * a4.size(1), " and weights of K = ",
+                    2 * w4.size(1));
+  const at::Device dev = a4.device();
+  on_device(w4, dev, what, "w4");
+  const int64_t M = a4.size(0), N = w4.size(0), K = 2 * a4.size(1);
+  TORCH_CHECK_VALUE(!bias || (bias->scalar_type() == at::kBFloat16 && bias->numel() == N && bias->is_contiguous()), what,
+                    "bias must be ", N, " contiguous bf16 values");
+  if (bias) on_device(*bias, dev, what, "bias");
+  Tensor out = empty({M, N}, a4, at::kBFloat16);
+  const c10::DeviceGuard guard(dev);
+  check(mxf8_gemm_mxfp4(static_cast<const uint8_t*>(a4.data_ptr()), static_cast<const uint8_t*>(w4.data_ptr()),
+                        static_cast<const uint8_t*>(sa.data_ptr()), static_cast<const uint8_t*>(sw.data_ptr()),
+                        bias ? bias->data_ptr() : nullptr, static_cast<int>(act), out.data_ptr(), M, N, K, N,
+                        stream_of(a4)),
+        "gemm_mxfp4");
+  return out;
+}
+
 // The ops have no derivative.  With grad mode on, an output of an input that requires grad
 // requires grad and its backward raises; otherwise the call goes on below autograd (as the
 // Python declarations' autograd kernel does; forward-mode tangents end here).
@@ -325,9 +550,16 @@ TORCH_LIBRARY_IMPL(mxf8, CUDA, m) {
   m.impl("lora_down", &lora_down);
   m.impl("attn_quant_kv", &attn_quant_kv);
   m.impl("attn_fwd_q", &attn_fwd_q);
+  m.impl("rotary_table", &rotary_table);
+  m.impl("rotate_qk", &rotate_qk);
+  m.impl("gated_residual_norm", &gated_residual_norm);
+  m.impl("mxfp4_quant", &mxfp4_quant);
+  m.impl("mxfp4_dequant", &mxfp4_dequant);
+  m.impl("gemm_mxfp4", &gemm_mxfp4);
 }
 
 TORCH_LIBRARY_IMPL(mxf8, AutogradCUDA, m) {
-  for (const char* op : {"quant_rows", "adaln_quant_rows", "gemm_rowwise", "lora_down", "attn_quant_kv", "attn_fwd_q"})
+  for (const char* op : {"quant_rows", "adaln_quant_rows", "gemm_rowwise", "lora_down", "attn_quant_kv", "attn_fwd_q",
+                         "rotary_table", "rotate_qk", "gated_residual_norm", "mxfp4_quant", "mxfp4_dequant", "gemm_mxfp4"})
     m.impl(op, torch::CppFunction::makeFromBoxedFunction<&no_derivative>());
 }

@@ -296,15 +296,15 @@ def find_primary_block_list(transformer: nn.Module) -> tuple[str, nn.ModuleList]
     return max(pool, key=lambda nm: len(nm[1]))
 
 
-def _fuse_gelu_modules(block: nn.Module) -> None:
-    """Fold a tanh-GELU activation module into its FP8 projection (GEMM epilogue).
+def _fuse_gelu_modules(block: nn.Module, kind: type = FP8Linear) -> None:
+    """Fold a tanh-GELU activation module into its quantized projection (GEMM epilogue).
 
     Matches the activation modules of diffusers-style FFNs: a module with a ``proj``
     sub-module and ``approximate == "tanh"`` whose forward is gelu_tanh(proj(x)).
     """
     for name, mod in list(block.named_modules()):
         proj = getattr(mod, "proj", None)
-        if isinstance(proj, FP8Linear) and getattr(mod, "approximate", None) == "tanh" and proj.act == ACT_NONE:
+        if isinstance(proj, kind) and getattr(mod, "approximate", None) == "tanh" and proj.act == ACT_NONE:
             proj.act = ACT_GELU_TANH
             mod.forward = proj.forward  # the module's own forward would apply GELU a second time
 
@@ -322,6 +322,12 @@ def convert_transformer_to_fp8(
     Returns the number of converted modules.  ``fuse_gelu`` additionally folds tanh-GELU
     activations into the preceding FP8 GEMM (an extension; off by default).
     """
+    return _convert_blocks(transformer, exclude_patterns, keep_edge_blocks, fuse_gelu, FP8Linear, 16)
+
+
+def _convert_blocks(transformer: nn.Module, exclude_patterns: str | list[str], keep_edge_blocks: int, fuse_gelu: bool,
+                    kind: type, in_multiple: int) -> int:
+    """The conversion to ``kind`` (``FP8Linear``, or another class with its ``from_linear`` and ``act``)."""
     if isinstance(exclude_patterns, str):
         exclude_patterns = exclude_patterns.split(",")
     patterns = [p.strip().lower() for p in exclude_patterns if p.strip()]
@@ -334,12 +340,12 @@ def convert_transformer_to_fp8(
         for sub_name, sub in list(block.named_modules()):
             if not isinstance(sub, nn.Linear):
                 continue
-            if sub.in_features % 16 or sub.out_features % 16:
+            if sub.in_features % in_multiple or sub.out_features % 16:
                 continue
             path = (f"{list_name}.{idx}.{sub_name}" if sub_name else f"{list_name}.{idx}").lower()
             if any(p in path for p in patterns):
                 continue
-            new = FP8Linear.from_linear(sub)
+            new = kind.from_linear(sub)
             if not sub_name:
                 blocks[idx] = new
             else:
@@ -348,7 +354,7 @@ def convert_transformer_to_fp8(
                 setattr(parent, attr, new)
             converted += 1
         if fuse_gelu:
-            _fuse_gelu_modules(blocks[idx])
+            _fuse_gelu_modules(blocks[idx], kind)
     if torch.cuda.is_available():
         torch.cuda.empty_cache()
     return converted

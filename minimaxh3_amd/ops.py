@@ -6,7 +6,8 @@ torch.compile: the DiT blocks are compiled with ``fullgraph=False``
 breaks.  Outputs come from torch's caching allocator; launches go to the current stream.
 
 The ops of the hot path (quant_rows, adaln_quant_rows, gemm_rowwise, lora_down,
-attn_quant_kv, attn_fwd_q) run as native dispatcher kernels (csrc/torch_ops.cpp), which are
+attn_quant_kv, attn_fwd_q) and of the rest of a DiT block (rotary_table, rotate_qk,
+gated_residual_norm, mxfp4_quant, mxfp4_dequant, gemm_mxfp4) run as native dispatcher kernels (csrc/torch_ops.cpp), which are
 registered when this module is imported: the dispatcher reads an operator's kernels without
 a lock, so none may be added while another thread calls it.  Their Python bodies see only
 what has no native kernel: other devices, and a library built after the import.  The other
@@ -16,6 +17,7 @@ from __future__ import annotations
 
 import math
 import os
+from collections.abc import Sequence
 
 import torch
 
@@ -419,6 +421,106 @@ def _(q, c, k8, v8t, sk, sv, key_mask, key_bias, repair_tau, Sk, kv_mode=0):
 def softmax_c(scale: float | None, D: int) -> float:
     """c = (scale or 1/sqrt(D)) * log2(e) (kernels/fp8_attention.py:315)."""
     return (scale if scale is not None else 1.0 / math.sqrt(D)) * 1.4426950408889634
+
+
+# ---------------------------------------------------------------------------------------
+# Rotary positions, gated residual norms, 4-bit linear
+# ---------------------------------------------------------------------------------------
+
+@torch.library.custom_op("mxf8::rotary_table", mutates_args=())
+def rotary_table(positions: torch.Tensor, axis_dims: Sequence[int], theta: float) -> torch.Tensor:
+    """positions [..., A] (fp32 / fp64 / int32 / int64), axis_dims A even channel counts ->
+    [..., P, 2] fp32 pairs (cos, sin) of pos[a] * theta^(-2 i / axis_dims[a]), P = sum(axis_dims) / 2."""
+    return _native(positions, "rotary_table")(positions, axis_dims, theta)
+
+
+@rotary_table.register_fake
+def _(positions, axis_dims, theta):
+    return positions.new_empty((*positions.shape[:-1], sum(d // 2 for d in axis_dims), 2), dtype=torch.float32)
+
+
+@torch.library.custom_op("mxf8::rotate_qk", mutates_args=())
+def rotate_qk(q: torch.Tensor, k: torch.Tensor | None, table: torch.Tensor, q_weight: torch.Tensor | None,
+              k_weight: torch.Tensor | None, eps: float, interleaved: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """Per-head RMS norm (with weights) and rotation of q [B, H, S, D] and k [B, Hk, S, D] by table
+    [S, P, 2] or [B, S, P, 2]; k None: the second output is empty.  Outputs keep the inputs' order
+    of dimensions in memory."""
+    return _native(q, "rotate_qk")(q, k, table, q_weight, k_weight, eps, interleaved)
+
+
+@rotate_qk.register_fake
+def _(q, k, table, q_weight, k_weight, eps, interleaved):
+    def like(x):
+        o = torch.empty_like(x if x.stride(-1) == 1 or x.shape[-1] <= 1 else x.contiguous())
+        return o if o.stride(-1) == 1 else x.new_empty(x.shape)
+
+    return like(q), q.new_empty((0,)) if k is None else like(k)
+
+
+@torch.library.custom_op("mxf8::gated_residual_norm", mutates_args=())
+def gated_residual_norm(x: torch.Tensor, branch: torch.Tensor | None, gate: torch.Tensor | None,
+                        shift: torch.Tensor | None, scale: torch.Tensor | None, branch_weight: torch.Tensor | None,
+                        weight: torch.Tensor | None, layer: bool, eps: float, residual_scale: float, quant: int,
+                        want_y: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """r = residual_scale x + gate PN(branch), y = N(r) weight (1 + scale) + shift -> (r [B, S, C] or
+    empty without a branch, y [B, S, C] or empty, codes, scales); quant: N.QUANT_NONE (codes and
+    scales empty), N.QUANT_E4M3 (those of quant_rows(y)), N.QUANT_MXFP4 (those of mxfp4_quant(y))."""
+    return _native(x, "gated_residual_norm")(x, branch, gate, shift, scale, branch_weight, weight, layer, eps,
+                                             residual_scale, quant, want_y)
+
+
+@gated_residual_norm.register_fake
+def _(x, branch, gate, shift, scale, branch_weight, weight, layer, eps, residual_scale, quant, want_y):
+    B, S, C = x.shape
+    r = x.new_empty((B, S, C) if branch is not None else (0,))
+    y = x.new_empty((B, S, C) if want_y or quant == N.QUANT_NONE else (0,))
+    if quant == N.QUANT_E4M3:
+        return r, y, x.new_empty((B * S, C), dtype=E4M3), x.new_empty((B * S, 1), dtype=torch.float32)
+    if quant == N.QUANT_MXFP4:
+        return (r, y, x.new_empty((B * S, C // 2), dtype=torch.uint8),
+                x.new_empty(mxfp4_scale_shape(B * S, C), dtype=torch.uint8))
+    return r, y, x.new_empty((0,), dtype=torch.uint8), x.new_empty((0,), dtype=torch.uint8)
+
+
+def mxfp4_scale_shape(M: int, K: int) -> tuple[int, int, int]:
+    """Shape of the block scales of an M x K matrix: [ceil(K / 256), M, 8] (slab of 256 columns;
+    row; block of 32)."""
+    return (_cdiv(K, 256), M, 8)
+
+
+@torch.library.custom_op("mxf8::mxfp4_quant", mutates_args=())
+def mxfp4_quant(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """[M, K] bf16/fp16/fp32 -> 4-bit codes [M, K / 2] uint8 and block scales [ceil(K / 256), M, 8] uint8."""
+    return _native(x, "mxfp4_quant")(x)
+
+
+@mxfp4_quant.register_fake
+def _(x):
+    M, K = x.shape
+    return x.new_empty((M, K // 2), dtype=torch.uint8), x.new_empty(mxfp4_scale_shape(M, K), dtype=torch.uint8)
+
+
+@torch.library.custom_op("mxf8::mxfp4_dequant", mutates_args=())
+def mxfp4_dequant(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """The values of mxfp4_quant's codes and scales, [M, K] of `dtype`."""
+    return _native(codes, "mxfp4_dequant")(codes, scales, dtype)
+
+
+@mxfp4_dequant.register_fake
+def _(codes, scales, dtype):
+    return codes.new_empty((codes.shape[0], 2 * codes.shape[1]), dtype=dtype)
+
+
+@torch.library.custom_op("mxf8::gemm_mxfp4", mutates_args=())
+def gemm_mxfp4(a4: torch.Tensor, w4: torch.Tensor, sa: torch.Tensor, sw: torch.Tensor, bias: torch.Tensor | None,
+               act: int) -> torch.Tensor:
+    """bf16(act(a w^T + bias)) of 4-bit activations (a4, sa) [M, K] and weights (w4, sw) [N, K], bf16 [M, N]."""
+    return _native(a4, "gemm_mxfp4")(a4, w4, sa, sw, bias, act)
+
+
+@gemm_mxfp4.register_fake
+def _(a4, w4, sa, sw, bias, act):
+    return a4.new_empty((a4.shape[0], w4.shape[0]), dtype=torch.bfloat16)
 
 
 def _register() -> None:
