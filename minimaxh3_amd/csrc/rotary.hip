@@ -7,6 +7,8 @@
 //   (u, v) = (a cos - b sin, a sin + b cos) for the pairs (a, b) of y: channels (2 j, 2 j + 1), or (j, j + P)
 //            with P pairs; channels from 2 P on stay as they are
 // Everything is fp32 between the load and the one rounding at the store.
+#include <type_traits>
+
 #include "common.h"
 #include "rowio.h"
 
@@ -89,18 +91,56 @@ struct RotArgs {
   int64_t S;
   int D, P, B;
   int steps[2], per;  // head steps of q and k, and how many one wave takes
-  float eps;
+  float eps, inv_d;
 };
 
-// One wave per token and span of head steps: L lanes hold a head (8 channels each), so a step moves 64 / L
-// heads, 16 bytes a lane, and the token's cos / sin stay in registers over the heads.
-template <int DT, int L, bool INTERLEAVED>
+// Sum over the L lanes that hold a head, in each of them.
+template <int L>
+__device__ __forceinline__ float head_sum(float v) {
+  auto dpp = [](float x, auto ctrl) {
+    return __builtin_bit_cast(
+        float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  v += dpp(v, std::integral_constant<int, 0xb1>{});   // lane ^ 1
+  v += dpp(v, std::integral_constant<int, 0x4e>{});   // lane ^ 2
+  v += dpp(v, std::integral_constant<int, 0x141>{});  // the other half of eight
+  if constexpr (L >= 16) v += dpp(v, std::integral_constant<int, 0x140>{});  // the other half of sixteen
+  if constexpr (L >= 32) {
+    const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+  }
+  if constexpr (L >= 64) {
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+  }
+  return v;
+}
+
+// One wave per token and span of head steps: L lanes hold a head (8 channels each), so a step moves 64 / L heads,
+// 16 bytes a lane.  The token's cos / sin and the norm's weights stay in registers over the heads, and the
+// next ROT_UNROLL steps' loads are in flight together.
+//
+// HEAD_FULL: a head fills its lanes (D = 8 L); HEAD_CHUNKS: whole chunks of 8 channels, and half-split pairs at the
+// same place of two lanes' chunks (P % 8 == 0); HEAD_ANY: the last chunk may be cut, and half-split partners
+// come through LDS.
+//
+// Bound by memory: 20280 tokens x (24 + 24) heads x 128 in bf16, 509 MB, 92 us (5.5 TB/s), the same without the
+// norm; one step at a time 96.5, with stores that stay in the caches 100.
+constexpr int ROT_UNROLL = 6;
+enum { HEAD_FULL, HEAD_CHUNKS, HEAD_ANY };
+
+template <int DT, int L, bool INTERLEAVED, int MODE>
 __global__ __launch_bounds__(256) void rotate_qk_kernel(const RotArgs a) {
+  constexpr int G = 64 / L, ES = DT == MXF8_F32 ? 4 : 2;
+  __shared__ float exchange[MODE == HEAD_ANY && !INTERLEAVED ? 4 * 512 : 1];
   const int lane = threadIdx.x & 63, l = lane % L, hg = lane / L;
-  const int64_t token = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t token = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (token >= a.S * a.B) return;
-  const int64_t b = token / a.S, s = token - b * a.S;
-  const int c0 = 8 * l, n = min(a.D - c0, 8);  // this lane's channels (n <= 0: none)
+  const int b = (uint32_t)token / (uint32_t)a.S;
+  const int64_t s = token - (int64_t)b * a.S;
+  const int c0 = 8 * l;                       // this lane's channels
+  const bool there = MODE == HEAD_FULL || c0 < a.D;  // any of them
+  const int n = MODE == HEAD_ANY ? min(max(a.D - c0, 0), 8) : 8;  // how many, if any
   const float2* tab = reinterpret_cast<const float2*>(a.table + b * a.table_batch) + s * a.P;
   constexpr int NP = INTERLEAVED ? 4 : 8;
   float co[NP], si[NP];
@@ -114,59 +154,109 @@ __global__ __launch_bounds__(256) void rotate_qk_kernel(const RotArgs a) {
     co[i] = t.x;
     si[i] = INTERLEAVED || c >= a.P ? t.y : -t.y;
   }
-  const int total = a.steps[0] + a.steps[1];
-  const int first = blockIdx.y * a.per, last = min(first + a.per, total);
-  // half-split partner: channel c +- P is in lane l +- P / 8, at the same place of its eight when P % 8 == 0
-  const int plane = INTERLEAVED ? lane : (lane - l) + min(max(c0 < a.P ? l + a.P / 8 : l - a.P / 8, 0), L - 1);
-#pragma unroll 4
-  for (int it = first; it < last; ++it) {
-    const int part = it >= a.steps[0];
-    const int h = (it - (part ? a.steps[0] : 0)) * (64 / L) + hg;
-    const bool on = h < a.heads[part] && n > 0;
-    Raw8<DT> v;
-    if (on)
-      v.load(a.x[part], b * a.xs[part][0] + h * a.xs[part][1] + s * a.xs[part][2] + c0);
-    else
-      v.zero();
-    float f[8];
-    v.get(f);
-    if (a.w[part]) {
-      float ss = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(f[i], f[i], ss);
-#pragma unroll
-      for (int off = L / 2; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, 64);
-      const float r = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, (float)a.D) + a.eps));
-      Raw8<DT> wv;
-      if (n > 0)
-        wv.load(a.w[part], c0);
+  // half-split partner: channel c +- P is in lane l +- P / 8, at the same place of its eight as P % 8 == 0
+  const int plane = (lane - l) + min(max(c0 < a.P ? l + a.P / 8 : l - a.P / 8, 0), L - 1);
+  const int first = blockIdx.y * a.per, last = min(first + a.per, a.steps[0] + a.steps[1]);
+
+  auto part = [&](auto p_tag) {
+    constexpr int p = decltype(p_tag)::value;
+    const int s0 = max(first - (p ? a.steps[0] : 0), 0), s1 = min(last - (p ? a.steps[0] : 0), a.steps[p]);
+    if (s0 >= s1) return;
+    const bool norm = a.w[p] != nullptr;
+    Raw8<DT> wv, wp;
+    wv.zero();
+    if (norm && there) {
+      if (MODE != HEAD_ANY || n == 8)
+        wv.load(a.w[p], c0);
       else
-        wv.zero();
-      float wf[8];
-      wv.get(wf);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] *= r * wf[i];
+        wv.load_part(a.w[p], c0, n);
     }
-    float o[8];
-    if constexpr (INTERLEAVED) {
+    wp = wv;
+    if constexpr (!INTERLEAVED && MODE != HEAD_ANY) wp.from_lane(plane);
+    const char* x = static_cast<const char*>(a.x[p]) + ((int64_t)b * a.xs[p][0] + s * a.xs[p][2]) * ES;
+    char* o = static_cast<char*>(a.o[p]) + ((int64_t)b * a.os[p][0] + s * a.os[p][2]) * ES;
+    // byte offsets of this lane's head and channels within a step; heads past the last one read it again
+    const uint32_t xo = (uint32_t)(hg * a.xs[p][1] + (there ? c0 : 0)) * ES, oo = (uint32_t)(hg * a.os[p][1] + c0) * ES;
+    const int in_last = a.heads[p] - (a.steps[p] - 1) * G;  // heads of the last step
+    const uint32_t xo_last = (uint32_t)(min(hg, in_last - 1) * a.xs[p][1] + (there ? c0 : 0)) * ES;
+    const int64_t xstep = a.xs[p][1] * G * ES, ostep = a.os[p][1] * G * ES;
+    for (int st = s0; st < s1; st += ROT_UNROLL) {
+      Raw8<DT> v[ROT_UNROLL];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        o[2 * i] = f[2 * i] * co[i] - f[2 * i + 1] * si[i];
-        o[2 * i + 1] = f[2 * i] * si[i] + f[2 * i + 1] * co[i];
+      for (int u = 0; u < ROT_UNROLL; ++u)
+        if (st + u < s1) {
+          const uint32_t off = st + u + 1 == a.steps[p] ? xo_last : xo;
+          if (MODE != HEAD_ANY || n == 8)
+            v[u].load_off(x + (st + u) * xstep, off);
+          else
+            v[u].load_part(x + (st + u) * xstep + off, 0, n);
+        }
+#pragma unroll
+      for (int u = 0; u < ROT_UNROLL; ++u) {
+        if (st + u >= s1) break;
+        float f[8], q[8];
+        if (!there) v[u].zero();
+        v[u].get(f);
+        if constexpr (!INTERLEAVED && MODE != HEAD_ANY) {
+          v[u].from_lane(plane);
+          v[u].get(q);
+        }
+        if (norm) {
+          float ss = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(f[i], f[i], ss);
+          const float r = rsqrtf(__builtin_fmaf(head_sum<L>(ss), a.inv_d, a.eps));
+          float k[8];
+          wv.get(k);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] *= r * k[i];
+          if constexpr (!INTERLEAVED && MODE != HEAD_ANY) {
+            wp.get(k);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[i] *= r * k[i];
+          }
+        }
+        if constexpr (!INTERLEAVED && MODE == HEAD_ANY) {
+          // (this wave's part of the exchange alone: LDS operations of a wave complete in order)
+          float* mine = exchange + (threadIdx.x & ~63) * 8;
+          *reinterpret_cast<v4f*>(mine + lane * 8) = v4f{f[0], f[1], f[2], f[3]};
+          *reinterpret_cast<v4f*>(mine + lane * 8 + 4) = v4f{f[4], f[5], f[6], f[7]};
+          __builtin_amdgcn_wave_barrier();
+          const float* head = mine + hg * L * 8;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int c = c0 + i, j = c < a.P ? c + a.P : c - a.P;
+            q[i] = head[c < 2 * a.P ? j : c];
+          }
+          __builtin_amdgcn_wave_barrier();
+        }
+        float y[8];
+        if constexpr (INTERLEAVED) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            y[2 * i] = f[2 * i] * co[i] - f[2 * i + 1] * si[i];
+            y[2 * i + 1] = f[2 * i] * si[i] + f[2 * i + 1] * co[i];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = f[i] * co[i] + q[i] * si[i];
+        }
+        Raw8<DT> w;
+        w.set(y);
+        if (there && (st + u + 1 < a.steps[p] || hg < in_last)) {
+          if (MODE != HEAD_ANY || n == 8)
+            w.stream_off(o + (st + u) * ostep, oo);
+          else
+            w.store_part(o + (st + u) * ostep + oo, 0, n);
+        }
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = f[i] * co[i] + __shfl(f[i], plane, 64) * si[i];
     }
-    if (on) {
-      Raw8<DT> w;
-      w.set(o);
-      w.store(a.o[part], b * a.os[part][0] + h * a.os[part][1] + s * a.os[part][2] + c0);
-    }
-  }
+  };
+  part(std::integral_constant<int, 0>{});
+  part(std::integral_constant<int, 1>{});
 }
 
-// Any head width: one wave per head, element by element.
+// Heads wider than a wave's 512 channels or far apart in memory: one wave per head, element by element.
 template <int DT, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void rotate_qk_any_kernel(const RotArgs a) {
   typedef typename Elem<DT>::T T;
@@ -207,9 +297,12 @@ __global__ __launch_bounds__(256) void rotate_qk_any_kernel(const RotArgs a) {
 template <int DT, bool INTERLEAVED>
 static void launch_rotate(RotArgs& a, hipStream_t st) {
   const int64_t tokens = a.S * a.B;
-  // lanes per head: the 8-channel chunks of a head, up to a power of two.  A half-split pair's channels must
-  // stand at the same place of their lanes' chunks.
-  if (a.D % 8 || a.D > 512 || (!INTERLEAVED && a.P % 8)) {
+  // lanes per head: the 8-channel chunks of a head, up to a power of two.  Heads wider than a wave, or far apart,
+  // go element by element.
+  bool near_heads = true;  // (32-bit offsets within a step of up to 8 heads)
+  for (int p = 0; p < 2; ++p)
+    for (const int64_t hs : {a.xs[p][1], a.os[p][1]}) near_heads = near_heads && hs >= 0 && hs < (1 << 24);
+  if (a.D > 512 || !near_heads) {
     rotate_qk_any_kernel<DT, INTERLEAVED><<<dim3((unsigned)cdiv(tokens * (a.heads[0] + a.heads[1]), 4)), 256, 0, st>>>(a);
     return;
   }
@@ -222,12 +315,23 @@ static void launch_rotate(RotArgs& a, hipStream_t st) {
   a.per = total;
   while (a.per > 1 && tokens * cdiv(total, a.per) < 2048) a.per = (a.per + 1) / 2;
   const dim3 grid((unsigned)cdiv(tokens, 4), (unsigned)cdiv(total, a.per));
+  const bool any = a.D % 8 || (!INTERLEAVED && a.P % 8);
+#define MXF8_CASE(LL)                                                                \
+  case LL:                                                                           \
+    if (any)                                                                         \
+      rotate_qk_kernel<DT, LL, INTERLEAVED, HEAD_ANY><<<grid, 256, 0, st>>>(a);      \
+    else if (a.D == 8 * LL)                                                          \
+      rotate_qk_kernel<DT, LL, INTERLEAVED, HEAD_FULL><<<grid, 256, 0, st>>>(a);     \
+    else                                                                             \
+      rotate_qk_kernel<DT, LL, INTERLEAVED, HEAD_CHUNKS><<<grid, 256, 0, st>>>(a);   \
+    break;
   switch (L) {
-    case 8: rotate_qk_kernel<DT, 8, INTERLEAVED><<<grid, 256, 0, st>>>(a); break;
-    case 16: rotate_qk_kernel<DT, 16, INTERLEAVED><<<grid, 256, 0, st>>>(a); break;
-    case 32: rotate_qk_kernel<DT, 32, INTERLEAVED><<<grid, 256, 0, st>>>(a); break;
-    default: rotate_qk_kernel<DT, 64, INTERLEAVED><<<grid, 256, 0, st>>>(a); break;
+    MXF8_CASE(8)
+    MXF8_CASE(16)
+    MXF8_CASE(32)
+    MXF8_CASE(64)
   }
+#undef MXF8_CASE
 }
 
 }  // namespace mxf8
@@ -312,6 +416,7 @@ extern "C" int mxf8_rotate_qk(const void* q, const int64_t q_strides[4], int64_t
   a.table_batch = table_batch_stride;
   a.S = S, a.B = (int)B, a.D = (int)D, a.P = (int)P;
   a.eps = eps;
+  a.inv_d = 1.0f / (float)D;
 #define MXF8_CASE(DT)                                   \
   if (dtype == DT) {                                    \
     if (interleaved) launch_rotate<DT, true>(a, stream); \
