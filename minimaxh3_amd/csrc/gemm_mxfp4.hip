@@ -10,22 +10,10 @@
 // both operands follow it, and with this one the four scales that a lane needs in a stage are one aligned dword
 // of the slab's eight bytes per row, which the instruction picks bytes from.
 #include "gemm_common.h"
+#include "gemm_mxfp4_ring.h"
 #include "mxfp4.h"
 
 namespace mxf8 {
-
-__device__ __forceinline__ v8i mx_wide(const v4i& v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
-
-// One instruction on block 4 g + T of the stage: 16 bytes of each operand per lane, byte T of the scale dwords.
-template <int T>
-__device__ __forceinline__ v16f mx_mma(const v4i& a, const v4i& b, const v16f& c, uint32_t sa, uint32_t sb) {
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_wide(a), mx_wide(b), c, 4, 4, T, (int)sa, T, (int)sb);
-}
-
-// 16 bytes: logical chunk `chunk` of `row` (swizzled storage).
-__device__ __forceinline__ v4i mx_frag(const uint8_t* tile, int row, int chunk) {
-  return *reinterpret_cast<const v4i*>(tile + row * GEMM_BK + ((chunk ^ lds_swz<GEMM_BK>(row)) << 4));
-}
 
 // Scale dwords of one stage: this lane's rows of the W and X tiles, blocks 4 g .. 4 g + 3.
 template <class C>
@@ -40,17 +28,6 @@ struct MxScales {
     for (int b = 0; b < C::TM; ++b) asm volatile("v_mov_b32 %0, %1" : "=v"(x[b]) : "v"(o.x[b]));
   }
 };
-
-template <int ACT>
-__device__ __forceinline__ uint2 mx_out_quad(const v4f& x, const v4f& b) {
-  float v[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    v[e] = x[e] + b[e];
-    if constexpr (ACT == MXF8_ACT_GELU_TANH) v[e] = gelu_tanh_f32(v[e]);
-  }
-  return make_uint2(bf16x2(v[0], v[1]), bf16x2(v[2], v[3]));
-}
 
 template <class C, int ACT, bool KTAIL>
 __global__ __launch_bounds__(C::THREADS) void gemm_mxfp4_kernel(const uint8_t* __restrict__ a4, const uint8_t* __restrict__ w4,
@@ -224,53 +201,32 @@ __global__ __launch_bounds__(C::THREADS) void gemm_mxfp4_kernel(const uint8_t* _
     asm volatile("" : "+v"(ln));
     const int r = ln & 31, g = ln >> 5;
     auto quad = [&](const v16f& c, int q) { return v4f{c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]}; };
-    const bool staged = ((ld_out & 7) == 0) && ((((uintptr_t)out) & 15) == 0) && (m0 + C::BM <= M) && (n0 + C::BN <= N);
-    if (staged) {
-      // whole tile: each 32-token round of a wave goes through its own 1 / NW of the last stage's buffer, and
-      // leaves as 16-byte stores of whole row segments
-      constexpr int RB = TN * 64, NCH = RB / 16, RPI = 64 / NCH;
-      static_assert(32 * RB <= C::STAGE / C::NW, "per-wave staging region");
-      uint8_t* const wreg = smem + ((gs + 1) & 1) * C::STAGE + wave * (C::STAGE / C::NW);
+    // Each 32-token round of a wave goes through its own 1 / NW of the last stage's buffer and leaves as 16-byte stores
+    // of whole row segments, at any alignment; what a tile at the matrix's edge cuts is stored one by one.
+    constexpr int RB = TN * 64, NCH = RB / 16, RPI = 64 / NCH;
+    static_assert(32 * RB <= C::STAGE / C::NW, "per-wave staging region");
+    uint8_t* const wreg = smem + ((gs + 1) & 1) * C::STAGE + wave * (C::STAGE / C::NW);
+    const bool inside = m0 + C::BM <= M && n0 + C::BN <= N;
 #pragma unroll
-      for (int b = 0; b < TM; ++b) {
+    for (int b = 0; b < TM; ++b) {
 #pragma unroll
-        for (int a = 0; a < TN; ++a)
+      for (int a = 0; a < TN; ++a)
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<uint2*>(wreg + r * RB + (((4 * a + q) ^ (r & (NCH - 1))) << 4) + 8 * g) =
-                mx_out_quad<ACT>(quad(acc[a][b], q), *reinterpret_cast<const v4f*>(ep_b + wrow0 + 32 * a + 8 * q + 4 * g));
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<uint2*>(wreg + r * RB + (((4 * a + q) ^ (r & (NCH - 1))) << 4) + 8 * g) =
+              mx_out_quad<ACT>(quad(acc[a][b], q), *reinterpret_cast<const v4f*>(ep_b + wrow0 + 32 * a + 8 * q + 4 * g));
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-        for (int i = 0; i < 32 / RPI; ++i) {
-          const int row = i * RPI + ln / NCH, ch = ln % NCH;
-          const uint4 val = *reinterpret_cast<const uint4*>(wreg + row * RB + ((ch ^ (row & (NCH - 1))) << 4));
-          store_out16(out + (int64_t)(m0 + xrow0 + 32 * b + row) * ld_out + n0 + wrow0 + ch * 8, val);
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      for (int i = 0; i < 32 / RPI; ++i) {
+        const int row = i * RPI + ln / NCH, ch = ln % NCH;
+        const uint4 val = *reinterpret_cast<const uint4*>(wreg + row * RB + ((ch ^ (row & (NCH - 1))) << 4));
+        const int m = m0 + xrow0 + 32 * b + row, n = n0 + wrow0 + ch * 8;
+        if (inside)
+          mx_store8<true>(out + (int64_t)m * ld_out + n, val, 8);
+        else if (m < M)
+          mx_store8<true>(out + (int64_t)m * ld_out + n, val, N - n);
       }
-    } else {
-      const bool vec_ok = ((ld_out & 3) == 0) && ((((uintptr_t)out) & 7) == 0);
-#pragma unroll
-      for (int b = 0; b < TM; ++b) {
-        const int m = m0 + xrow0 + 32 * b + r;
-        if (m >= M) continue;
-#pragma unroll
-        for (int a = 0; a < TN; ++a)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int nl = wrow0 + 32 * a + 8 * q + 4 * g, n = n0 + nl;
-            const uint2 o = mx_out_quad<ACT>(quad(acc[a][b], q), *reinterpret_cast<const v4f*>(ep_b + nl));
-            uint16_t* dst = out + (int64_t)m * ld_out + n;
-            if (vec_ok && n + 3 < N) {
-              *reinterpret_cast<uint2*>(dst) = o;
-            } else {
-              const uint16_t oo[4] = {(uint16_t)o.x, (uint16_t)(o.x >> 16), (uint16_t)o.y, (uint16_t)(o.y >> 16)};
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (n + e < N) dst[e] = oo[e];
-            }
-          }
-      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
     tm = tm_n;
     tn = tn_n;
@@ -288,6 +244,42 @@ static void launch_mxfp4(const uint8_t* a4, const uint8_t* w4, const uint8_t* sa
   const int group_m = Kb >= 8192 ? 4 : 8;
   gemm_mxfp4_kernel<C, ACT, KTAIL><<<dim3(grid), dim3(C::THREADS), 0, st>>>(a4, w4, sa, sw, bias, out, M, N, Kb, ld_out,
                                                                             tiles_m, tiles_n, group_m);
+}
+
+typedef MxRing<32, 64, 1, 2, 6> MxRing32x64;      // 77 KB of LDS: two workgroups per CU
+typedef MxRing<64, 64, 2, 2, 4> MxRing64x64;      // 68 KB: two
+typedef MxRing<128, 64, 4, 2, 3> MxRing128x64;    // 77 KB: two
+typedef MxRing<128, 128, 2, 4, 4> MxRing128x128;  // 136 KB: one
+
+template <class C>
+static void launch_mxfp4_ring(int act, const uint8_t* a4, const uint8_t* w4, const uint8_t* sa, const uint8_t* sw,
+                              const uint16_t* bias, uint16_t* out, int M, int N, int Kb, int64_t ld_out, hipStream_t st) {
+  const int tiles_m = (int)cdiv(M, C::BM), tiles_n = (int)cdiv(N, C::BN);
+  const bool ktail = Kb % GEMM_BK != 0;
+#define MXF8_CASE(A, T)                                                                                        \
+  if (act == A && ktail == T)                                                                                  \
+    gemm_mxfp4_ring_kernel<C, A, T><<<dim3(tiles_m * tiles_n), dim3(C::THREADS), 0, st>>>(                     \
+        a4, w4, sa, sw, bias, out, M, N, Kb, ld_out, tiles_m, tiles_n);
+  MXF8_CASE(MXF8_ACT_NONE, false)
+  MXF8_CASE(MXF8_ACT_NONE, true)
+  MXF8_CASE(MXF8_ACT_GELU_TANH, false)
+  MXF8_CASE(MXF8_ACT_GELU_TANH, true)
+#undef MXF8_CASE
+}
+
+template <int TM, int NW>
+static void launch_mxfp4_rows(int act, const uint8_t* a4, const uint8_t* w4, const uint8_t* sa, const uint8_t* sw,
+                              const uint16_t* bias, uint16_t* out, int M, int N, int Kb, int64_t ld_out, hipStream_t st) {
+  const dim3 grid((unsigned)cdiv(N, 16), (unsigned)cdiv(M, 16 * TM));
+  const bool ktail = Kb % GEMM_BK != 0;
+#define MXF8_CASE(A, T)                                                                                                 \
+  if (act == A && ktail == T)                                                                                           \
+    gemm_mxfp4_rows_kernel<TM, NW, A, T><<<grid, 64 * NW, 0, st>>>(a4, w4, sa, sw, bias, out, M, N, Kb, ld_out);
+  MXF8_CASE(MXF8_ACT_NONE, false)
+  MXF8_CASE(MXF8_ACT_NONE, true)
+  MXF8_CASE(MXF8_ACT_GELU_TANH, false)
+  MXF8_CASE(MXF8_ACT_GELU_TANH, true)
+#undef MXF8_CASE
 }
 
 }  // namespace mxf8
@@ -312,7 +304,23 @@ extern "C" int mxf8_gemm_mxfp4(const uint8_t* a4, const uint8_t* w4, const uint8
   if (cdiv(M, 128) * cdiv(N, 128) > 0x7fffffff) return set_error(MXF8_EINVAL, "%s: shape too large", what);
   const uint16_t* b16 = static_cast<const uint16_t*>(bias);
   uint16_t* o16 = static_cast<uint16_t*>(out);
-  const bool ktail = Kb % GEMM_BK != 0, big = cdiv(M, 256) * cdiv(N, 256) >= 256;
+#define MXF8_MX_SMALL(launch)                                                        \
+  launch(act, a4, w4, sa, sw, b16, o16, iM, iN, Kb, ld_out, stream);                 \
+  return check_launch(what);
+  const bool ktail = Kb % GEMM_BK != 0;
+  const int pick = mxfp4_pick(M, N, K, cus);
+  switch (pick) {
+    case MX_ROWS16_4: MXF8_MX_SMALL((launch_mxfp4_rows<1, 4>))
+    case MX_ROWS16_8: MXF8_MX_SMALL((launch_mxfp4_rows<1, 8>))
+    case MX_ROWS16_16: MXF8_MX_SMALL((launch_mxfp4_rows<1, 16>))
+    case MX_ROWS32: MXF8_MX_SMALL((launch_mxfp4_rows<2, 4>))
+    case MX_RING_32x64: MXF8_MX_SMALL(launch_mxfp4_ring<MxRing32x64>)
+    case MX_RING_64x64: MXF8_MX_SMALL(launch_mxfp4_ring<MxRing64x64>)
+    case MX_RING_128x64: MXF8_MX_SMALL(launch_mxfp4_ring<MxRing128x64>)
+    case MX_RING_128x128: MXF8_MX_SMALL(launch_mxfp4_ring<MxRing128x128>)
+    default: break;
+  }
+#undef MXF8_MX_SMALL
 #define MXF8_MX_CASE(Cfg, A, T)                                                                       \
   if (act == A && ktail == T) {                                                                       \
     launch_mxfp4<Cfg, A, T>(a4, w4, sa, sw, b16, o16, iM, iN, Kb, ld_out, cus, stream);               \
@@ -321,7 +329,7 @@ extern "C" int mxf8_gemm_mxfp4(const uint8_t* a4, const uint8_t* w4, const uint8
 #define MXF8_MX_CASES(Cfg)                                                                                   \
   MXF8_MX_CASE(Cfg, MXF8_ACT_NONE, false) MXF8_MX_CASE(Cfg, MXF8_ACT_NONE, true)                             \
   MXF8_MX_CASE(Cfg, MXF8_ACT_GELU_TANH, false) MXF8_MX_CASE(Cfg, MXF8_ACT_GELU_TANH, true)
-  if (big) {
+  if (pick == MX_TILE_256) {
     MXF8_MX_CASES(GemmBig)
   } else {
     MXF8_MX_CASES(GemmSmall)

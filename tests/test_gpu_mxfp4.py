@@ -113,9 +113,19 @@ def test_product(m, n, k):
     product(m, n, k, seed=m + n)
 
 
-@pytest.mark.parametrize("m,n,k", [(4100, 4104, 256), (4096, 4096, 96), (8200, 2100, 288), (4097, 4224, 800)])
+@pytest.mark.parametrize("m,n,k", [(4096, 8192, 96), (4097, 4224, 800)])
 def test_product_of_many_tiles(m, n, k):
     product(m, n, k, seed=m)
+
+
+@pytest.mark.parametrize("act", [0, 1])
+@pytest.mark.parametrize("m,n,k", [(1, 9216, 3072), (7, 1001, 288), (3, 64, 8224), (17, 130, 512), (33, 2100, 96),
+                                   (130, 4100, 800), (300, 4100, 320), (256, 9216, 2080), (513, 12288, 800),
+                                   (2100, 1001, 768), (4100, 4104, 256), (6000, 4100, 288)])
+def test_every_kernel(m, n, k, act):
+    """Each of the product's kernels (tests/test_mxfp4_tiles.py), with whole and cut stages and tiles, rows of
+    outputs at any alignment."""
+    product(m, n, k, seed=m + k, act=act)
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 48, 3072), (20, 70, 96), (130, 300, 320), (700, 256, 768), (4500, 4100, 64)])
