@@ -66,6 +66,8 @@ _SIGNATURES = {
     "mxf8_mxfp4_scale_bytes": (_i64, [_i64, _i64]),
     "mxf8_mxfp4_quant": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp]),
     "mxf8_mxfp4_dequant": (_i32, [_vp, _vp, _i64, _i64, _vp, _i32, _vp]),
+    "mxf8_mxfp4_linear_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32]),
+    "mxf8_mxfp4_linear": (_i32, [_vp, _i32, _i64, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _i64, _vp, _vp]),
     "mxf8_gemm_mxfp4": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _i64, _vp]),
 }
 EXPORTS = tuple(_SIGNATURES)

@@ -19,8 +19,7 @@ namespace mxf8 {
 template <class C>
 struct MxScales {
   uint32_t w[C::TN], x[C::TM];
-  // *this = o, as moves that the compiler cannot fold: it would leave the values where they are and put the
-  // loads that follow into `o` elsewhere, to be moved at the end of the stage while they are in flight.
+  // *this = o, as moves that the compiler does not fold: it would sink the reads of `o` to their first use.
   __device__ __forceinline__ void take(const MxScales& o) {
 #pragma unroll
     for (int a = 0; a < C::TN; ++a) asm volatile("v_mov_b32 %0, %1" : "=v"(w[a]) : "v"(o.w[a]));
@@ -37,8 +36,10 @@ __global__ __launch_bounds__(C::THREADS) void gemm_mxfp4_kernel(const uint8_t* _
                                                                 uint16_t* __restrict__ out, int M, int N, int Kb,
                                                                 int64_t ld_out, int tiles_m, int tiles_n, int group_m) {
   constexpr int TM = C::TM, TN = C::TN;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * C::STAGE + C::BN * 4];
-  float* const ep_b = reinterpret_cast<float*>(smem + 2 * C::STAGE);  // [BN]
+  constexpr int SCALES = (C::BM + C::BN) * MX_SLAB;  // a stage's scales: W rows, then X rows
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * C::STAGE + 2 * SCALES + C::BN * 4];
+  uint8_t* const sc_smem = smem + 2 * C::STAGE;
+  float* const ep_b = reinterpret_cast<float*>(sc_smem + 2 * SCALES);  // [BN]
 
   const int ntiles = tiles_m * tiles_n;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -59,46 +60,28 @@ __global__ __launch_bounds__(C::THREADS) void gemm_mxfp4_kernel(const uint8_t* _
   int s = blockIdx.x;
   int tm, tn;
   tile_coords(s, tiles_m, tiles_n, group_m, tm, tn);
+  int tm_c = tm, tn_c = tn;  // the tile that is being copied
   __amdgpu_buffer_rsrc_t wrs = rsrc(w4, tn * C::BN, N, C::BN), xrs = rsrc(a4, tm * C::BM, M, C::BM);
-  gemm_dma<C>(wrs, xrs, smem, lane_off, Kb, wave, 0);
+  // Stage ks of tile (tm, tn), whose operands' buffers wrs and xrs are, into stage buffer `buf`.
+  auto copy = [&](int buf, int ks) {
+    gemm_dma<C>(wrs, xrs, smem + buf * C::STAGE, lane_off, Kb, wave, ks * GEMM_BK);
+    mx_copy_scales<C>(sw + ((int64_t)ks * N + tn_c * C::BN) * MX_SLAB, sa + ((int64_t)ks * M + tm_c * C::BM) * MX_SLAB,
+                      min(N - tn_c * C::BN, C::BN), min(M - tm_c * C::BM, C::BM), sc_smem + buf * SCALES, wave, lane);
+  };
+  copy(0, 0);
+  // an epilogue round is 32 tokens of a wave's 32 TN channels, 64 x 16 bytes per store
+  constexpr int RB = TN * 64, NCH = RB / 16, RPI = 64 / NCH, STORES = TM * (32 / RPI);
+  bool stores_behind = false;
   int gs = 0;  // global stage counter: stage buffer parity runs on across tiles
 
   for (; s < ntiles; s += gridDim.x) {
     const int m0 = tm * C::BM, n0 = tn * C::BN;
-    // this tile's bias, handed over through LDS after the mainloop
-    const float ep_v = bias && (int)threadIdx.x < C::BN && n0 + (int)threadIdx.x < N
-                           ? bf16_bits_to_f32(bias[n0 + threadIdx.x]) : 0.0f;
+    // this tile's bias, handed over through LDS after the mainloop (an unconditional load from a valid address, which
+    // nothing waits for here)
+    const uint16_t ep_v = *(bias ? bias + min(n0 + (int)(threadIdx.x % C::BN), N - 1) : reinterpret_cast<const uint16_t*>(sw));
     const int s_next = s + gridDim.x;
     int tm_n = 0, tn_n = 0;
     if (s_next < ntiles) tile_coords(s_next, tiles_m, tiles_n, group_m, tm_n, tn_n);
-
-    // rows past the end read the last row's scales (their products are not stored)
-    uint32_t ow[TN], ox[TM];
-#pragma unroll
-    for (int a = 0; a < TN; ++a) ow[a] = min(wrow0 + 32 * a + r, N - 1 - n0) * MX_SLAB + 4 * g;
-#pragma unroll
-    for (int b = 0; b < TM; ++b) ox[b] = min(xrow0 + 32 * b + r, M - 1 - m0) * MX_SLAB + 4 * g;
-    auto load_scales = [&](int ks, MxScales<C>& sc) {
-      // (buffer loads: a uniform base and a 32-bit offset, where plain loads would hold six 64-bit addresses)
-      const __amdgpu_buffer_rsrc_t pw = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)(sw + ((int64_t)ks * N + n0) * MX_SLAB), 0, C::BN * MX_SLAB, 0x00020000);
-      const __amdgpu_buffer_rsrc_t px = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)(sa + ((int64_t)ks * M + m0) * MX_SLAB), 0, C::BM * MX_SLAB, 0x00020000);
-#pragma unroll
-      for (int a = 0; a < TN; ++a) sc.w[a] = __builtin_amdgcn_raw_buffer_load_b32(pw, ow[a], 0, 0);
-#pragma unroll
-      for (int b = 0; b < TM; ++b) sc.x[b] = __builtin_amdgcn_raw_buffer_load_b32(px, ox[b], 0, 0);
-    };
-    // Blocks past K in the last stage have zeros for codes; their scale bytes, which may hold anything,
-    // become 1 (127), as a NaN there would meet the zeros.
-    auto mend_scales = [&](MxScales<C>& sc) {
-      const int valid = min(max(((Kb % GEMM_BK) >> 4) - 4 * g, 0), 4);
-      const uint32_t keep = valid == 4 ? 0xffffffffu : (1u << (8 * valid)) - 1u;
-#pragma unroll
-      for (int a = 0; a < TN; ++a) sc.w[a] = (sc.w[a] & keep) | (0x7f7f7f7fu & ~keep);
-#pragma unroll
-      for (int b = 0; b < TM; ++b) sc.x[b] = (sc.x[b] & keep) | (0x7f7f7f7fu & ~keep);
-    };
 
     v16f acc[TN][TM];
 #pragma unroll
@@ -108,42 +91,59 @@ __global__ __launch_bounds__(C::THREADS) void gemm_mxfp4_kernel(const uint8_t* _
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.0f;
 
-    auto after_last = [&](uint8_t* dst) {
+    // the next tile's first stage
+    auto after_last = [&](int buf) {
       if (s_next < ntiles) {
+        tm_c = tm_n;
+        tn_c = tn_n;
         wrs = rsrc(w4, tn_n * C::BN, N, C::BN);
         xrs = rsrc(a4, tm_n * C::BM, M, C::BM);
-        gemm_dma<C>(wrs, xrs, dst, lane_off, Kb, wave, 0);
+        copy(buf, 0);
       }
     };
-    // Stage 0 of this tile is in flight into buffer gs & 1.
-    MxScales<C> cur_s, nxt_s;
-    load_scales(0, cur_s);
-    wait_vm0();
-    block_barrier();
-    if (KTAIL && nk == 1) {
-      zero_tail<C>(smem + (gs & 1) * C::STAGE, (Kb % GEMM_BK) >> 4);
-      mend_scales(cur_s);
+    // Blocks past K in the last stage: zero codes, and scales of 1 (127) in the place of bytes that may hold anything
+    // (a NaN would meet the zeros).
+    auto mend = [&](int buf) {
+      const int valid = (Kb % GEMM_BK) >> 4;
+      zero_tail<C>(smem + buf * C::STAGE, valid);
+      for (int i = threadIdx.x; i < SCALES; i += C::THREADS)
+        if (i % MX_SLAB >= valid) sc_smem[buf * SCALES + i] = 127;
       block_barrier();
-    }
-    if (nk > 1) {
-      load_scales(1, nxt_s);
-      gemm_dma<C>(wrs, xrs, smem + ((gs + 1) & 1) * C::STAGE, lane_off, Kb, wave, GEMM_BK);
-    } else {
-      nxt_s = cur_s;
-      after_last(smem + ((gs + 1) & 1) * C::STAGE);
-    }
+    };
+    // Stage 0 of this tile is in flight into buffer gs & 1; of what was issued after it, the last tile's output stores
+    // (STORES a wave, of a tile inside the matrix) and the bias, nothing is waited for.
+    if (stores_behind)
+      wait_vm<STORES + 1>();
+    else
+      wait_vm0();
+    block_barrier();
+    if (KTAIL && nk == 1) mend(gs & 1);
+    if (nk > 1)
+      copy((gs + 1) & 1, 1);
+    else
+      after_last((gs + 1) & 1);
     // A stage is four steps, one block of each lane's four per step.  A step's fragments are read while the
     // step before it runs: W's into the registers of the fragment whose products have just been issued, X's
     // into the other of two sets.  Step 3's are the stage's last reads, so the barrier stands before it.
     v4i af[TN], bf[2][TM];
+    MxScales<C> sc, sc_next;
+    auto read_scales = [&](int buf, MxScales<C>& to) {
+      const uint8_t* p = sc_smem + buf * SCALES + 4 * g;
+#pragma unroll
+      for (int a = 0; a < TN; ++a) to.w[a] = *reinterpret_cast<const uint32_t*>(p + (wrow0 + 32 * a + r) * MX_SLAB);
+#pragma unroll
+      for (int b = 0; b < TM; ++b)
+        to.x[b] = *reinterpret_cast<const uint32_t*>(p + (C::BN + xrow0 + 32 * b + r) * MX_SLAB);
+    };
     {
       const uint8_t* cur = smem + (gs & 1) * C::STAGE;
 #pragma unroll
       for (int a = 0; a < TN; ++a) af[a] = mx_frag(cur, wrow0 + 32 * a + r, 4 * g);
 #pragma unroll
       for (int b = 0; b < TM; ++b) bf[0][b] = mx_frag(cur + C::BN * GEMM_BK, xrow0 + 32 * b + r, 4 * g);
+      read_scales(gs & 1, sc);
     }
-    auto step = [&](auto t_tag, const uint8_t* from, int chunk, const MxScales<C>& sc) {
+    auto step = [&](auto t_tag, const uint8_t* from, int chunk) {
       constexpr int T = decltype(t_tag)::value;
 #pragma unroll
       for (int b = 0; b < TM; ++b) bf[(T + 1) & 1][b] = mx_frag(from + C::BN * GEMM_BK, xrow0 + 32 * b + r, chunk);
@@ -157,43 +157,36 @@ __global__ __launch_bounds__(C::THREADS) void gemm_mxfp4_kernel(const uint8_t* _
     };
     int ks = 0;
     do {
-      uint8_t* cur = smem + (gs & 1) * C::STAGE;
-      uint8_t* nxt = smem + ((gs + 1) & 1) * C::STAGE;
-      step(std::integral_constant<int, 0>{}, cur, 4 * g + 1, cur_s);
-      step(std::integral_constant<int, 1>{}, cur, 4 * g + 2, cur_s);
-      step(std::integral_constant<int, 2>{}, cur, 4 * g + 3, cur_s);
+      const int cb = gs & 1, nb = cb ^ 1;
+      uint8_t* cur = smem + cb * C::STAGE;
+      uint8_t* nxt = smem + nb * C::STAGE;
+      step(std::integral_constant<int, 0>{}, cur, 4 * g + 1);
+      step(std::integral_constant<int, 1>{}, cur, 4 * g + 2);
+      step(std::integral_constant<int, 2>{}, cur, 4 * g + 3);
       // (products have no side effect, and the compiler would move those above past the barrier to their next use)
 #pragma unroll
       for (int a = 0; a < TN; ++a)
 #pragma unroll
         for (int b = 0; b < TM; ++b) asm volatile("" : "+v"(acc[a][b]));
-      // (step 3's scales move out of the way here, where the next stage's have landed: moving those while the
-      // ones after them are in flight would wait for these)
-      const MxScales<C> step3_s = cur_s;
       if (ks + 1 < nk) {
         wait_vm0();
         block_barrier();
-        if (KTAIL && ks + 2 == nk) {
-          zero_tail<C>(nxt, (Kb % GEMM_BK) >> 4);
-          mend_scales(nxt_s);
-          block_barrier();
-        }
-        cur_s.take(nxt_s);
-        if (ks + 2 < nk) {
-          load_scales(ks + 2, nxt_s);
-          gemm_dma<C>(wrs, xrs, cur, lane_off, Kb, wave, (ks + 2) * GEMM_BK);
-        } else {
-          after_last(cur);
-        }
+        if (KTAIL && ks + 2 == nk) mend(nb);
+        if (ks + 2 < nk)
+          copy(cb, ks + 2);
+        else
+          after_last(cb);
       }
       // (after the last stage the reads fetch nothing that is used)
-      step(std::integral_constant<int, 3>{}, nxt, 4 * g, step3_s);
+      read_scales(nb, sc_next);
+      step(std::integral_constant<int, 3>{}, nxt, 4 * g);
+      sc.take(sc_next);
       ++gs;
     } while (++ks < nk);
 
     // ---- epilogue: acc[a][b] register i is channel n0 + wrow0 + 32 a + 8 (i / 4) + 4 g + i % 4 of token
     // m0 + xrow0 + 32 b + r
-    if ((int)threadIdx.x < C::BN) ep_b[threadIdx.x] = ep_v;
+    if ((int)threadIdx.x < C::BN) ep_b[threadIdx.x] = bias ? bf16_bits_to_f32(ep_v) : 0.0f;
     block_barrier();
     // (the lane index is made opaque here, or the epilogue's addresses, the same for every tile, would be held in
     // registers across the mainloop, where there are none left for them)
@@ -203,7 +196,6 @@ __global__ __launch_bounds__(C::THREADS) void gemm_mxfp4_kernel(const uint8_t* _
     auto quad = [&](const v16f& c, int q) { return v4f{c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]}; };
     // Each 32-token round of a wave goes through its own 1 / NW of the last stage's buffer and leaves as 16-byte stores
     // of whole row segments, at any alignment; what a tile at the matrix's edge cuts is stored one by one.
-    constexpr int RB = TN * 64, NCH = RB / 16, RPI = 64 / NCH;
     static_assert(32 * RB <= C::STAGE / C::NW, "per-wave staging region");
     uint8_t* const wreg = smem + ((gs + 1) & 1) * C::STAGE + wave * (C::STAGE / C::NW);
     const bool inside = m0 + C::BM <= M && n0 + C::BN <= N;
@@ -228,6 +220,7 @@ __global__ __launch_bounds__(C::THREADS) void gemm_mxfp4_kernel(const uint8_t* _
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
+    stores_behind = inside;
     tm = tm_n;
     tn = tn_n;
   }
@@ -237,7 +230,7 @@ template <class C, int ACT, bool KTAIL>
 static void launch_mxfp4(const uint8_t* a4, const uint8_t* w4, const uint8_t* sa, const uint8_t* sw, const uint16_t* bias,
                          uint16_t* out, int M, int N, int Kb, int64_t ld_out, int cus, hipStream_t st) {
   const int tiles_m = (int)cdiv(M, C::BM), tiles_n = (int)cdiv(N, C::BN), ntiles = tiles_m * tiles_n;
-  constexpr int per_cu = (160 * 1024) / (2 * C::STAGE + C::BN * 4);
+  constexpr int per_cu = (160 * 1024) / (2 * C::STAGE + 2 * (C::BM + C::BN) * MX_SLAB + C::BN * 4);
   int grid = cus * per_cu;
   grid = grid >= 8 ? grid & ~7 : ntiles;
   if (grid > ntiles) grid = ntiles;
@@ -267,19 +260,47 @@ static void launch_mxfp4_ring(int act, const uint8_t* a4, const uint8_t* w4, con
 #undef MXF8_CASE
 }
 
-template <int TM, int NW>
-static void launch_mxfp4_rows(int act, const uint8_t* a4, const uint8_t* w4, const uint8_t* sa, const uint8_t* sw,
+template <int TM, int NW, int XT>
+static void launch_mxfp4_rows(int act, const void* x, int64_t ldx, const uint8_t* sa, const uint8_t* w4, const uint8_t* sw,
                               const uint16_t* bias, uint16_t* out, int M, int N, int Kb, int64_t ld_out, hipStream_t st) {
   const dim3 grid((unsigned)cdiv(N, 16), (unsigned)cdiv(M, 16 * TM));
   const bool ktail = Kb % GEMM_BK != 0;
-#define MXF8_CASE(A, T)                                                                                                 \
-  if (act == A && ktail == T)                                                                                           \
-    gemm_mxfp4_rows_kernel<TM, NW, A, T><<<grid, 64 * NW, 0, st>>>(a4, w4, sa, sw, bias, out, M, N, Kb, ld_out);
+#define MXF8_CASE(A, T)                                                                                             \
+  if (act == A && ktail == T)                                                                                       \
+    gemm_mxfp4_rows_kernel<TM, NW, A, T, XT><<<grid, 64 * NW, 0, st>>>(x, ldx, sa, w4, sw, bias, out, M, N, Kb, ld_out);
   MXF8_CASE(MXF8_ACT_NONE, false)
   MXF8_CASE(MXF8_ACT_NONE, true)
   MXF8_CASE(MXF8_ACT_GELU_TANH, false)
   MXF8_CASE(MXF8_ACT_GELU_TANH, true)
 #undef MXF8_CASE
+}
+
+// The rows kernel that mxfp4_pick chose.
+template <int XT>
+static void launch_mxfp4_few(int pick, int act, const void* x, int64_t ldx, const uint8_t* sa, const uint8_t* w4,
+                             const uint8_t* sw, const uint16_t* bias, uint16_t* out, int M, int N, int Kb, int64_t ld_out,
+                             hipStream_t st) {
+  switch (pick) {
+    case MX_ROWS16_4: launch_mxfp4_rows<1, 4, XT>(act, x, ldx, sa, w4, sw, bias, out, M, N, Kb, ld_out, st); break;
+    case MX_ROWS16_8: launch_mxfp4_rows<1, 8, XT>(act, x, ldx, sa, w4, sw, bias, out, M, N, Kb, ld_out, st); break;
+    case MX_ROWS16_16: launch_mxfp4_rows<1, 16, XT>(act, x, ldx, sa, w4, sw, bias, out, M, N, Kb, ld_out, st); break;
+    default:
+      if constexpr (XT == MX_CODES) launch_mxfp4_rows<2, 4, XT>(act, x, ldx, sa, w4, sw, bias, out, M, N, Kb, ld_out, st);
+  }
+}
+
+// Checks of the product that its two entries share.
+static int mxfp4_check(const char* what, const uint8_t* w4, const uint8_t* sw, int act, const void* out, int64_t M, int64_t N,
+                       int64_t K, int64_t ld_out) {
+  if (K <= 0 || K % MX_BLOCK) return set_error(MXF8_EINVAL, "%s: K=%lld must be a positive multiple of 32", what, (long long)K);
+  if (!w4 || !sw || !out) return set_error(MXF8_EINVAL, "%s: null pointer", what);
+  if (ld_out < N) return set_error(MXF8_EINVAL, "%s: ld_out < N", what);
+  if (act != MXF8_ACT_NONE && act != MXF8_ACT_GELU_TANH) return set_error(MXF8_EINVAL, "%s: bad act", what);
+  if (M > (1 << 27) || N > (1 << 27) || K > (1 << 22) || cdiv(M, 32) * cdiv(N, 64) > 0x7fffffff)
+    return set_error(MXF8_EINVAL, "%s: shape too large", what);
+  if (((uintptr_t)w4 % 16) || ((uintptr_t)sw % 8))
+    return set_error(MXF8_EINVAL, "%s: codes must be 16-byte and scales 8-byte aligned", what);
+  return MXF8_OK;
 }
 
 }  // namespace mxf8
@@ -291,50 +312,84 @@ extern "C" int mxf8_gemm_mxfp4(const uint8_t* a4, const uint8_t* w4, const uint8
   const char* what = "gemm_mxfp4";
   if (M < 0 || N < 0 || K < 0) return set_error(MXF8_EINVAL, "%s: negative shape", what);
   if (M == 0 || N == 0) return MXF8_OK;
-  if (K == 0 || K % MX_BLOCK) return set_error(MXF8_EINVAL, "%s: K=%lld must be a positive multiple of 32", what, (long long)K);
-  if (!a4 || !w4 || !sa || !sw || !out) return set_error(MXF8_EINVAL, "%s: null pointer", what);
-  if (ld_out < N) return set_error(MXF8_EINVAL, "%s: ld_out < N", what);
-  if (act != MXF8_ACT_NONE && act != MXF8_ACT_GELU_TANH) return set_error(MXF8_EINVAL, "%s: bad act", what);
-  if (M > (1 << 27) || N > (1 << 27) || K > (1 << 22)) return set_error(MXF8_EINVAL, "%s: shape too large", what);
-  if (((uintptr_t)a4 % 16) || ((uintptr_t)w4 % 16) || ((uintptr_t)sa % 8) || ((uintptr_t)sw % 8))
+  if (const int rc = mxfp4_check(what, w4, sw, act, out, M, N, K, ld_out)) return rc;
+  if (!a4 || !sa) return set_error(MXF8_EINVAL, "%s: null pointer", what);
+  if (((uintptr_t)a4 % 16) || ((uintptr_t)sa % 8))
     return set_error(MXF8_EINVAL, "%s: codes must be 16-byte and scales 8-byte aligned", what);
   const int cus = device_cus();
   if (cus <= 0) return set_error(MXF8_ELAUNCH, "%s: the device's compute-unit count is unavailable", what);
   const int iM = (int)M, iN = (int)N, Kb = (int)(K / 2);
-  if (cdiv(M, 128) * cdiv(N, 128) > 0x7fffffff) return set_error(MXF8_EINVAL, "%s: shape too large", what);
   const uint16_t* b16 = static_cast<const uint16_t*>(bias);
   uint16_t* o16 = static_cast<uint16_t*>(out);
-#define MXF8_MX_SMALL(launch)                                                        \
-  launch(act, a4, w4, sa, sw, b16, o16, iM, iN, Kb, ld_out, stream);                 \
-  return check_launch(what);
   const bool ktail = Kb % GEMM_BK != 0;
   const int pick = mxfp4_pick(M, N, K, cus);
+#define MXF8_MX_RING(Cfg)                                                                             \
+  launch_mxfp4_ring<Cfg>(act, a4, w4, sa, sw, b16, o16, iM, iN, Kb, ld_out, stream);                  \
+  break;
+#define MXF8_MX_CASE(Cfg, A, T) \
+  if (act == A && ktail == T) launch_mxfp4<Cfg, A, T>(a4, w4, sa, sw, b16, o16, iM, iN, Kb, ld_out, cus, stream);
+#define MXF8_MX_TILE(Cfg)                                                                             \
+  MXF8_MX_CASE(Cfg, MXF8_ACT_NONE, false)                                                             \
+  MXF8_MX_CASE(Cfg, MXF8_ACT_NONE, true)                                                              \
+  MXF8_MX_CASE(Cfg, MXF8_ACT_GELU_TANH, false)                                                        \
+  MXF8_MX_CASE(Cfg, MXF8_ACT_GELU_TANH, true)                                                         \
+  break;
   switch (pick) {
-    case MX_ROWS16_4: MXF8_MX_SMALL((launch_mxfp4_rows<1, 4>))
-    case MX_ROWS16_8: MXF8_MX_SMALL((launch_mxfp4_rows<1, 8>))
-    case MX_ROWS16_16: MXF8_MX_SMALL((launch_mxfp4_rows<1, 16>))
-    case MX_ROWS32: MXF8_MX_SMALL((launch_mxfp4_rows<2, 4>))
-    case MX_RING_32x64: MXF8_MX_SMALL(launch_mxfp4_ring<MxRing32x64>)
-    case MX_RING_64x64: MXF8_MX_SMALL(launch_mxfp4_ring<MxRing64x64>)
-    case MX_RING_128x64: MXF8_MX_SMALL(launch_mxfp4_ring<MxRing128x64>)
-    case MX_RING_128x128: MXF8_MX_SMALL(launch_mxfp4_ring<MxRing128x128>)
-    default: break;
+    case MX_RING_32x64: MXF8_MX_RING(MxRing32x64)
+    case MX_RING_64x64: MXF8_MX_RING(MxRing64x64)
+    case MX_RING_128x64: MXF8_MX_RING(MxRing128x64)
+    case MX_RING_128x128: MXF8_MX_RING(MxRing128x128)
+    case MX_TILE_128: MXF8_MX_TILE(GemmSmall)
+    case MX_TILE_256: MXF8_MX_TILE(GemmBig)
+    default: launch_mxfp4_few<MX_CODES>(pick, act, a4, 0, sa, w4, sw, b16, o16, iM, iN, Kb, ld_out, stream);
   }
-#undef MXF8_MX_SMALL
-#define MXF8_MX_CASE(Cfg, A, T)                                                                       \
-  if (act == A && ktail == T) {                                                                       \
-    launch_mxfp4<Cfg, A, T>(a4, w4, sa, sw, b16, o16, iM, iN, Kb, ld_out, cus, stream);               \
-    return check_launch(what);                                                                        \
-  }
-#define MXF8_MX_CASES(Cfg)                                                                                   \
-  MXF8_MX_CASE(Cfg, MXF8_ACT_NONE, false) MXF8_MX_CASE(Cfg, MXF8_ACT_NONE, true)                             \
-  MXF8_MX_CASE(Cfg, MXF8_ACT_GELU_TANH, false) MXF8_MX_CASE(Cfg, MXF8_ACT_GELU_TANH, true)
-  if (pick == MX_TILE_256) {
-    MXF8_MX_CASES(GemmBig)
-  } else {
-    MXF8_MX_CASES(GemmSmall)
-  }
-#undef MXF8_MX_CASES
+#undef MXF8_MX_TILE
 #undef MXF8_MX_CASE
-  return set_error(MXF8_EINVAL, "%s: no kernel", what);
+#undef MXF8_MX_RING
+  return check_launch(what);
+}
+
+// Whether the product quantizes its activations itself: the rows kernel's tokens, in 16 bits, and a weight small
+// enough that the same quantization in every 16 channels' workgroup costs less than a launch.  MI355X, in one
+// launch / two: 1 x 3072 x 3072 4.4 / 5.3 us, 16 x 3072 x 3072 6.3 / 6.6; past the limit 1 x 9216 x 3072 9.3 / 8.2,
+// 1 x 3072 x 12288 11.0 / 9.6.
+static bool mxfp4_one_launch(int64_t M, int64_t N, int64_t K, int dtype) {
+  return M <= 16 && dtype != MXF8_F32 && N * K <= (1 << 24);
+}
+
+extern "C" int64_t mxf8_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
+  if (M <= 0 || N <= 0 || K <= 0 || N > (1 << 27) || K > (1 << 22) || mxfp4_one_launch(M, N, K, dtype)) return 0;
+  return M * (K / 2) + mx_slabs(K) * M * MX_SLAB;  // codes, then scales (K / 2 is a multiple of 16)
+}
+
+extern "C" int mxf8_mxfp4_linear(const void* x, int dtype, int64_t ldx, const uint8_t* w4, const uint8_t* sw, const void* bias,
+                                 int act, void* out, int64_t M, int64_t N, int64_t K, int64_t ld_out, void* workspace,
+                                 hipStream_t stream) {
+  const char* what = "mxfp4_linear";
+  if (M < 0 || N < 0 || K < 0) return set_error(MXF8_EINVAL, "%s: negative shape", what);
+  if (M == 0 || N == 0) return MXF8_OK;
+  if (const int rc = mxfp4_check(what, w4, sw, act, out, M, N, K, ld_out)) return rc;
+  if (!x) return set_error(MXF8_EINVAL, "%s: null pointer", what);
+  if (ldx < K && M > 1) return set_error(MXF8_EINVAL, "%s: ldx < K", what);
+  if (dtype != MXF8_BF16 && dtype != MXF8_F16 && dtype != MXF8_F32)
+    return set_error(MXF8_EINVAL, "%s: bad dtype %d", what, dtype);
+  if (!mxfp4_one_launch(M, N, K, dtype)) {
+    if (!workspace || (uintptr_t)workspace % 16) return set_error(MXF8_EINVAL, "%s: a 16-byte aligned workspace is needed", what);
+    uint8_t* codes = static_cast<uint8_t*>(workspace);
+    uint8_t* scales = codes + M * (K / 2);
+    if (const int rc = mxf8_mxfp4_quant(x, dtype, M, K, ldx, codes, scales, stream)) return rc;
+    return mxf8_gemm_mxfp4(codes, w4, scales, sw, bias, act, out, M, N, K, ld_out, stream);
+  }
+  const int cus = device_cus();
+  if (cus <= 0) return set_error(MXF8_ELAUNCH, "%s: the device's compute-unit count is unavailable", what);
+  const int pick = mxfp4_pick(M, N, K, cus);  // (up to 16 tokens: a rows kernel)
+  const uint16_t* b16 = static_cast<const uint16_t*>(bias);
+  uint16_t* o16 = static_cast<uint16_t*>(out);
+#define MXF8_CASE(DT)                                                                                                 \
+  if (dtype == DT)                                                                                                    \
+    launch_mxfp4_few<DT>(pick, act, x, ldx, nullptr, w4, sw, b16, o16, (int)M, (int)N, (int)(K / 2), ld_out, stream);
+  MXF8_CASE(MXF8_BF16)
+  MXF8_CASE(MXF8_F16)
+#undef MXF8_CASE
+  return check_launch(what);
 }

@@ -28,13 +28,20 @@ __device__ __forceinline__ v4i mx_frag(const uint8_t* tile, int row, int chunk) 
   return *reinterpret_cast<const v4i*>(tile + row * GEMM_BK + ((chunk ^ lds_swz<GEMM_BK>(row)) << 4));
 }
 
+// GELU-tanh, z sigmoid(2 u) with u = sqrt(2 / pi) (z + 0.044715 z^3), as z / (1 + 2^t): t = -2 u log2(e), whose two
+// coefficients hold all constants (at 12288 channels the activation is an eighth of the kernel's cycles).
+__device__ __forceinline__ float mx_gelu(float z) {
+  const float t = z * __builtin_fmaf(-0.10294324f, z * z, -2.3022082f);
+  return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t));
+}
+
 template <int ACT>
 __device__ __forceinline__ uint2 mx_out_quad(const v4f& x, const v4f& b) {
   float v[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     v[e] = x[e] + b[e];
-    if constexpr (ACT == MXF8_ACT_GELU_TANH) v[e] = gelu_tanh_f32(v[e]);
+    if constexpr (ACT == MXF8_ACT_GELU_TANH) v[e] = mx_gelu(v[e]);
   }
   return make_uint2(bf16x2(v[0], v[1]), bf16x2(v[2], v[3]));
 }
@@ -58,6 +65,27 @@ __device__ __forceinline__ void mx_store8(uint16_t* dst, const uint4& v, int n) 
   }
 }
 
+// A wave's share of the copies of a stage's scales, BN rows of W, then BM rows of X, from the tile's first rows of the
+// slab: 256-byte instructions of 32 rows, two dwords a row.  Rows past the operand's end (wrows, xrows of them are
+// there) read as zeros (2^-127, with zero codes).  Every wave issues as many instructions (some copy rows again), so
+// that one count of instructions in flight holds for all.
+template <class C>
+__device__ __forceinline__ void mx_copy_scales(const uint8_t* w, const uint8_t* x, int wrows, int xrows, uint8_t* dst,
+                                               int wave, int lane) {
+  constexpr int ALL = (C::BM + C::BN) / 32;
+#pragma unroll
+  for (int j = 0; j < (ALL + C::NW - 1) / C::NW; ++j) {
+    // (whole rounds of the waves over each operand: known here which)
+    constexpr bool whole = C::BN / 32 % C::NW == 0 && ALL % C::NW == 0;
+    const int J = whole ? wave + j * C::NW : (wave + j * C::NW) % ALL;
+    const bool is_w = whole ? j * C::NW < C::BN / 32 : J < C::BN / 32;
+    const __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc((void*)(is_w ? w : x), 0, (is_w ? wrows : xrows) * MX_SLAB, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, LDS_PTR(dst + J * 256), 4, lane * 4,
+                                             (is_w ? 32 * J : 32 * J - C::BN) * MX_SLAB, 0, 0);
+  }
+}
+
 template <int BM_, int BN_, int WM_, int WN_, int NS_>
 struct MxRing {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NS = NS_;
@@ -66,9 +94,7 @@ struct MxRing {
   static constexpr int CODES = (BM + BN) * GEMM_BK;          // LDS bytes of a stage: W rows, then X rows,
   static constexpr int STAGE = CODES + (BM + BN) * MX_SLAB;  // and their scales in the same order
   static constexpr int DMA_CODES = (BM + BN) / 8 / NW;       // 1 KB instructions per wave and stage
-  // 256-byte instructions for the scales of 32 rows each; every wave issues as many (some copy rows again),
-  // so that one count of instructions in flight holds for all
-  static constexpr int DMA_SCALES = ((BM + BN) / 32 + NW - 1) / NW;
+  static constexpr int DMA_SCALES = ((BM + BN) / 32 + NW - 1) / NW;      // and of mx_copy_scales
   static constexpr int PER_STAGE = DMA_CODES + DMA_SCALES;
   static constexpr int OUT_PITCH = BN * 2 + 16;
   static_assert((BM + BN) / 8 % NW == 0 && BN % 32 == 0 && BM % 32 == 0, "DMA shares");
@@ -86,20 +112,6 @@ struct MxRing {
       const __amdgpu_buffer_rsrc_t rs = is_w ? wrs : xrs;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, LDS_PTR(stage + J * 1024), 16, lane_off[J & 1],
                                                (is_w ? 8 * J : 8 * J - BN) * Kb + k0, 0, 0);
-    }
-  }
-  // Its share of the scales: two dwords per row, from the tile's first rows of the slab; rows past the operand's end
-  // read as zeros (2^-127, with zero codes).
-  static __device__ __forceinline__ void copy_scales(const uint8_t* w, const uint8_t* x, int wrows, int xrows,
-                                                     uint8_t* dst, int wave, int lane) {
-#pragma unroll
-    for (int j = 0; j < DMA_SCALES; ++j) {
-      const int J = (wave + j * NW) % ((BM + BN) / 32);
-      const bool is_w = J < BN / 32;
-      const __amdgpu_buffer_rsrc_t rs =
-          __builtin_amdgcn_make_buffer_rsrc((void*)(is_w ? w : x), 0, (is_w ? wrows : xrows) * MX_SLAB, 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, LDS_PTR(dst + J * 256), 4, lane * 4,
-                                               (is_w ? 32 * J : 32 * J - BN) * MX_SLAB, 0, 0);
     }
   }
 };
@@ -134,7 +146,7 @@ __global__ __launch_bounds__(C::THREADS) void gemm_mxfp4_ring_kernel(const uint8
   const __amdgpu_buffer_rsrc_t wrs = rsrc(w4, n0, N, C::BN), xrs = rsrc(a4, m0, M, C::BM);
   auto dma = [&](uint8_t* stage, int ks) {
     C::copy_codes(wrs, xrs, stage, lane_off, Kb, wave, ks * GEMM_BK);
-    C::copy_scales(sw + ((int64_t)ks * N + n0) * MX_SLAB, sa + ((int64_t)ks * M + m0) * MX_SLAB, min(N - n0, C::BN),
+    mx_copy_scales<C>(sw + ((int64_t)ks * N + n0) * MX_SLAB, sa + ((int64_t)ks * M + m0) * MX_SLAB, min(N - n0, C::BN),
                    min(M - m0, C::BM), stage + C::CODES, wave, lane);
   };
   // the bias, read before the copies that the waits below count, handed over through LDS
@@ -254,20 +266,25 @@ __global__ __launch_bounds__(C::THREADS) void gemm_mxfp4_ring_kernel(const uint8
 
 // 16 channels x 16 TM tokens per workgroup of NW waves.  A unit is one slab of K (256 elements, 128 bytes of a
 // row): lane group g = lane / 16 of the 16 x 16 x 128 instruction takes blocks 2 g and 2 g + 1 of its row, one
-// per instruction, 32 bytes and two scale bytes.  Wave w takes units w, w + NW, ..., two at a time in flight
-// beside the two that are being multiplied.
+// per instruction, 32 bytes and two scale bytes.  Wave w takes units w, w + NW, ..., up to four in flight.
 template <int T>
 __device__ __forceinline__ v4f mx_mma16(const v4i& a, const v4i& b, const v4f& c, uint32_t sa, uint32_t sb) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_wide(a), mx_wide(b), c, 4, 4, T, (int)sa, T, (int)sb);
 }
 
-template <int TM, int NW, int ACT, bool KTAIL>
-__global__ __launch_bounds__(64 * NW) void gemm_mxfp4_rows_kernel(const uint8_t* __restrict__ a4, const uint8_t* __restrict__ w4,
+// XT: the activations are codes and scales (MX_CODES), or 16-bit elements of that type, row stride ldx, which each
+// lane quantizes for itself (mx_quant_block), where that costs less than a launch of its own.
+constexpr int MX_CODES = -1;
+
+template <int TM, int NW, int ACT, bool KTAIL, int XT>
+__global__ __launch_bounds__(64 * NW) void gemm_mxfp4_rows_kernel(const void* __restrict__ x, int64_t ldx,
                                                                   const uint8_t* __restrict__ sa,
+                                                                  const uint8_t* __restrict__ w4,
                                                                   const uint8_t* __restrict__ sw,
                                                                   const uint16_t* __restrict__ bias,
                                                                   uint16_t* __restrict__ out, int M, int N, int Kb,
                                                                   int64_t ld_out) {
+  typedef uint16_t T;
   __shared__ __attribute__((aligned(16))) v4f part[NW][TM][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int r = lane & 15, g = lane >> 4;
@@ -278,45 +295,58 @@ __global__ __launch_bounds__(64 * NW) void gemm_mxfp4_rows_kernel(const uint8_t*
   const uint8_t* const wp = w4 + (int64_t)wrow * Kb + 32 * g;
   const uint8_t* const swp = sw + (int64_t)wrow * MX_SLAB + 2 * g;
   const uint8_t *xp[TM], *sxp[TM];
+  const T* xe[TM];
 #pragma unroll
   for (int b = 0; b < TM; ++b) {
     const int xrow = min(m0 + 16 * b + r, M - 1);
-    xp[b] = a4 + (int64_t)xrow * Kb + 32 * g;
-    sxp[b] = sa + (int64_t)xrow * MX_SLAB + 2 * g;
+    if constexpr (XT == MX_CODES) {
+      xp[b] = static_cast<const uint8_t*>(x) + (int64_t)xrow * Kb + 32 * g;
+      sxp[b] = sa + (int64_t)xrow * MX_SLAB + 2 * g;
+    } else {
+      xe[b] = static_cast<const T*>(x) + xrow * ldx + 64 * g;
+    }
   }
   struct Unit {
     v4i w[2], x[TM][2];
     uint32_t sw, sx[TM];
   };
-  auto load = [&](int ks, Unit& u) {
-    const int64_t off = (int64_t)ks * GEMM_BK;
-    const int64_t ws = (int64_t)ks * N * MX_SLAB, xs = (int64_t)ks * M * MX_SLAB;
-    // blocks 2 g and 2 g + 1 of the slab; those past K are zero codes under a scale of 1
-    const int valid = KTAIL ? (Kb >> 4) - 8 * ks - 2 * g : 2;
-    if (valid >= 2) {
-      u.w[0] = *reinterpret_cast<const v4i*>(wp + off);
-      u.w[1] = *reinterpret_cast<const v4i*>(wp + off + 16);
-      u.sw = *reinterpret_cast<const uint16_t*>(swp + ws);
-#pragma unroll
-      for (int b = 0; b < TM; ++b) {
-        u.x[b][0] = *reinterpret_cast<const v4i*>(xp[b] + off);
-        u.x[b][1] = *reinterpret_cast<const v4i*>(xp[b] + off + 16);
-        u.sx[b] = *reinterpret_cast<const uint16_t*>(sxp[b] + xs);
-      }
+  // blocks 2 g and 2 g + 1 of the slab; those past K are zero codes under a scale of 1
+  auto there = [&](int ks) { return KTAIL ? (Kb >> 4) - 8 * ks - 2 * g : 2; };
+  const v4i none = {0, 0, 0, 0};
+  auto load_w = [&](int ks, Unit& u) {
+    const uint8_t *p = wp + (int64_t)ks * GEMM_BK, *s = swp + (int64_t)ks * N * MX_SLAB;
+    const int n = there(ks);
+    if (n >= 2) {
+      u.w[0] = *reinterpret_cast<const v4i*>(p);
+      u.w[1] = *reinterpret_cast<const v4i*>(p + 16);
+      u.sw = *reinterpret_cast<const uint16_t*>(s);
     } else {
-      const v4i zero = {0, 0, 0, 0};
-      u.w[0] = u.w[1] = zero;
-      u.sw = 0x7f7fu;
+      u.w[0] = n == 1 ? *reinterpret_cast<const v4i*>(p) : none;
+      u.w[1] = none;
+      u.sw = 0x7f00u | (n == 1 ? s[0] : 127u);
+    }
+  };
+  auto load_x = [&](int ks, Unit& u) {
+    const int n = there(ks);
 #pragma unroll
-      for (int b = 0; b < TM; ++b) u.x[b][0] = u.x[b][1] = zero, u.sx[b] = 0x7f7fu;
-      if (valid == 1) {
-        u.w[0] = *reinterpret_cast<const v4i*>(wp + off);
-        u.sw = 0x7f00u | swp[ws];
-#pragma unroll
-        for (int b = 0; b < TM; ++b) {
-          u.x[b][0] = *reinterpret_cast<const v4i*>(xp[b] + off);
-          u.sx[b] = 0x7f00u | sxp[b][xs];
+    for (int b = 0; b < TM; ++b) {
+      if constexpr (XT == MX_CODES) {
+        const uint8_t *p = xp[b] + (int64_t)ks * GEMM_BK, *s = sxp[b] + (int64_t)ks * M * MX_SLAB;
+        if (n >= 2) {
+          u.x[b][0] = *reinterpret_cast<const v4i*>(p);
+          u.x[b][1] = *reinterpret_cast<const v4i*>(p + 16);
+          u.sx[b] = *reinterpret_cast<const uint16_t*>(s);
+        } else {
+          u.x[b][0] = n == 1 ? *reinterpret_cast<const v4i*>(p) : none;
+          u.x[b][1] = none;
+          u.sx[b] = 0x7f00u | (n == 1 ? s[0] : 127u);
         }
+      } else {
+        const T* p = xe[b] + (int64_t)ks * 2 * GEMM_BK;
+        u.x[b][0] = u.x[b][1] = none;
+        u.sx[b] = 0x7f7fu;
+        if (n >= 1) u.sx[b] = 0x7f00u | mx_quant_block<XT>(p, u.x[b][0]);
+        if (n >= 2) u.sx[b] = (u.sx[b] & 255u) | mx_quant_block<XT>(p + MX_BLOCK, u.x[b][1]) << 8;
       }
     }
   };
@@ -330,17 +360,23 @@ __global__ __launch_bounds__(64 * NW) void gemm_mxfp4_rows_kernel(const uint8_t*
       acc[b] = mx_mma16<1>(u.w[1], u.x[b][1], acc[b], u.sw, u.sx[b]);
     }
   };
-  constexpr int DEPTH = 4;
+  constexpr int DEPTH = NW == 16 ? 2 : 4;
   Unit u[DEPTH];
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d)
-    if (wave + d * NW < nk) load(wave + d * NW, u[d]);
+    if (wave + d * NW < nk) load_w(wave + d * NW, u[d]);
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d)
+    if (wave + d * NW < nk) load_x(wave + d * NW, u[d]);
   for (int ks = wave; ks < nk; ks += DEPTH * NW) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
       if (ks + d * NW < nk) {
         products(u[d]);
-        if (ks + (d + DEPTH) * NW < nk) load(ks + (d + DEPTH) * NW, u[d]);
+        if (ks + (d + DEPTH) * NW < nk) {
+          load_w(ks + (d + DEPTH) * NW, u[d]);
+          load_x(ks + (d + DEPTH) * NW, u[d]);
+        }
       }
     }
   }

@@ -1,6 +1,6 @@
 // The hot torch.library ops (mxf8::quant_rows, adaln_quant_rows, gemm_rowwise, lora_down,
 // attn_quant_kv, attn_fwd_q, rotary_table, rotate_qk, gated_residual_norm, mxfp4_quant,
-// mxfp4_dequant, gemm_mxfp4) as native kernels over the C ABI of libmxf8.  Their schemas and
+// mxfp4_dequant, gemm_mxfp4, mxfp4_linear) as native kernels over the C ABI of libmxf8.  Their schemas and
 // fake kernels are declared in minimaxh3_amd/ops.py; the kernels here take the CUDA and
 // AutogradCUDA entries of the dispatcher (the device type of a ROCm GPU), where they stand in
 // for the Python kernels of the declarations.
@@ -507,6 +507,29 @@ Tensor gemm_mxfp4(const Tensor& a4, const Tensor& w4, const Tensor& sa, const Te
   return out;
 }
 
+Tensor mxfp4_linear(const Tensor& x_in, const Tensor& w4, const Tensor& sw, const optional<Tensor>& bias, int64_t act) {
+  const char* what = "mxfp4_linear: ";
+  require_gfx950(x_in, "mxfp4_linear");
+  check_mxfp4(w4, sw, what, "weight");
+  const int64_t K = 2 * w4.size(1), N = w4.size(0);
+  TORCH_CHECK_VALUE(x_in.dim() == 2 && x_in.size(1) == K, what, "x [M, ", K, "] expected, got ", x_in.sizes());
+  const at::Device dev = x_in.device();
+  on_device(w4, dev, what, "w4");
+  TORCH_CHECK_VALUE(!bias || (bias->scalar_type() == at::kBFloat16 && bias->numel() == N && bias->is_contiguous()), what,
+                    "bias must be ", N, " contiguous bf16 values");
+  if (bias) on_device(*bias, dev, what, "bias");
+  const Tensor x = x_in.stride(1) != 1 || x_in.stride(0) < K ? x_in.contiguous() : x_in;
+  const int dt = dtype_code(x);
+  const int64_t M = x.size(0), ws = mxf8_mxfp4_linear_workspace_bytes(M, N, K, dt);
+  Tensor out = empty({M, N}, x, at::kBFloat16), work = ws ? empty({ws}, x, at::kByte) : Tensor();
+  const c10::DeviceGuard guard(dev);
+  check(mxf8_mxfp4_linear(x.data_ptr(), dt, std::max(x.stride(0), K), static_cast<const uint8_t*>(w4.data_ptr()),
+                          static_cast<const uint8_t*>(sw.data_ptr()), bias ? bias->data_ptr() : nullptr,
+                          static_cast<int>(act), out.data_ptr(), M, N, K, N, ws ? work.data_ptr() : nullptr, stream_of(x)),
+        "mxfp4_linear");
+  return out;
+}
+
 // The ops have no derivative.  With grad mode on, an output of an input that requires grad
 // requires grad and its backward raises; otherwise the call goes on below autograd (as the
 // Python declarations' autograd kernel does; forward-mode tangents end here).
@@ -556,10 +579,12 @@ TORCH_LIBRARY_IMPL(mxf8, CUDA, m) {
   m.impl("mxfp4_quant", &mxfp4_quant);
   m.impl("mxfp4_dequant", &mxfp4_dequant);
   m.impl("gemm_mxfp4", &gemm_mxfp4);
+  m.impl("mxfp4_linear", &mxfp4_linear);
 }
 
 TORCH_LIBRARY_IMPL(mxf8, AutogradCUDA, m) {
   for (const char* op : {"quant_rows", "adaln_quant_rows", "gemm_rowwise", "lora_down", "attn_quant_kv", "attn_fwd_q",
-                         "rotary_table", "rotate_qk", "gated_residual_norm", "mxfp4_quant", "mxfp4_dequant", "gemm_mxfp4"})
+                         "rotary_table", "rotate_qk", "gated_residual_norm", "mxfp4_quant", "mxfp4_dequant", "gemm_mxfp4",
+                         "mxfp4_linear"})
     m.impl(op, torch::CppFunction::makeFromBoxedFunction<&no_derivative>());
 }

@@ -80,8 +80,10 @@ class MXFP4Linear(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         x2d = x.reshape(-1, self.in_features)
-        x4, x_scale = quantize_mxfp4(x2d)
-        out = self.forward_quantized(x4, x_scale, x2d if self.adapters else None)
+        if self.adapters:
+            out = self.forward_quantized(*quantize_mxfp4(x2d), x2d)
+        else:
+            out = ops.mxfp4_linear(x2d, self.w4, self.w_scale, self.bias, int(self.act))
         return out.reshape(*x.shape[:-1], self.out_features).to(x.dtype)
 
     def forward_quantized(self, x4: torch.Tensor, x_scale: torch.Tensor,

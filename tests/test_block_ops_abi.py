@@ -138,6 +138,26 @@ def test_mxfp4(lib):
     refused(lib, gemm(sw=ctypes.c_void_p(260)), "aligned")
     assert gemm(m=0, a=None) == 0 and gemm(n=0, w=None) == 0
 
+    def linear(x=D, dtype=0, ldx=64, w=D, sw=D, act=0, out=D, m=40, n=8, k=64, ld=8, ws=D):
+        return lib.mxf8_mxfp4_linear(x, dtype, ldx, w, sw, None, act, out, m, n, k, ld, ws, None)
+
+    need = lib.mxf8_mxfp4_linear_workspace_bytes
+    assert need(16, 96, 288, 0) == 0 and need(0, 96, 288, 0) == 0
+    assert need(17, 96, 288, 0) == 17 * 144 + 2 * 17 * 8 and need(1, 96, 288, 2) == 144 + 16
+    assert need(1, 9216, 3072, 0) == 1536 + 12 * 8
+    refused(lib, linear(m=-1), "negative")
+    refused(lib, linear(k=0), "multiple of 32")
+    for null in ("x", "w", "sw", "out"):
+        refused(lib, linear(**{null: None}), "null")
+    refused(lib, linear(ldx=63), "ldx")
+    refused(lib, linear(ld=7), "ld_out")
+    refused(lib, linear(dtype=3), "dtype")
+    refused(lib, linear(act=9), "act")
+    refused(lib, linear(ws=None), "workspace")
+    refused(lib, linear(ws=ctypes.c_void_p(264)), "workspace")
+    refused(lib, linear(w=ctypes.c_void_p(264)), "aligned")
+    assert linear(m=0, x=None) == 0 and linear(n=0, w=None) == 0
+
 
 def test_cpu_tensors_are_refused():
     x = torch.zeros((4, 64))

@@ -139,6 +139,39 @@ def test_product_of_widely_scaled_blocks(m, n, k):
     product(m, n, k, seed=k, spread=6)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("m,n,k", [(1, 9216, 3072), (1, 3, 32), (5, 1001, 288), (16, 64, 8224), (16, 5200, 3072), (11, 5200, 4640), (2, 96, 288), (17, 96, 544),
+                                   (600, 300, 96)])
+def test_linear_in_one_call_is_the_quantizer_and_the_product(m, n, k, dtype):
+    x, w, b = randn(m, m, k, dtype=DT[dtype]), randn(n, n, k, std=0.05), randn(3, n)
+    x[0, :32] = 0
+    x[m // 2, 5] = 1e-7
+    w4, sw = quantize_mxfp4(w)
+    for act in (0, 1):
+        want = ops.gemm_mxfp4(*[(q, w4, s, sw) for q, s in [quantize_mxfp4(x)]][0], b, act)
+        assert torch.equal(ops.mxfp4_linear(x, w4, sw, b, act), want)
+    wide = torch.zeros((m, k + 7), dtype=x.dtype, device="cuda")
+    wide[:, 3: k + 3] = x
+    assert torch.equal(ops.mxfp4_linear(wide[:, 3: k + 3], w4, sw, b, 1), want)
+    assert torch.equal(ops.mxfp4_linear(x.t().contiguous().t(), w4, sw, b, 1), want)
+    x[m - 1, k - 1] = float("nan")
+    x[0, 2] = -float("inf")
+    out = ops.mxfp4_linear(x, w4, sw, b, 0)
+    assert out[m - 1].isnan().all() and out[0].isnan().all() and torch.isfinite(out[1: m - 1]).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_linear_quantizes_every_16_bit_value_as_the_quantizer(dtype):
+    v = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(torch.float16 if dtype == "fp16" else torch.bfloat16)
+    v = v[torch.randperm(65536, generator=torch.Generator().manual_seed(1))].float()
+    v = v.nan_to_num(0.5, 1.0, -1.0).to(DT[dtype]).reshape(-1, 1024).cuda()
+    w4, sw = quantize_mxfp4(torch.eye(1024, device="cuda"))  # (each output is one value of the row)
+    for rows in v.split(16):
+        (a4, sa), got = quantize_mxfp4(rows), ops.mxfp4_linear(rows, w4, sw, None, 0)
+        assert torch.equal(got, ops.gemm_mxfp4(a4, w4, sa, sw, None, 0))
+        assert torch.equal(got, dequantize_mxfp4(a4, sa))
+
+
 def test_scale_bytes_past_k_are_ignored():
     """K = 288 fills one block of the second slab; the others' bytes may hold anything, NaN among it."""
     for m in (3, 40, 140, 4100):
@@ -294,6 +327,12 @@ def test_refusals():
             ops.gemm_mxfp4(*args)
     with pytest.raises(RuntimeError, match="act"):
         ops.gemm_mxfp4(a4, w4, sa, sw, b, 5)
+    for args in ((x[:, :32], w4, sw, b, 0), (x[0], w4, sw, b, 0), (x.cpu(), w4, sw, b, 0), (x, w4, sw[:, :3], b, 0),
+                 (x, w4, sw, b[:2], 0), (x.double(), w4, sw, b, 0), (x, w4.cpu(), sw.cpu(), None, 0)):
+        with pytest.raises(ValueError):
+            ops.mxfp4_linear(*args)
+    with pytest.raises(RuntimeError, match="act"):
+        ops.mxfp4_linear(x, w4, sw, b, 2)
     with pytest.raises(ValueError):
         MXFP4Linear.from_quantized(w4, sw[:, :3])
     with pytest.raises(ValueError):
