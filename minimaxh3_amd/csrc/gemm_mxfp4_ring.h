@@ -264,19 +264,20 @@ __global__ __launch_bounds__(C::THREADS) void gemm_mxfp4_ring_kernel(const uint8
   }
 }
 
-// 16 channels x 16 TM tokens per workgroup of NW waves.  A unit is one slab of K (256 elements, 128 bytes of a
+// 16 TN channels x 16 TM tokens per workgroup of NW waves.  A unit is one slab of K (256 elements, 128 bytes of a
 // row): lane group g = lane / 16 of the 16 x 16 x 128 instruction takes blocks 2 g and 2 g + 1 of its row, one
 // per instruction, 32 bytes and two scale bytes.  Wave w takes units w, w + NW, ..., up to four in flight.
+//
+// XT: the activations are codes and scales (MX_CODES), or 16-bit elements of that type, row stride ldx, which each
+// lane quantizes for itself (mx_quant_block), where that costs less than a launch of its own.
+constexpr int MX_CODES = -1;
+
 template <int T>
 __device__ __forceinline__ v4f mx_mma16(const v4i& a, const v4i& b, const v4f& c, uint32_t sa, uint32_t sb) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_wide(a), mx_wide(b), c, 4, 4, T, (int)sa, T, (int)sb);
 }
 
-// XT: the activations are codes and scales (MX_CODES), or 16-bit elements of that type, row stride ldx, which each
-// lane quantizes for itself (mx_quant_block), where that costs less than a launch of its own.
-constexpr int MX_CODES = -1;
-
-template <int TM, int NW, int ACT, bool KTAIL, int XT>
+template <int TM, int TN, int NW, int ACT, bool KTAIL, int XT>
 __global__ __launch_bounds__(64 * NW) void gemm_mxfp4_rows_kernel(const void* __restrict__ x, int64_t ldx,
                                                                   const uint8_t* __restrict__ sa,
                                                                   const uint8_t* __restrict__ w4,
@@ -284,81 +285,87 @@ __global__ __launch_bounds__(64 * NW) void gemm_mxfp4_rows_kernel(const void* __
                                                                   const uint16_t* __restrict__ bias,
                                                                   uint16_t* __restrict__ out, int M, int N, int Kb,
                                                                   int64_t ld_out) {
-  typedef uint16_t T;
-  __shared__ __attribute__((aligned(16))) v4f part[NW][TM][64];
+  __shared__ __attribute__((aligned(16))) v4f part[NW][TN * TM][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int r = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * TM;
+  const int n0 = blockIdx.x * 16 * TN, m0 = blockIdx.y * 16 * TM;
   const int nk = (Kb + GEMM_BK - 1) / GEMM_BK;
   // rows past the end are the last row again (not stored)
-  const int wrow = min(n0 + r, N - 1);
-  const uint8_t* const wp = w4 + (int64_t)wrow * Kb + 32 * g;
-  const uint8_t* const swp = sw + (int64_t)wrow * MX_SLAB + 2 * g;
-  const uint8_t *xp[TM], *sxp[TM];
-  const T* xe[TM];
+  const uint8_t *wp[TN], *swp[TN], *xp[TM], *sxp[TM];
+  const uint16_t* xe[TM];
+#pragma unroll
+  for (int a = 0; a < TN; ++a) {
+    const int row = min(n0 + 16 * a + r, N - 1);
+    wp[a] = w4 + (int64_t)row * Kb + 32 * g;
+    swp[a] = sw + (int64_t)row * MX_SLAB + 2 * g;
+  }
 #pragma unroll
   for (int b = 0; b < TM; ++b) {
-    const int xrow = min(m0 + 16 * b + r, M - 1);
+    const int row = min(m0 + 16 * b + r, M - 1);
     if constexpr (XT == MX_CODES) {
-      xp[b] = static_cast<const uint8_t*>(x) + (int64_t)xrow * Kb + 32 * g;
-      sxp[b] = sa + (int64_t)xrow * MX_SLAB + 2 * g;
+      xp[b] = static_cast<const uint8_t*>(x) + (int64_t)row * Kb + 32 * g;
+      sxp[b] = sa + (int64_t)row * MX_SLAB + 2 * g;
     } else {
-      xe[b] = static_cast<const T*>(x) + xrow * ldx + 64 * g;
+      xe[b] = static_cast<const uint16_t*>(x) + row * ldx + 64 * g;
     }
   }
-  struct Unit {
-    v4i w[2], x[TM][2];
-    uint32_t sw, sx[TM];
+  struct Operand {
+    v4i c[2];
+    uint32_t s;
   };
   // blocks 2 g and 2 g + 1 of the slab; those past K are zero codes under a scale of 1
   auto there = [&](int ks) { return KTAIL ? (Kb >> 4) - 8 * ks - 2 * g : 2; };
   const v4i none = {0, 0, 0, 0};
-  auto load_w = [&](int ks, Unit& u) {
-    const uint8_t *p = wp + (int64_t)ks * GEMM_BK, *s = swp + (int64_t)ks * N * MX_SLAB;
-    const int n = there(ks);
+  auto load = [&](const uint8_t* p, const uint8_t* s, int n, Operand& o) {
     if (n >= 2) {
-      u.w[0] = *reinterpret_cast<const v4i*>(p);
-      u.w[1] = *reinterpret_cast<const v4i*>(p + 16);
-      u.sw = *reinterpret_cast<const uint16_t*>(s);
+      o.c[0] = *reinterpret_cast<const v4i*>(p);
+      o.c[1] = *reinterpret_cast<const v4i*>(p + 16);
+      o.s = *reinterpret_cast<const uint16_t*>(s);
     } else {
-      u.w[0] = n == 1 ? *reinterpret_cast<const v4i*>(p) : none;
-      u.w[1] = none;
-      u.sw = 0x7f00u | (n == 1 ? s[0] : 127u);
+      o.c[0] = n == 1 ? *reinterpret_cast<const v4i*>(p) : none;
+      o.c[1] = none;
+      o.s = 0x7f00u | (n == 1 ? s[0] : 127u);
     }
+  };
+  struct Unit {
+    Operand w[TN], x[TM];
+  };
+  auto load_w = [&](int ks, Unit& u) {
+#pragma unroll
+    for (int a = 0; a < TN; ++a)
+      load(wp[a] + (int64_t)ks * GEMM_BK, swp[a] + (int64_t)ks * N * MX_SLAB, there(ks), u.w[a]);
   };
   auto load_x = [&](int ks, Unit& u) {
     const int n = there(ks);
 #pragma unroll
     for (int b = 0; b < TM; ++b) {
       if constexpr (XT == MX_CODES) {
-        const uint8_t *p = xp[b] + (int64_t)ks * GEMM_BK, *s = sxp[b] + (int64_t)ks * M * MX_SLAB;
-        if (n >= 2) {
-          u.x[b][0] = *reinterpret_cast<const v4i*>(p);
-          u.x[b][1] = *reinterpret_cast<const v4i*>(p + 16);
-          u.sx[b] = *reinterpret_cast<const uint16_t*>(s);
-        } else {
-          u.x[b][0] = n == 1 ? *reinterpret_cast<const v4i*>(p) : none;
-          u.x[b][1] = none;
-          u.sx[b] = 0x7f00u | (n == 1 ? s[0] : 127u);
-        }
+        load(xp[b] + (int64_t)ks * GEMM_BK, sxp[b] + (int64_t)ks * M * MX_SLAB, n, u.x[b]);
       } else {
-        const T* p = xe[b] + (int64_t)ks * 2 * GEMM_BK;
-        u.x[b][0] = u.x[b][1] = none;
-        u.sx[b] = 0x7f7fu;
-        if (n >= 1) u.sx[b] = 0x7f00u | mx_quant_block<XT>(p, u.x[b][0]);
-        if (n >= 2) u.sx[b] = (u.sx[b] & 255u) | mx_quant_block<XT>(p + MX_BLOCK, u.x[b][1]) << 8;
+        const uint16_t* p = xe[b] + (int64_t)ks * 2 * GEMM_BK;
+        MxElems e[2];
+        if (n >= 1) e[0].load(p);
+        if (n >= 2) e[1].load(p + MX_BLOCK);
+        u.x[b].c[0] = u.x[b].c[1] = none;
+        u.x[b].s = 0x7f7fu;
+        if (n >= 1) u.x[b].s = 0x7f00u | e[0].quantize<XT>(u.x[b].c[0]);
+        if (n >= 2) u.x[b].s = (u.x[b].s & 255u) | e[1].quantize<XT>(u.x[b].c[1]) << 8;
       }
     }
   };
-  v4f acc[TM];
+  v4f acc[TN][TM];
 #pragma unroll
-  for (int b = 0; b < TM; ++b) acc[b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int a = 0; a < TN; ++a)
+#pragma unroll
+    for (int b = 0; b < TM; ++b) acc[a][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   auto products = [&](const Unit& u) {
 #pragma unroll
-    for (int b = 0; b < TM; ++b) {
-      acc[b] = mx_mma16<0>(u.w[0], u.x[b][0], acc[b], u.sw, u.sx[b]);
-      acc[b] = mx_mma16<1>(u.w[1], u.x[b][1], acc[b], u.sw, u.sx[b]);
-    }
+    for (int a = 0; a < TN; ++a)
+#pragma unroll
+      for (int b = 0; b < TM; ++b) {
+        acc[a][b] = mx_mma16<0>(u.w[a].c[0], u.x[b].c[0], acc[a][b], u.w[a].s, u.x[b].s);
+        acc[a][b] = mx_mma16<1>(u.w[a].c[1], u.x[b].c[1], acc[a][b], u.w[a].s, u.x[b].s);
+      }
   };
   constexpr int DEPTH = NW == 16 ? 2 : 4;
   Unit u[DEPTH];
@@ -381,15 +388,17 @@ __global__ __launch_bounds__(64 * NW) void gemm_mxfp4_rows_kernel(const void* __
     }
   }
 #pragma unroll
-  for (int b = 0; b < TM; ++b) part[wave][b][lane] = acc[b];
-  __syncthreads();
-  // part[.][b][lane]: channels n0 + 4 g .. 4 g + 3 of token m0 + 16 b + r; thread t sums entry t over the waves
-  for (int e = threadIdx.x; e < TM * 64; e += 64 * NW) {
-    const int b = e >> 6, l = e & 63, m = m0 + 16 * b + (l & 15), n = n0 + 4 * (l >> 4);
-    if (m >= M || n >= N) continue;
-    v4f s = part[0][b][l];
+  for (int a = 0; a < TN; ++a)
 #pragma unroll
-    for (int w = 1; w < NW; ++w) s += part[w][b][l];
+    for (int b = 0; b < TM; ++b) part[wave][a * TM + b][lane] = acc[a][b];
+  __syncthreads();
+  // part[.][a TM + b][lane]: channels n0 + 16 a + 4 g .. + 3 of token m0 + 16 b + r; thread t sums entry t over the waves
+  for (int e = threadIdx.x; e < TN * TM * 64; e += 64 * NW) {
+    const int t = e >> 6, l = e & 63, m = m0 + 16 * (t % TM) + (l & 15), n = n0 + 16 * (t / TM) + 4 * (l >> 4);
+    if (m >= M || n >= N) continue;
+    v4f s = part[0][t][l];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) s += part[w][t][l];
     v4f bq = {0.0f, 0.0f, 0.0f, 0.0f};
     if (bias) {
 #pragma unroll

@@ -44,41 +44,45 @@ __device__ __forceinline__ uint32_t mx_codes8(const float (&f)[8], uint32_t byte
   return w;
 }
 
-// A whole block of 16-bit elements in one lane: 32 from `p` (any alignment) to 16 bytes of codes and the scale byte,
-// the same as above.  The elements stay packed: their magnitudes are ordered like integers.
-template <int DT>
-__device__ __forceinline__ uint32_t mx_quant_block(const uint16_t* p, v4i& codes) {
+// A whole block of 16-bit elements in one lane: loaded from any alignment, and quantized to 16 bytes of codes and
+// the scale byte, the same as above.  The elements stay packed: their magnitudes are ordered like integers.
+struct MxElems {
   typedef uint32_t words4 __attribute__((ext_vector_type(4), aligned(2)));
   typedef unsigned short v2us __attribute__((ext_vector_type(2)));
   words4 w[4];
-  v2us m = {0, 0};
+  __device__ __forceinline__ void load(const uint16_t* p) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    w[q] = reinterpret_cast<const words4*>(p)[q];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(v2us, w[q][i] & 0x7fff7fffu));
+    for (int q = 0; q < 4; ++q) w[q] = reinterpret_cast<const words4*>(p)[q];
   }
-  const uint32_t byte = mx_scale_byte(__float_as_uint(Elem<DT>::to_f32(max(m[0], m[1]))));
-  const float s = mx_scale_value(byte);
+  template <int DT>
+  __device__ __forceinline__ uint32_t quantize(v4i& codes) const {
+    v2us m = {0, 0};
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const uint32_t a = w[q][0], b = w[q][1], c = w[q][2], d = w[q][3];
-    uint32_t o = 0;
-    if constexpr (DT == MXF8_BF16) {
-      o = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o, __builtin_bit_cast(v2bf, a), s, 0);
-      o = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o, __builtin_bit_cast(v2bf, b), s, 1);
-      o = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o, __builtin_bit_cast(v2bf, c), s, 2);
-      o = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o, __builtin_bit_cast(v2bf, d), s, 3);
-    } else {
-      o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, __builtin_bit_cast(v2h, a), s, 0);
-      o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, __builtin_bit_cast(v2h, b), s, 1);
-      o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, __builtin_bit_cast(v2h, c), s, 2);
-      o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, __builtin_bit_cast(v2h, d), s, 3);
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(v2us, w[q][i] & 0x7fff7fffu));
+    const uint32_t byte = mx_scale_byte(__float_as_uint(Elem<DT>::to_f32(max(m[0], m[1]))));
+    const float s = mx_scale_value(byte);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t a = w[q][0], b = w[q][1], c = w[q][2], d = w[q][3];
+      uint32_t o = 0;
+      if constexpr (DT == MXF8_BF16) {
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o, __builtin_bit_cast(v2bf, a), s, 0);
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o, __builtin_bit_cast(v2bf, b), s, 1);
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o, __builtin_bit_cast(v2bf, c), s, 2);
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o, __builtin_bit_cast(v2bf, d), s, 3);
+      } else {
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, __builtin_bit_cast(v2h, a), s, 0);
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, __builtin_bit_cast(v2h, b), s, 1);
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, __builtin_bit_cast(v2h, c), s, 2);
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, __builtin_bit_cast(v2h, d), s, 3);
+      }
+      codes[q] = (int)o;
     }
-    codes[q] = (int)o;
+    return byte;
   }
-  return byte;
-}
+};
 
 // The largest |f| as bits (a NaN is larger than every number) over eight values and the four lanes of a quad,
 // which together hold one block.

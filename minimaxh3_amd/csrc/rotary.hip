@@ -74,10 +74,16 @@ __global__ __launch_bounds__(256) void rotary_table_kernel(const void* __restric
   __syncthreads();
   const int64_t t0 = (int64_t)blockIdx.x * rows;
   const int cnt = (int)min((int64_t)rows, n - t0) * P;
-  for (int e = threadIdx.x; e < cnt; e += 256) {
-    const int t = e / P, j = e - t * P;
-    const v2f cs = rot_cos_sin(rot_pos<PT>(pos, (t0 + t) * axes + axis[j]) * freq[j]);
-    *reinterpret_cast<v2f*>(table + (t0 * P + e) * 2) = cs;
+  // entry e = t P + j, 256 further each time: t and j move by the same amounts but for a carry
+  const int dt = 256 / P, dj = 256 - dt * P;
+  int t = threadIdx.x / P, j = threadIdx.x - t * P;
+  float* o = table + (t0 * P + threadIdx.x) * 2;
+  for (int e = threadIdx.x; e < cnt; e += 256, o += 512) {
+    const double p = rot_pos<PT>(pos, (t0 + t) * axes + axis[j]);
+    *reinterpret_cast<v2f*>(o) = rot_cos_sin(p * freq[j]);
+    t += dt;
+    j += dj;
+    if (j >= P) j -= P, ++t;
   }
 }
 

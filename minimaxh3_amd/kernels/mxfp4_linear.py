@@ -79,12 +79,14 @@ class MXFP4Linear(nn.Module):
         return mod
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        x2d = x.reshape(-1, self.in_features)
+        x2d = x if x.ndim == 2 else x.reshape(-1, self.in_features)
         if self.adapters:
             out = self.forward_quantized(*quantize_mxfp4(x2d), x2d)
         else:
             out = ops.mxfp4_linear(x2d, self.w4, self.w_scale, self.bias, int(self.act))
-        return out.reshape(*x.shape[:-1], self.out_features).to(x.dtype)
+        if x.ndim != 2:
+            out = out.reshape(*x.shape[:-1], self.out_features)
+        return out if x.dtype == torch.bfloat16 else out.to(x.dtype)
 
     def forward_quantized(self, x4: torch.Tensor, x_scale: torch.Tensor,
                           x_modulated: torch.Tensor | None = None) -> torch.Tensor:
