@@ -22,21 +22,25 @@ struct RotAxes {
   double log2_theta;
 };
 
+// Position i from the uniform `base` on, of pos_type PT.
 template <int PT>
-__device__ __forceinline__ double rot_pos(const void* p, int64_t i);
-template <> __device__ __forceinline__ double rot_pos<0>(const void* p, int64_t i) { return static_cast<const float*>(p)[i]; }
-template <> __device__ __forceinline__ double rot_pos<1>(const void* p, int64_t i) { return static_cast<const double*>(p)[i]; }
-template <> __device__ __forceinline__ double rot_pos<2>(const void* p, int64_t i) { return static_cast<const int*>(p)[i]; }
-template <> __device__ __forceinline__ double rot_pos<3>(const void* p, int64_t i) {
-  return (double)static_cast<const int64_t*>(p)[i];
+__device__ __forceinline__ double rot_pos(const void* p, int64_t base, int i) {
+  if constexpr (PT == 0)
+    return (static_cast<const float*>(p) + base)[i];
+  else if constexpr (PT == 1)
+    return (static_cast<const double*>(p) + base)[i];
+  else if constexpr (PT == 2)
+    return (static_cast<const int*>(p) + base)[i];
+  else
+    return (double)(static_cast<const int64_t*>(p) + base)[i];
 }
 
 // cos and sin of `rev` revolutions.  The angle is reduced in fp64 to an eighth of a turn either way, exactly, so
 // positions in the millions lose nothing; there the Taylor series to the 9th and 10th power are within 2^-26.
 __device__ __forceinline__ v2f rot_cos_sin(double rev) {
-  const double q = __builtin_rint(4.0 * rev);
-  const double turn = q - 4.0 * __builtin_rint(0.25 * q);  // -2 .. 2 (fp64: whole at any magnitude)
-  const float x = (float)(__builtin_fma(q, -0.25, rev) * 6.283185307179586);
+  const double turn = rev - __builtin_rint(rev);  // -1/2 .. 1/2
+  const float q = __builtin_rintf(4.0f * (float)turn);  // -2 .. 2 (either neighbour of a tie will do)
+  const float x = (float)(__builtin_fma((double)q, -0.25, turn) * 6.283185307179586);
   const float x2 = x * x;
   float s = __builtin_fmaf(x2, 2.7557319e-6f, -1.9841270e-4f);
   s = __builtin_fmaf(x2, s, 8.3333333e-3f);
@@ -47,7 +51,7 @@ __device__ __forceinline__ v2f rot_cos_sin(double rev) {
   c = __builtin_fmaf(x2, c, 4.1666667e-2f);
   c = __builtin_fmaf(x2, c, -0.5f);
   c = __builtin_fmaf(x2, c, 1.0f);
-  const int k = (int)turn & 3;
+  const int k = (int)q & 3;
   const float cc = k & 1 ? s : c, ss = k & 1 ? c : s;
   return v2f{k == 1 || k == 2 ? -cc : cc, k >= 2 ? -ss : ss};
 }
@@ -77,13 +81,13 @@ __global__ __launch_bounds__(256) void rotary_table_kernel(const void* __restric
   // entry e = t P + j, 256 further each time: t and j move by the same amounts but for a carry
   const int dt = 256 / P, dj = 256 - dt * P;
   int t = threadIdx.x / P, j = threadIdx.x - t * P;
+  int row = t * axes;  // of the block's first token's positions
   float* o = table + (t0 * P + threadIdx.x) * 2;
   for (int e = threadIdx.x; e < cnt; e += 256, o += 512) {
-    const double p = rot_pos<PT>(pos, (t0 + t) * axes + axis[j]);
-    *reinterpret_cast<v2f*>(o) = rot_cos_sin(p * freq[j]);
-    t += dt;
+    *reinterpret_cast<v2f*>(o) = rot_cos_sin(rot_pos<PT>(pos, t0 * axes, row + axis[j]) * freq[j]);
+    row += dt * axes;
     j += dj;
-    if (j >= P) j -= P, ++t;
+    if (j >= P) j -= P, row += axes;
   }
 }
 
