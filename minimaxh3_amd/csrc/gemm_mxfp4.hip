@@ -110,10 +110,11 @@ __global__ __launch_bounds__(C::THREADS) void gemm_mxfp4_kernel(const uint8_t* _
         if (i % MX_SLAB >= valid) sc_smem[buf * SCALES + i] = 127;
       block_barrier();
     };
-    // Stage 0 of this tile is in flight into buffer gs & 1; of what was issued after it, the last tile's output stores
-    // (STORES a wave, of a tile inside the matrix) and the bias, nothing is waited for.
+    // Stage 0 of this tile is in flight into buffer gs & 1; the last tile's output stores (STORES a wave, of a tile
+    // inside the matrix), issued after it, are not waited for.  The bias load is not counted: the compiler may place it
+    // on either side of the wait, and one operation too many here would leave a copy in flight.
     if (stores_behind)
-      wait_vm<STORES + 1>();
+      wait_vm<STORES>();
     else
       wait_vm0();
     block_barrier();
