@@ -18,6 +18,12 @@ template <int DT>
 struct Raw8 {
   uint32_t w[4];
   __device__ __forceinline__ void load(const void* base, int64_t i) { load_at((gbytes)base + i * 2); }
+  // non-temporal: for operands that are read once and too large for the caches
+  __device__ __forceinline__ void load_stream(const void* base, int64_t i) {
+    const words4 v = __builtin_nontemporal_load((gwords4)((gbytes)base + i * 2));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = v[j];
+  }
   // `off`: bytes from a base that is the same for the whole wave
   __device__ __forceinline__ void load_off(const void* base, uint32_t off) { load_at((gbytes)base + off); }
   __device__ __forceinline__ void load_at(gbytes p) {
@@ -81,6 +87,12 @@ template <>
 struct Raw8<MXF8_F32> {
   float w[8];
   __device__ __forceinline__ void load(const void* base, int64_t i) { load_at((gbytes)base + i * 4); }
+  __device__ __forceinline__ void load_stream(const void* base, int64_t i) {
+    const floats4 a = __builtin_nontemporal_load((gfloats4)((gbytes)base + i * 4));
+    const floats4 b = __builtin_nontemporal_load((gfloats4)((gbytes)base + i * 4 + 16));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = a[j], w[j + 4] = b[j];
+  }
   __device__ __forceinline__ void load_off(const void* base, uint32_t off) { load_at((gbytes)base + off); }
   __device__ __forceinline__ void load_at(gbytes p) {
     const floats4 a = *(gfloats4)p, b = *(gfloats4)(p + 16);

@@ -39,7 +39,7 @@ def check_quant(x):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
-@pytest.mark.parametrize("m,k", [(1, 32), (1, 3072), (5, 96), (17, 288), (33, 4640), (130, 1056), (3, 12288)])
+@pytest.mark.parametrize("m,k", [(1, 32), (1, 3072), (5, 96), (17, 288), (33, 4640), (130, 1056), (3, 12288), (6000, 3072)])
 def test_quantizer(m, k, dtype):
     check_quant(randn(m + k, m, k, dtype=DT[dtype]))
 
