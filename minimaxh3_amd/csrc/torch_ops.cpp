@@ -560,8 +560,10 @@ void no_derivative(const c10::OperatorHandle& op, c10::DispatchKeySet ks, torch:
       "Trying to backward through mxf8." + name + ".default but no autograd formula was registered. Please use "
       "register_autograd to add one.", std::move(edges));
   const size_t nret = op.schema().returns().size();
-  for (size_t i = 0; i < nret; ++i)
-    torch::autograd::set_history(torch::jit::peek(*stack, i, nret).toTensor(), node);
+  for (size_t i = 0; i < nret; ++i) {
+    const at::Tensor& out = torch::jit::peek(*stack, i, nret).toTensor();
+    if (torch::autograd::isDifferentiableType(out.scalar_type())) torch::autograd::set_history(out, node);  // not 4-bit codes
+  }
 }
 
 }  // namespace

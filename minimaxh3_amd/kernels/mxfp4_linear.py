@@ -80,10 +80,9 @@ class MXFP4Linear(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         x2d = x if x.ndim == 2 else x.reshape(-1, self.in_features)
+        out = ops.mxfp4_linear(x2d, self.w4, self.w_scale, self.bias, ACT_NONE if self.adapters else int(self.act))
         if self.adapters:
-            out = self.forward_quantized(*quantize_mxfp4(x2d), x2d)
-        else:
-            out = ops.mxfp4_linear(x2d, self.w4, self.w_scale, self.bias, int(self.act))
+            out = self._adapted(x2d, out)
         if x.ndim != 2:
             out = out.reshape(*x.shape[:-1], self.out_features)
         return out if x.dtype == torch.bfloat16 else out.to(x.dtype)
@@ -99,7 +98,10 @@ class MXFP4Linear(nn.Module):
         if x_modulated is None:
             raise ValueError("forward_quantized: LoRA adapters need the unquantized input (x_modulated)")
         out = ops.gemm_mxfp4(x4, self.w4, x_scale, self.w_scale, self.bias, ACT_NONE)
-        out = apply_lora_adapters(x_modulated.reshape(-1, self.in_features), out, self.adapters)
+        return self._adapted(x_modulated.reshape(-1, self.in_features), out)
+
+    def _adapted(self, x2d: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+        out = apply_lora_adapters(x2d, out, self.adapters)
         return torch.nn.functional.gelu(out, approximate="tanh") if self.act == ACT_GELU_TANH else out
 
     def extra_repr(self) -> str:

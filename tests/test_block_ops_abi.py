@@ -193,3 +193,13 @@ def test_fake_kernels_give_the_shapes_of_the_real_ones():
     assert codes.shape == (5, 144) and scales.shape == (2, 5, 8)
     assert ops.gemm_mxfp4(codes, codes, scales, scales, None, 0).shape == (5, 5)
     assert ops.mxfp4_dequant(codes, scales, torch.float16).dtype == torch.float16
+
+
+def test_import_registers_the_native_kernels():
+    """Before any call: a kernel registered later would change a table that the dispatcher reads without a lock."""
+    import minimaxh3_amd.ops  # noqa: F401
+
+    for op in ("rotary_table", "rotate_qk", "gated_residual_norm", "mxfp4_quant", "mxfp4_dequant", "gemm_mxfp4",
+               "mxfp4_linear"):
+        for key in ("CUDA", "AutogradCUDA"):
+            assert torch._C._dispatch_has_kernel_for_dispatch_key("mxf8::" + op, key), (op, key)

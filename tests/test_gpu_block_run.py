@@ -1,0 +1,279 @@
+"""The operators of a DiT block in a run, as a denoiser uses them: norm and modulation into the 4-bit QKV
+projection, rotary positions on its views, FP8 attention, 4-bit output projection, gated residual and norm into an
+8-bit MLP, gated residual.  Each stage against its 64-bit form on the inputs that the run hands it; the whole run
+captured, on two streams at once, compiled, and under the dispatcher's checks."""
+import numpy as np
+import pytest
+import torch
+import torch.nn as nn
+
+from minimaxh3_amd import _native as N
+from minimaxh3_amd import ops
+from minimaxh3_amd.kernels.block_norms import gated_residual_norm
+from minimaxh3_amd.kernels.fp8_attention import fp8_attention
+from minimaxh3_amd.kernels.fp8_linear import ACT_GELU_TANH, FP8Linear
+from minimaxh3_amd.kernels.mxfp4_linear import MXFP4Linear, quantize_mxfp4
+from minimaxh3_amd.kernels.rotary import rotary_table, rotate_qk
+from oracle import attention as oa
+from oracle import dit_block as ob
+from oracle import linear as ol
+from tests.helpers import assert_gemm_close, cos
+
+pytestmark = pytest.mark.gpu
+H, D = 3, 128
+C, F = H * D, 2 * H * D
+DIMS = (44, 42, 42)
+
+
+def f64(t):
+    return t.detach().to("cpu", torch.float64).numpy()
+
+
+def values(codes, scales):
+    return ob.mxfp4_values(codes.cpu().numpy(), scales.cpu().numpy())
+
+
+def e4m3(codes, scales):
+    return f64(codes) * f64(scales).reshape(-1, 1)
+
+
+class Block(nn.Module):
+    def __init__(self, mlp4):
+        super().__init__()
+        g = torch.Generator().manual_seed(7)
+        lin = lambda k, n: self._linear(g, k, n)  # noqa: E731
+        self.qkv, self.proj = MXFP4Linear.from_linear(lin(C, 3 * C)), MXFP4Linear.from_linear(lin(C, C))
+        self.mlp4 = mlp4
+        kind = MXFP4Linear if mlp4 else FP8Linear
+        self.up, self.down = kind.from_linear(lin(C, F)), kind.from_linear(lin(F, C))
+        self.up.act = ACT_GELU_TANH
+        w = lambda n: nn.Buffer((1 + 0.2 * torch.randn(n, generator=g)).bfloat16().cuda())  # noqa: E731
+        self.qw, self.kw, self.post = w(D), w(D), w(C)
+
+    @staticmethod
+    def _linear(g, k, n):
+        lin = nn.Linear(k, n, device="cuda", dtype=torch.bfloat16)
+        with torch.no_grad():
+            lin.weight.copy_(torch.randn(n, k, generator=g) * k ** -0.5)
+            lin.bias.copy_(torch.randn(n, generator=g) * 0.1)
+        return lin
+
+    def forward(self, x, mod, table, kept=None):
+        B, S, _ = x.shape
+        shift1, scale1, gate1, shift2, scale2, gate2 = mod.unbind(-2)  # [B, G, C], rows 6 C apart
+        _, h4, hs = gated_residual_norm(x, None, None, shift1, scale1, quantize="mxfp4")
+        qkv = self.qkv.forward_quantized(h4, hs)
+        q, k, v = (t.transpose(1, 2) for t in qkv.view(B, S, 3, H, D).unbind(2))
+        qr, kr = rotate_qk(q, k, table, self.qw, self.kw)
+        a = fp8_attention(qr, kr, v)
+        o = self.proj(a.transpose(1, 2).reshape(B, S, C))
+        r, u8, us = gated_residual_norm(x, o, gate1, shift2, scale2, branch_weight=self.post, norm="rms",
+                                        quantize="mxfp4" if self.mlp4 else "e4m3")
+        up = self.up.forward_quantized(u8, us)
+        down = self.down(up).view(B, S, C)
+        out, y = gated_residual_norm(r, down, gate2)
+        if kept is not None:
+            kept.update(h4=h4, hs=hs, qkv=qkv, q=q, k=k, v=v, qr=qr, kr=kr, a=a, o=o, r=r, u8=u8, us=us, up=up, down=down)
+        return out, y
+
+
+def inputs(seed, b, s, groups=1):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(b, s, C, generator=g).bfloat16().cuda()
+    mod = (torch.randn(b, groups, 6, C, generator=g) * 0.4).bfloat16().cuda()
+    pos = torch.stack([torch.arange(s) // 12, torch.arange(s) // 4 % 3, torch.arange(s) % 4], -1).cuda()
+    return x, mod, rotary_table(pos, DIMS)
+
+
+def close(got, ref, bound, what):
+    err = np.abs(f64(got).reshape(ref.shape) - ref)
+    ok = err <= bound + ob.half_step(np.abs(ref) + bound, "bf16")
+    assert ok.all(), (what, (err - bound).max(), np.argwhere(~ok)[:4])
+
+
+@pytest.mark.parametrize("mlp4", [False, True])
+@pytest.mark.parametrize("b,s,groups", [(1, 1, 1), (2, 7, 1), (1, 132, 11), (2, 300, 3)])
+@torch.no_grad()
+def test_every_stage_of_a_run(b, s, groups, mlp4):
+    x, mod, table = inputs(s, b, s, groups)
+    blk, t = Block(mlp4), {}
+    out, y = blk(x, mod, table, t)
+    shift1, scale1, gate1, shift2, scale2, gate2 = (f64(m) for m in mod.unbind(-2))
+
+    # the norm's codes are those of the value that it would store
+    _, _, _, stored = gated_residual_norm(x, None, None, mod[:, :, 0], mod[:, :, 1], quantize="mxfp4", return_modulated=True)
+    h4, hs = quantize_mxfp4(stored.view(-1, C))
+    assert torch.equal(h4, t["h4"]) and torch.equal(hs, t["hs"])
+    _, ref, _, bound = ob.gated_residual_norm(f64(x), None, None, shift1, scale1)
+    close(stored, ref, bound, "first norm")
+
+    def linear4(mod4, codes, scales, act=False):
+        return ob.mxfp4_linear(values(codes, scales), values(mod4.w4, mod4.w_scale), f64(mod4.bias), act)
+
+    close(t["qkv"], *linear4(blk.qkv, t["h4"], t["hs"]), "qkv")
+    for x_, w, got in ((t["q"], blk.qw, t["qr"]), (t["k"], blk.kw, t["kr"])):
+        assert got.transpose(1, 2).is_contiguous()
+        close(got, *ob.rotate(f64(x_), f64(table), f64(w)), "rotation")
+    ref = oa.fp8_attention(f64(t["qr"]), f64(t["kr"]), f64(t["v"]))[0].astype(np.float64)
+    # the attention's own bar, and a step of bf16 (outputs reach 4 and more here)
+    assert cos(f64(t["a"]), ref) >= 0.999 and (np.abs(f64(t["a"]) - ref) <= 2e-2 + 2.0 ** -7 * np.abs(ref)).all()
+    flat = t["a"].transpose(1, 2).reshape(-1, C)
+    close(t["o"], *linear4(blk.proj, *quantize_mxfp4(flat)), "projection")
+    r, u, br, bu = ob.gated_residual_norm(f64(x), f64(t["o"]), gate1, shift2, scale2, f64(blk.post), norm="rms")
+    close(t["r"], r, br, "residual")
+    if mlp4:
+        close(t["up"], *linear4(blk.up, t["u8"], t["us"], True), "up")
+        close(t["down"], *linear4(blk.down, *quantize_mxfp4(t["up"])), "down")
+        # a block's largest is 3.5 to 7 of its units; half the widest step and what 7 loses at 6 are one unit (and bf16's
+        # roundings of the value and of the largest before it)
+        rows, bound = np.abs(u).reshape(b * s, -1, 32), bu.reshape(b * s, -1, 32)
+        most = (rows.max(-1, keepdims=True) * (1 / 3.5 + 2.0 ** -7) + 2 * bound.max(-1, keepdims=True))
+        err = np.abs(values(t["u8"], t["us"]) - u.reshape(-1, C)).reshape(rows.shape)
+        assert (err <= most).all()
+    else:
+        w = e4m3(blk.up.w8, blk.up.w_scale)
+        assert_gemm_close(f64(t["up"]), ol.gelu_tanh(e4m3(t["u8"], t["us"]) @ w.T + f64(blk.up.bias)))
+        d8, ds = ops.quant_rows(t["up"])
+        assert_gemm_close(f64(t["down"]).reshape(-1, C), e4m3(d8, ds) @ e4m3(blk.down.w8, blk.down.w_scale).T + f64(blk.down.bias))
+        # half a step of e4m3 (2^-4 relative, 2^-10 units below the normals) and of bf16
+        u2, bound = u.reshape(-1, C), bu.reshape(-1, C)
+        unit = np.abs(u2).max(-1, keepdims=True) / 448 * (1 + 2.0 ** -7)
+        err = np.abs(e4m3(t["u8"], t["us"]) - u2)
+        assert (err <= (np.abs(u2) + bound) * (2.0 ** -4 + 2.0 ** -7) + unit * 2.0 ** -9 + bound).all()
+    r2, y2, br2, by2 = ob.gated_residual_norm(f64(t["r"]), f64(t["down"]), gate2)
+    close(out, r2, br2, "last residual")
+    close(y, y2, by2, "last norm")
+
+
+@pytest.mark.parametrize("mlp4", [False, True])
+@torch.no_grad()
+def test_captured_run_replays(mlp4):
+    """Every replay equals the eager run on the inputs of the moment, with eager work in between."""
+    blk = Block(mlp4)
+    x, mod, table = inputs(1, 2, 300, 3)
+    other = inputs(2, 1, 40)
+    blk(x, mod, table), blk(*other)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = blk(x, mod, table)
+    for seed in range(4):
+        nx, nmod, _ = inputs(10 + seed, 2, 300, 3)
+        x.copy_(nx), mod.copy_(nmod)
+        for t in got:
+            t.fill_(float("nan"))
+        graph.replay()
+        blk(*other)
+        torch.cuda.synchronize()
+        want = blk(x, mod, table)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), seed
+
+
+@torch.no_grad()
+def test_runs_on_two_streams_at_once():
+    blk = Block(True)
+    cases = [inputs(1, 2, 300, 3), inputs(2, 1, 777)]
+    want = [blk(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(blk(*cases[i]))
+    torch.cuda.synchronize()
+    for i, w in enumerate(want):
+        for g in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(g, w))
+
+
+@pytest.mark.parametrize("mlp4", [False, True])
+@pytest.mark.parametrize("dynamic", [False, True])
+@torch.no_grad()
+def test_compiled_run_is_one_graph_with_the_same_result(mlp4, dynamic):
+    """Through the shape kernels too ("aot_eager" plans the views after each op from them)."""
+    torch._dynamo.reset()
+    try:
+        blk = Block(mlp4)
+        run = torch.compile(blk, backend="aot_eager", fullgraph=True, dynamic=dynamic)
+        for case in (inputs(1, 2, 36), inputs(2, 2, 300)):
+            assert all(torch.equal(a, b) for a, b in zip(run(*case), blk(*case)))
+    finally:
+        torch._dynamo.reset()
+
+
+def _calls():
+    g = torch.Generator().manual_seed(3)
+    rn = lambda *s: torch.randn(s, generator=g).bfloat16().cuda()  # noqa: E731
+    qkv = rn(2, 9, 3, 4, 64)
+    q, k = (qkv[:, :, i].transpose(1, 2) for i in range(2))
+    table = rotary_table(torch.arange(27).view(9, 3).cuda(), (16, 8, 8))
+    x, w, b = rn(2, 9, 288), rn(40, 288), rn(40)
+    x4, xs = quantize_mxfp4(x.view(18, 288))
+    w4, ws = quantize_mxfp4(w)
+    return {
+        "rotary_table": [(torch.arange(12).view(2, 2, 3).cuda(), [4, 6, 2], 1e4), (rn(5, 1).float(), [8], 1e3)],
+        "rotate_qk": [(q, k, table, None, None, 1e-6, True), (q, None, table, rn(64), None, 1e-6, False),
+                      (q, k[:, :1].expand(2, 3, 9, 64), table, None, rn(64), 1e-6, True),
+                      (q.transpose(2, 3).contiguous().transpose(2, 3), k.contiguous(), table, None, None, 1e-6, True)],
+        "gated_residual_norm": [(x, x, x[:, :1], x[:, :1], x[:, :1], None, None, True, 1e-6, 1.0, n, y)
+                                for n in (N.QUANT_NONE, N.QUANT_E4M3, N.QUANT_MXFP4) for y in (False, True)]
+        + [(x.transpose(0, 1), None, None, None, None, None, None, False, 1e-6, 1.0, N.QUANT_NONE, True)],
+        "mxfp4_quant": [(x.view(18, 288),), (x.view(18, 288)[::2, 32:],), (x.view(288, 18).t(),)],
+        "mxfp4_dequant": [(x4, xs, dt) for dt in (torch.bfloat16, torch.float16, torch.float32)],
+        "gemm_mxfp4": [(x4, w4, xs, ws, b, 1), (x4, w4, xs, ws, None, 0)],
+        "mxfp4_linear": [(x.view(18, 288), w4, ws, b, 1), (x.view(18, 288).float(), w4, ws, None, 0)],
+    }
+
+
+@pytest.mark.parametrize("op", ["rotary_table", "rotate_qk", "gated_residual_norm", "mxfp4_quant", "mxfp4_dequant",
+                                "gemm_mxfp4", "mxfp4_linear"])
+def test_declarations(op):
+    """What the schema and the shape kernel say (shapes, strides, types, nothing written in place or aliased) is what
+    the native kernel does; it has no derivative and says so; a batch under vmap is the calls one by one."""
+    call = getattr(ops, op)
+    for args in _calls()[op]:
+        torch.library.opcheck(getattr(torch.ops.mxf8, op).default, args, test_utils=("test_schema", "test_faketensor"))
+        real = call(*args)
+        first = args[0]
+        if first.is_floating_point():
+            got = call(first.clone().requires_grad_(), *args[1:])
+            for t in got if isinstance(got, tuple) else (got,):
+                assert t.requires_grad == t.is_floating_point()
+                if t.requires_grad:
+                    with pytest.raises(RuntimeError, match="no autograd formula"):
+                        t.float().sum().backward()
+        if op in ("mxfp4_quant", "mxfp4_linear", "rotary_table"):
+            batch = torch.vmap(lambda t: call(t, *args[1:]))(torch.stack([first, first + 1]))
+            for i, t in enumerate((first, first + 1)):
+                want = call(t, *args[1:])
+                pairs = zip(batch, want) if isinstance(want, tuple) else ((batch, want),)
+                assert all(torch.equal(a[i], b) for a, b in pairs)
+        with torch.inference_mode():
+            again = call(*args)
+        pairs = zip(again, real) if isinstance(real, tuple) else ((again, real),)
+        as_bytes = lambda t: t.contiguous().view(torch.uint8)  # noqa: E731
+        assert all(torch.equal(as_bytes(a), as_bytes(b)) for a, b in pairs)
+
+
+@pytest.mark.parametrize("lora", [False, True])
+def test_the_module_refuses_its_backward(lora):
+    """With adapters too, whose own products could be differentiated: half a gradient is none."""
+    mod = MXFP4Linear.from_linear(nn.Linear(64, 32, device="cuda", dtype=torch.bfloat16))
+    x = torch.randn(5, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    if lora:
+        mod.adapters.append((x.new_zeros(16, 64).detach(), x.new_zeros(32, 16).detach(), 1.0))
+    y = mod(x)
+    assert y.requires_grad
+    with pytest.raises(RuntimeError, match="no autograd formula"):
+        y.float().sum().backward()
+    with torch.no_grad():
+        assert not mod(x).requires_grad
+
+
+def test_large_operands_off_16_byte_boundaries():
+    """Past the size from which the quantizer streams, from an address and rows of two bytes' alignment."""
+    base = torch.randn(6000 * 3073 + 1, generator=torch.Generator().manual_seed(5)).bfloat16().cuda()
+    x = base[1:].view(6000, 3073)[:, 1:]
+    got, want = quantize_mxfp4(x), quantize_mxfp4(x.contiguous())
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
