@@ -251,6 +251,10 @@ __global__ __launch_bounds__(256) void rotate_qk_kernel(const RotArgs a) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) y[i] = f[i] * co[i] + q[i] * si[i];
         }
+        if (2 * a.P < a.D) {  // what passes through does so as it is: 0 times an infinity would make it NaN
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = c0 + i < 2 * a.P ? y[i] : f[i];
+        }
         Raw8<DT> w;
         w.set(y);
         if (there && (st + u + 1 < a.steps[p] || hg < in_last)) {

@@ -123,6 +123,24 @@ def test_non_finite_values_stay_in_their_head():
     assert torch.isfinite(o[~bad]).all() and o[0, 1, 2].isnan().all() and not torch.isfinite(o[0, 2, 0, 6:8]).any()
 
 
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("d,p", [(64, 24), (64, 20), (96, 40), (96, 37), (50, 20), (128, 0), (520, 200)])
+def test_channels_that_pass_through_are_untouched(d, p, dtype, interleaved):
+    """Bit for bit, infinities and negative zeros too, and nothing of them in the channels that turn."""
+    q, k, table, _, _ = make(d, 1, 9, 3, 2, d, p, dtype, False, False)
+    q, k = q.contiguous(), k.contiguous()
+    for x in (q, k):
+        x[..., 2 * p:: 3] = -0.0
+        x[..., 2 * p + 1:: 5] = float("inf")
+        x[..., 2 * p + 2:: 7] = float("nan")
+    for x, o in zip((q, k), rotate_qk(q, k, table, interleaved=interleaved)):
+        bits = torch.int32 if dtype == "fp32" else torch.int16
+        nan = x.isnan()
+        same = (o.view(bits) == x.view(bits)) | (o.isnan() & nan)
+        assert same[..., 2 * p:].all() and torch.isfinite(o[..., : 2 * p]).all()
+
+
 def test_zero_heads_and_zero_tokens():
     q, k, table, qw, kw = make(5, 1, 0, 3, 1, 64, 32, "bf16", True, False)
     qo, ko = rotate_qk(q, k, table, qw, kw)
