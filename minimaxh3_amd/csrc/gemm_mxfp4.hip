@@ -294,8 +294,11 @@ static void launch_mxfp4_few(int pick, int act, const void* x, int64_t ldx, cons
         MXF8_ROWS(1, 1, 8);
       break;
     case MX_ROWS16_16: MXF8_ROWS(1, 1, 16); break;
+    case MX_ROWS32x32:
+      if constexpr (XT == MX_CODES) MXF8_ROWS(2, 2, 8);
+      break;
     default:
-      if constexpr (XT == MX_CODES) MXF8_ROWS(2, 1, 4);
+      if constexpr (XT == MX_CODES) MXF8_ROWS(2, 1, 8);
   }
 #undef MXF8_ROWS
 }

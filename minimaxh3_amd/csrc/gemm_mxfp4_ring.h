@@ -5,9 +5,9 @@
 // for FP8.  What bounds it is the chain of stages: a stage's copies are issued NS - 1 stages ahead, and its
 // fragments are read from LDS while the previous stage's products run.
 //
-// gemm_mxfp4_rows_kernel: a few tens of tokens.  Nothing is shared there but the activations, so no operand goes
-// through LDS and no wave waits for another: each of a workgroup's waves streams the weights of 16 channels
-// over its own slabs of K straight into fragments, and the partial sums meet in LDS at the end.
+// gemm_mxfp4_rows_kernel: products too small to give every compute unit a tile.  Little is shared there, so no
+// operand goes through LDS and no wave waits for another: each of a workgroup's waves streams the weights of
+// 16 or 32 channels over its own slabs of K straight into fragments, and the partial sums meet in LDS at the end.
 #pragma once
 
 #include "gemm_common.h"

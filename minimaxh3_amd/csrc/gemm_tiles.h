@@ -91,23 +91,28 @@ inline int gemm_pick(int64_t M, int64_t N, int64_t K, int64_t r, int cus) {
 
 // The kernel of an M x N x K product of 4-bit blocks (gemm_mxfp4.hip, gemm_mxfp4_ring.h).
 //
-// The rows kernel for 16 tokens always, for 32 up to 4608 channels, for 64 up to 2048 (past that a ring, which
-// reads the activations once for 64 channels, is faster).  It splits K over 4 to 16 waves, more where there are
-// few channels to give the chip work.  Else the fastest by gemm_time's estimates; its constants (start, time
-// per 256 elements of K with one and with two workgroups on a CU) are fitted to MI355X times, weights from
-// HBM, of 154 products with M 33-22515, N 64-12288 and K 512-12288, over which the choice takes 1.006 of the
-// best kernel's time each time, and with 1001 channels up to 1.37 (before their stores were vectors), else 1.07 at
-// worst.  128 x 128 tiles / ring / rows: 1 x 3072 x 3072 14.2 / 6.9 / 3.9 us, 1 x 3072 x 12288 48 / 19 / 8.5,
-// 513 x 3072 x 3072 15.3 / 9.3; 2048 x 3072 x 3072 20.0 with 128 x 128 tiles, 24.1 with 256 x 256.
+// The rows kernel up to 16 tokens; beyond, in workgroups of 32 tokens by 16 or 32 channels as long as there is a
+// compute unit for each: it splits K over 4 to 16 waves, so that no wave waits for another before the end, where the
+// ring's chain of stages would leave most of the chip idle.  (Past one workgroup per unit it reads too much from
+// L2: 64 x 4608 x 3072 9.9 us against the ring's 7.1.)  32 x 16 / 32 x 32 / fastest ring: 100 x 1024 x 3072 5.0 / 5.8 / 7.0,
+// 64 x 4096 x 3072 8.5 / 6.0 / 7.1, 17 x 6144 x 12288 20.4 / 14.8 / 20.2, 512 x 512 x 1024 5.5 / 3.9 / 4.2.
+//
+// Else the fastest by gemm_time's estimates; its constants (start, time per 256 elements of K with one and with two
+// workgroups on a CU) are fitted to MI355X times, weights from HBM, of 154 products with M 33-22515, N 64-12288 and
+// K 512-12288, over which the choice took 1.006 of the best such kernel's time, 1.07 at worst where the channels are a
+// multiple of 8.  128 x 128 tiles / ring / rows: 1 x 3072 x 3072 14.2 / 6.9 / 3.7 us, 1 x 3072 x 12288 48 / 19 / 8.1,
+// 513 x 3072 x 3072 15.3 / 8.9; 2048 x 3072 x 3072 20.0 with 128 x 128 tiles, 24.1 with 256 x 256.
 enum {
   MX_ROWS16_4, MX_ROWS16_8, MX_ROWS16_16, MX_ROWS32,
-  MX_RING_32x64, MX_RING_64x64, MX_RING_128x64, MX_RING_128x128, MX_TILE_128, MX_TILE_256
+  MX_RING_32x64, MX_RING_64x64, MX_RING_128x64, MX_RING_128x128, MX_TILE_128, MX_TILE_256,
+  MX_ROWS32x32
 };
 inline int mxfp4_pick(int64_t M, int64_t N, int64_t K, int cus) {
   if (M <= 16) return N > 5120 ? (K > 4096 ? MX_ROWS16_8 : MX_ROWS16_4) : K >= 8192 ? MX_ROWS16_16 : MX_ROWS16_8;
-  if ((M <= 32 && N <= 4608) || (M <= 64 && N <= 2048)) return MX_ROWS32;
   const int64_t ns = cdiv(K, 2 * GEMM_BK);
   auto tiles = [&](int bm, int bn) { return cdiv(M, bm) * cdiv(N, bn); };
+  if (tiles(32, 16) <= cus) return MX_ROWS32;
+  if (tiles(32, 32) <= cus) return MX_ROWS32x32;
   const float time[6] = {gemm_time(tiles(32, 64), cus, 2, ns, 2.6f, 0.37f, 0.60f, 0.0f),
                          gemm_time(tiles(64, 64), cus, 2, ns, 3.3f, 0.36f, 0.58f, 0.0f),
                          gemm_time(tiles(128, 64), cus, 2, ns, 2.85f, 0.50f, 0.94f, 0.0f),

@@ -39,7 +39,8 @@ def check_quant(x):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
-@pytest.mark.parametrize("m,k", [(1, 32), (1, 3072), (5, 96), (17, 288), (33, 4640), (130, 1056), (3, 12288), (6000, 3072)])
+@pytest.mark.parametrize("m,k", [(1, 32), (1, 3072), (5, 96), (17, 288), (33, 4640), (130, 1056), (3, 12288),
+                                 (6000, 3072)])
 def test_quantizer(m, k, dtype):
     check_quant(randn(m + k, m, k, dtype=DT[dtype]))
 
@@ -120,8 +121,9 @@ def test_product_of_many_tiles(m, n, k):
 
 @pytest.mark.parametrize("act", [0, 1])
 @pytest.mark.parametrize("m,n,k", [(1, 9216, 3072), (7, 1001, 288), (3, 64, 8224), (17, 130, 512), (33, 2100, 96),
-                                   (130, 4100, 800), (300, 4100, 320), (256, 9216, 2080), (513, 12288, 800),
-                                   (2100, 1001, 768), (4100, 4104, 256), (6000, 4100, 288)])
+                                   (33, 8200, 96), (70, 1999, 2080), (130, 4100, 800), (300, 4100, 320),
+                                   (256, 9216, 2080), (513, 12288, 800), (2100, 1001, 768), (4100, 4104, 256),
+                                   (6000, 4100, 288)])
 def test_every_kernel(m, n, k, act):
     """Each of the product's kernels (tests/test_mxfp4_tiles.py), with whole and cut stages and tiles, rows of
     outputs at any alignment."""
