@@ -265,10 +265,11 @@ template <int TM, int TN, int NW, int XT>
 static void launch_mxfp4_rows(int act, const void* x, int64_t ldx, const uint8_t* sa, const uint8_t* w4, const uint8_t* sw,
                               const uint16_t* bias, uint16_t* out, int M, int N, int Kb, int64_t ld_out, hipStream_t st) {
   const dim3 grid((unsigned)cdiv(N, 16 * TN), (unsigned)cdiv(M, 16 * TM));
+  const int lds = XT == MX_CODES ? 0 : M * mx_row_pitch((int)cdiv(Kb, GEMM_BK));
   const bool ktail = Kb % GEMM_BK != 0;
 #define MXF8_CASE(A, T)                                                                                             \
   if (act == A && ktail == T)                                                                                       \
-    gemm_mxfp4_rows_kernel<TM, TN, NW, A, T, XT><<<grid, 64 * NW, 0, st>>>(x, ldx, sa, w4, sw, bias, out, M, N, Kb, ld_out);
+    gemm_mxfp4_rows_kernel<TM, TN, NW, A, T, XT><<<grid, 64 * NW, lds, st>>>(x, ldx, sa, w4, sw, bias, out, M, N, Kb, ld_out);
   MXF8_CASE(MXF8_ACT_NONE, false)
   MXF8_CASE(MXF8_ACT_NONE, true)
   MXF8_CASE(MXF8_ACT_GELU_TANH, false)
@@ -283,16 +284,9 @@ static void launch_mxfp4_few(int pick, int act, const void* x, int64_t ldx, cons
                              hipStream_t st) {
 #define MXF8_ROWS(TM, TN, NW) \
   launch_mxfp4_rows<TM, TN, NW, XT>(act, x, ldx, sa, w4, sw, bias, out, M, N, Kb, ld_out, st)
-  // (quantizing for itself, a workgroup of 32 channels does so half as often, once there are many channels)
-  constexpr int WIDE = XT == MX_CODES ? 1 : 2;
   switch (pick) {
-    case MX_ROWS16_4: MXF8_ROWS(1, WIDE, 4); break;
-    case MX_ROWS16_8:
-      if (N > 5120)
-        MXF8_ROWS(1, WIDE, 8);
-      else
-        MXF8_ROWS(1, 1, 8);
-      break;
+    case MX_ROWS16_4: MXF8_ROWS(1, 1, 4); break;
+    case MX_ROWS16_8: MXF8_ROWS(1, 1, 8); break;
     case MX_ROWS16_16: MXF8_ROWS(1, 1, 16); break;
     case MX_ROWS32x32:
       if constexpr (XT == MX_CODES) MXF8_ROWS(2, 2, 8);
@@ -363,14 +357,14 @@ extern "C" int mxf8_gemm_mxfp4(const uint8_t* a4, const uint8_t* w4, const uint8
   return check_launch(what);
 }
 
-// Whether the product quantizes its activations itself: the rows kernel's tokens, in 16 bits, where the same
-// quantization in every workgroup costs little more than the launch it saves (and the host a launch).  MI355X, in
-// one launch / two, in a graph: 1 x 3072 x 3072 4.4 / 5.3 us, 16 x 3072 x 3072 6.2 / 6.6, 1 x 9216 x 3072 8.7 / 8.2,
-// 4 x 9216 x 3072 9.4 / 9.2, 1 x 6144 x 6144 9.0 / 9.5; past the limits 16 x 9216 x 3072 12.1 / 10.7, 1 x 3072 x 12288
-// 10.8 / 9.6.
+// Whether the product quantizes its activations itself: the rows kernel's tokens, in 16 bits, as long as what every
+// workgroup spends on it (M K elements, the first of them while the weights are on their way) is less than the launch
+// it saves (and the host a launch).  With more than one workgroup per compute unit the limit is lower.  MI355X, one
+// launch / two, in a graph: 1 x 3072 x 3072 3.5 / 5.2 us, 16 x 3072 x 3072 5.1 / 6.2, 1 x 9216 x 3072 6.4 / 8.3,
+// 8 x 9216 x 3072 8.9 / 9.8, 1 x 3072 x 12288 7.7 / 9.6, 1 x 12288 x 12288 16.6 / 19.3; past the limits
+// 12 x 9216 x 3072 10.6 / 9.7, 16 x 3072 x 6144 8.6 / 8.3.
 static bool mxfp4_one_launch(int64_t M, int64_t N, int64_t K, int dtype) {
-  if (M > 16 || dtype == MXF8_F32) return false;
-  return N * K <= (1 << 24) || (M <= 4 && N > 5120 && N * K <= 40000000);
+  return M <= 16 && dtype != MXF8_F32 && M * K <= (N > 4096 ? 32768 : 65536);
 }
 
 extern "C" int64_t mxf8_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
@@ -398,7 +392,7 @@ extern "C" int mxf8_mxfp4_linear(const void* x, int dtype, int64_t ldx, const ui
   }
   const int cus = device_cus();
   if (cus <= 0) return set_error(MXF8_ELAUNCH, "%s: the device's compute-unit count is unavailable", what);
-  const int pick = mxfp4_pick(M, N, K, cus);  // (up to 16 tokens: a rows kernel)
+  const int pick = mxfp4_pick(M, N, K, cus);  // a rows kernel
   const uint16_t* b16 = static_cast<const uint16_t*>(bias);
   uint16_t* o16 = static_cast<uint16_t*>(out);
 #define MXF8_CASE(DT)                                                                                                 \

@@ -269,13 +269,16 @@ __global__ __launch_bounds__(C::THREADS) void gemm_mxfp4_ring_kernel(const uint8
 // per instruction, 32 bytes and two scale bytes.  Wave w takes units w, w + NW, ..., up to four in flight.
 //
 // XT: the activations are codes and scales (MX_CODES), or 16-bit elements of that type, row stride ldx, which each
-// lane quantizes for itself (mx_quant_block), where that costs less than a launch of its own.
+// workgroup quantizes for itself into LDS, where that costs less than a launch of its own.
 constexpr int MX_CODES = -1;
 
 template <int T>
 __device__ __forceinline__ v4f mx_mma16(const v4i& a, const v4i& b, const v4f& c, uint32_t sa, uint32_t sb) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_wide(a), mx_wide(b), c, 4, 4, T, (int)sa, T, (int)sb);
 }
+
+// LDS bytes of one such row of nk slabs, and 16 more (rows of a multiple of 128 bytes would all start in one bank).
+__host__ __device__ constexpr int mx_row_pitch(int nk) { return nk * GEMM_BK + ((nk * MX_SLAB + 15) & ~15) + 16; }
 
 template <int TM, int TN, int NW, int ACT, bool KTAIL, int XT>
 __global__ __launch_bounds__(64 * NW) void gemm_mxfp4_rows_kernel(const void* __restrict__ x, int64_t ldx,
@@ -290,9 +293,10 @@ __global__ __launch_bounds__(64 * NW) void gemm_mxfp4_rows_kernel(const void* __
   const int r = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * 16 * TN, m0 = blockIdx.y * 16 * TM;
   const int nk = (Kb + GEMM_BK - 1) / GEMM_BK;
+  extern __shared__ __attribute__((aligned(16))) uint8_t xq[];  // activations quantized here: a row's codes, then its scales
+  const int pitch = mx_row_pitch(nk);
   // rows past the end are the last row again (not stored)
   const uint8_t *wp[TN], *swp[TN], *xp[TM], *sxp[TM];
-  const uint16_t* xe[TM];
 #pragma unroll
   for (int a = 0; a < TN; ++a) {
     const int row = min(n0 + 16 * a + r, N - 1);
@@ -306,18 +310,19 @@ __global__ __launch_bounds__(64 * NW) void gemm_mxfp4_rows_kernel(const void* __
       xp[b] = static_cast<const uint8_t*>(x) + (int64_t)row * Kb + 32 * g;
       sxp[b] = sa + (int64_t)row * MX_SLAB + 2 * g;
     } else {
-      xe[b] = static_cast<const uint16_t*>(x) + row * ldx + 64 * g;
+      xp[b] = xq + row * pitch + 32 * g;
+      sxp[b] = xq + row * pitch + nk * GEMM_BK + 2 * g;
     }
   }
   struct Operand {
     v4i c[2];
     uint32_t s;
   };
-  // blocks 2 g and 2 g + 1 of the slab; those past K are zero codes under a scale of 1
-  auto there = [&](int ks) { return KTAIL ? (Kb >> 4) - 8 * ks - 2 * g : 2; };
+  // blocks 2 g and 2 g + 1 of slab ks; those past K, in the last one, are zero codes under a scale of 1
   const v4i none = {0, 0, 0, 0};
-  auto load = [&](const uint8_t* p, const uint8_t* s, int n, Operand& o) {
-    if (n >= 2) {
+  auto load = [&](const uint8_t* p, const uint8_t* s, int ks, Operand& o) {
+    const int n = KTAIL && ks + 1 == nk ? (Kb >> 4) - 8 * ks - 2 * g : 2;
+    if (!KTAIL || ks + 1 < nk || n >= 2) {
       o.c[0] = *reinterpret_cast<const v4i*>(p);
       o.c[1] = *reinterpret_cast<const v4i*>(p + 16);
       o.s = *reinterpret_cast<const uint16_t*>(s);
@@ -333,23 +338,17 @@ __global__ __launch_bounds__(64 * NW) void gemm_mxfp4_rows_kernel(const void* __
   auto load_w = [&](int ks, Unit& u) {
 #pragma unroll
     for (int a = 0; a < TN; ++a)
-      load(wp[a] + (int64_t)ks * GEMM_BK, swp[a] + (int64_t)ks * N * MX_SLAB, there(ks), u.w[a]);
+      load(wp[a] + (int64_t)ks * GEMM_BK, swp[a] + (int64_t)ks * N * MX_SLAB, ks, u.w[a]);
   };
   auto load_x = [&](int ks, Unit& u) {
-    const int n = there(ks);
 #pragma unroll
     for (int b = 0; b < TM; ++b) {
       if constexpr (XT == MX_CODES) {
-        load(xp[b] + (int64_t)ks * GEMM_BK, sxp[b] + (int64_t)ks * M * MX_SLAB, n, u.x[b]);
+        load(xp[b] + (int64_t)ks * GEMM_BK, sxp[b] + (int64_t)ks * M * MX_SLAB, ks, u.x[b]);
       } else {
-        const uint16_t* p = xe[b] + (int64_t)ks * 2 * GEMM_BK;
-        MxElems e[2];
-        if (n >= 1) e[0].load(p);
-        if (n >= 2) e[1].load(p + MX_BLOCK);
-        u.x[b].c[0] = u.x[b].c[1] = none;
-        u.x[b].s = 0x7f7fu;
-        if (n >= 1) u.x[b].s = 0x7f00u | e[0].quantize<XT>(u.x[b].c[0]);
-        if (n >= 2) u.x[b].s = (u.x[b].s & 255u) | e[1].quantize<XT>(u.x[b].c[1]) << 8;
+        u.x[b].c[0] = *reinterpret_cast<const v4i*>(xp[b] + ks * GEMM_BK);
+        u.x[b].c[1] = *reinterpret_cast<const v4i*>(xp[b] + ks * GEMM_BK + 16);
+        u.x[b].s = *reinterpret_cast<const uint16_t*>(sxp[b] + ks * MX_SLAB);
       }
     }
   };
@@ -369,20 +368,64 @@ __global__ __launch_bounds__(64 * NW) void gemm_mxfp4_rows_kernel(const void* __
   };
   constexpr int DEPTH = NW == 16 ? 2 : 4;
   Unit u[DEPTH];
+  auto load_ahead = [&] {
 #pragma unroll
-  for (int d = 0; d < DEPTH; ++d)
-    if (wave + d * NW < nk) load_w(wave + d * NW, u[d]);
+    for (int d = 0; d < DEPTH; ++d)
+      if (wave + d * NW < nk) load_w(wave + d * NW, u[d]);
+  };
+  if constexpr (XT == MX_CODES) {
+    load_ahead();
 #pragma unroll
-  for (int d = 0; d < DEPTH; ++d)
-    if (wave + d * NW < nk) load_x(wave + d * NW, u[d]);
+    for (int d = 0; d < DEPTH; ++d)
+      if (wave + d * NW < nk) load_x(wave + d * NW, u[d]);
+  } else {
+    // A block per thread at a time, the first ones loaded before the weights: loads return in order, and what
+    // quantizing takes passes while the weights come.
+    constexpr int THREADS = 64 * NW, FIRST = 2;
+    const int per_row = nk * MX_SLAB, blocks = M * per_row;
+    MxElems e[FIRST];
+    auto source = [&](int i, int& row, int& kb) {
+      row = i / per_row;
+      kb = i - row * per_row;
+      return i < blocks && kb < Kb >> 4;
+    };
+    auto fetch = [&](int i, MxElems& to) {
+      int row, kb;
+      if (source(i, row, kb)) to.load(static_cast<const uint16_t*>(x) + row * ldx + kb * MX_BLOCK);
+    };
+    auto put = [&](int i, const MxElems& from) {
+      int row, kb;
+      const bool is = source(i, row, kb);
+      v4i c = none;
+      uint32_t byte = 127;  // blocks past K: zeros under a scale of 1
+      if (is) byte = from.template quantize<XT>(c);
+      if (i < blocks) {
+        *reinterpret_cast<v4i*>(xq + row * pitch + kb * 16) = c;
+        xq[row * pitch + nk * GEMM_BK + kb] = (uint8_t)byte;
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < FIRST; ++j) fetch(threadIdx.x + j * THREADS, e[j]);
+    __builtin_amdgcn_sched_barrier(0);
+    load_ahead();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < FIRST; ++j) put(threadIdx.x + j * THREADS, e[j]);
+    for (int i = threadIdx.x + FIRST * THREADS; i < blocks; i += THREADS) {
+      fetch(i, e[0]);
+      put(i, e[0]);
+    }
+    block_barrier();
+  }
   for (int ks = wave; ks < nk; ks += DEPTH * NW) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
       if (ks + d * NW < nk) {
+        if (XT != MX_CODES) load_x(ks + d * NW, u[d]);
         products(u[d]);
         if (ks + (d + DEPTH) * NW < nk) {
           load_w(ks + (d + DEPTH) * NW, u[d]);
-          load_x(ks + (d + DEPTH) * NW, u[d]);
+          if (XT == MX_CODES) load_x(ks + (d + DEPTH) * NW, u[d]);
         }
       }
     }

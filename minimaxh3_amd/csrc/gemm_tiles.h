@@ -93,9 +93,11 @@ inline int gemm_pick(int64_t M, int64_t N, int64_t K, int64_t r, int cus) {
 //
 // The rows kernel up to 16 tokens; beyond, in workgroups of 32 tokens by 16 or 32 channels as long as there is a
 // compute unit for each: it splits K over 4 to 16 waves, so that no wave waits for another before the end, where the
-// ring's chain of stages would leave most of the chip idle.  (Past one workgroup per unit it reads too much from
-// L2: 64 x 4608 x 3072 9.9 us against the ring's 7.1.)  32 x 16 / 32 x 32 / fastest ring: 100 x 1024 x 3072 5.0 / 5.8 / 7.0,
-// 64 x 4096 x 3072 8.5 / 6.0 / 7.1, 17 x 6144 x 12288 20.4 / 14.8 / 20.2, 512 x 512 x 1024 5.5 / 3.9 / 4.2.
+// ring's chain of stages would leave most of the chip idle.  (Past one workgroup per unit it reads too much from L2:
+// 64 x 4608 x 3072 9.9 us against the ring's 7.1.)  4 / 8 / 16 waves: 1 x 9216 x 3072 5.8 / 6.7 / 7.2 us,
+// 1 x 3072 x 12288 9.7 / 8.2 / 7.7, and 16 x 3072 x 3072, quantizing its activations too, 6.8 / 5.6 / 5.1.  32 x 16 /
+// 32 x 32 / fastest ring: 100 x 1024 x 3072 5.0 / 5.8 / 7.0, 64 x 4096 x 3072 8.5 / 6.0 / 7.1, 17 x 6144 x 12288
+// 20.4 / 14.8 / 20.2, 512 x 512 x 1024 5.5 / 3.9 / 4.2.
 //
 // Else the fastest by gemm_time's estimates; its constants (start, time per 256 elements of K with one and with two
 // workgroups on a CU) are fitted to MI355X times, weights from HBM, of 154 products with M 33-22515, N 64-12288 and
@@ -108,9 +110,12 @@ enum {
   MX_ROWS32x32
 };
 inline int mxfp4_pick(int64_t M, int64_t N, int64_t K, int cus) {
-  if (M <= 16) return N > 5120 ? (K > 4096 ? MX_ROWS16_8 : MX_ROWS16_4) : K >= 8192 ? MX_ROWS16_16 : MX_ROWS16_8;
   const int64_t ns = cdiv(K, 2 * GEMM_BK);
   auto tiles = [&](int bm, int bn) { return cdiv(M, bm) * cdiv(N, bn); };
+  if (M <= 16) {
+    if (tiles(16, 16) <= cus) return K > 2048 ? MX_ROWS16_16 : MX_ROWS16_8;
+    return K > 4096 ? MX_ROWS16_8 : MX_ROWS16_4;
+  }
   if (tiles(32, 16) <= cus) return MX_ROWS32;
   if (tiles(32, 32) <= cus) return MX_ROWS32x32;
   const float time[6] = {gemm_time(tiles(32, 64), cus, 2, ns, 2.6f, 0.37f, 0.60f, 0.0f),

@@ -7,11 +7,11 @@ breaks.  Outputs come from torch's caching allocator; launches go to the current
 
 The ops of the hot path (quant_rows, adaln_quant_rows, gemm_rowwise, lora_down,
 attn_quant_kv, attn_fwd_q) and of the rest of a DiT block (rotary_table, rotate_qk,
-gated_residual_norm, mxfp4_quant, mxfp4_dequant, gemm_mxfp4, mxfp4_linear) run as native dispatcher kernels (csrc/torch_ops.cpp), which are
-registered when this module is imported: the dispatcher reads an operator's kernels without
-a lock, so none may be added while another thread calls it.  Their Python bodies see only
-what has no native kernel: other devices, and a library built after the import.  The other
-ops call the C ABI from here.
+gated_residual_norm, mxfp4_quant, mxfp4_dequant, gemm_mxfp4, mxfp4_linear) run as native
+dispatcher kernels (csrc/torch_ops.cpp), which are registered when this module is imported:
+the dispatcher reads an operator's kernels without a lock, so none may be added while another
+thread calls it.  Their Python bodies see only what has no native kernel: other devices, and a
+library built after the import.  The other ops call the C ABI from here.
 """
 from __future__ import annotations
 
@@ -527,7 +527,7 @@ def _(a4, w4, sa, sw, bias, act):
 def mxfp4_linear(x: torch.Tensor, w4: torch.Tensor, sw: torch.Tensor, bias: torch.Tensor | None,
                  act: int) -> torch.Tensor:
     """gemm_mxfp4(*mxfp4_quant(x), ...) of x [M, K] bf16/fp16/fp32, bf16 [M, N], in one
-    dispatch (and one launch for a few tokens and a small weight)."""
+    dispatch (and one launch for a few tokens)."""
     return _native(x, "mxfp4_linear")(x, w4, sw, bias, act)
 
 

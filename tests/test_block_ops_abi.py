@@ -144,8 +144,8 @@ def test_mxfp4(lib):
     need = lib.mxf8_mxfp4_linear_workspace_bytes
     assert need(16, 96, 288, 0) == 0 and need(0, 96, 288, 0) == 0
     assert need(17, 96, 288, 0) == 17 * 144 + 2 * 17 * 8 and need(1, 96, 288, 2) == 144 + 16
-    assert need(1, 9216, 3072, 0) == 0 and need(5, 9216, 3072, 0) == 5 * (1536 + 12 * 8)
-    assert need(1, 3072, 12288, 0) == 6144 + 48 * 8 and need(1, 12288, 12288, 0) > 0
+    assert need(1, 9216, 3072, 0) == 0 and need(12, 9216, 3072, 0) == 12 * (1536 + 12 * 8)
+    assert need(1, 3072, 12288, 0) == 0 and need(6, 3072, 12288, 0) == 6 * (6144 + 48 * 8)
     refused(lib, linear(m=-1), "negative")
     refused(lib, linear(k=0), "multiple of 32")
     for null in ("x", "w", "sw", "out"):

@@ -142,8 +142,10 @@ def test_product_of_widely_scaled_blocks(m, n, k):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
-@pytest.mark.parametrize("m,n,k", [(1, 9216, 3072), (1, 3, 32), (5, 1001, 288), (16, 64, 8224), (16, 5200, 3072), (11, 5200, 4640), (2, 96, 288), (4, 5201, 288), (3, 6145, 6176), (17, 96, 544),
-                                   (600, 300, 96)])
+@pytest.mark.parametrize("m,n,k", [(1, 9216, 3072), (1, 3, 32), (5, 1001, 288), (16, 64, 8224), (16, 5200, 3072),
+                                   (11, 5200, 4640), (2, 96, 288), (4, 5201, 288), (3, 6145, 6176), (17, 96, 544),
+                                   (600, 300, 96), (16, 64, 4000), (12, 4001, 5280), (7, 5200, 4640), (1, 48, 65536),
+                                   (8, 100, 8192), (1, 33, 65568)])
 def test_linear_in_one_call_is_the_quantizer_and_the_product(m, n, k, dtype):
     x, w, b = randn(m, m, k, dtype=DT[dtype]), randn(n, n, k, std=0.05), randn(3, n)
     x[0, :32] = 0

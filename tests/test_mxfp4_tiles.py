@@ -41,7 +41,7 @@ def test_the_choice_is_close_to_the_fastest(pick):
 
 
 def test_few_tokens_go_to_the_rows_kernel(pick):
-    assert pick([(m, n, 3072) for m in (1, 16) for n in (1, 3072, 12288)]) == [1, 1, 0, 1, 1, 0]
+    assert pick([(m, n, 3072) for m in (1, 16) for n in (1, 3072, 12288)]) == [2, 2, 0, 2, 2, 0]
     assert pick([(1, 3072, 12288), (1, 12288, 12288), (32, 3072, 3072), (32, 9216, 3072), (64, 2048, 512)])[:3] == [2, 1, 3]
     assert pick([(32, 9216, 3072)])[0] >= 4 and pick([(64, 2048, 512)]) == [3] and pick([(65, 2048, 512)])[0] >= 4
 
