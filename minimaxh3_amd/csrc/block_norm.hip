@@ -77,13 +77,18 @@ constexpr int min_waves(int dt, int chunks, bool weights) {
 }
 
 // NT threads per row (64: four rows per block), NC chunks of 8 elements per thread, of which the last one alone may
-// lie past the row's end; with TAIL, the C % 8 elements behind the row's last whole chunk are one element each
-// of its first threads.  WEIGHTS: branch_weight or weight may be there.
+// lie past the row's end.  TAIL_BACK (C % 8 != 0): the row's last chunk starts 8 elements before its end instead; what
+// it shares with the chunk before it counts there, and is stored twice alike (10166 x 2730: 46.5 us, with the elements
+// behind the last whole chunk one by one 50.3; 2728 channels 45.8).  TAIL_SHORT (C < 8): one chunk of C
+// elements.  WEIGHTS: branch_weight or weight may be there.
 //
 // What bounds it is memory, as long as the loads do not wait for each other: an operand's chunks are loaded with
 // no condition between them (an absent operand is eight constants that every lane reads), the row's and the
-// gate's first, the modulation's before the sums.
-template <int DT, int NT, int NC, int QM, bool TAIL, bool WEIGHTS>
+// gate's first, the modulation's before the sums.  20280 x 3072 in bf16: 86-88 us, 498 MB at 5.7 TB/s, with e4m3 codes
+// 79 (5.5 TB/s), with mxfp4 codes 76 (5.4); with norms before and behind 90, 83 and 81.
+enum { TAIL_NONE, TAIL_BACK, TAIL_SHORT };
+
+template <int DT, int NT, int NC, int QM, int TAIL, bool WEIGHTS>
 __global__ __launch_bounds__(NT > 256 ? NT : 256, min_waves(DT, NC, WEIGHTS)) void block_norm_kernel(const BlockNormArgs a) {
   __shared__ float red[NT / 64];
   const int t = threadIdx.x % NT;
@@ -91,11 +96,14 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256, min_waves(DT, NC, WEIGHTS)) vo
   const int m = blockIdx.x * ((NT > 256 ? NT : 256) / NT) + wave;
   if (m >= a.M) return;  // (whole waves; whole blocks where a block is a row)
   const int b = m / a.S, s = m - b * a.S, span = s / a.span;
-  const int C = a.C, C8 = C & ~7;
-  auto at = [&](int c) { return 8 * (c * NT + t); };  // chunk c: elements [at, at + 8) of the row
-  const bool whole = at(NC - 1) < C8;                  // the last chunk is there
-  const int te = C8 + t;                               // the tail element
-  const bool tail = TAIL && te < C;
+  const int C = a.C;
+  const int at_last = 8 * ((NC - 1) * NT + t);
+  const bool whole = at_last < C;  // the last chunk is there
+  // chunk c: elements [at, at + 8) of the row, of which [lo, hi) of the last one are not another chunk's
+  const int back = TAIL == TAIL_BACK ? min(at_last, C - 8) : at_last;
+  const int lo = at_last - back, hi = TAIL == TAIL_SHORT ? C : 8;
+  auto at = [&](int c) { return c < NC - 1 ? 8 * (c * NT + t) : back; };
+  auto own = [&](int c, int i) { return TAIL == TAIL_NONE || c < NC - 1 || (i >= lo && i < hi); };
   typedef typename Elem<DT>::T T;
   const bool has_br = a.branch != nullptr, has_g = a.gate != nullptr, has_sh = a.shift != nullptr,
              has_sc = a.scale != nullptr;
@@ -116,7 +124,11 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256, min_waves(DT, NC, WEIGHTS)) vo
 #pragma unroll
     for (int c = 0; c < NC - 1; ++c) v[c].load_off(p, first + c * step);
     v[NC - 1].zero();
-    if (whole) v[NC - 1].load_off(p, first + (NC - 1) * step);
+    if (TAIL == TAIL_SHORT && there) {
+      if (whole) v[NC - 1].load_part(p, 0, hi);
+    } else if (whole) {
+      v[NC - 1].load_off(p, TAIL == TAIL_BACK ? (there ? back * sizeof(T) : 0) : first + (NC - 1) * step);
+    }
   };
   // The scheduler fills waits with whatever follows, and unpacking the operands of a later phase early costs it
   // the registers of four waves.
@@ -128,29 +140,22 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256, min_waves(DT, NC, WEIGHTS)) vo
   load(xv, x, true);
   load(bv, br, has_br);
   load(gv, g, has_g);
-  float rt = 0.0f, bt = 0.0f, gt = 1.0f;
-  if (tail) {
-    rt = load1<DT>(x, te) * a.residual_scale;
-    if (has_br) bt = load1<DT>(br, te);
-    if (has_g) gt = load1<DT>(g, te);
-  }
   Raw8<DT> wv[WEIGHTS ? NC : 1];
   float post = 1.0f;
   if constexpr (WEIGHTS) {
     load(wv, bw, has_bw);
     if (has_bw) {
-      float ss = bt * bt;
+      float ss = 0.0f;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         float f[8];
         bv[c].get(f);
         bv[c].hide();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(f[i], f[i], ss);
+        for (int i = 0; i < 8; ++i) ss = own(c, i) ? __builtin_fmaf(f[i], f[i], ss) : ss;
         __builtin_amdgcn_sched_barrier(0);
       }
       post = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(row_sum<NT>(ss, red), (float)C) + a.eps));
-      if (tail) bt *= post * load1<DT>(bw, te);
     }
   }
   float r[NC][8];
@@ -170,29 +175,33 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256, min_waves(DT, NC, WEIGHTS)) vo
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       r[c][i] = __builtin_fmaf(h[i], u[i], f[i] * a.residual_scale);
-      sum += r[c][i];
+      sum += own(c, i) ? r[c][i] : 0.0f;
     }
     __builtin_amdgcn_sched_barrier(0);
   }
-  rt = __builtin_fmaf(gt, bt, rt);
-  sum += rt;
   // the next norm's modulation, in flight over the sums
   phase();
   Raw8<DT> sv[NC], hv[NC];
   load(sv, sc, has_sc);
   load(hv, sh, has_sh);
+  auto put = [&](const Raw8<DT>& o, void* to, int c) {
+    if (c == NC - 1 && !whole) return;
+    if (TAIL == TAIL_SHORT)
+      o.store_part(to, ro, hi);
+    else
+      o.stream(to, ro + at(c));
+  };
   if (has_br) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       Raw8<DT> o;
       o.set(r[c]);
-      if (c < NC - 1 || whole) o.stream(a.r, ro + at(c));
+      put(o, a.r, c);
     }
-    if (tail) store1<DT>(a.r, ro + te, rt);
   }
   phase();
   const float mean = a.layer ? __fdiv_rn(row_sum<NT>(sum, red), (float)C) : 0.0f;
-  float ss = tail ? (rt - mean) * (rt - mean) : 0.0f;
+  float ss = 0.0f;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
 #pragma unroll
@@ -202,7 +211,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256, min_waves(DT, NC, WEIGHTS)) vo
       for (int i = 0; i < 8; ++i) r[c][i] = 0.0f;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(r[c][i], r[c][i], ss);
+    for (int i = 0; i < 8; ++i) ss = own(c, i) ? __builtin_fmaf(r[c][i], r[c][i], ss) : ss;
   }
   const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(row_sum<NT>(ss, red), (float)C) + a.eps));
   phase();
@@ -225,21 +234,13 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256, min_waves(DT, NC, WEIGHTS)) vo
     for (int i = 0; i < 8; ++i) r[c][i] = __builtin_fmaf(r[c][i], 1.0f + f[i], h[i]);
     Raw8<DT> o;
     o.set(r[c]);
-    if ((QM == MXF8_QUANT_NONE || a.y) && (c < NC - 1 || whole)) o.stream(a.y, ro + at(c));
+    if (QM == MXF8_QUANT_NONE || a.y) put(o, a.y, c);
     if constexpr (QM != MXF8_QUANT_NONE) o.get(r[c]);  // y as it is stored (0 past the row's end)
     if constexpr (QM == MXF8_QUANT_E4M3) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(r[c][i]));
+      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, TAIL == TAIL_SHORT && i >= hi ? 0.0f : fabsf(r[c][i]));
     }
     __builtin_amdgcn_sched_barrier(0);
-  }
-  if (tail) {
-    rt = (rt - mean) * rstd;
-    if (WEIGHTS && has_w) rt *= load1<DT>(w, te);
-    rt = __builtin_fmaf(rt, 1.0f + (has_sc ? load1<DT>(sc, te) : 0.0f), has_sh ? load1<DT>(sh, te) : 0.0f);
-    if (QM == MXF8_QUANT_NONE || a.y) store1<DT>(a.y, ro + te, rt);
-    rt = round1<DT>(rt);
-    amax = fmaxf(amax, fabsf(rt));
   }
   if constexpr (QM == MXF8_QUANT_E4M3) {
     const float s8 = e4m3_scale(row_max<NT>(amax, red));
@@ -251,12 +252,16 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256, min_waves(DT, NC, WEIGHTS)) vo
       for (int i = 0; i < 8; ++i) f[i] = clamp448(div_by_scale(r[c][i], s8, inv));
       struct __attribute__((packed, aligned(1))) W2 {
         uint32_t w[2];
-      };
-      if (c < NC - 1 || whole)
-        *reinterpret_cast<W2*>(a.codes + ro + at(c)) =
-            W2{{cvt4_e4m3(f[0], f[1], f[2], f[3]), cvt4_e4m3(f[4], f[5], f[6], f[7])}};
+      } const q = {{cvt4_e4m3(f[0], f[1], f[2], f[3]), cvt4_e4m3(f[4], f[5], f[6], f[7])}};
+      if (c == NC - 1 && !whole) continue;
+      if constexpr (TAIL == TAIL_SHORT) {
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+          if (i < hi) a.codes[ro + i] = (uint8_t)(q.w[i >> 2] >> (8 * (i & 3)));
+      } else {
+        *reinterpret_cast<W2*>(a.codes + ro + at(c)) = q;
+      }
     }
-    if (tail) a.codes[ro + te] = (uint8_t)(cvt2_e4m3(clamp448(div_by_scale(rt, s8, inv)), 0.0f) & 0xff);
     if (t == 0) a.row_scale[m] = s8;
   }
   if constexpr (QM == MXF8_QUANT_MXFP4) {
@@ -278,20 +283,26 @@ static void launch_block_norm_nc(const BlockNormArgs& a, hipStream_t st) {
   const bool weights = a.branch_weight || a.weight;
   if constexpr (QM != MXF8_QUANT_MXFP4) {
     if (a.C % 8) {
-      block_norm_kernel<DT, NT, NC, QM, true, true><<<grid, block, 0, st>>>(a);
+      if constexpr (NT == 64 && NC == 1) {
+        if (a.C < 8) {
+          block_norm_kernel<DT, NT, NC, QM, TAIL_SHORT, true><<<grid, block, 0, st>>>(a);
+          return;
+        }
+      }
+      block_norm_kernel<DT, NT, NC, QM, TAIL_BACK, true><<<grid, block, 0, st>>>(a);
       return;
     }
   }
   if (weights)
-    block_norm_kernel<DT, NT, NC, QM, false, true><<<grid, block, 0, st>>>(a);
+    block_norm_kernel<DT, NT, NC, QM, TAIL_NONE, true><<<grid, block, 0, st>>>(a);
   else
-    block_norm_kernel<DT, NT, NC, QM, false, false><<<grid, block, 0, st>>>(a);
+    block_norm_kernel<DT, NT, NC, QM, TAIL_NONE, false><<<grid, block, 0, st>>>(a);
 }
 
 template <int DT, int QM>
 static int launch_block_norm(const BlockNormArgs& a, hipStream_t st) {
-  // whole chunks of a row (with mxfp4, of the padded row whose scale bytes are written), one for a shorter row
-  int64_t chunks = a.C / 8 > 0 ? a.C / 8 : 1;
+  // chunks of a row (with mxfp4, of the padded row whose scale bytes are written)
+  int64_t chunks = cdiv(a.C, 8);
   if (QM == MXF8_QUANT_MXFP4) chunks = mx_slabs(a.C) * MX_BLOCK * MX_SLAB / 8;
   // One wave per row where a lane has two chunks at most, or up to six (three in fp32) once there are rows for every
   // wave that fits; else four waves per row, whose parts of a row wait for each other at the sums but load it

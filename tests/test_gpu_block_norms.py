@@ -41,7 +41,7 @@ def check(a, dtype, norm, rs=1.0, eps=1e-6):
 
 SHAPES = [(1, 1, 3072), (2, 3, 3072), (1, 2, 1), (2, 5, 7), (1, 3, 8), (3, 4, 33), (1, 6, 512), (1, 3, 2730),
           (1, 2, 4096), (1, 2, 4104), (2, 2, 8192), (1, 1, 12288), (1, 1, 16384), (1, 1, 16383), (1, 4099, 72),
-          (1, 4097, 96), (1, 4200, 1000)]
+          (1, 4097, 96), (1, 4200, 1000), (1, 9000, 9), (1, 8200, 515)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
@@ -113,7 +113,7 @@ def test_quantized_outputs_are_the_quantizers_of_y(b, s, c, dtype):
         assert torch.equal(scales, want[1])
 
 
-@pytest.mark.parametrize("c", [33, 2730, 1001])
+@pytest.mark.parametrize("c", [1, 5, 7, 9, 15, 33, 1001, 2730, 4099, 16383])
 def test_e4m3_codes_of_odd_widths(c):
     a = make(c, 2, 5, c, "bf16")
     _, y = gated_residual_norm(**a)
