@@ -366,8 +366,8 @@ int64_t mxf8_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int d
 
 /*
  * mxf8_mxfp4_quant of x [M, K] (`dtype`, row stride ldx, any alignment) followed by mxf8_gemm_mxfp4, the same
- * output bit for bit; for a few tokens of 16-bit elements and weights that are not too many in one launch, in
- * which the product quantizes its activations itself.
+ * output bit for bit; for a few tokens of 16-bit elements in one launch, in which the product quantizes its
+ * activations itself.
  *   workspace: mxf8_mxfp4_linear_workspace_bytes(M, N, K, dtype) bytes, 16-byte aligned (NULL where that is 0)
  */
 int mxf8_mxfp4_linear(const void* x, int dtype, int64_t ldx, const uint8_t* w4, const uint8_t* sw, const void* bias,

@@ -9,6 +9,13 @@
 // of its row, one per instruction: any assignment of K to lanes and instructions gives the same sum as long as
 // both operands follow it, and with this one the four scales that a lane needs in a stage are one aligned dword
 // of the slab's eight bytes per row, which the instruction picks bytes from.
+//
+// What bounds it: a stage of a 256 x 256 tile is 2048 cycles of products and takes about 3600, with the fragment reads
+// (LDS active 30% of the time) and the copies on LDS's one port beside them, at a clock that the power limit holds at
+// 1.7-1.9 GHz; an epilogue takes 9300 cycles a tile.  20280 tokens: 3072 -> 12288 428 us (3580 TFLOP/s; the FP8 GEMM
+// 600) and 433 with GELU, 12288 -> 3072 369 (4150; 590), 3072 -> 3072 106; 8192^3 257 us, 4280 TFLOP/s.
+// Measured and not kept: four waves of 128 x 128 (spills), W fragments a step ahead too, a barrier in the middle of a
+// stage's products, raised wave priority around them.
 #include "gemm_common.h"
 #include "gemm_mxfp4_ring.h"
 #include "mxfp4.h"

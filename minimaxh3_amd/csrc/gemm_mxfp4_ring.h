@@ -3,11 +3,15 @@
 //
 // gemm_mxfp4_ring_kernel: one small tile per workgroup, stages of K in a deep LDS ring, as gemm_ring.h has it
 // for FP8.  What bounds it is the chain of stages: a stage's copies are issued NS - 1 stages ahead, and its
-// fragments are read from LDS while the previous stage's products run.
+// fragments are read from LDS while the previous stage's products run.  513 x 3072 x 3072 8.9-10.7 us, a stage of a 128 x 64
+// tile about 1050 cycles, of which LDS serves reads and copies for 700.  Rings twice as deep (9.4), two or three stages
+// to a barrier (10.4, 9.6) and waves of 64 x 32 outputs (10.9) were slower.
 //
 // gemm_mxfp4_rows_kernel: products too small to give every compute unit a tile.  Little is shared there, so no
 // operand goes through LDS and no wave waits for another: each of a workgroup's waves streams the weights of
 // 16 or 32 channels over its own slabs of K straight into fragments, and the partial sums meet in LDS at the end.
+// 1 x 9216 x 3072, activations quantized here, 6.1 us: 15.3 MB at 2.5 TB/s, the latency of two rounds of loads and of
+// the launch (1.9 us).
 #pragma once
 
 #include "gemm_common.h"
