@@ -12,6 +12,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
@@ -82,6 +83,12 @@ void on_device(const Tensor& t, at::Device dev, const char* what, const char* na
 
 Tensor empty(at::IntArrayRef sizes, const Tensor& like, at::ScalarType dt) {
   return at::empty(sizes, like.options().dtype(dt));
+}
+
+// The same straight from the caching allocator: a kernel that writes all of it and costs a few us should not go through
+// the dispatcher for each output.
+Tensor fresh(at::IntArrayRef sizes, const Tensor& like, at::ScalarType dt) {
+  return at::detail::empty_cuda(sizes, dt, like.device(), std::nullopt);
 }
 
 constexpr auto kE4M3 = at::kFloat8_e4m3fn;
@@ -309,7 +316,7 @@ Tensor rotary_table(const Tensor& positions, at::IntArrayRef axis_dims, double t
   std::vector<int64_t> shape(positions.sizes().begin(), positions.sizes().end() - 1);
   shape.push_back(pairs);
   shape.push_back(2);
-  Tensor table = empty(shape, pos, at::kFloat);
+  Tensor table = fresh(shape, pos, at::kFloat);
   const c10::DeviceGuard guard(pos.device());
   check(mxf8_rotary_table(pos.data_ptr(), type, axes ? pos.numel() / axes : 0, axes, axis_dims.data(), theta,
                           table.data_ptr<float>(), stream_of(pos)),
@@ -353,7 +360,7 @@ std::tuple<Tensor, Tensor> rotate_qk(const Tensor& q_in, const optional<Tensor>&
   check_weight(q_weight, D, q_in, what, "q_weight");
   check_weight(k_weight, D, q_in, what, "k_weight");
   const Tensor q = rows_of(q_in), k = k_in ? rows_of(*k_in) : Tensor();
-  Tensor qo = at::empty_like(q), ko = k_in ? at::empty_like(k) : empty({0}, q, q.scalar_type());
+  Tensor qo = at::empty_like(q), ko = k_in ? at::empty_like(k) : fresh({0}, q, q.scalar_type());
   if (qo.stride(3) != 1) qo = at::empty(q.sizes(), q.options());
   if (k_in && ko.stride(3) != 1) ko = at::empty(k.sizes(), k.options());
   const int64_t P = table.size(-2);
@@ -415,19 +422,19 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_residual_norm(
   };
   const ModRows g = rows(gate, "gate"), sh = rows(shift, "shift"), sc = rows(scale, "scale");
   const Tensor x = rows_of(x_in), br = branch_in ? rows_of(*branch_in) : Tensor();
-  Tensor r = empty(branch_in ? at::IntArrayRef{B, S, C} : at::IntArrayRef{0}, x, x.scalar_type());
+  Tensor r = fresh(branch_in ? at::IntArrayRef{B, S, C} : at::IntArrayRef{0}, x, x.scalar_type());
   const bool y_out = want_y || quant == MXF8_QUANT_NONE;
-  Tensor y = empty(y_out ? at::IntArrayRef{B, S, C} : at::IntArrayRef{0}, x, x.scalar_type());
+  Tensor y = fresh(y_out ? at::IntArrayRef{B, S, C} : at::IntArrayRef{0}, x, x.scalar_type());
   Tensor codes, scales;
   if (quant == MXF8_QUANT_E4M3) {
-    codes = empty({M, C}, x, kE4M3);
-    scales = empty({M, 1}, x, at::kFloat);
+    codes = fresh({M, C}, x, kE4M3);
+    scales = fresh({M, 1}, x, at::kFloat);
   } else if (quant == MXF8_QUANT_MXFP4) {
-    codes = empty({M, C / 2}, x, at::kByte);
-    scales = empty({cdiv(C, 256), M, 8}, x, at::kByte);
+    codes = fresh({M, C / 2}, x, at::kByte);
+    scales = fresh({cdiv(C, 256), M, 8}, x, at::kByte);
   } else {
-    codes = empty({0}, x, at::kByte);
-    scales = empty({0}, x, at::kByte);
+    codes = fresh({0}, x, at::kByte);
+    scales = fresh({0}, x, at::kByte);
   }
   const c10::DeviceGuard guard(dev);
   check(mxf8_gated_residual_norm(x.data_ptr(), x.stride(0), x.stride(1), branch_in ? br.data_ptr() : nullptr,
@@ -450,7 +457,7 @@ std::tuple<Tensor, Tensor> mxfp4_quant(const Tensor& x_in) {
   dtype_code(x_in);
   const Tensor x = x_in.stride(1) != 1 || x_in.stride(0) < x_in.size(1) ? x_in.contiguous() : x_in;
   const int64_t M = x.size(0), K = x.size(1);
-  Tensor codes = empty({M, K / 2}, x, at::kByte), scales = empty({cdiv(K, 256), M, 8}, x, at::kByte);
+  Tensor codes = fresh({M, K / 2}, x, at::kByte), scales = fresh({cdiv(K, 256), M, 8}, x, at::kByte);
   const c10::DeviceGuard guard(x.device());
   check(mxf8_mxfp4_quant(x.data_ptr(), dtype_code(x), M, K, std::max(x.stride(0), K),
                          static_cast<uint8_t*>(codes.data_ptr()), static_cast<uint8_t*>(scales.data_ptr()),
@@ -475,7 +482,7 @@ void check_mxfp4(const Tensor& codes, const Tensor& scales, const char* what, co
 Tensor mxfp4_dequant(const Tensor& codes, const Tensor& scales, at::ScalarType dtype) {
   require_gfx950(codes, "mxfp4_dequant");
   check_mxfp4(codes, scales, "mxfp4_dequant: ", "x");
-  Tensor out = empty({codes.size(0), 2 * codes.size(1)}, codes, dtype);
+  Tensor out = fresh({codes.size(0), 2 * codes.size(1)}, codes, dtype);
   const c10::DeviceGuard guard(codes.device());
   check(mxf8_mxfp4_dequant(static_cast<const uint8_t*>(codes.data_ptr()), static_cast<const uint8_t*>(scales.data_ptr()),
                            out.size(0), out.size(1), out.data_ptr(), dtype_code(out), stream_of(codes)),
@@ -497,7 +504,7 @@ Tensor gemm_mxfp4(const Tensor& a4, const Tensor& w4, const Tensor& sa, const Te
   TORCH_CHECK_VALUE(!bias || (bias->scalar_type() == at::kBFloat16 && bias->numel() == N && bias->is_contiguous()), what,
                     "bias must be ", N, " contiguous bf16 values");
   if (bias) on_device(*bias, dev, what, "bias");
-  Tensor out = empty({M, N}, a4, at::kBFloat16);
+  Tensor out = fresh({M, N}, a4, at::kBFloat16);
   const c10::DeviceGuard guard(dev);
   check(mxf8_gemm_mxfp4(static_cast<const uint8_t*>(a4.data_ptr()), static_cast<const uint8_t*>(w4.data_ptr()),
                         static_cast<const uint8_t*>(sa.data_ptr()), static_cast<const uint8_t*>(sw.data_ptr()),
@@ -521,7 +528,7 @@ Tensor mxfp4_linear(const Tensor& x_in, const Tensor& w4, const Tensor& sw, cons
   const Tensor x = x_in.stride(1) != 1 || x_in.stride(0) < K ? x_in.contiguous() : x_in;
   const int dt = dtype_code(x);
   const int64_t M = x.size(0), ws = mxf8_mxfp4_linear_workspace_bytes(M, N, K, dt);
-  Tensor out = empty({M, N}, x, at::kBFloat16), work = ws ? empty({ws}, x, at::kByte) : Tensor();
+  Tensor out = fresh({M, N}, x, at::kBFloat16), work = ws ? fresh({ws}, x, at::kByte) : Tensor();
   const c10::DeviceGuard guard(dev);
   check(mxf8_mxfp4_linear(x.data_ptr(), dt, std::max(x.stride(0), K), static_cast<const uint8_t*>(w4.data_ptr()),
                           static_cast<const uint8_t*>(sw.data_ptr()), bias ? bias->data_ptr() : nullptr,
