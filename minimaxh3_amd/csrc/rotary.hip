@@ -105,28 +105,6 @@ struct RotArgs {
   float eps, inv_d;
 };
 
-// Sum over the L lanes that hold a head, in each of them.
-template <int L>
-__device__ __forceinline__ float head_sum(float v) {
-  auto dpp = [](float x, auto ctrl) {
-    return __builtin_bit_cast(
-        float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, true));
-  };
-  v += dpp(v, std::integral_constant<int, 0xb1>{});   // lane ^ 1
-  v += dpp(v, std::integral_constant<int, 0x4e>{});   // lane ^ 2
-  v += dpp(v, std::integral_constant<int, 0x141>{});  // the other half of eight
-  if constexpr (L >= 16) v += dpp(v, std::integral_constant<int, 0x140>{});  // the other half of sixteen
-  if constexpr (L >= 32) {
-    const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(x[0]) + __uint_as_float(x[1]);
-  }
-  if constexpr (L >= 64) {
-    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(x[0]) + __uint_as_float(x[1]);
-  }
-  return v;
-}
-
 // One wave per token and span of head steps: L lanes hold a head (8 channels each), so a step moves 64 / L heads,
 // 16 bytes a lane.  The token's cos / sin and the norm's weights stay in registers over the heads, and the
 // next ROT_UNROLL steps' loads are in flight together.
@@ -216,7 +194,7 @@ __global__ __launch_bounds__(256) void rotate_qk_kernel(const RotArgs a) {
           float ss = 0.0f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(f[i], f[i], ss);
-          const float r = rsqrtf(__builtin_fmaf(head_sum<L>(ss), a.inv_d, a.eps));
+          const float r = rsqrtf(__builtin_fmaf(lanes_sum<L>(ss), a.inv_d, a.eps));
           float k[8];
           wv.get(k);
 #pragma unroll

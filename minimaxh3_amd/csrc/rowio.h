@@ -141,24 +141,34 @@ struct Raw8<MXF8_F32> {
   }
 };
 
-// Wave-wide sum and maximum in every lane: four steps within rows of 16 lanes and two swaps of rows, all on
-// the vector unit (a shuffle goes through LDS, with some 100 cycles a step on a row's critical path).
-template <class F>
-__device__ __forceinline__ float wave_reduce_fast(float v, F f) {
+// f over the L (8 to 64, a power of two) neighbouring lanes that hold a row or a head, in every one of them: steps within
+// rows of 16 lanes and two swaps of rows, all on the vector unit (a shuffle goes through LDS, with some 100 cycles
+// a step on a row's critical path).
+template <int L, class F>
+__device__ __forceinline__ float lanes_reduce(float v, F f) {
+  static_assert(L == 8 || L == 16 || L == 32 || L == 64, "lanes of a group");
   v = f(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0xb1, 0xf, 0xf, true)));
   v = f(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x4e, 0xf, 0xf, true)));
   v = f(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x141, 0xf, 0xf, true)));
-  v = f(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x140, 0xf, 0xf, true)));
-  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  if constexpr (L >= 16)
+    v = f(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x140, 0xf, 0xf, true)));
+  if constexpr (L >= 32) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  }
+  if constexpr (L >= 64) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  }
+  return v;
 }
-__device__ __forceinline__ float wave_sum_fast(float v) {
-  return wave_reduce_fast(v, [](float a, float b) { return a + b; });
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
+  return lanes_reduce<L>(v, [](float a, float b) { return a + b; });
 }
-__device__ __forceinline__ float wave_max_fast(float v) {
-  return wave_reduce_fast(v, [](float a, float b) { return fmaxf(a, b); });
+template <int L>
+__device__ __forceinline__ float lanes_max(float v) {
+  return lanes_reduce<L>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
 // One element.

@@ -41,7 +41,8 @@ def check(a, dtype, norm, rs=1.0, eps=1e-6):
 
 SHAPES = [(1, 1, 3072), (2, 3, 3072), (1, 2, 1), (2, 5, 7), (1, 3, 8), (3, 4, 33), (1, 6, 512), (1, 3, 2730),
           (1, 2, 4096), (1, 2, 4104), (2, 2, 8192), (1, 1, 12288), (1, 1, 16384), (1, 1, 16383), (1, 4099, 72),
-          (1, 4097, 96), (1, 4200, 1000), (1, 9000, 9), (1, 8200, 515)]
+          (1, 4097, 96), (1, 4200, 1000), (1, 9000, 9), (1, 8200, 515),
+          (3, 43, 64), (2, 35, 120), (1, 37, 128), (1, 21, 250), (5, 17, 256), (1, 9, 257)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
@@ -96,7 +97,7 @@ def test_layouts():
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("b,s,c", [(1, 1, 3072), (2, 7, 96), (1, 4098, 288), (1, 3, 4640), (1, 2, 8192), (1, 2, 16384),
-                                   (2, 3, 32), (1, 4100, 4096)])
+                                   (2, 3, 32), (1, 4100, 4096), (3, 37, 160), (1, 45, 256), (1, 19, 64)])
 def test_quantized_outputs_are_the_quantizers_of_y(b, s, c, dtype):
     a = make(c, b, s, c, dtype, sandwich=c == 96, weighted=c == 288)
     a["x"][0, 0, :32] = 0
