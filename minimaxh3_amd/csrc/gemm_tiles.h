@@ -99,16 +99,26 @@ inline int gemm_pick(int64_t M, int64_t N, int64_t K, int64_t r, int cus) {
 // 32 x 32 / fastest ring: 100 x 1024 x 3072 5.0 / 5.8 / 7.0, 64 x 4096 x 3072 8.5 / 6.0 / 7.1, 17 x 6144 x 12288
 // 20.4 / 14.8 / 20.2, 512 x 512 x 1024 5.5 / 3.9 / 4.2.
 //
-// Else the fastest by gemm_time's estimates; its constants (start, time per 256 elements of K with one and with two
-// workgroups on a CU) are fitted to MI355X times, weights from HBM, of 154 products with M 33-22515, N 64-12288 and
-// K 512-12288, over which the choice took 1.006 of the best such kernel's time, 1.07 at worst where the channels are a
-// multiple of 8.  128 x 128 tiles / ring / rows: 1 x 3072 x 3072 14.2 / 6.9 / 3.7 us, 1 x 3072 x 12288 48 / 19 / 8.1,
-// 513 x 3072 x 3072 15.3 / 8.9; 2048 x 3072 x 3072 20.0 with 128 x 128 tiles, 24.1 with 256 x 256.
+// Else the fastest by mx_time's estimates; its constants are fitted to MI355X times of 230 products with M 34-21388,
+// N 64-12288 and K 32-12288, over which the choice took 1.003 of the best kernel's time, 1.06 at worst.
+// 128 x 128 tiles / ring / rows: 1 x 3072 x 3072 14.2 / 6.9 / 3.7 us, 1 x 3072 x 12288 48 / 19 / 7.7, 513 x 3072 x 3072
+// 15.3 / 8.9; 2048 x 3072 x 3072 19.5 with 128 x 128 tiles, 23.1 with 256 x 256.
 enum {
   MX_ROWS16_4, MX_ROWS16_8, MX_ROWS16_16, MX_ROWS32,
   MX_RING_32x64, MX_RING_64x64, MX_RING_128x64, MX_RING_128x128, MX_TILE_128, MX_TILE_256,
   MX_ROWS32x32
 };
+// Estimated time (us) as gemm_time's: t1 and t2 per 256 elements of K, `each` for every workgroup's epilogue, and
+// `early`, how much less than in a full round a CU's second workgroup costs where few CUs have one.
+inline float mx_time(int64_t tiles, int cus, int per_cu, int64_t ns, float start, float t1, float t2, float each,
+                     float early) {
+  const float one = t1 * (float)ns + each, two = t2 * (float)ns + 2.0f * each;
+  if (per_cu == 1) return start + (float)cdiv(tiles, cus) * one;
+  const int64_t full = tiles / (2 * cus), rem = tiles - full * 2 * cus;
+  return start + (float)full * two +
+         (rem == 0 ? 0.0f : rem <= cus ? one : two - early * (two - one) * (float)(2 * cus - rem) / (float)cus);
+}
+
 inline int mxfp4_pick(int64_t M, int64_t N, int64_t K, int cus) {
   const int64_t ns = cdiv(K, 2 * GEMM_BK);
   auto tiles = [&](int bm, int bn) { return cdiv(M, bm) * cdiv(N, bn); };
@@ -118,12 +128,12 @@ inline int mxfp4_pick(int64_t M, int64_t N, int64_t K, int cus) {
   }
   if (tiles(32, 16) <= cus) return MX_ROWS32;
   if (tiles(32, 32) <= cus) return MX_ROWS32x32;
-  const float time[6] = {gemm_time(tiles(32, 64), cus, 2, ns, 2.6f, 0.37f, 0.60f, 0.0f),
-                         gemm_time(tiles(64, 64), cus, 2, ns, 3.3f, 0.36f, 0.58f, 0.0f),
-                         gemm_time(tiles(128, 64), cus, 2, ns, 2.85f, 0.50f, 0.94f, 0.0f),
-                         gemm_time(tiles(128, 128), cus, 1, ns, 4.3f, 0.76f, 0.0f, 0.0f),
-                         gemm_time(tiles(128, 128), cus, 2, ns, 3.0f, 0.95f, 1.42f, 0.0f),
-                         gemm_time(tiles(256, 256), cus, 1, ns, 4.0f, 1.85f, 0.0f, 0.0f)};
+  const float time[6] = {mx_time(tiles(32, 64), cus, 2, ns, 2.22f, 0.37f, 0.43f, 0.98f, 0.52f),
+                         mx_time(tiles(64, 64), cus, 2, ns, 2.5f, 0.36f, 0.48f, 1.06f, 0.66f),
+                         mx_time(tiles(128, 64), cus, 2, ns, 2.75f, 0.40f, 0.79f, 1.28f, 0.29f),
+                         mx_time(tiles(128, 128), cus, 1, ns, 1.65f, 0.69f, 0.0f, 3.32f, 0.0f),
+                         mx_time(tiles(128, 128), cus, 2, ns, 3.35f, 0.91f, 1.27f, 1.65f, 0.63f),
+                         mx_time(tiles(256, 256), cus, 1, ns, -0.05f, 1.55f, 0.0f, 6.83f, 0.0f)};
   int best = 0;
   for (int i = 1; i < 6; ++i)
     if (time[i] < time[best]) best = i;

@@ -121,7 +121,7 @@ def test_product_of_many_tiles(m, n, k):
 
 @pytest.mark.parametrize("act", [0, 1])
 @pytest.mark.parametrize("m,n,k", [(1, 9216, 3072), (7, 1001, 288), (3, 64, 8224), (17, 130, 512), (33, 2100, 96),
-                                   (33, 8200, 96), (70, 1999, 2080), (130, 4100, 800), (300, 4100, 320),
+                                   (200, 2100, 800), (70, 1999, 2080), (130, 4100, 800), (300, 4100, 320),
                                    (256, 9216, 2080), (513, 12288, 800), (2100, 1001, 768), (4100, 4104, 256),
                                    (6000, 4100, 288)])
 def test_every_kernel(m, n, k, act):

@@ -19,7 +19,7 @@ TIMES = {
 }
 # kernels that the GPU tests' shapes are meant to reach
 SHAPES = {(1, 9216, 3072): 0, (7, 1001, 288): 1, (3, 64, 8224): 2, (17, 130, 512): 3, (33, 2100, 96): 10,
-          (33, 8200, 96): 4, (130, 4100, 800): 5, (300, 4100, 320): 6, (256, 9216, 2080): 7, (513, 12288, 800): 8, (2100, 1001, 768): 6,
+          (200, 2100, 800): 4, (130, 4100, 800): 5, (300, 4100, 320): 6, (256, 9216, 2080): 7, (513, 12288, 800): 8, (2100, 1001, 768): 6,
           (4100, 4104, 256): 8, (6000, 4100, 288): 9}
 
 
