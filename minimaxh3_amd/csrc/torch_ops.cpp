@@ -12,6 +12,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/ExpandUtils.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -89,6 +90,13 @@ Tensor empty(at::IntArrayRef sizes, const Tensor& like, at::ScalarType dt) {
 // the dispatcher for each output.
 Tensor fresh(at::IntArrayRef sizes, const Tensor& like, at::ScalarType dt) {
   return at::detail::empty_cuda(sizes, dt, like.device(), std::nullopt);
+}
+
+// As at::empty_like: the dimensions in x's memory order.
+Tensor fresh_like(const Tensor& x) {
+  const std::vector<int64_t> strides =
+      x.is_non_overlapping_and_dense() ? x.strides().vec() : at::infer_dense_strides(x.sizes(), x.strides());
+  return at::detail::empty_strided_cuda(x.sizes(), strides, x.scalar_type(), x.device());
 }
 
 constexpr auto kE4M3 = at::kFloat8_e4m3fn;
@@ -360,7 +368,7 @@ std::tuple<Tensor, Tensor> rotate_qk(const Tensor& q_in, const optional<Tensor>&
   check_weight(q_weight, D, q_in, what, "q_weight");
   check_weight(k_weight, D, q_in, what, "k_weight");
   const Tensor q = rows_of(q_in), k = k_in ? rows_of(*k_in) : Tensor();
-  Tensor qo = at::empty_like(q), ko = k_in ? at::empty_like(k) : fresh({0}, q, q.scalar_type());
+  Tensor qo = fresh_like(q), ko = k_in ? fresh_like(k) : fresh({0}, q, q.scalar_type());
   if (qo.stride(3) != 1) qo = at::empty(q.sizes(), q.options());
   if (k_in && ko.stride(3) != 1) ko = at::empty(k.sizes(), k.options());
   const int64_t P = table.size(-2);
