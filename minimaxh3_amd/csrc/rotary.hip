@@ -105,6 +105,10 @@ struct RotArgs {
   float eps, inv_d;
 };
 
+// a x + b y.  Which product the compiler fuses with the sum is its choice at every place, and with it the last bit:
+// written out, a token's result does not depend on where in the unrolled steps its head falls.
+__device__ __forceinline__ float turn(float a, float x, float b, float y) { return __builtin_fmaf(a, x, b * y); }
+
 // One wave per token and span of head steps: L lanes hold a head (8 channels each), so a step moves 64 / L heads,
 // 16 bytes a lane.  The token's cos / sin and the norm's weights stay in registers over the heads, and the
 // next ROT_UNROLL steps' loads are in flight together.
@@ -223,12 +227,12 @@ __global__ __launch_bounds__(256) void rotate_qk_kernel(const RotArgs a) {
         if constexpr (INTERLEAVED) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            y[2 * i] = f[2 * i] * co[i] - f[2 * i + 1] * si[i];
-            y[2 * i + 1] = f[2 * i] * si[i] + f[2 * i + 1] * co[i];
+            y[2 * i] = turn(f[2 * i], co[i], f[2 * i + 1], -si[i]);
+            y[2 * i + 1] = turn(f[2 * i], si[i], f[2 * i + 1], co[i]);
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = f[i] * co[i] + q[i] * si[i];
+          for (int i = 0; i < 8; ++i) y[i] = turn(f[i], co[i], q[i], si[i]);
         }
         if (2 * a.P < a.D) {  // what passes through does so as it is: 0 times an infinity would make it NaN
 #pragma unroll
@@ -281,8 +285,8 @@ __global__ __launch_bounds__(256) void rotate_qk_any_kernel(const RotArgs a) {
     const int c0 = INTERLEAVED ? 2 * j : j, c1 = INTERLEAVED ? 2 * j + 1 : j + a.P;
     const float2 t = tab[j];
     const float u = get(c0), v = get(c1);
-    put(c0, u * t.x - v * t.y);
-    put(c1, u * t.y + v * t.x);
+    put(c0, turn(u, t.x, v, -t.y));
+    put(c1, turn(u, t.y, v, t.x));
   }
   for (int c = 2 * a.P + lane; c < a.D; c += 64) put(c, get(c));
 }

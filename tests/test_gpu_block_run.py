@@ -277,3 +277,47 @@ def test_large_operands_off_16_byte_boundaries():
     x = base[1:].view(6000, 3073)[:, 1:]
     got, want = quantize_mxfp4(x), quantize_mxfp4(x.contiguous())
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def _far(*shape):
+    """bf16 zeros with random last rows (dimension 1 of three or more, else 0)."""
+    x = torch.zeros(shape, dtype=torch.bfloat16, device="cuda")
+    end = x[:, -5:] if x.ndim > 2 else x[-5:]
+    end.copy_(torch.randn(end.shape, generator=torch.Generator().manual_seed(9)))
+    return x
+
+
+@torch.no_grad()
+def test_operands_past_32_bit_offsets():
+    """The last rows of operands of more than 2^31 elements, against the same rows alone (bit for bit)."""
+    n = 700_001
+    x = _far(n, C * 8)  # 2.15e9 elements
+    codes, scales = quantize_mxfp4(x)
+    c5, s5 = quantize_mxfp4(x[-5:])
+    assert torch.equal(codes[-5:], c5) and torch.equal(scales[:, -5:], s5)
+    assert torch.equal(ops.mxfp4_dequant(codes, scales, torch.bfloat16)[-5:], ops.mxfp4_dequant(c5, s5, torch.bfloat16))
+    x3 = x.view(1, n, C * 8)
+    for fmt in (None, "e4m3", "mxfp4"):
+        got = gated_residual_norm(x3, x3, quantize=fmt)
+        # (as many rows as take one wave each, as the whole does: four waves a row add in another order)
+        want = gated_residual_norm(x3[:, -9000:], x3[:, -9000:], quantize=fmt)
+        assert torch.equal(got[0][:, -5:], want[0][:, -5:])
+        if fmt == "mxfp4":
+            assert torch.equal(got[1][-5:], want[1][-5:]) and torch.equal(got[2][:, -5:], want[2][:, -5:])
+        else:
+            last = lambda t: (t[0] if fmt is None else t)[-5:].view(torch.uint8)  # noqa: E731
+            assert torch.equal(last(got[1]), last(want[1]))
+        del got
+    q = x.view(1, n, 24, D).transpose(1, 2)
+    table = torch.rand(n, 64, 2, device="cuda")
+    for halves in (True, False):
+        got = rotate_qk(q, None, table, interleaved=halves)[0][:, :, -5:]
+        assert torch.equal(got, rotate_qk(q[:, :, -5:], None, table[-5:].contiguous(), interleaved=halves)[0])
+    del x, x3, q, codes, scales, table, got
+    # one block of K: its products add without rounding, whatever kernel takes them
+    a, w = _far(180_001, 32), _far(12288, 32)
+    a4, sa = quantize_mxfp4(a)
+    w4, sw = quantize_mxfp4(w)
+    out = ops.gemm_mxfp4(a4, w4, sa, sw, None, 0)  # 2.2e9 elements
+    t4, ts = quantize_mxfp4(a[-5:])
+    assert out[-5:, -5:].any() and torch.equal(out[-5:], ops.gemm_mxfp4(t4, w4, ts, sw, None, 0))

@@ -141,6 +141,20 @@ def test_channels_that_pass_through_are_untouched(d, p, dtype, interleaved):
         assert same[..., 2 * p:].all() and torch.isfinite(o[..., : 2 * p]).all()
 
 
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("weights", [True, False])
+@pytest.mark.parametrize("d,p", [(128, 64), (96, 37)])
+def test_a_token_does_not_depend_on_the_others(d, p, weights, interleaved):
+    """Bit for bit: few tokens split their heads over waves, many do not."""
+    q, k, table, qw, kw = make(4, 1, 3000, 24, 5, d, p, "bf16", weights, False)
+    qo, ko = rotate_qk(q, k, table, qw, kw, interleaved=interleaved)
+    for n in (1, 5, 80, 700):
+        for i in (0, 1500, 3000 - n):
+            part = rotate_qk(q[:, :, i: i + n], k[:, :, i: i + n], table[i: i + n].contiguous(), qw, kw,
+                             interleaved=interleaved)
+            assert torch.equal(part[0], qo[:, :, i: i + n]) and torch.equal(part[1], ko[:, :, i: i + n])
+
+
 def test_zero_heads_and_zero_tokens():
     q, k, table, qw, kw = make(5, 1, 0, 3, 1, 64, 32, "bf16", True, False)
     qo, ko = rotate_qk(q, k, table, qw, kw)
