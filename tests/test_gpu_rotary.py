@@ -155,6 +155,54 @@ def test_a_token_does_not_depend_on_the_others(d, p, weights, interleaved):
             assert torch.equal(part[0], qo[:, :, i: i + n]) and torch.equal(part[1], ko[:, :, i: i + n])
 
 
+def _apart(x, stride):
+    """x [B, H, S, D] as a view whose heads lie `stride` elements apart."""
+    b, h, s, d = x.shape
+    store = torch.empty((h - 1) * stride + b * s * d, dtype=x.dtype, device="cuda")
+    return store.as_strided((b, h, s, d), (s * d, stride, d, 1)).copy_(x)
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("weights", [True, False])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("b,s,hq,hk,d,p", [(2, 9, 5, 3, 128, 64), (1, 37, 9, 1, 64, 24), (1, 5, 3, 2, 96, 37),
+                                           (2, 4, 3, 1, 50, 25), (1, 3, 2, 2, 256, 128), (1, 3, 2, 1, 72, 36)])
+def test_heads_far_apart(b, s, hq, hk, d, p, dtype, weights, interleaved):
+    """The values, bit for bit, that heads which are neighbours get."""
+    q, k, table, qw, kw = make(d + s, b, s, hq, hk, d, p, dtype, weights, False)
+    want = rotate_qk(q, k, table, qw, kw, interleaved=interleaved)
+    got = rotate_qk(_apart(q, 2 ** 24 + 24), _apart(k, 2 ** 24 + 56), table, qw, kw, interleaved=interleaved)
+    for x, w, g, n in ((q, qw, got[0], want[0]), (k, kw, got[1], want[1])):
+        check(g, x, table, w, dtype, interleaved)
+        assert torch.equal(g, n)
+
+
+@pytest.mark.parametrize("stride", [306_783_300, 306_783_400, 320_000_000])
+@pytest.mark.parametrize("weights,interleaved", [(True, True), (False, False), (True, False)])
+@pytest.mark.parametrize("d,p", [(64, 32), (50, 25)])
+def test_heads_at_and_past_32_bit_offsets(d, p, weights, interleaved, stride):
+    """Eight heads: the last one's offset is on either side of 2^32 bytes."""
+    q, _, table, qw, _ = make(d, 1, 3, 8, 0, d, p, "bf16", weights, False)
+    want = rotate_qk(q, None, table, qw, interleaved=interleaved)[0]
+    assert torch.equal(rotate_qk(_apart(q, stride), None, table, qw, interleaved=interleaved)[0], want)
+
+
+@pytest.mark.parametrize("h,s,d,p", [(5, 140_001, 128, 64), (8, 5_000_001, 64, 4)])
+def test_long_head_major_sequences(h, s, d, p):
+    """[B, H, S, D] as it lies in memory, results too; a token as it is in a short sequence, bit for bit."""
+    q = torch.zeros((1, h, s, d), dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator().manual_seed(s)
+    spots = [0, 1, s // 2, s - 2, s - 1]
+    q[:, :, spots] = torch.randn((1, h, 5, d), generator=g).bfloat16().cuda()
+    table, w = torch.rand((s, p, 2), device="cuda"), (1 + 0.2 * torch.randn(d, generator=g)).bfloat16().cuda()
+    for interleaved in (True, False):
+        got = rotate_qk(q, None, table, w, interleaved=interleaved)[0]
+        assert got.is_contiguous()
+        few = rotate_qk(q[:, :, spots], None, table[spots], w, interleaved=interleaved)[0]
+        assert torch.equal(got[:, :, spots], few)
+        check(few, q[:, :, spots], table[spots], w, "bf16", interleaved)
+
+
 def test_zero_heads_and_zero_tokens():
     q, k, table, qw, kw = make(5, 1, 0, 3, 1, 64, 32, "bf16", True, False)
     qo, ko = rotate_qk(q, k, table, qw, kw)
