@@ -35,7 +35,8 @@ class MXFP4Linear(nn.Module):
 
     The output is bf16(act(x w^T + bias)) with one rounding, in the input's dtype.  ``adapters`` holds
     LoRA triples as ``FP8Linear`` does; they and the activation then run after the product as torch
-    ops."""
+    ops, in the input's dtype (``forward_quantized``: bf16).  Code that attaches adapters to
+    ``nn.Linear`` and ``FP8Linear`` by type has to be told of this class."""
 
     def __init__(self, in_features: int, out_features: int) -> None:
         super().__init__()
@@ -81,11 +82,11 @@ class MXFP4Linear(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         x2d = x if x.ndim == 2 else x.reshape(-1, self.in_features)
         out = ops.mxfp4_linear(x2d, self.w4, self.w_scale, self.bias, ACT_NONE if self.adapters else int(self.act))
+        if x.dtype != torch.bfloat16:
+            out = out.to(x.dtype)
         if self.adapters:
             out = self._adapted(x2d, out)
-        if x.ndim != 2:
-            out = out.reshape(*x.shape[:-1], self.out_features)
-        return out if x.dtype == torch.bfloat16 else out.to(x.dtype)
+        return out if x.ndim == 2 else out.reshape(*x.shape[:-1], self.out_features)
 
     def forward_quantized(self, x4: torch.Tensor, x_scale: torch.Tensor,
                           x_modulated: torch.Tensor | None = None) -> torch.Tensor:

@@ -278,6 +278,23 @@ def test_module(dtype):
         mod.forward_quantized(*quantize_mxfp4(x2))
 
 
+@pytest.mark.parametrize("act", [0, 1])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_adapters_add_in_the_input_s_dtype(dtype, act):
+    """The product, then each branch and the activation, in x's dtype, as FP8Linear does it."""
+    mod = MXFP4Linear.from_linear(nn.Linear(288, 176, device="cuda", dtype=torch.bfloat16))
+    x = randn(5, 2, 9, 288, dtype=DT[dtype])
+    want = mod(x)
+    mod.act = act
+    for i, (rank, scale) in enumerate(((8, 0.5), (3, 1.7))):
+        A, B = randn(6 + i, rank, 288, std=0.1), randn(8 + i, 176, rank, std=0.1)
+        mod.adapters.append((A, B, scale))
+        want = want + (((x.to(A.dtype) @ A.t()) @ B.t()) * scale).to(x.dtype)
+    if act:
+        want = torch.nn.functional.gelu(want, approximate="tanh")
+    assert want.dtype == DT[dtype] and torch.equal(mod(x), want)
+
+
 def test_conversion_of_a_transformer():
     class Proj(nn.Module):
         def __init__(self):
