@@ -277,26 +277,30 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256, min_waves(DT, NC, WEIGHTS)) vo
 }
 
 template <int DT, int NT, int NC, int QM>
-static void launch_block_norm_nc(const BlockNormArgs& a, hipStream_t st) {
+static int launch_block_norm_nc(const BlockNormArgs& a, hipStream_t st) {
+  const char* what = "gated_residual_norm";
   constexpr int block = NT > 256 ? NT : 256;
-  const dim3 grid((unsigned)cdiv(a.M, block / NT));
+  const int64_t blocks = cdiv(a.M, block / NT);
+  if (!grid_fits(blocks, block)) return set_error(MXF8_EINVAL, "%s: shape too large", what);
+  const dim3 grid((unsigned)blocks);
   const bool weights = a.branch_weight || a.weight;
   if constexpr (QM != MXF8_QUANT_MXFP4) {
     if (a.C % 8) {
       if constexpr (NT == 8) {
         if (a.C < 8) {
           block_norm_kernel<DT, NT, NC, QM, TAIL_SHORT, true><<<grid, block, 0, st>>>(a);
-          return;
+          return check_launch(what);
         }
       }
       block_norm_kernel<DT, NT, NC, QM, TAIL_BACK, true><<<grid, block, 0, st>>>(a);
-      return;
+      return check_launch(what);
     }
   }
   if (weights)
     block_norm_kernel<DT, NT, NC, QM, TAIL_NONE, true><<<grid, block, 0, st>>>(a);
   else
     block_norm_kernel<DT, NT, NC, QM, TAIL_NONE, false><<<grid, block, 0, st>>>(a);
+  return check_launch(what);
 }
 
 template <int DT, int QM>
@@ -310,15 +314,12 @@ static int launch_block_norm(const BlockNormArgs& a, hipStream_t st) {
   // 20280 88.8 / 92.0; 1024 channels: 512 tokens 4.1 / 4.4, 10166 16.0 / 23.4.
   const bool wave = chunks <= 128 || (chunks <= (DT == MXF8_F32 ? 192 : 384) && a.M >= 8192);
 #define MXF8_BN(NT, NC) \
-  case NC: launch_block_norm_nc<DT, NT, NC, QM>(a, st); break;
+  case NC: return launch_block_norm_nc<DT, NT, NC, QM>(a, st);
   // Short rows share a wave: 51597 x 33 30.0 -> 8.2 us, 20000 x 256 13.2 -> 10.0.
   if (chunks <= 32) {
-    if (chunks <= 8)
-      launch_block_norm_nc<DT, 8, 1, QM>(a, st);
-    else if (chunks <= 16)
-      launch_block_norm_nc<DT, 16, 1, QM>(a, st);
-    else
-      launch_block_norm_nc<DT, 32, 1, QM>(a, st);
+    return chunks <= 8    ? launch_block_norm_nc<DT, 8, 1, QM>(a, st)
+           : chunks <= 16 ? launch_block_norm_nc<DT, 16, 1, QM>(a, st)
+                          : launch_block_norm_nc<DT, 32, 1, QM>(a, st);
   } else if (wave) {
     switch (cdiv(chunks, 64)) {
       MXF8_BN(64, 1) MXF8_BN(64, 2) MXF8_BN(64, 3)
@@ -333,7 +334,7 @@ static int launch_block_norm(const BlockNormArgs& a, hipStream_t st) {
     switch (cdiv(chunks, 512)) { MXF8_BN(512, 3) MXF8_BN(512, 4) }
   }
 #undef MXF8_BN
-  return check_launch("gated_residual_norm");
+  return set_error(MXF8_EINVAL, "gated_residual_norm: no kernel for C=%d", a.C);
 }
 
 }  // namespace mxf8

@@ -169,6 +169,9 @@ __device__ __forceinline__ float block256_max(float v, float* red4) {
 
 __host__ __device__ constexpr int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Whether a launch of so many blocks is possible: a grid holds less than 2^32 threads a dimension.
+constexpr bool grid_fits(int64_t blocks, int64_t threads) { return blocks < (1LL << 32) / threads; }
+
 // LDS tiles with 64- or 128-byte rows are stored as 16-byte chunks, logical chunk c of row
 // r at physical chunk c ^ lds_swz(r).  A ds_read_b128 is served 16 lanes at a time over
 // 64 four-byte banks (256 bytes); when 16 consecutive rows read the same logical chunk,

@@ -79,10 +79,15 @@ __global__ __launch_bounds__(256) void mxfp4_dequant_kernel(const uint8_t* __res
   }
 }
 
+// Workgroups of both: two rows a wave for small matrices, else four.
+static bool mx_small(int64_t M, int64_t K) { return M * K <= MX_SMALL; }
+static int64_t mx_blocks(int64_t M, int64_t K) { return cdiv(M, mx_small(M, K) ? 8 : 16) * cdiv(K, 512); }
+
 static int mx_check(const char* what, int64_t M, int64_t K) {
   if (M < 0 || K <= 0) return set_error(MXF8_EINVAL, "%s: bad shape", what);
   if (K % MX_BLOCK) return set_error(MXF8_EINVAL, "%s: K=%lld must be a multiple of 32", what, (long long)K);
-  if (M > 0x7fffffff / 2 || K > (1 << 22) || cdiv(M, 8) * cdiv(K, 512) > 0x7fffffff) return set_error(MXF8_EINVAL, "%s: shape too large", what);
+  if (M > 0x7fffffff / 2 || K > (1 << 22) || !grid_fits(mx_blocks(M, K), 256))
+    return set_error(MXF8_EINVAL, "%s: shape too large", what);
   return MXF8_OK;
 }
 
@@ -101,8 +106,8 @@ extern "C" int mxf8_mxfp4_quant(const void* x, int dtype, int64_t M, int64_t K, 
   if (M == 0) return MXF8_OK;
   if (!x || !codes || !scales) return set_error(MXF8_EINVAL, "mxfp4_quant: null pointer");
   if ((uintptr_t)codes % 4) return set_error(MXF8_EINVAL, "mxfp4_quant: codes must be 4-byte aligned");
-  const bool small = M * K <= MX_SMALL;
-  const dim3 grid((unsigned)(cdiv(M, small ? 8 : 16) * cdiv(K, 512)));
+  const bool small = mx_small(M, K);
+  const dim3 grid((unsigned)mx_blocks(M, K));
   switch (dtype) {
 #define MXF8_CASE(DT)                                                                                           \
   case DT:                                                                                                      \
@@ -126,8 +131,8 @@ extern "C" int mxf8_mxfp4_dequant(const uint8_t* codes, const uint8_t* scales, i
   if (M == 0) return MXF8_OK;
   if (!out || !codes || !scales) return set_error(MXF8_EINVAL, "mxfp4_dequant: null pointer");
   if ((uintptr_t)codes % 4) return set_error(MXF8_EINVAL, "mxfp4_dequant: codes must be 4-byte aligned");
-  const bool small = M * K <= MX_SMALL;
-  const dim3 grid((unsigned)(cdiv(M, small ? 8 : 16) * cdiv(K, 512)));
+  const bool small = mx_small(M, K);
+  const dim3 grid((unsigned)mx_blocks(M, K));
   switch (dtype) {
 #define MXF8_CASE(DT)                                                                                            \
   case DT:                                                                                                       \

@@ -292,11 +292,14 @@ __global__ __launch_bounds__(256) void rotate_qk_any_kernel(const RotArgs a) {
 }
 
 template <int DT, bool INTERLEAVED>
-static void launch_rotate(RotArgs& a, hipStream_t st) {
+static int launch_rotate(RotArgs& a, hipStream_t st) {
+  const char* what = "rotate_qk";
   const int64_t tokens = a.S * a.B;
+  const int64_t blocks = cdiv(a.D > 512 ? tokens * (a.heads[0] + a.heads[1]) : tokens, 4);
+  if (!grid_fits(blocks, 256)) return set_error(MXF8_EINVAL, "%s: shape too large", what);
   if (a.D > 512) {
-    rotate_qk_any_kernel<DT, INTERLEAVED><<<dim3((unsigned)cdiv(tokens * (a.heads[0] + a.heads[1]), 4)), 256, 0, st>>>(a);
-    return;
+    rotate_qk_any_kernel<DT, INTERLEAVED><<<dim3((unsigned)blocks), 256, 0, st>>>(a);
+    return check_launch(what);
   }
   // Lanes per head: the 8-channel chunks of a head, up to a power of two.  A lane's offset within a step of 64 / L
   // heads is 32 bits of bytes; heads that lie too far apart for that take a wave each, with the same result bit for bit
@@ -315,7 +318,7 @@ static void launch_rotate(RotArgs& a, hipStream_t st) {
   // All heads of a token in one wave once that gives every SIMD two waves; fewer tokens split the heads.
   a.per = total;
   while (a.per > 1 && tokens * cdiv(total, a.per) < 2048) a.per = (a.per + 1) / 2;
-  const dim3 grid((unsigned)cdiv(tokens, 4), (unsigned)cdiv(total, a.per));
+  const dim3 grid((unsigned)blocks, (unsigned)cdiv(total, a.per));
   const bool any = a.D % 8 || (!INTERLEAVED && a.P % 8);
 #define MXF8_CASE(LL)                                                                \
   case LL:                                                                           \
@@ -333,6 +336,7 @@ static void launch_rotate(RotArgs& a, hipStream_t st) {
     MXF8_CASE(64)
   }
 #undef MXF8_CASE
+  return check_launch(what);
 }
 
 }  // namespace mxf8
@@ -365,7 +369,7 @@ extern "C" int mxf8_rotary_table(const void* pos, int pos_type, int64_t n, int64
   int rows = (int)cdiv(2048, P);
   const int cus = device_cus();
   while (rows > 1 && cdiv(n, rows) < 4 * cus) rows = (rows + 1) / 2;
-  if (cdiv(n, rows) > 0x7fffffff) return set_error(MXF8_EINVAL, "rotary_table: too many positions");
+  if (!grid_fits(cdiv(n, rows), 256)) return set_error(MXF8_EINVAL, "rotary_table: too many positions");
   const dim3 grid((unsigned)cdiv(n, rows));
   switch (pos_type) {
     case 0: rotary_table_kernel<0><<<grid, 256, 0, stream>>>(pos, n, (int)axes, ax, rows, table); break;
@@ -418,14 +422,11 @@ extern "C" int mxf8_rotate_qk(const void* q, const int64_t q_strides[4], int64_t
   a.S = S, a.B = (int)B, a.D = (int)D, a.P = (int)P;
   a.eps = eps;
   a.inv_d = 1.0f / (float)D;
-#define MXF8_CASE(DT)                                   \
-  if (dtype == DT) {                                    \
-    if (interleaved) launch_rotate<DT, true>(a, stream); \
-    else launch_rotate<DT, false>(a, stream);           \
-  }
-  MXF8_CASE(MXF8_BF16)
-  MXF8_CASE(MXF8_F16)
-  MXF8_CASE(MXF8_F32)
-#undef MXF8_CASE
-  return check_launch(what);
+  auto launch = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    return interleaved ? launch_rotate<DT, true>(a, stream) : launch_rotate<DT, false>(a, stream);
+  };
+  return dtype == MXF8_BF16  ? launch(std::integral_constant<int, MXF8_BF16>{})
+         : dtype == MXF8_F16 ? launch(std::integral_constant<int, MXF8_F16>{})
+                             : launch(std::integral_constant<int, MXF8_F32>{});
 }

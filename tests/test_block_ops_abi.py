@@ -160,6 +160,28 @@ def test_mxfp4(lib):
     assert linear(m=0, x=None) == 0 and linear(n=0, w=None) == 0
 
 
+def test_sizes_that_no_launch_takes(lib):
+    """2^32 threads or more: refused with their own words, not at the launch."""
+    refused(lib, lib.mxf8_rotary_table(D, 0, 1 << 35, 1, dims(2), 1e4, D, None), "too many")
+    st = N._I64x4(64, 16, 8, 1)
+    for s, d in ((1 << 27, 8), (1 << 26, 128), (1 << 25, 1024)):
+        for dtype in (0, 1, 2):
+            for inter in (0, 1):
+                rc = lib.mxf8_rotate_qk(D, st, 2, D, st, 1, dtype, 1, s, d, D, 0, 4, None, None, 1e-6, inter, D, st, D, st,
+                                        None)
+                refused(lib, rc, "too large")
+    # (tokens, channels): a row takes 8 threads, 64 and 256 of 256, 512
+    for s, c in ((1 << 29, 32), (1 << 26, 1024), (1 << 24, 4096), (1 << 23, 16384)):
+        for dtype in (0, 2):
+            for quant in (0, 1, 2):
+                rc = lib.mxf8_gated_residual_norm(D, 0, c, D, 0, c, dtype, 1, s, c, None, 0, 0, None, 0, 0, None, 0, 0, 1,
+                                                  None, None, 1, 1e-6, 1.0, quant, D, D, D, D, None)
+                refused(lib, rc, "too large")
+    for m, k in ((1 << 28, 32), (1 << 24, 1 << 13)):
+        refused(lib, lib.mxf8_mxfp4_quant(D, 0, m, k, k, D, D, None), "too large")
+        refused(lib, lib.mxf8_mxfp4_dequant(D, D, m, k, D, 0, None), "too large")
+
+
 def test_cpu_tensors_are_refused():
     x = torch.zeros((4, 64))
     with pytest.raises(ValueError):
