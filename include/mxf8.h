@@ -316,7 +316,8 @@ enum { MXF8_QUANT_NONE = 0, MXF8_QUANT_E4M3 = 1, MXF8_QUANT_MXFP4 = 2 };
  *   r [B, S, C] contiguous; y [B, S, C] contiguous, required when quant == MXF8_QUANT_NONE, else optional
  *   quant == MXF8_QUANT_E4M3: codes [B S, C] and fp32 scales [B S], mxf8_quant_rows(y) bit for bit
  *   quant == MXF8_QUANT_MXFP4: codes [B S, C / 2] and scales, mxf8_mxfp4_quant(y) bit for bit; C % 32 == 0
- * fp32 arithmetic; C <= 16384.  Outputs must not overlap inputs.
+ * fp32 arithmetic, in an order that C alone determines: a token's results do not depend, to the bit, on the other
+ * tokens of the call or on how many there are.  C <= 16384.  Outputs must not overlap inputs.
  */
 int mxf8_gated_residual_norm(const void* x, int64_t x_batch, int64_t x_token, const void* branch, int64_t br_batch,
                              int64_t br_token, int dtype, int64_t B, int64_t S, int64_t C, const void* gate,

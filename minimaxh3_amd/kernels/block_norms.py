@@ -39,8 +39,9 @@ def gated_residual_norm(
     gate, shift and scale hold a row per batch item, [B, C], or one per S / G consecutive tokens (a
     frame), [B, G, C]; each may be None (1, 0, 0), and so may ``weight`` [C].  All tensors have x's
     dtype: bf16, fp16 or fp32.  Arithmetic is fp32, y is taken from the unrounded r, and each output is
-    rounded once.  With ``branch=None`` r is x itself (residual_scale must be 1): the norm before a
-    model's first branch.  C <= 16384.
+    rounded once; a token's results do not depend on the others of the call, to the bit.  With
+    ``branch=None`` r is x itself (residual_scale must be 1): the norm before a model's first branch.
+    C <= 16384.
 
     ``quantize="e4m3"`` returns (r, x8 [B S, C], x_scale [B S, 1]) for ``FP8Linear.forward_quantized``,
     ``quantize="mxfp4"`` (r, x4 [B S, C / 2], x_scale [ceil(C / 256), B S, 8]) for

@@ -63,8 +63,9 @@ def gated_residual_norm(x, branch, gate=None, shift=None, scale=None, branch_wei
                         norm: str = "layer", eps: float = 1e-6, residual_scale: float = 1.0):
     """(r, y, bound of r, bound of y), [B, S, C] each.
 
-    A row's sums run over at most 64 elements of one thread, 6 levels of a wave and 3 waves: a relative
-    error of g = 80 U in a sum of squares, and of g mean|r| in the mean.  u then has g / 2 + 6 U, r adds a
+    A row's sums run over at most 48 elements of one thread, 6 levels between the lanes of a wave and the
+    parts of up to 8 waves, under 62 roundings and those of the products' sum: a relative error of under
+    g = 80 U in a sum of squares, and of g mean|r| in the mean.  u then has g / 2 + 6 U, r adds a
     product and a sum.  y: the errors of r and of the mean times rstd, g / 2 + 6 U of n, and a rounding for
     each further product and sum."""
     g = 80 * U

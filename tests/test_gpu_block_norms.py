@@ -123,6 +123,31 @@ def test_e4m3_codes_of_odd_widths(c):
     assert torch.equal(codes.view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(scales, want[1])
 
 
+@pytest.mark.parametrize("norm,sandwich,weighted", [("layer", False, False), ("rms", True, True), ("layer", True, False)])
+@pytest.mark.parametrize("dtype,c", [("bf16", 3072), ("bf16", 1032), ("fp16", 2730), ("bf16", 2048), ("fp16", 1600),
+                                     ("fp32", 1536), ("fp32", 1030), ("fp32", 3072), ("bf16", 1024), ("bf16", 33),
+                                     ("bf16", 4104)])
+def test_a_token_does_not_depend_on_the_others(c, dtype, norm, sandwich, weighted):
+    """Bit for bit: from 8192 tokens on one wave holds a row that four share below."""
+    s = 8300
+    a = make(c, 1, s, c, dtype, sandwich=sandwich, weighted=weighted)
+    per_call = {"norm": norm}
+    formats = [None, "e4m3"] + ["mxfp4"] * (c % 32 == 0)
+    whole = {q: gated_residual_norm(**a, **per_call, quantize=q) for q in formats}
+    as_bytes = lambda t: t.contiguous().view(torch.uint8)  # noqa: E731
+    for n in (1, 5, 700, 8191):
+        for i in (0, s - n):
+            cut = {**a, "x": a["x"][:, i: i + n], "branch": a["branch"][:, i: i + n]}
+            for q in formats:
+                got, want = gated_residual_norm(**cut, **per_call, quantize=q), whole[q]
+                assert torch.equal(got[0], want[0][:, i: i + n])
+                if q is None:
+                    assert torch.equal(got[1], want[1][:, i: i + n])
+                else:
+                    scale = want[2][:, i: i + n] if q == "mxfp4" else want[2][i: i + n]
+                    assert torch.equal(as_bytes(got[1]), as_bytes(want[1][i: i + n])) and torch.equal(got[2], scale)
+
+
 @pytest.mark.parametrize("s", [3, 4100])
 def test_non_finite_values_stay_in_their_token(s):
     a = make(8, 1, s, 96, "bf16", sandwich=True)
