@@ -123,6 +123,31 @@ def test_e4m3_codes_of_odd_widths(c):
     assert torch.equal(codes.view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(scales, want[1])
 
 
+LARGE = [("bf16", 8200, 3072), ("fp16", 8197, 2730), ("bf16", 8192, 1032), ("bf16", 8200, 2000), ("fp16", 8192, 2560),
+         ("fp32", 8200, 1536), ("fp32", 8195, 1029)]
+
+
+@pytest.mark.parametrize("norm,sandwich", [("layer", False), ("rms", True)])
+@pytest.mark.parametrize("dtype,s,c", LARGE)
+def test_one_wave_a_row_against_the_oracle(dtype, s, c, norm, sandwich):
+    """1025 channels and more, from 8192 rows on."""
+    check(make(c + s, 1, s, c, dtype, sandwich=sandwich, weighted=sandwich), dtype, norm, rs=0.75 if sandwich else 1.0)
+
+
+@pytest.mark.parametrize("sandwich", [False, True])
+@pytest.mark.parametrize("dtype,s,c", [*LARGE, ("bf16", 8200, 1056), ("fp16", 8200, 2336), ("fp32", 8192, 1312)])
+def test_codes_of_one_wave_a_row_are_the_quantizers_of_y(dtype, s, c, sandwich):
+    a = make(c, 1, s, c, dtype, sandwich=sandwich, weighted=sandwich)
+    a["x"][0, 0, :32] = 0
+    r, y = gated_residual_norm(**a)
+    for fmt, quant in (("e4m3", quantize_rows), ("mxfp4", quantize_mxfp4)):
+        if fmt == "e4m3" or c % 32 == 0:
+            want = quant(y[0])
+            r1, codes, scales = gated_residual_norm(**a, quantize=fmt)
+            assert torch.equal(r1, r) and torch.equal(codes.view(torch.uint8), want[0].view(torch.uint8)), fmt
+            assert torch.equal(scales, want[1]), fmt
+
+
 @pytest.mark.parametrize("norm,sandwich,weighted", [("layer", False, False), ("rms", True, True), ("layer", True, False)])
 @pytest.mark.parametrize("dtype,c", [("bf16", 3072), ("bf16", 1032), ("fp16", 2730), ("bf16", 2048), ("fp16", 1600),
                                      ("fp32", 1536), ("fp32", 1030), ("fp32", 3072), ("bf16", 1024), ("bf16", 33),
