@@ -358,6 +358,9 @@ int mxf8_mxfp4_dequant(const uint8_t* codes, const uint8_t* scales, int64_t M, i
  *   a4, sa: activations [M, K]; w4, sw: weights [N, K]; both as mxf8_mxfp4_quant writes them; codes 16-byte
  *   and scales 8-byte aligned
  *   bias [N] bf16 or NULL; out [M, N] bf16, row stride ld_out >= N
+ * Products too small to give every compute unit a 32 x 32 tile of out, and those of up to 16 tokens, split K over waves,
+ * and add in another order than larger ones: a token's output may then differ in the last bit with M.  Among the larger
+ * ones, and among those of up to 16 tokens, it does not depend on M.
  */
 int mxf8_gemm_mxfp4(const uint8_t* a4, const uint8_t* w4, const uint8_t* sa, const uint8_t* sw, const void* bias,
                     int act, void* out, int64_t M, int64_t N, int64_t K, int64_t ld_out, hipStream_t stream);

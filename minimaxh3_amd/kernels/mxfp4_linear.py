@@ -36,7 +36,10 @@ class MXFP4Linear(nn.Module):
     The output is bf16(act(x w^T + bias)) with one rounding, in the input's dtype.  ``adapters`` holds
     LoRA triples as ``FP8Linear`` does; they and the activation then run after the product as torch
     ops, in the input's dtype (``forward_quantized``: bf16).  Code that attaches adapters to
-    ``nn.Linear`` and ``FP8Linear`` by type has to be told of this class."""
+    ``nn.Linear`` and ``FP8Linear`` by type has to be told of this class.
+
+    The fp32 sum's order depends on the size of the product: a token's output may differ in its last
+    bit between a call of a few tokens and one of many (``mxf8_gemm_mxfp4`` in include/mxf8.h)."""
 
     def __init__(self, in_features: int, out_features: int) -> None:
         super().__init__()

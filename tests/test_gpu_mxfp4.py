@@ -130,6 +130,32 @@ def test_every_kernel(m, n, k, act):
     product(m, n, k, seed=m + k, act=act)
 
 
+@pytest.mark.parametrize("act", [0, 1])
+@pytest.mark.parametrize("m,n,k", [(200, 2100, 768), (130, 4100, 768), (300, 4100, 768), (256, 9216, 2048),
+                                   (513, 12288, 768), (8200, 4100, 768), (4097, 8200, 1024), (2100, 4100, 1536)])
+def test_every_tile_kernel_with_whole_stages(m, n, k, act):
+    """K in whole stages of 256, three and more of them (tests/test_mxfp4_tiles.py: the ring and the persistent kernels,
+    256 x 256 tiles in one round of workgroups and in several)."""
+    product(m, n, k, seed=m + k, act=act)
+
+
+@pytest.mark.parametrize("k", [768, 800, 1280])
+def test_a_token_does_not_depend_on_the_others(k):
+    """Bit for bit, among the sizes that go to the ring and the persistent kernels, which add in one order; and among
+    those of up to 16 tokens."""
+    n = 4100
+    (a4, sa), (w4, sw) = quantize_mxfp4(randn(1, 8200, k)), quantize_mxfp4(randn(2, n, k))
+    b = randn(3, n)
+    whole = ops.gemm_mxfp4(a4, w4, sa, sw, b, 1)
+    part = lambda i, m: ops.gemm_mxfp4(a4[i: i + m], w4, sa[:, i: i + m].contiguous(), sw, b, 1)  # noqa: E731
+    for m in (60, 130, 300, 700, 1100, 2100, 4200):
+        for i in (0, 8200 - m):
+            assert torch.equal(part(i, m), whole[i: i + m]), (m, i)
+    few = part(3, 16)
+    for m in (1, 2, 7, 15):
+        assert torch.equal(part(3, m), few[:m])
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 48, 3072), (20, 70, 96), (130, 300, 320), (700, 256, 768), (4500, 4100, 64)])
 @pytest.mark.parametrize("bias", [True, False])
 def test_product_with_activation(m, n, k, bias):

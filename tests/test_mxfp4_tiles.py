@@ -52,5 +52,16 @@ def test_every_size_has_a_kernel(pick, cus):
     assert all(0 <= p <= 10 for p in pick(sizes, cus))
 
 
+def test_gpu_test_shapes_of_whole_stages_reach_every_tile_kernel(pick):
+    """The shapes of tests/test_gpu_mxfp4.py's test of that name, and those whose slices it compares bit for bit."""
+    shapes = {(200, 2100, 768): 4, (130, 4100, 768): 5, (300, 4100, 768): 6, (256, 9216, 2048): 7, (513, 12288, 768): 8,
+              (8200, 4100, 768): 9, (4097, 8200, 1024): 9, (2100, 4100, 1536): 9}
+    assert dict(zip(shapes, pick(shapes))) == shapes
+    for k in (768, 800, 1280):
+        slices = [(m, 4100, k) for m in (60, 130, 300, 700, 1100, 2100, 4200, 8200)]
+        assert min(pick(slices)) == 4 and max(pick(slices)) == 9 and 10 not in pick(slices)
+        assert len(set(pick([(m, 4100, k) for m in range(1, 17)]))) == 1
+
+
 def test_gpu_test_shapes_reach_every_kernel(pick):
     assert dict(zip(SHAPES, pick(SHAPES))) == SHAPES and set(SHAPES.values()) == set(range(11))
