@@ -18,7 +18,6 @@ constexpr int ROT_MAX_AXES = 4, ROT_MAX_PAIRS = 256;
 
 struct RotAxes {
   int first[ROT_MAX_AXES + 1];  // first pair of each axis, and the number of pairs
-  int n;
   double log2_theta;
 };
 
@@ -350,7 +349,6 @@ extern "C" int mxf8_rotary_table(const void* pos, int pos_type, int64_t n, int64
     return set_error(MXF8_EINVAL, "rotary_table: 1 to %d axes expected", ROT_MAX_AXES);
   if (!(theta > 0.0) || !(theta < 1.0e30)) return set_error(MXF8_EINVAL, "rotary_table: theta must be positive");
   RotAxes ax{};
-  ax.n = (int)axes;
   ax.log2_theta = __builtin_log2(theta);
   int64_t P = 0;
   for (int64_t i = 0; i < axes; ++i) {

@@ -71,9 +71,6 @@ struct Raw8 {
 #pragma unroll
     for (int j = 0; j < 4; ++j) w[j] = cvt_pk_16<DT>(f[2 * j], f[2 * j + 1]);
   }
-  __device__ __forceinline__ void store(void* base, int64_t i) const {
-    *reinterpret_cast<words4*>(static_cast<uint16_t*>(base) + i) = words4{w[0], w[1], w[2], w[3]};
-  }
   // non-temporal: for results that the caches would not hold until they are read
   __device__ __forceinline__ void stream(void* base, int64_t i) const {
     stream_off(static_cast<uint16_t*>(base) + i, 0);
@@ -128,11 +125,6 @@ struct Raw8<MXF8_F32> {
 #pragma unroll
     for (int j = 0; j < 8; ++j) w[j] = f[j];
   }
-  __device__ __forceinline__ void store(void* base, int64_t i) const {
-    float* p = static_cast<float*>(base) + i;
-    *reinterpret_cast<floats4*>(p) = floats4{w[0], w[1], w[2], w[3]};
-    *reinterpret_cast<floats4*>(p + 4) = floats4{w[4], w[5], w[6], w[7]};
-  }
   __device__ __forceinline__ void stream(void* base, int64_t i) const { stream_off(static_cast<float*>(base) + i, 0); }
   __device__ __forceinline__ void stream_off(void* base, uint32_t off) const {
     float* p = reinterpret_cast<float*>(static_cast<char*>(base) + off);
@@ -171,19 +163,7 @@ __device__ __forceinline__ float lanes_max(float v) {
   return lanes_reduce<L>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
-// One element.
-template <int DT>
-__device__ __forceinline__ float load1(const void* base, int64_t i) {
-  return Elem<DT>::to_f32(static_cast<const typename Elem<DT>::T*>(base)[i]);
-}
-// f rounded to the type.
-template <int DT>
-__device__ __forceinline__ float round1(float f) {
-  if constexpr (DT == MXF8_F32)
-    return f;
-  else
-    return Elem<DT>::lo(cvt_pk_16<DT>(f, f));
-}
+// One element, rounded.
 template <int DT>
 __device__ __forceinline__ void store1(void* base, int64_t i, float f) {
   if constexpr (DT == MXF8_F32)
