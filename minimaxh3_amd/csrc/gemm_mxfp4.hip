@@ -10,10 +10,12 @@
 // both operands follow it, and with this one the four scales that a lane needs in a stage are one aligned dword
 // of the slab's eight bytes per row, which the instruction picks bytes from.
 //
-// What bounds it: a stage of a 256 x 256 tile is 2048 cycles of products and takes about 3600, with the fragment reads
-// (LDS active 30% of the time) and the copies on LDS's one port beside them, at a clock that the power limit holds at
-// 1.7-1.9 GHz; an epilogue takes 9300 cycles a tile.  20280 tokens: 3072 -> 12288 428 us (3580 TFLOP/s; the FP8 GEMM
-// 600) and 433 with GELU, 12288 -> 3072 369 (4150; 590), 3072 -> 3072 106; 8192^3 257 us, 4280 TFLOP/s.
+// What bounds it: a stage of a 256 x 256 tile is 2048 cycles of products and takes about 3600, an epilogue 9300 a tile, at
+// a clock that the power limit holds at 1.9-1.95 GHz.  No unit is busy throughout (matrix cores 44-55%, the vector unit 25-42%,
+// LDS active 28-30% of the cycles); waves wait for a third of them.  Without the output stores of whole tiles 4-8% less
+// at K = 3072, 2% at 12288.  20280 tokens, once the clock has settled under load (after an idle spell calls take up to 1.3 times as
+// long for some ten milliseconds): 3072 -> 12288 403 us (3800 TFLOP/s; the FP8 GEMM 605) and 441 with GELU (651),
+// 12288 -> 3072 371 (4130; 616), 3072 -> 9216 314 (467), 3072 -> 3072 108 (161); 8192^3 257 us, 4270 TFLOP/s (407).
 // Measured and not kept: four waves of 128 x 128 (spills), W fragments a step ahead too, a barrier in the middle of a
 // stage's products, raised wave priority around them.
 #include "gemm_common.h"

@@ -8,7 +8,8 @@ namespace mxf8 {
 // A lane holds 8 elements (a 16-byte load, 4 bytes of codes), a quad of lanes one block, a wave 512 elements of
 // ROWS rows, whose loads are in flight together.  Workgroups go along the rows first, so that those running at the
 // same time read and write neighbouring memory (20280 x 12288 bf16: 133 -> 107 us), and past the caches (quantize
-// 20280 x 3072 30.4 -> 27.2 us, 5.8 TB/s; back 33.7 -> 25.1, 6.3 TB/s).
+// 20280 x 3072 30.4 -> 27.2 us, 5.8 TB/s; back 33.7 -> 25.1, 6.3 TB/s).  A wave spans 512 columns, so a matrix of few leaves
+// lanes idle: 62 million elements in rows of 32 take 212 us (back 129), of 288 32 (25), of 1056 32 (28).
 constexpr int64_t MX_SMALL = 1 << 24;  // elements up to which two rows and plain loads do (2048 x 3072: 5.5 -> 5.2 us)
 
 // This wave's first row and lane's first column, of workgroups that hold 512 columns of 4 ROWS rows each.
