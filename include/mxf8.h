@@ -1,7 +1,8 @@
 /*
  * mxf8.h - C ABI of the MI355X (gfx950) FP8 hot path: dynamic e4m3 quantizers, the
  * row-wise scaled FP8 GEMM with a fused epilogue, and the FP8 flash-attention forward; and of
- * what a DiT block has around them: rotary positions, gated residual norms, the 4-bit linear.
+ * what a DiT block has around them: rotary positions, gated residual norms, the 4-bit linear, and a
+ * paged e4m3 cache of keys and values with the attention over it.
  *
  * Conventions
  *  - Every pointer is a device pointer; every size, leading dimension and stride is in
@@ -377,6 +378,64 @@ int64_t mxf8_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int d
 int mxf8_mxfp4_linear(const void* x, int dtype, int64_t ldx, const uint8_t* w4, const uint8_t* sw, const void* bias,
                       int act, void* out, int64_t M, int64_t N, int64_t K, int64_t ld_out, void* workspace,
                       hipStream_t stream);
+
+/*
+ * Paged e4m3 cache of keys and values (no counterpart in the reference).  A pool of `pages` pages holds
+ * page_size (16, 32, 64 or 128) tokens of H heads each:
+ *   k_codes, v_codes [pages, H, page_size, D] e4m3, 16-byte aligned, D 64 or 128
+ *   k_scale, v_scale [pages, H] uint8: exponent + 127 of the power of two that the page's codes are times
+ * Sequence b's tokens t are in page page_table[b, t / page_size] (int32, row stride table_stride, table_width
+ * entries a row) at t % page_size.  An entry outside [0, pages) names no page: nothing is written there,
+ * it reads as zeros, and no query sees it; nor do tokens behind the table's last entry exist.
+ */
+
+/*
+ * Appends S new tokens of k, v [B, H, S, D] (`dtype` bf16, fp16 or fp32, any strides with contiguous channels)
+ * to each sequence, from its token starts[b] (int32) on; counts NULL, or only the first counts[b] of them.
+ * Tokens from there on are taken as not there before; other tokens and pages stay as they are.
+ *   keys are normed per head with k_weight [D] (or NULL) and turned by turns [S, P, 2] fp32 (cos, sin) with
+ *   batch stride turns_batch_stride (0: one for all; P = 0: none), as in mxf8_rotate_qk, in fp32
+ *   a page and head's exponent e is the smallest in [-32, 63] with max |x| <= 448 * 2^e over the new tokens in it,
+ *   or the one it has where that is larger and the page holds tokens before starts[b]; their codes are then
+ *   rounded again where e grew.  A code is the e4m3 number nearest to x * 2^-e, ties to even, an infinity the
+ *   largest.  A NaN in a token's key or value makes its key NaN (in its first channel) and is held as 0
+ * A page may be in one sequence of a call only, as far as tokens are written to it.
+ */
+int mxf8_kv_append(const void* k, const int64_t k_strides[4], const void* v, const int64_t v_strides[4], int dtype,
+                   int64_t B, int64_t H, int64_t S, int64_t D, const float* turns, int64_t turns_batch_stride,
+                   int64_t P, const void* k_weight, float eps, int interleaved, const int32_t* page_table,
+                   int64_t table_stride, int64_t table_width, const int32_t* starts, const int32_t* counts,
+                   uint8_t* k_codes, uint8_t* v_codes, uint8_t* k_scale, uint8_t* v_scale, int64_t pages,
+                   int64_t page_size, hipStream_t stream);
+
+/* The values of T tokens of each sequence from starts[b] (int32) on, k and v [B, H, T, D] of `dtype`: exact in bf16
+ * and fp32, rounded in fp16; zeros from token lengths[b] (int32, NULL: none) on and where there is no page. */
+int mxf8_kv_read(const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_scale, const uint8_t* v_scale,
+                 int64_t pages, int64_t H, int64_t page_size, int64_t D, const int32_t* page_table,
+                 int64_t table_stride, int64_t table_width, int64_t B, const int32_t* starts, int64_t T,
+                 const int32_t* lengths, void* k, void* v, int dtype, hipStream_t stream);
+
+/* Scratch bytes that mxf8_kv_attend needs (0 where one launch does). */
+int64_t mxf8_kv_attend_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t S, int64_t D, int64_t table_width,
+                                       int64_t page_size);
+
+/*
+ * Attention of q [B, H, S, D] (bf16 or fp16, any strides with contiguous channels) over the first lengths[b]
+ * (int32) tokens of each sequence; head h reads key head h / (H / Hk), H a multiple of Hk.
+ *   q_lengths NULL, or only the first q_lengths[b] (int32) queries of item b are there; the others' outputs are 0
+ *   causal: query i of n sees the keys up to lengths[b] - n + i (its own token, where the queries are the last
+ *   tokens of the cache); a query that sees no key gives 0
+ *   out [B, H, S, D] of q's dtype, any strides with contiguous channels
+ *   workspace: mxf8_kv_attend_workspace_bytes(...) bytes, 16-byte aligned (NULL where that is 0)
+ * Products of 16-bit floating point numbers (q and the probabilities in fp16 under scales of their own, codes
+ * exactly), sums and softmax statistics in fp32.  The same call gives the same bits; how keys are split, and with
+ * it the order of the sums, depends on the shapes of the call and on lengths[b].
+ */
+int mxf8_kv_attend(const void* q, const int64_t q_strides[4], int dtype, int64_t B, int64_t H, int64_t S, int64_t D,
+                   const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_scale, const uint8_t* v_scale,
+                   int64_t pages, int64_t Hk, int64_t page_size, const int32_t* page_table, int64_t table_stride,
+                   int64_t table_width, const int32_t* lengths, const int32_t* q_lengths, int causal, float scale,
+                   void* out, const int64_t out_strides[4], void* workspace, hipStream_t stream);
 
 #ifdef __cplusplus
 }

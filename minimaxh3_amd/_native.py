@@ -68,6 +68,13 @@ _SIGNATURES = {
     "mxf8_mxfp4_dequant": (_i32, [_vp, _vp, _i64, _i64, _vp, _i32, _vp]),
     "mxf8_mxfp4_linear_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32]),
     "mxf8_mxfp4_linear": (_i32, [_vp, _i32, _i64, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "mxf8_kv_append": (_i32, [_vp, _I64x4, _vp, _I64x4, _i32, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _f32, _i32,
+                              _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp]),
+    "mxf8_kv_read": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp,
+                            _i32, _vp]),
+    "mxf8_kv_attend_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "mxf8_kv_attend": (_i32, [_vp, _I64x4, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64,
+                              _i64, _vp, _vp, _i32, _f32, _vp, _I64x4, _vp, _vp]),
     "mxf8_gemm_mxfp4": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _i64, _vp]),
 }
 EXPORTS = tuple(_SIGNATURES)

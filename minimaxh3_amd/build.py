@@ -31,6 +31,8 @@ SOURCES = [
     ("mxfp4.hip", "mxfp4", []),
     ("rotary.hip", "rotary", []),
     ("block_norm.hip", "block_norm", []),
+    ("kv_cache.hip", "kv_cache", []),
+    ("kv_attend.hip", "kv_attend", []),
     ("attn.hip", "attn", []),
 ] + [
     ("attn_inst.hip", f"attn_d{d}_o{o}", [f"-DMXF8_ATTN_D={d}", f"-DMXF8_ATTN_ODT={o}"])

@@ -1,6 +1,7 @@
 // The hot torch.library ops (mxf8::quant_rows, adaln_quant_rows, gemm_rowwise, lora_down,
 // attn_quant_kv, attn_fwd_q, rotary_table, rotate_qk, gated_residual_norm, mxfp4_quant,
-// mxfp4_dequant, gemm_mxfp4, mxfp4_linear) as native kernels over the C ABI of libmxf8.  Their schemas and
+// mxfp4_dequant, gemm_mxfp4, mxfp4_linear, kv_append, kv_read, kv_attend) as native kernels over the C ABI of
+// libmxf8.  Their schemas and
 // fake kernels are declared in minimaxh3_amd/ops.py; the kernels here take the CUDA and
 // AutogradCUDA entries of the dispatcher (the device type of a ROCm GPU), where they stand in
 // for the Python kernels of the declarations.
@@ -545,6 +546,127 @@ Tensor mxfp4_linear(const Tensor& x_in, const Tensor& w4, const Tensor& sw, cons
   return out;
 }
 
+// ---- paged e4m3 cache of keys and values ---------------------------------------------------------
+
+// The four tensors of a cache, and a call's page table.
+struct Pool {
+  int64_t pages, H, page, D;
+  Tensor table;
+};
+
+Pool pool_of(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, const Tensor& table, int64_t B,
+             at::Device dev, const char* what) {
+  TORCH_CHECK_VALUE(kc.dim() == 4 && kc.is_contiguous() && vc.is_contiguous() && vc.sizes() == kc.sizes() &&
+                        kc.scalar_type() == kE4M3 && vc.scalar_type() == kE4M3,
+                    what, "codes must be two contiguous e4m3 tensors [pages, heads, page_size, head_dim], got ",
+                    kc.scalar_type(), " ", kc.sizes(), " and ", vc.scalar_type(), " ", vc.sizes());
+  TORCH_CHECK_VALUE(ks.sizes() == kc.sizes().slice(0, 2) && vs.sizes() == ks.sizes() && ks.is_contiguous() &&
+                        vs.is_contiguous() && ks.scalar_type() == at::kByte && vs.scalar_type() == at::kByte,
+                    what, "scales must be two contiguous uint8 tensors [pages, heads], got ", ks.scalar_type(), " ",
+                    ks.sizes(), " and ", vs.scalar_type(), " ", vs.sizes());
+  TORCH_CHECK_VALUE(table.dim() == 2 && (B < 0 || table.size(0) == B) && table.scalar_type() == at::kInt, what,
+                    "page_table must be int32 [B, pages of a sequence], got ", table.scalar_type(), " ", table.sizes());
+  for (const Tensor* t : {&kc, &vc, &ks, &vs, &table}) on_device(*t, dev, what, "the cache and its page table");
+  const bool rows = (table.stride(1) == 1 || table.size(1) <= 1) && (table.size(0) <= 1 || table.stride(0) >= table.size(1));
+  return {kc.size(0), kc.size(1), kc.size(2), kc.size(3), rows ? table : table.contiguous()};
+}
+
+void check_per_item(const optional<Tensor>& t, int64_t B, at::Device dev, const char* what, const char* name) {
+  if (!t) return;
+  TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == B && t->scalar_type() == at::kInt && t->is_contiguous(), what, name,
+                    " must be ", B, " contiguous int32 values, got ", t->scalar_type(), " ", t->sizes());
+  on_device(*t, dev, what, name);
+}
+
+const int32_t* ints(const optional<Tensor>& t) { return t ? t->data_ptr<int32_t>() : nullptr; }
+uint8_t* bytes(const Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
+
+void kv_append(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, const Tensor& page_table,
+               const Tensor& starts, const Tensor& k_in, const Tensor& v_in, const optional<Tensor>& counts,
+               const optional<Tensor>& table, const optional<Tensor>& k_weight, double eps, bool interleaved) {
+  const char* what = "kv_append: ";
+  require_gfx950(k_in, "kv_append");
+  TORCH_CHECK_VALUE(k_in.dim() == 4 && v_in.sizes() == k_in.sizes() && v_in.scalar_type() == k_in.scalar_type(), what,
+                    "k and v must be [B, H, S, D] of one shape and dtype, got ", k_in.sizes(), " and ", v_in.sizes());
+  dtype_code(k_in);
+  const at::Device dev = k_in.device();
+  on_device(v_in, dev, what, "v");
+  const int64_t B = k_in.size(0), H = k_in.size(1), S = k_in.size(2), D = k_in.size(3);
+  const Pool p = pool_of(kc, vc, ks, vs, page_table, B, dev, what);
+  TORCH_CHECK_VALUE(p.H == H && p.D == D, what, "the cache holds ", p.H, " heads of ", p.D, ", got ", k_in.sizes());
+  check_per_item(starts, B, dev, what, "starts");
+  check_per_item(counts, B, dev, what, "counts");
+  if (table) {
+    TORCH_CHECK_VALUE(table->scalar_type() == at::kFloat && table->is_contiguous() &&
+                          (table->dim() == 3 || (table->dim() == 4 && table->size(0) == B)) && table->size(-1) == 2 &&
+                          table->size(-3) == S && 2 * table->size(-2) <= D,
+                      what, "table must be contiguous fp32 [S, P, 2] or [B, S, P, 2] with 2 P <= D, got ",
+                      table->scalar_type(), " ", table->sizes(), " for k ", k_in.sizes());
+    on_device(*table, dev, what, "table");
+  }
+  check_weight(k_weight, D, k_in, what, "k_weight");
+  const Tensor k = rows_of(k_in), v = rows_of(v_in);
+  const int64_t P = table ? table->size(-2) : 0;
+  const c10::DeviceGuard guard(dev);
+  check(mxf8_kv_append(k.data_ptr(), k.strides().data(), v.data_ptr(), v.strides().data(), dtype_code(k), B, H, S, D,
+                       table ? table->data_ptr<float>() : nullptr, table && table->dim() == 4 ? S * P * 2 : 0, P,
+                       k_weight ? k_weight->data_ptr() : nullptr, static_cast<float>(eps), interleaved,
+                       p.table.data_ptr<int32_t>(), p.table.stride(0), p.table.size(1), starts.data_ptr<int32_t>(),
+                       ints(counts), bytes(kc), bytes(vc), bytes(ks), bytes(vs), p.pages, p.page, stream_of(k)),
+        "kv_append");
+}
+
+std::tuple<Tensor, Tensor> kv_read(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs,
+                                   const Tensor& page_table, const Tensor& starts, int64_t tokens,
+                                   const optional<Tensor>& lengths, at::ScalarType dtype) {
+  const char* what = "kv_read: ";
+  require_gfx950(kc, "kv_read");
+  const at::Device dev = kc.device();
+  const Pool p = pool_of(kc, vc, ks, vs, page_table, -1, dev, what);
+  const int64_t B = page_table.size(0);
+  check_per_item(starts, B, dev, what, "starts");
+  check_per_item(lengths, B, dev, what, "lengths");
+  TORCH_CHECK_VALUE(tokens >= 0 && tokens <= (1 << 30), what, "tokens must be from 0 to 2^30, got ", tokens);
+  TORCH_CHECK_VALUE(dtype == at::kBFloat16 || dtype == at::kHalf || dtype == at::kFloat, what, "unsupported dtype ",
+                    dtype);
+  Tensor k = fresh({B, p.H, tokens, p.D}, kc, dtype), v = fresh({B, p.H, tokens, p.D}, kc, dtype);
+  const c10::DeviceGuard guard(dev);
+  check(mxf8_kv_read(bytes(kc), bytes(vc), bytes(ks), bytes(vs), p.pages, p.H, p.page, p.D, p.table.data_ptr<int32_t>(),
+                     p.table.stride(0), p.table.size(1), B, starts.data_ptr<int32_t>(), tokens, ints(lengths),
+                     k.data_ptr(), v.data_ptr(), dtype_code(k), stream_of(kc)),
+        "kv_read");
+  return {k, v};
+}
+
+Tensor kv_attend(const Tensor& q_in, const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs,
+                 const Tensor& page_table, const Tensor& lengths, const optional<Tensor>& q_lengths, bool causal,
+                 double scale) {
+  const char* what = "kv_attend: ";
+  require_gfx950(q_in, "kv_attend");
+  TORCH_CHECK_VALUE(q_in.dim() == 4 && (q_in.scalar_type() == at::kBFloat16 || q_in.scalar_type() == at::kHalf), what,
+                    "q must be bf16 or fp16 [B, H, S, D], got ", q_in.scalar_type(), " ", q_in.sizes());
+  const at::Device dev = q_in.device();
+  const int64_t B = q_in.size(0), H = q_in.size(1), S = q_in.size(2), D = q_in.size(3);
+  const Pool p = pool_of(kc, vc, ks, vs, page_table, B, dev, what);
+  TORCH_CHECK_VALUE(p.D == D && p.H > 0 && H % p.H == 0, what, "the cache holds ", p.H, " heads of ", p.D, ", got q ",
+                    q_in.sizes());
+  check_per_item(lengths, B, dev, what, "lengths");
+  check_per_item(q_lengths, B, dev, what, "q_lengths");
+  const Tensor q = rows_of(q_in);
+  Tensor out = fresh_like(q);
+  if (out.stride(3) != 1) out = at::empty(q.sizes(), q.options());
+  const c10::DeviceGuard guard(dev);
+  const int64_t need = mxf8_kv_attend_workspace_bytes(B, H, p.H, S, D, p.table.size(1), p.page);
+  Tensor work;
+  if (need) work = fresh({need}, q, at::kByte);
+  check(mxf8_kv_attend(q.data_ptr(), q.strides().data(), dtype_code(q), B, H, S, D, bytes(kc), bytes(vc), bytes(ks),
+                       bytes(vs), p.pages, p.H, p.page, p.table.data_ptr<int32_t>(), p.table.stride(0), p.table.size(1),
+                       lengths.data_ptr<int32_t>(), ints(q_lengths), causal, static_cast<float>(scale), out.data_ptr(),
+                       out.strides().data(), need ? work.data_ptr() : nullptr, stream_of(q)),
+        "kv_attend");
+  return out;
+}
+
 // The ops have no derivative.  With grad mode on, an output of an input that requires grad
 // requires grad and its backward raises; otherwise the call goes on below autograd (as the
 // Python declarations' autograd kernel does; forward-mode tangents end here).
@@ -597,11 +719,14 @@ TORCH_LIBRARY_IMPL(mxf8, CUDA, m) {
   m.impl("mxfp4_dequant", &mxfp4_dequant);
   m.impl("gemm_mxfp4", &gemm_mxfp4);
   m.impl("mxfp4_linear", &mxfp4_linear);
+  m.impl("kv_append", &kv_append);
+  m.impl("kv_read", &kv_read);
+  m.impl("kv_attend", &kv_attend);
 }
 
 TORCH_LIBRARY_IMPL(mxf8, AutogradCUDA, m) {
   for (const char* op : {"quant_rows", "adaln_quant_rows", "gemm_rowwise", "lora_down", "attn_quant_kv", "attn_fwd_q",
                          "rotary_table", "rotate_qk", "gated_residual_norm", "mxfp4_quant", "mxfp4_dequant", "gemm_mxfp4",
-                         "mxfp4_linear"})
+                         "mxfp4_linear", "kv_append", "kv_read", "kv_attend"})
     m.impl(op, torch::CppFunction::makeFromBoxedFunction<&no_derivative>());
 }

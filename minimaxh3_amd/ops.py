@@ -7,8 +7,8 @@ breaks.  Outputs come from torch's caching allocator; launches go to the current
 
 The ops of the hot path (quant_rows, adaln_quant_rows, gemm_rowwise, lora_down,
 attn_quant_kv, attn_fwd_q) and of the rest of a DiT block (rotary_table, rotate_qk,
-gated_residual_norm, mxfp4_quant, mxfp4_dequant, gemm_mxfp4, mxfp4_linear) run as native
-dispatcher kernels (csrc/torch_ops.cpp), which are registered when this module is imported:
+gated_residual_norm, mxfp4_quant, mxfp4_dequant, gemm_mxfp4, mxfp4_linear), and those of the
+key / value cache (kv_append, kv_read, kv_attend) run as native dispatcher kernels (csrc/torch_ops.cpp), which are registered when this module is imported:
 the dispatcher reads an operator's kernels without a lock, so none may be added while another
 thread calls it.  Their Python bodies see only what has no native kernel: other devices, and a
 library built after the import.  The other ops call the C ABI from here.
@@ -534,6 +534,55 @@ def mxfp4_linear(x: torch.Tensor, w4: torch.Tensor, sw: torch.Tensor, bias: torc
 @mxfp4_linear.register_fake
 def _(x, w4, sw, bias, act):
     return x.new_empty((x.shape[0], w4.shape[0]), dtype=torch.bfloat16)
+
+
+# ---------------------------------------------------------------------------------------
+# Paged e4m3 cache of keys and values
+# ---------------------------------------------------------------------------------------
+
+@torch.library.custom_op("mxf8::kv_append", mutates_args=("k_codes", "v_codes", "k_scale", "v_scale"))
+def kv_append(k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+              page_table: torch.Tensor, starts: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+              counts: torch.Tensor | None, table: torch.Tensor | None, k_weight: torch.Tensor | None, eps: float,
+              interleaved: bool) -> None:
+    """Quantizes k, v [B, H, S, D] into the pages behind each sequence's first starts[b] tokens, the keys normed
+    (with a weight) and turned (with a table) before."""
+    _native(k, "kv_append")(k_codes, v_codes, k_scale, v_scale, page_table, starts, k, v, counts, table, k_weight, eps,
+                            interleaved)
+
+
+@kv_append.register_fake
+def _(k_codes, v_codes, k_scale, v_scale, page_table, starts, k, v, counts, table, k_weight, eps, interleaved):
+    return None
+
+
+@torch.library.custom_op("mxf8::kv_read", mutates_args=())
+def kv_read(k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+            page_table: torch.Tensor, starts: torch.Tensor, tokens: int, lengths: torch.Tensor | None,
+            dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    """The values of `tokens` tokens of each sequence from starts[b] on, k and v [B, H, tokens, D] of `dtype`."""
+    return _native(k_codes, "kv_read")(k_codes, v_codes, k_scale, v_scale, page_table, starts, tokens, lengths, dtype)
+
+
+@kv_read.register_fake
+def _(k_codes, v_codes, k_scale, v_scale, page_table, starts, tokens, lengths, dtype):
+    shape = (page_table.shape[0], k_codes.shape[1], tokens, k_codes.shape[3])
+    return k_codes.new_empty(shape, dtype=dtype), k_codes.new_empty(shape, dtype=dtype)
+
+
+@torch.library.custom_op("mxf8::kv_attend", mutates_args=())
+def kv_attend(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor,
+              v_scale: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, q_lengths: torch.Tensor | None,
+              causal: bool, scale: float) -> torch.Tensor:
+    """softmax(scale q k^T) v of q [B, H, S, D] over the first lengths[b] tokens of each sequence's pages; the output
+    keeps q's order of dimensions in memory."""
+    return _native(q, "kv_attend")(q, k_codes, v_codes, k_scale, v_scale, page_table, lengths, q_lengths, causal, scale)
+
+
+@kv_attend.register_fake
+def _(q, k_codes, v_codes, k_scale, v_scale, page_table, lengths, q_lengths, causal, scale):
+    o = torch.empty_like(q if q.stride(-1) == 1 else q.contiguous())
+    return o if o.stride(-1) == 1 else q.new_empty(q.shape)
 
 
 def _register() -> None:

@@ -1,0 +1,633 @@
+"""The paged e4m3 cache of keys and values, and the attention over it, against the 64-bit oracle.
+
+Codes are exact but where the unrounded key lies within its 32-bit evaluation's bound of a border between two.
+The attention's outputs: half a step of the output type, and 2^-10 of sum p |v| / sum p.  Of that half are the
+probabilities' own half steps in fp16 (2^-11 each); the scores' fp32 sums over D products (D 2^-24 of
+sum |q k| scale, under 2^-13 for scores of size 10), exp2, the row sum and probabilities below fp16's normal range (2^-25
+of the largest each) share the other half."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from minimaxh3_amd import ops
+from minimaxh3_amd.kernels.kv_cache import FP8KVCache, append_kv, cached_attention, read_kv
+from minimaxh3_amd.kernels.rotary import rotary_table, rotate_qk
+from oracle import dit_block as ob
+from oracle import kv_cache as ok
+from oracle.numerics import e4m3_decode
+
+pytestmark = pytest.mark.gpu
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def f64(t):
+    return t.detach().to("cpu", torch.float64).numpy()
+
+
+def i32(*v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def raw(cache):
+    return ([t.view(torch.uint8).cpu().numpy() for t in (cache.k, cache.v)],
+            [t.cpu().numpy() for t in (cache.k_scale, cache.v_scale)])
+
+
+def random_cache(seed, pages, heads, page, d, spread=3):
+    """Any codes but NaN, under exponents of -spread - 6 ... spread - 6."""
+    g = torch.Generator().manual_seed(seed)
+    codes = [torch.randint(0, 127, (pages, heads, page, d), generator=g, dtype=torch.uint8)
+             + 128 * torch.randint(0, 2, (pages, heads, page, d), generator=g, dtype=torch.uint8) for _ in range(2)]
+    # (sizes up to 448 would let one product decide a row: most codes of 1 and below)
+    codes = [torch.where(c % 128 > 56, c - 56 // 8 * 8, c) for c in codes]
+    scales = [torch.randint(121 - spread, 122 + spread, (pages, heads), generator=g, dtype=torch.uint8) for _ in range(2)]
+    return FP8KVCache.from_tensors(*[t.cuda() for t in codes + scales])
+
+
+def normal_cache(seed, pages, heads, page, d, table, lengths, k_std=1.0, v_std=1.0):
+    """A cache that holds normal keys and values, appended."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    cache = FP8KVCache(pages, heads, d, page)
+    S, B = table.shape[1] * page, table.shape[0]
+    k, v = (torch.randn((B, heads, S, d), generator=g, device="cuda") * s for s in (k_std, v_std))
+    append_kv(cache, table, torch.zeros(B, dtype=torch.int32, device="cuda"), k, v, counts=lengths)
+    return cache
+
+
+def pages_for(seed, b, width, extra=3):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randperm(b * width + extra, generator=g)[: b * width].to(torch.int32).view(b, width).cuda()
+
+
+# ---------------------------------------------------------------------------------------
+# append, read
+# ---------------------------------------------------------------------------------------
+
+def check_append(cache, table, starts, k, v, counts=None, turns=None, weight=None, interleaved=True):
+    pool = ok.Pool(*raw(cache))
+    before = pool.copy()
+    append_kv(cache, table, starts, k, v, counts=counts, table=turns, k_weight=weight, interleaved=interleaved)
+    tb, st = table.cpu().numpy(), starts.cpu().numpy()
+    cn = None if counts is None else counts.cpu().numpy()
+    key, _, bound = ok.append(pool, tb, st, f64(k), f64(v), cn, None if turns is None else f64(turns),
+                              None if weight is None else f64(weight), 1e-6, interleaved)
+    codes, scales = raw(cache)
+    assert np.array_equal(scales[0], pool.scales[0]) and np.array_equal(scales[1], pool.scales[1])
+    assert np.array_equal(codes[1], pool.codes[1])
+    wrong = codes[0] != pool.codes[0]
+    if turns is None and weight is None:
+        assert not wrong.any()
+    elif wrong.any():
+        # each as near to the unrounded key as the oracle's, within what 32 bits may add
+        for b in range(len(st)):
+            for s in range(k.shape[2] if cn is None else min(max(cn[b], 0), k.shape[2])):
+                at = pool.at(tb, b, int(st[b]) + s)
+                if at is None or not wrong[at[0], :, at[1]].any():
+                    continue
+                e = pool.scales[0][at[0]].astype(int)[:, None] - 127
+                got, ref = (np.ldexp(e4m3_decode(c[0][at[0], :, at[1]]).astype(np.float64), e) for c in (codes, pool.codes))
+                x, near = key[b, :, s], bound[b, :, s]
+                assert (np.abs(got - x) <= np.abs(ref - x) + 2 * near).all()
+                wrong[at[0], :, at[1]] = False
+        assert not wrong.any()  # and nothing else differs
+    return before, pool
+
+
+@pytest.mark.parametrize("d,page", [(128, 16), (128, 32), (128, 64), (128, 128), (64, 16), (64, 32), (64, 64), (64, 128)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_append_plain(d, page, dtype):
+    g = torch.Generator().manual_seed(page + d)
+    b, h, s = 3, 3, 2 * page + 5
+    cache = random_cache(1, 40, h, page, d)
+    table = pages_for(2, b, 6)
+    qkv = (torch.randn((b, s, 3, h, d), generator=g) * torch.exp2(torch.randint(-9, 9, (b, s, 1, 1, 1), generator=g))).to(DT[dtype]).cuda()
+    k, v = (qkv[:, :, i].transpose(1, 2) for i in (1, 2))
+    check_append(cache, table, i32(0, page - 1, 2 * page + 3), k, v)
+    check_append(cache, table, i32(5, page, 3 * page - 7), k, v, counts=i32(s, 1, s + 9))
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("weighted", [True, False])
+@pytest.mark.parametrize("d,p", [(128, 64), (128, 48), (128, 21), (64, 32), (64, 8), (64, 1), (64, 0)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_append_turned(interleaved, weighted, d, p, dtype):
+    g = torch.Generator().manual_seed(p)
+    b, h, s, page = 2, 2, 83, 32
+    cache, table = random_cache(3, 16, h, page, d), pages_for(4, b, 5)
+    k, v = (torch.randn((b, h, s, d), generator=g).to(DT[dtype]).cuda() for _ in range(2))
+    angle = torch.rand((b, s, p) if p == 48 else (s, p), generator=g) * 7
+    turns = torch.stack([angle.cos(), angle.sin()], -1).cuda()
+    w = (1 + 0.2 * torch.randn(d, generator=g)).to(DT[dtype]).cuda() if weighted else None
+    check_append(cache, table, i32(0, 40), k, v, turns=turns, weight=w, interleaved=interleaved)
+
+
+@pytest.mark.parametrize("d,page", [(128, 64), (64, 16), (128, 128)])
+def test_append_one_token_at_a_time(d, page):
+    """Sizes that grow and fall: pages whose exponent rises under what they hold."""
+    g = torch.Generator().manual_seed(5)
+    cache, table = FP8KVCache(12, 2, d, page), pages_for(6, 2, 3)
+    for t in range(0, 2 * page + 3, 3 if page > 16 else 1):
+        k, v = (torch.randn((2, 2, 1, d), generator=g) * 2.0 ** float(torch.randint(-6, 7, (1,), generator=g)) for _ in range(2))
+        check_append(cache, table, i32(t, max(0, t - 5)), k.bfloat16().cuda(), v.bfloat16().cuda())
+
+
+def test_append_special_values():
+    cache, table = FP8KVCache(8, 1, 64, 16), pages_for(1, 1, 4)
+    x = torch.randn((1, 1, 48, 64), generator=torch.Generator().manual_seed(1))
+    x[0, 0, 3, 7], x[0, 0, 20] = float("inf"), 0.0
+    x[0, 0, 33, 5], x[0, 0, 34, 5], x[0, 0, 35] = 3e38, -1e-38, 1e25
+    v = x.clone()
+    v[0, 0, 9, 63], x[0, 0, 11, 1] = float("nan"), float("nan")
+    x[0, 0, 16:32], v[0, 0, 16:32] = 0.0, -0.0
+    check_append(cache, table, i32(0), x.cuda(), v.cuda())
+    k, w = read_kv(cache, table, i32(0), 48, dtype=torch.float32)
+    assert torch.isnan(k[0, 0, 9, 0]) and torch.isnan(k[0, 0, 11, 0]) and torch.isfinite(w).all()
+    assert torch.isnan(k).sum() == 2 and (k[0, 0, 16:32] == 0).all()
+    # a value of the page is the largest, an infinity as large as the scale allows; the other tokens keep theirs
+    assert k[0, 0, 3, 7] == k[0, 0, 3, 7].abs() > 2 and (w[0, 0, 0] - v[0, 0, 0].cuda()).abs().max() < 0.2
+
+
+def test_append_where_there_is_no_page():
+    page, d = 16, 64
+    cache, g = random_cache(8, 6, 2, page, d), torch.Generator().manual_seed(2)
+    k, v = (torch.randn((4, 2, 40, d), generator=g).bfloat16().cuda() for _ in range(2))
+    table = torch.tensor([[0, -1, 1], [6, 2, 2 ** 31 - 1], [-(2 ** 31), 3, 4], [5, -1, -1]], dtype=torch.int32, device="cuda")
+    # behind the table's end, before its beginning, and all of a sequence
+    check_append(cache, table, i32(3, 30, -20, 2 ** 30), k, v)
+    before = raw(cache)
+    for kwargs in ({"counts": i32(0, -3, 0, 0)}, {}):
+        append_kv(cache, table[:, :0] if not kwargs else table, i32(0, 0, 0, 0), k, v, **kwargs)
+    append_kv(cache, table[:0], i32(), k[:0], v[:0])
+    append_kv(cache, table, i32(0, 0, 0, 0), k[:, :, :0], v[:, :, :0])
+    assert all(np.array_equal(a, b) for x, y in zip(before, raw(cache)) for a, b in zip(x, y))
+
+
+def test_append_any_strides():
+    g = torch.Generator().manual_seed(3)
+    base = torch.randn((2, 3, 41, 2 * 64 + 1), generator=g).bfloat16().cuda()
+    for view in (base[..., 1:65], base[..., ::2][..., :64], base[..., :64].transpose(0, 1)[:2], base[:1, :, :, :64].expand(2, -1, -1, -1)):
+        h = view.shape[1]
+        a, b = FP8KVCache(12, h, 64, 16), FP8KVCache(12, h, 64, 16)
+        table = pages_for(3, 2, 4, extra=4)
+        for cache, x in ((a, view), (b, view.contiguous())):
+            append_kv(cache, table, i32(7, 16), x, x)
+        assert all(torch.equal(s.view(torch.uint8), t.view(torch.uint8)) for s, t in zip(a.tensors(), b.tensors()))
+    wide = torch.full((2, 9), -1, dtype=torch.int32, device="cuda")
+    wide[:, 2:6] = table
+    c = FP8KVCache(12, h, 64, 16)
+    append_kv(c, wide[:, 2:6], i32(7, 16), view, view)  # a view of a table
+    assert torch.equal(c.k.view(torch.uint8), b.k.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("d,page", [(128, 64), (64, 16)])
+def test_read(dtype, d, page):
+    cache, table = random_cache(4, 9, 3, page, d), pages_for(5, 2, 4, extra=0)
+    table[1, 1] = -1
+    pool = ok.Pool(*raw(cache))
+    for starts, t, lengths in ((i32(0, 3), 4 * page + 3, None), (i32(page - 1, -2), 11, i32(page + 4, 5)), (i32(1, 1), 0, None)):
+        got = read_kv(cache, table, starts, t, lengths=lengths, dtype=DT[dtype])
+        ref = ok.read(pool, table.cpu().numpy(), starts.cpu().numpy(), t, None if lengths is None else lengths.cpu().numpy())
+        for a, b in zip(got, ref):
+            assert a.dtype == DT[dtype] and torch.equal(a.cpu(), torch.from_numpy(b).to(DT[dtype]))
+
+
+# ---------------------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------------------
+
+def check_attend(q, cache, table, lengths, causal=False, q_lengths=None, scale=None):
+    got = cached_attention(q, cache, table, lengths, causal=causal, q_lengths=q_lengths, scale=scale)
+    assert got.shape == q.shape and got.dtype == q.dtype
+    pool = ok.Pool(*raw(cache))
+    tb, T = table.cpu().numpy(), table.shape[1] * cache.page_size
+    k, v = ok.read(pool, tb, np.zeros(len(tb), int), T)
+    there = np.repeat((tb >= 0) & (tb < cache.pages), cache.page_size, 1)
+    c = q.shape[-1] ** -0.5 if scale is None else scale
+    o, a = ok.attend(f64(q), k, v, there, lengths.cpu().numpy(), c, causal,
+                     None if q_lengths is None else q_lengths.cpu().numpy())
+    name = "bf16" if q.dtype == torch.bfloat16 else "fp16"
+    tol = 2.0 ** -10 * a
+    err = np.abs(f64(got) - o)
+    assert (err <= tol + ob.half_step(np.abs(o) + tol, name)).all(), ((err - tol).max(), np.argwhere(err > tol + ob.half_step(np.abs(o) + tol, name))[:5])
+    assert (f64(got)[a.sum(-1) == 0] == 0).all()  # rows that see nothing
+    return got
+
+
+SHAPES = [  # B, H, Hk, S, D, page
+    (1, 1, 1, 1, 64, 16), (2, 4, 4, 1, 128, 64), (3, 8, 2, 1, 128, 16), (2, 7, 1, 1, 64, 32), (1, 16, 1, 1, 128, 128),
+    (2, 5, 5, 3, 64, 64), (1, 40, 8, 5, 64, 32), (2, 8, 1, 2, 128, 64), (1, 4, 2, 13, 128, 16), (2, 3, 1, 17, 128, 32),
+    (1, 2, 2, 64, 64, 16), (1, 2, 2, 65, 128, 64), (1, 6, 2, 100, 128, 16), (2, 1, 1, 129, 64, 128), (1, 2, 1, 150, 64, 32),
+    (1, 2, 2, 257, 128, 64),
+]
+
+
+@pytest.mark.parametrize("B,H,Hk,S,D,page", SHAPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_attend(B, H, Hk, S, D, page, causal, dtype):
+    g = torch.Generator().manual_seed(S + H)
+    width = -(-(S + 70) // page) + 1
+    table = pages_for(S, B, width)
+    T = width * page
+    lengths = torch.tensor([T, S + 33, 1][:B], dtype=torch.int32, device="cuda")
+    cache = normal_cache(D + page, B * width + 3, Hk, page, D, table, lengths)
+    q = torch.randn((B, S, H, D), generator=g).to(DT[dtype]).cuda().transpose(1, 2)
+    got = check_attend(q, cache, table, lengths, causal)
+    assert got.transpose(1, 2).is_contiguous()
+
+
+@pytest.mark.parametrize("S,H,Hk", [(1, 4, 4), (1, 8, 2), (5, 4, 1), (70, 2, 2), (140, 2, 1)])
+@pytest.mark.parametrize("length", [0, 1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 127, 128, 129, 255, 300])
+def test_attend_lengths(S, H, Hk, length):
+    table = pages_for(length, 1, 20)
+    cache = normal_cache(length, 23, Hk, 16, 64, table, i32(length))
+    q = torch.randn((1, H, S, 64), generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    check_attend(q, cache, table, i32(length))
+    check_attend(q, cache, table, i32(length), causal=True)
+
+
+@pytest.mark.parametrize("S,H,Hk,D", [(1, 4, 4, 128), (3, 8, 2, 64), (90, 2, 2, 128), (200, 4, 2, 64)])
+def test_attend_ragged(S, H, Hk, D):
+    """Queries that are not there, sequences longer than their tables, shorter than nothing, or fewer than the queries."""
+    B, page, width = 6, 32, 7
+    table = pages_for(9, B, width)
+    lengths = i32(100, 224, 3, 0, 10 ** 6, -5)
+    cache = normal_cache(2, B * width + 3, Hk, page, D, table, lengths)
+    q = torch.randn((B, H, S, D), generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    q[1, :, 1:] = float("nan")  # not there
+    q_lengths = i32(S, 1, S, S, S + 5, S)
+    for causal in (False, True):
+        check_attend(torch.nan_to_num(q), cache, table, lengths, causal, q_lengths)
+        got = cached_attention(q, cache, table, lengths, causal=causal, q_lengths=q_lengths)
+        assert torch.equal(got, cached_attention(torch.nan_to_num(q), cache, table, lengths, causal=causal, q_lengths=q_lengths))
+        assert (got[1, :, 1:] == 0).all()
+    check_attend(torch.nan_to_num(q), cache, table, lengths, True, i32(0, -1, S, 1, S, S))
+
+
+@pytest.mark.parametrize("S,H,Hk", [(1, 4, 2), (2, 4, 1), (80, 2, 2)])
+def test_attend_missing_pages(S, H, Hk):
+    table = pages_for(3, 2, 12)
+    cache = normal_cache(3, 27, Hk, 16, 128, table, i32(192, 192))
+    table[0, 2:5], table[0, 11], table[1, :] = -1, 27, 2 ** 31 - 1
+    q = torch.randn((2, H, S, 128), generator=torch.Generator().manual_seed(3)).half().cuda()
+    got = check_attend(q, cache, table, i32(190, 192))
+    assert (got[1] == 0).all()
+    check_attend(q, cache, table, i32(190, 192), causal=True)
+
+
+@pytest.mark.parametrize("S,H,Hk", [(1, 4, 2), (6, 4, 1), (130, 2, 2)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attend_what_is_not_there_changes_nothing(S, H, Hk, D):
+    """NaN codes and any scales behind a sequence's end and in pages that it does not name."""
+    table = pages_for(4, 1, 12)
+    lengths = i32(16 * 9 + 5)
+    cache = normal_cache(4, 15, Hk, 16, D, table, lengths)
+    q = torch.randn((1, H, S, D), generator=torch.Generator().manual_seed(4)).bfloat16().cuda()
+    want = [cached_attention(q, cache, table, lengths, causal=c) for c in (False, True)]
+    used = set(table[0, :10].tolist())
+    for t in (cache.k, cache.v):
+        t.view(torch.uint8)[int(table[0, 9]), :, 5:] = 0x7F
+        for p in set(range(15)) - used:
+            t.view(torch.uint8)[p] = 0xFF
+            cache.k_scale[p], cache.v_scale[p] = 255, 0
+    for c, w in zip((False, True), want):
+        assert torch.equal(cached_attention(q, cache, table, lengths, causal=c), w)
+
+
+@pytest.mark.parametrize("S,H,Hk", [(1, 4, 2), (20, 2, 1), (150, 2, 2)])
+def test_attend_nan_reaches_those_that_see_it(S, H, Hk):
+    """A NaN in one token's value: rows that see the token are NaN, causal rows before it are not."""
+    table, n = pages_for(5, 1, 12), 180
+    g = torch.Generator().manual_seed(5)
+    k, v = (torch.randn((1, Hk, n, 64), generator=g).bfloat16().cuda() for _ in range(2))
+    at = n - S // 2 - 1
+    v[0, 0, at, 3] = float("nan")
+    cache = FP8KVCache(15, Hk, 64, 16)
+    append_kv(cache, table, i32(0), k, v)
+    q = torch.randn((1, H, S, 64), generator=g).bfloat16().cuda()
+    bad = torch.isnan(cached_attention(q, cache, table, i32(n), causal=True)).all(-1)
+    part = torch.isnan(cached_attention(q, cache, table, i32(n), causal=True)).any(-1)
+    sees = (torch.arange(S) + n - S >= at).cuda()
+    heads = (torch.arange(H) // (H // Hk) == 0).cuda()
+    assert torch.equal(bad[0], sees & heads[:, None]) and torch.equal(bad, part)
+
+
+@pytest.mark.parametrize("S,H,Hk", [(1, 4, 2), (3, 8, 1), (100, 2, 2)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attend_any_scales(S, H, Hk, D):
+    """Pages, values, queries and scores of very different sizes."""
+    table = pages_for(6, 1, 12)
+    q = torch.randn((1, H, S, D), generator=torch.Generator().manual_seed(6)).bfloat16().cuda()
+    cache = random_cache(6, 15, Hk, 16, D, spread=5)
+    check_attend(q, cache, table, i32(185), scale=0.3)
+    cache.v_scale.copy_(torch.randint(95, 191, cache.v_scale.shape, generator=torch.Generator().manual_seed(7)))
+    check_attend(q, cache, table, i32(185), scale=0.01)
+    # one page of the largest values, one of the smallest, the others zeros of the lowest exponent
+    cache = FP8KVCache.from_tensors(cache.k.view(torch.uint8), torch.zeros_like(cache.v.view(torch.uint8)), cache.k_scale,
+                                    torch.full_like(cache.v_scale, 95))
+    cache.v_scale[int(table[0, 1])], cache.v_scale[int(table[0, 8])] = 190, 95
+    cache.v[int(table[0, 1])], cache.v[int(table[0, 8])] = 448.0, 0.5
+    check_attend(q, cache, table, i32(185), scale=0.05)
+    cache.v_scale[int(table[0, 1])] = 127
+    for size in (2.0 ** -40, 2.0 ** 30):  # queries beyond fp16's range under a scale that brings the scores back
+        check_attend((q.float() * size).bfloat16(), cache, table, i32(185), scale=0.1 / size)
+    check_attend(torch.zeros_like(q), cache, table, i32(185))
+
+
+@pytest.mark.parametrize("S,H,Hk", [(1, 2, 2), (4, 8, 2), (70, 2, 1)])
+def test_attend_scores_that_grow(S, H, Hk):
+    """Each page's scores larger than the last's, and the other way round: the running maximum moves at every step."""
+    table = pages_for(7, 1, 16)
+    k = torch.randn((1, Hk, 256, 64), generator=torch.Generator().manual_seed(8))
+    v = torch.randn((1, Hk, 256, 64), generator=torch.Generator().manual_seed(9))
+    q = torch.randn((1, H, S, 64), generator=torch.Generator().manual_seed(10)).bfloat16()
+    q[..., 0] = 8.0
+    for ramp in (torch.linspace(0, 60, 256), torch.linspace(60, 0, 256), 30 * torch.sin(torch.arange(256.0))):
+        k[..., 0] = ramp
+        cache = FP8KVCache(19, Hk, 64, 16)
+        append_kv(cache, table, i32(0), k.cuda(), v.cuda())
+        check_attend(q.cuda(), cache, table, i32(256), scale=0.125)
+
+
+def test_attend_strides():
+    table = pages_for(8, 2, 10)
+    cache = normal_cache(8, 23, 2, 16, 64, table, i32(150, 160))
+    base = torch.randn((2, 4, 90, 2 * 64 + 1), generator=torch.Generator().manual_seed(8)).bfloat16().cuda()
+    for n in (1, 3, 90):
+        for view in (base[:, :, :n, 1:65], base[:, :, :n, ::2][..., :64], base[:1, :, :n, 3:67].expand(2, -1, -1, -1),
+                     base[:, :2, :n, :64].repeat_interleave(2, 1)):
+            want = cached_attention(view.contiguous(), cache, table, i32(150, 160), causal=True)
+            assert torch.equal(cached_attention(view, cache, table, i32(150, 160), causal=True), want)
+    wide = torch.full((2, 15), -1, dtype=torch.int32, device="cuda")
+    wide[:, 2:12] = table
+    assert torch.equal(cached_attention(view, cache, wide[:, 2:12], i32(150, 160), causal=True), want)
+
+
+def test_attend_empty():
+    cache = FP8KVCache(2, 2, 64)
+    table = torch.zeros((1, 1), dtype=torch.int32, device="cuda")
+    q = torch.randn((1, 2, 3, 64), device="cuda").bfloat16()
+    assert (cached_attention(q, cache, table[:, :0], i32(5)) == 0).all()
+    assert cached_attention(q[:, :, :0], cache, table, i32(5)).shape == (1, 2, 0, 64)
+    assert cached_attention(q[:0], cache, table[:0], i32()).shape == (0, 2, 3, 64)
+    assert (cached_attention(q, FP8KVCache(0, 2, 64), table, i32(5)) == 0).all()
+
+
+def reference(q, cache, table, lengths, causal, q_lengths=None):
+    """Larger calls in 64 bits on the GPU: (o, sum p |v| / sum p)."""
+    B, H, S, D = q.shape
+    T = table.shape[1] * cache.page_size
+    k, v = (t.double() for t in read_kv(cache, table, torch.zeros_like(lengths), T, dtype=torch.float32))
+    o, a = torch.zeros((2, B, H, S, D), dtype=torch.float64, device="cuda")
+    for b in range(B):
+        n, length = S if q_lengths is None else int(q_lengths[b]), int(lengths[b])
+        for h in range(H):
+            kk, vv = (t[b, h * cache.heads // H, :length] for t in (k, v))
+            x = q[b, h, :n].double() @ kk.t() / math.sqrt(D)
+            if causal:
+                x = x.masked_fill(torch.arange(length, device="cuda") > length - n + torch.arange(n, device="cuda")[:, None], -math.inf)
+            p = torch.softmax(x, -1)
+            o[b, h, :n], a[b, h, :n] = p @ vv, p @ vv.abs()
+    return o, a
+
+
+@pytest.mark.parametrize("B,H,Hk,S,D,page,length,causal,dtype", [
+    (1, 24, 24, 1, 128, 64, 20281, False, "bf16"),    # one query of a whole clip
+    (1, 32, 8, 1, 128, 64, 131072, False, "bf16"),    # a very long cache, split
+    (5, 16, 2, 3, 64, 16, 5001, True, "fp16"),
+    (9, 8, 8, 1, 128, 128, 1999, True, "bf16"),
+    (1, 24, 24, 1560, 128, 64, 4680, False, "bf16"),  # a frame over three
+    (2, 8, 2, 777, 64, 32, 2049, True, "fp16"),
+    (1, 4, 4, 5000, 128, 64, 513, False, "bf16"),     # a clip over its text
+    (1, 2, 1, 3001, 128, 16, 3001, True, "bf16"),     # a prompt
+    (1, 1, 1, 300, 128, 64, 50001, False, "bf16"),    # few rows over many keys
+])
+def test_attend_large(B, H, Hk, S, D, page, length, causal, dtype):
+    width = -(-length // page)
+    lengths = torch.tensor([length - i * (length // (B + 1)) for i in range(B)], dtype=torch.int32, device="cuda")
+    q_lengths = None if B == 1 else torch.tensor([max(1, S - i * 40) for i in range(B)], dtype=torch.int32, device="cuda")
+    table = pages_for(length, B, width)
+    cache = normal_cache(length, B * width + 3, Hk, page, D, table, lengths, k_std=1.5)
+    q = torch.randn((B, S, H, D), generator=torch.Generator().manual_seed(S)).to(DT[dtype]).cuda().transpose(1, 2)
+    got = cached_attention(q, cache, table, lengths, causal=causal, q_lengths=q_lengths)
+    o, a = reference(q, cache, table, lengths, causal, q_lengths)
+    tol = 2.0 ** -10 * a
+    tol = tol + (o.abs() + tol) * torch.finfo(q.dtype).eps / 2 + 2.0 ** -25
+    assert ((got.double() - o).abs() <= tol).all(), ((got.double() - o).abs() / tol).max()
+    assert torch.equal(got, cached_attention(q, cache, table, lengths, causal=causal, q_lengths=q_lengths))
+
+
+def test_pages_beyond_four_gigabytes():
+    """Pages and tensors whose offsets need more than 32 bits."""
+    pages, page, h, d = 700_000, 16, 4, 128  # 5.7e9 codes each
+    cache = FP8KVCache(pages, h, d, page)
+    table = torch.tensor([[pages - 1, 5, pages - 2, pages // 2]], dtype=torch.int32, device="cuda")
+    small, low = FP8KVCache(4, h, d, page), torch.arange(4, dtype=torch.int32, device="cuda")[None]
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn((1, h, 60, d), generator=g).bfloat16().cuda() for _ in range(2))
+    for c, t in ((cache, table), (small, low)):
+        append_kv(c, t, i32(2), k, v)
+    for a, b in zip(read_kv(cache, table, i32(0), 62), read_kv(small, low, i32(0), 62)):
+        assert torch.equal(a, b)
+    for s in (1, 90):
+        q = torch.randn((1, 8, s, d), generator=g).bfloat16().cuda()
+        assert torch.equal(cached_attention(q, cache, table, i32(62)), cached_attention(q, small, low, i32(62)))
+
+
+# ---------------------------------------------------------------------------------------
+# a run of them
+# ---------------------------------------------------------------------------------------
+
+H, D, FRAME = 3, 128, 60
+
+
+class Clip:
+    """Frames generated one after another: each is appended at every denoising step at the same place, and attends to
+    the clip and itself."""
+
+    def __init__(self, frames=5, page=32):
+        self.cache = FP8KVCache(frames * FRAME // page + 3, H, D, page)
+        self.table = pages_for(11, 1, frames * FRAME // page + 1, extra=0)
+        g = torch.Generator().manual_seed(11)
+        self.qw, self.kw = ((1 + 0.2 * torch.randn(D, generator=g)).bfloat16().cuda() for _ in range(2))
+
+    def step(self, x, frame, start, length):
+        """x [1, S, 3, H, D]; start, length: device tensors."""
+        pos = torch.stack([torch.full((FRAME,), frame), torch.arange(FRAME) // 10, torch.arange(FRAME) % 10], -1)
+        table = self.turns[frame] if hasattr(self, "turns") else rotary_table(pos.cuda(), (44, 42, 42))
+        q, k, v = (t.transpose(1, 2) for t in x.unbind(2))
+        q, _ = rotate_qk(q, None, table, self.qw)
+        append_kv(self.cache, self.table, start, k, v, table=table, k_weight=self.kw)
+        return cached_attention(q, self.cache, self.table, length), q, table
+
+
+@torch.no_grad()
+def test_a_clip_frame_by_frame():
+    clip, g = Clip(), torch.Generator().manual_seed(12)
+    pool = ok.Pool(*raw(clip.cache))
+    tb = clip.table.cpu().numpy()
+    for frame in range(5):
+        start, length = i32(frame * FRAME), i32((frame + 1) * FRAME)
+        for step in range(2):
+            x = torch.randn((1, FRAME, 3, H, D), generator=g).bfloat16().cuda()
+            got, q, table = clip.step(x, frame, start, length)
+            k, v = (x[:, :, i].transpose(1, 2) for i in (1, 2))
+            ok.append(pool, tb, [frame * FRAME], f64(k), f64(v), None, f64(table), f64(clip.kw))
+            codes, scales = raw(clip.cache)
+            assert (codes[0] != pool.codes[0]).mean() < 1e-4 and np.array_equal(codes[1], pool.codes[1])
+            assert all(np.array_equal(s, t) for s, t in zip(scales, pool.scales))
+            pool.codes[0] = codes[0]  # (a border's other side, as above)
+            kk, vv = ok.read(pool, tb, [0], (frame + 1) * FRAME)
+            o, a = ok.attend(f64(q), kk, vv, np.ones((1, kk.shape[2]), bool), [kk.shape[2]], D ** -0.5)
+            tol = 2.0 ** -10 * a
+            assert (np.abs(f64(got) - o) <= tol + ob.half_step(np.abs(o) + tol, "bf16")).all()
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("S,Hq,Hk", [(FRAME, 3, 3), (1, 12, 3)])
+def test_a_captured_step_replays(S, Hq, Hk):
+    """One graph for every token or frame: starts and lengths are read on the device.  Eager work in between."""
+    cache, eager = FP8KVCache(40, Hk, D, 16), FP8KVCache(40, Hk, D, 16)
+    table = pages_for(13, 1, 30)
+    g = torch.Generator().manual_seed(13)
+    q, k, v = (torch.zeros((1, h, S, D), dtype=torch.bfloat16, device="cuda") for h in (Hq, Hk, Hk))
+    start, length = i32(0), i32(S)
+
+    def step():
+        append_kv(cache, table, start, k, v)
+        o = cached_attention(q, cache, table, length, causal=True)
+        start.add_(S)
+        length.add_(S)
+        return o
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    start.zero_(), length.fill_(S)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(6):
+        new = [torch.randn(t.shape, generator=g).bfloat16().cuda() for t in (q, k, v)]
+        for t, n in zip((q, k, v), new):
+            t.copy_(n)
+        graph.replay()
+        append_kv(eager, table, i32(i * S), new[1], new[2])
+        want = cached_attention(new[0], eager, table, i32(i * S + S), causal=True)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+
+
+@torch.no_grad()
+def test_two_streams_and_graphs_at_once():
+    table = pages_for(14, 1, 200)
+    caches = [normal_cache(s, 203, 4, 16, D, table, i32(3100)) for s in (1, 2)]
+    qs = [torch.randn((1, 8, s, D), generator=torch.Generator().manual_seed(s)).bfloat16().cuda() for s in (1, 130)]
+    lengths = i32(3100)
+    want = [[cached_attention(q, c, table, lengths) for q in qs] for c in caches]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in caches]
+    for _ in range(5):
+        got = []
+        for c, st in zip(caches, streams):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                got.append([cached_attention(q, c, table, lengths) for q in qs])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
+    graphs, outs = [], []
+    for c in caches:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append([cached_attention(q, c, table, lengths) for q in qs])
+    for _ in range(4):
+        for gr, st in zip(graphs, streams):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                gr.replay()
+        eager = cached_attention(qs[0], caches[0], table, lengths)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want[0][0])
+        assert all(torch.equal(a, b) for x, y in zip(outs, want) for a, b in zip(x, y))
+
+
+@torch.no_grad()
+def test_compiled_step():
+    clip, ref = Clip(), Clip()
+    x = torch.randn((1, FRAME, 3, H, D), generator=torch.Generator().manual_seed(15)).bfloat16().cuda()
+    pos = torch.stack([torch.zeros(FRAME), torch.arange(FRAME) // 10, torch.arange(FRAME) % 10], -1)
+    clip.turns = ref.turns = [rotary_table(pos.cuda(), (44, 42, 42))]
+    start, length = i32(0), i32(FRAME)
+    want = ref.step(x, 0, start, length)[0]
+
+    def f(x, start, length):
+        return clip.step(x, 0, start, length)[0]
+
+    compiled = torch.compile(f, backend="eager", fullgraph=True)
+    assert torch.equal(compiled(x, start, length), want)
+    assert torch.equal(clip.cache.k.view(torch.uint8), ref.cache.k.view(torch.uint8))
+
+
+def test_dispatcher_checks_and_derivatives():
+    cache, table = random_cache(1, 6, 2, 16, 64), pages_for(1, 1, 3)
+    k, v = (torch.randn((1, 2, 5, 64), device="cuda").bfloat16() for _ in range(2))
+    q = torch.randn((1, 4, 3, 64), device="cuda").bfloat16()
+    tests = ("test_faketensor",)  # (test_schema compares inputs by a product, which torch has none of in e4m3)
+    torch.library.opcheck(ops.kv_append, (*cache.tensors(), table, i32(3), k, v, None, None, None, 1e-6, True), test_utils=tests)
+    torch.library.opcheck(ops.kv_read, (*cache.tensors(), table, i32(3), 7, None, torch.float16), test_utils=tests)
+    torch.library.opcheck(ops.kv_attend, (q, *cache.tensors(), table, i32(30), None, False, 0.1), test_utils=tests)
+    version = cache.k._version
+    append_kv(cache, table, i32(3), k.requires_grad_(), v)
+    assert cache.k._version > version  # a write in place, for whoever saved the codes
+    out = cached_attention(q.requires_grad_(), cache, table, i32(30))
+    with pytest.raises(RuntimeError, match="kv_attend"):
+        out.float().sum().backward()
+
+
+def test_refusals():
+    cache, table = FP8KVCache(6, 2, 64, 16), pages_for(1, 1, 3)
+    k = torch.zeros((1, 2, 5, 64), device="cuda", dtype=torch.bfloat16)
+    q, n = torch.zeros((1, 4, 3, 64), device="cuda", dtype=torch.bfloat16), i32(3)
+    turns = torch.zeros((5, 32, 2), device="cuda")
+
+    def append(cache=cache, table=table, starts=n, k=k, v=k, **kw):
+        append_kv(cache, table, starts, k, v, **kw)
+
+    for bad in ({"k": k[0]}, {"v": k[:, :, :4]}, {"v": k.float()}, {"k": k.double(), "v": k.double()}, {"k": k[:, :1], "v": k[:, :1]},
+                {"k": k[..., :32], "v": k[..., :32]}, {"table": table.long()}, {"table": table[0]}, {"table": table.repeat(2, 1)},
+                {"starts": n.long()}, {"starts": i32(1, 2)}, {"starts": n.cpu()}, {"counts": i32(1, 2)}, {"counts": n.float()},
+                {"table": table.cpu()}, {"v": k.cpu()}):
+        with pytest.raises(ValueError):
+            append(**bad)
+    for bad in ({"table": turns.double()}, {"table": turns[:4]}, {"table": turns.repeat(1, 2, 1)}, {"table": turns.transpose(0, 1)},
+                {"table": turns.cpu()}, {"k_weight": k[0, 0, 0].float()}, {"k_weight": k[0, 0, 0, :32]}):
+        with pytest.raises(ValueError):
+            append_kv(cache, table, n, k, k, **bad)
+    with pytest.raises(RuntimeError, match="eps"):
+        append(eps=-1.0)
+
+    def attend(q=q, cache=cache, table=table, lengths=n, **kw):
+        return cached_attention(q, cache, table, lengths, **kw)
+
+    for bad in ({"q": q[0]}, {"q": q.float()}, {"q": q[:, :3]}, {"q": q[..., :32]}, {"table": table.long()}, {"table": table.cpu()},
+                {"table": table.repeat(2, 1)}, {"lengths": n.long()}, {"lengths": i32(1, 2)}, {"q_lengths": i32(1, 2)},
+                {"q_lengths": n.cpu()}):
+        with pytest.raises(ValueError):
+            attend(**bad)
+    with pytest.raises(RuntimeError, match="scale"):
+        attend(scale=float("nan"))
+    with pytest.raises(ValueError):
+        read_kv(cache, table, n, -1)
+    with pytest.raises(ValueError):
+        read_kv(cache, table, n, 3, dtype=torch.float64)
+    with pytest.raises(ValueError):
+        read_kv(cache, table, i32(1, 2), 3)
+    bad = FP8KVCache(6, 2, 64, 16)
+    bad.k_scale = bad.k_scale[:, :1]
+    with pytest.raises(ValueError):
+        attend(cache=bad)
