@@ -1,6 +1,16 @@
 // Attention over a paged e4m3 cache of keys and values.
 //
-//   o_i = sum_j p_ij v_j / sum_j p_ij, p_ij = exp(scale q_i . k_j), over the keys j that row i sees
+//   o_i = sum_j p_ij v_j / sum_j p_ij, p_ij = 2^x_ij, x_ij = scale log2(e) q_i . k_j, over the keys j that row i sees
+//
+// Keys and values are codes times a power of two for each page.  Codes become fp16 exactly and go into the fp16 matrix
+// instructions; a key's power of two multiplies the score, and a value's, 2^e_j, goes into the exponent:
+//   p'_ij = 2^(x_ij + e_j - m_i),  o_i = sum_j p'_ij code_j / sum_j p'_ij 2^-e_j
+// with m_i a running maximum of x_ij + e_j.  So p' is at most about 1 however the pages' sizes differ, and its half step
+// in fp16, 2^-11 of it, is all that the value product rounds; bf16 queries are exact in fp16 under a power of two per row.
+// (e4m3 probabilities would run twice as fast and be off by 2^-4, bf16 ones by 2^-8.)
+//
+// The products are made transposed, S' = K Q' and O' = V' P': then a lane holds one row's scores and outputs, the maximum
+// and the sum run within lanes, and the probabilities are in the layout that the second product reads.
 #include <type_traits>
 
 #include "kv_cache.h"
@@ -8,67 +18,639 @@
 
 namespace mxf8 {
 
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
 struct AttendArgs {
   KvPages c;
   const void* q;
   void* o;
   int64_t qs[3], os[3];  // strides of batch, head, token
   const int32_t *lengths, *q_lengths;
-  int B, H, S, causal;
-  float scale;  // times log2 e
+  int H, S, G, R, causal;  // G heads a key head, R = S G rows of it: row i G + g is query i of head g
+  float scale;             // times log2 e
+  int splits;              // parts of the keys
+  float *part, *stat;      // with more than one: sums [B, Hk, splits, R, D], and (maximum, sum of p) [.., 2]
 };
 
-// One wave a row.
-template <int DT, int D>
-__global__ __launch_bounds__(256) void kv_attend_row_kernel(const AttendArgs a) {
-  __shared__ float qrow[4][D];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t row = (int64_t)blockIdx.x * 4 + w;
-  const int h = blockIdx.y, b = blockIdx.z;
-  if (row >= a.S) return;
-  const int len = kv_length(a.c, a.lengths[b]);
-  const int qlen = a.q_lengths ? min(max(a.q_lengths[b], 0), a.S) : a.S;
-  const int64_t seen = row >= qlen ? 0 : a.causal ? (int64_t)len - qlen + row + 1 : len;
-  const int hk = h / (a.H / a.c.H);
-  typedef typename Elem<DT>::T T;
-  const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[1] + row * a.qs[2];
-  for (int d = lane; d < D; d += 64) qrow[w][d] = Elem<DT>::to_f32(q[d]);
-  __builtin_amdgcn_wave_barrier();
-  float m = -1e30f, l = 0.0f, o[D / 64] = {};
-  for (int64_t key0 = 0; key0 < seen; key0 += 64) {
-    const int64_t key = key0 + lane;
-    const int pid = key < seen ? kv_page(a.c, b, (int)(key >> a.c.shift)) : -1;
-    const int64_t ph = (int64_t)max(pid, 0) * a.c.H + hk;
-    const int64_t at = ((ph << a.c.shift) + (key & ((1 << a.c.shift) - 1))) * D;
-    float x = -1e30f, vs = 0.0f;
-    if (pid >= 0) {
-      x = 0.0f;
-      const int* k = reinterpret_cast<const int*>(a.c.k + at);
-      for (int d = 0; d < D; d += 4) {
-        const v2f u = __builtin_amdgcn_cvt_pk_f32_fp8(k[d / 4], false), v = __builtin_amdgcn_cvt_pk_f32_fp8(k[d / 4], true);
-        x += u[0] * qrow[w][d] + u[1] * qrow[w][d + 1] + v[0] * qrow[w][d + 2] + v[1] * qrow[w][d + 3];
-      }
-      x *= kv_scale(a.c.ks[ph]) * a.scale;
-      vs = kv_scale(a.c.vs[ph]);
+constexpr float KV_NONE = -1.0e30f;  // a maximum of no scores
+constexpr float KV_SLACK = 8.0f;     // p' may grow to 2^8 before the running maximum follows
+
+// ---- rows and splits -------------------------------------------------------------------
+struct KvSeq {
+  int len, n;  // keys and queries that are there
+};
+__device__ __forceinline__ KvSeq kv_seq(const AttendArgs& a, int b) {
+  KvSeq s;
+  s.len = kv_length(a.c, a.lengths[b]);
+  s.n = a.q_lengths ? min(max(a.q_lengths[b], 0), a.S) : a.S;
+  return s;
+}
+// How many keys row `row` sees, from the first on.
+__device__ __forceinline__ int kv_limit(const AttendArgs& a, KvSeq s, int row) {
+  const int i = (uint32_t)row / (uint32_t)a.G;
+  return i >= s.n ? 0 : a.causal ? max(s.len - s.n + i + 1, 0) : s.len;
+}
+// How many keys the rows [r0, r1) of a tile see, and how many of them one split takes (a multiple of `unit`).
+__device__ __forceinline__ int kv_end(const AttendArgs& a, KvSeq s, int r0, int r1) {
+  const int i1 = min((int)((uint32_t)(min(r1, a.R) - 1) / (uint32_t)a.G), s.n - 1);
+  return (int)((uint32_t)r0 / (uint32_t)a.G) >= s.n ? 0 : a.causal ? max(s.len - s.n + i1 + 1, 0) : s.len;
+}
+__device__ __forceinline__ int kv_chunk(const AttendArgs& a, int end, int unit) {
+  return ((end + a.splits - 1) / a.splits + unit - 1) / unit * unit;
+}
+
+// ---- codes -----------------------------------------------------------------------------
+__device__ __forceinline__ v8h codes_f16(uint32_t a, uint32_t b) {
+  const v2h p = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)a, 1.0f, false);
+  const v2h q = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)a, 1.0f, true);
+  const v2h r = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)b, 1.0f, false);
+  const v2h s = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)b, 1.0f, true);
+  return v8h{p[0], p[1], q[0], q[1], r[0], r[1], s[0], s[1]};
+}
+// Four words of four bytes -> word i holds byte i of each.
+__device__ __forceinline__ void transpose4(const uint32_t (&k)[4], uint32_t (&o)[4]) {
+  const uint32_t t0 = __builtin_amdgcn_perm(k[1], k[0], 0x05010400), t1 = __builtin_amdgcn_perm(k[1], k[0], 0x07030602);
+  const uint32_t u0 = __builtin_amdgcn_perm(k[3], k[2], 0x05010400), u1 = __builtin_amdgcn_perm(k[3], k[2], 0x07030602);
+  o[0] = __builtin_amdgcn_perm(u0, t0, 0x05040100), o[1] = __builtin_amdgcn_perm(u0, t0, 0x07060302);
+  o[2] = __builtin_amdgcn_perm(u1, t1, 0x05040100), o[3] = __builtin_amdgcn_perm(u1, t1, 0x07060302);
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) { return cvt_pk_16<MXF8_F16>(a, b); }
+
+// Max / sum over the lanes that hold one row: LANES 16 (four of them, lanes l + 16 i) or 32 (lanes l, l + 32).
+template <int LANES, class F>
+__device__ __forceinline__ float row_reduce(float v, F f) {
+  if constexpr (LANES == 16) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  }
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float sum_of(float a, float b) { return a + b; }
+
+// Eight channels of a query to fp16, and the largest of their sizes, for bf16 (bits).
+template <int DT>
+__device__ __forceinline__ v8h query_f16(const Raw8<DT>& r, float s) {
+  if constexpr (DT == MXF8_F16) {
+    return __builtin_bit_cast(v8h, v4i{(int)r.w[0], (int)r.w[1], (int)r.w[2], (int)r.w[3]});
+  } else {
+    float f[8];
+    r.get(f);
+    return __builtin_bit_cast(v8h, v4i{(int)pack_f16(f[0] * s, f[1] * s), (int)pack_f16(f[2] * s, f[3] * s),
+                                       (int)pack_f16(f[4] * s, f[5] * s), (int)pack_f16(f[6] * s, f[7] * s)});
+  }
+}
+
+// One row's fragments of a query: N pieces of eight channels at channel(i), and the factor of its scores.
+template <int DT, int LANES, int N, class F>
+__device__ __forceinline__ float load_query(const AttendArgs& a, int b, int hk, int row, bool there, v8h (&f)[N], F channel) {
+  const int i = (uint32_t)row / (uint32_t)a.G, g = row - i * a.G;
+  const int64_t at = b * a.qs[0] + (hk * a.G + g) * a.qs[1] + i * a.qs[2];
+  Raw8<DT> r[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    r[j].zero();
+    if (there) r[j].load(a.q, at + channel(j));
+  }
+  int e = 0;
+  if constexpr (DT == MXF8_BF16) {
+    float top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      float x[8];
+      r[j].get(x);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(x[k]));
     }
-    const float mn = fmaxf(m, wave_max(x)), alpha = __builtin_amdgcn_exp2f(m - mn);
-    const float p = pid >= 0 ? __builtin_amdgcn_exp2f(x - mn) : 0.0f;
-    m = mn;
-    l = l * alpha + p;
-    for (int i = 0; i < D / 64; ++i) o[i] *= alpha;
-    const uint32_t offset_lo = (uint32_t)at, offset_hi = (uint32_t)(at >> 32);
-    for (int j = 0; j < 64; ++j) {
-      const float pj = __shfl(p * vs, j, 64);
-      const int64_t atj = (int64_t)((uint64_t)(uint32_t)__shfl(offset_hi, j, 64) << 32 | (uint32_t)__shfl(offset_lo, j, 64));
-      if (__shfl(pid, j, 64) < 0) continue;
-      for (int i = 0; i < D / 64; ++i)
-        o[i] += pj * __builtin_amdgcn_cvt_f32_fp8(a.c.v[atj + lane + 64 * i], 0);
+    top = row_reduce<LANES>(top, max_of);
+    e = min(max((int)(__float_as_uint(top) >> 23) - 127, -126), 126);
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) f[j] = query_f16<DT>(r[j], __uint_as_float((uint32_t)(127 - e) << 23));
+  return a.scale * __uint_as_float((uint32_t)(127 + e) << 23);
+}
+
+// N consecutive channels of an output row.
+template <int DT, int N>
+__device__ __forceinline__ void store_row(void* base, int64_t i, const float (&f)[N]) {
+  typedef uint32_t words __attribute__((ext_vector_type(N / 2), aligned(2)));
+  words w;
+#pragma unroll
+  for (int j = 0; j < N / 2; ++j) w[j] = cvt_pk_16<DT>(f[2 * j], f[2 * j + 1]);
+  *reinterpret_cast<words*>(static_cast<uint16_t*>(base) + i) = w;
+}
+__device__ __forceinline__ int64_t out_row(const AttendArgs& a, int b, int hk, int row) {
+  const int i = (uint32_t)row / (uint32_t)a.G, g = row - i * a.G;
+  return b * a.os[0] + (hk * a.G + g) * a.os[1] + i * a.os[2];
+}
+
+// ---- few rows --------------------------------------------------------------------------
+// Up to 64 rows a key head (its G heads' S queries): a workgroup takes a part of the keys, its four waves every fourth
+// step of 32 keys each, straight from memory into the layout of 16 x 16 x 32 products, and joins their sums at the end.
+// No LDS on the way: a lane loads 16 channels of its key, and for the values 8 keys' D / 16 channels, which it transposes in
+// registers.  The next step's loads are in flight while a step is computed.
+constexpr int FEW_ROWS = 64, FEW_UNIT = 128;
+
+template <int D>
+struct FewStep {
+  v4i k[2][D / 64];
+  uint32_t v[8][D / 64];
+  int pid[2];
+  uint32_t ks[2], vs[2];
+};
+
+template <int DT, int D, int NR>
+__global__ __launch_bounds__(256) void kv_attend_few_kernel(const AttendArgs a) {
+  constexpr int KK = D / 32, DI = D / 16, W = D / 64;
+  __shared__ float om[4][16][D + 4];
+  __shared__ float ml[4][2][16 * NR];
+  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
+  const KvSeq seq = kv_seq(a, b);
+  const int end = kv_end(a, seq, 0, a.R), chunk = kv_chunk(a, end, FEW_UNIT);
+  const int k0 = split * chunk, k1 = min(k0 + chunk, end);
+  if (a.splits > 1 && k0 >= k1) return;
+
+  v8h qf[NR][KK];
+  float factor[NR];
+  int limit[NR], low = INT32_MAX;
+#pragma unroll
+  for (int t = 0; t < NR; ++t) {
+    const int row = 16 * t + c;
+    limit[t] = row < a.R ? kv_limit(a, seq, row) : 0;
+    low = min(low, row < a.R ? limit[t] : INT32_MAX);
+    factor[t] = load_query<DT, 16>(a, b, hk, min(row, a.R - 1), limit[t] > 0, qf[t],
+                                   [&](int j) { return 64 * (j / 2) + 16 * q + 8 * (j % 2); });
+  }
+#pragma unroll
+  for (int off = 8; off; off >>= 1) low = min(low, __shfl_xor(low, off, 64));
+  low = __builtin_amdgcn_readfirstlane(low);  // every row sees the keys before it
+
+  float m[NR], l[NR];
+  v4f o[NR][DI];
+#pragma unroll
+  for (int t = 0; t < NR; ++t) {
+    m[t] = KV_NONE, l[t] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < DI; ++i) o[t][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  const int mask = (1 << a.c.shift) - 1;
+  auto pages = [&](int key0, int (&pid)[2]) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int key = key0 + 16 * g;
+      pid[g] = -1;
+      if (key < k1) pid[g] = __builtin_amdgcn_readfirstlane(kv_page(a.c, b, key >> a.c.shift));
+    }
+  };
+  auto load = [&](int key0, const int (&pid)[2], FewStep<D>& s) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      // (no page: page 0 is read and not used)
+      const int64_t ph = (int64_t)max(pid[g], 0) * a.c.H + hk;
+      const int64_t at = ((ph << a.c.shift) + ((key0 + 16 * g) & mask)) * D;
+      s.pid[g] = pid[g];
+      s.ks[g] = a.c.ks[ph], s.vs[g] = a.c.vs[ph];
+      const uint8_t* k = a.c.k + at + c * D + 16 * q;
+      const uint8_t* v = a.c.v + at + 4 * q * D + c * DI;
+#pragma unroll
+      for (int j = 0; j < W; ++j) s.k[g][j] = *reinterpret_cast<const v4i*>(k + 64 * j);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if constexpr (W == 2) {
+          const v2i x = *reinterpret_cast<const v2i*>(v + j * D);
+          s.v[4 * g + j][0] = x[0], s.v[4 * g + j][W - 1] = x[1];
+        } else {
+          s.v[4 * g + j][0] = *reinterpret_cast<const uint32_t*>(v + j * D);
+        }
+    }
+  };
+  auto compute = [&](int key0, FewStep<D>& s) {
+    const bool whole = key0 + 32 <= low && s.pid[0] >= 0 && s.pid[1] >= 0;
+    float ks[2], ev[2], iv[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      ks[g] = kv_scale(__builtin_amdgcn_readfirstlane(s.ks[g]));
+      const int e = (int)__builtin_amdgcn_readfirstlane(s.vs[g]) - 127;
+      ev[g] = (float)e, iv[g] = __uint_as_float((uint32_t)(127 - e) << 23);
+    }
+    v8h pf[NR];
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+      v4f x[2];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              codes_f16((uint32_t)s.k[g][kk / 2][2 * (kk % 2)], (uint32_t)s.k[g][kk / 2][2 * (kk % 2) + 1]), qf[t][kk], acc,
+              0, 0, 0);
+        const float f = factor[t] * ks[g];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[g][r] = __builtin_fmaf(acc[r], f, ev[g]);
+      }
+      if (!whole) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            x[g][r] = key0 + 16 * g + 4 * q + r < limit[t] && s.pid[g] >= 0 ? x[g][r] : -INFINITY;
+      }
+      const float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
+                              fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+      if (__ballot(top > m[t] + KV_SLACK)) {
+        const float next = fmaxf(m[t], row_reduce<16>(top, max_of)), alpha = __builtin_amdgcn_exp2f(m[t] - next);
+        m[t] = next;
+        l[t] *= alpha;
+#pragma unroll
+        for (int i = 0; i < DI; ++i) o[t][i] *= alpha;
+      }
+      float p[2][4];
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[g][r] = __builtin_amdgcn_exp2f(x[g][r] - m[t]);
+#pragma unroll
+      for (int g = 0; g < 2; ++g) l[t] = __builtin_fmaf((p[g][0] + p[g][1]) + (p[g][2] + p[g][3]), iv[g], l[t]);
+      pf[t] = __builtin_bit_cast(v8h, v4i{(int)pack_f16(p[0][0], p[0][1]), (int)pack_f16(p[0][2], p[0][3]),
+                                          (int)pack_f16(p[1][0], p[1][1]), (int)pack_f16(p[1][2], p[1][3])});
+    }
+    if (!whole) {  // what is not there may be NaN, which 0 does not cancel
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (key0 + 16 * g + 4 * q + r >= k1 || s.pid[g] < 0)
+#pragma unroll
+            for (int d = 0; d < W; ++d) s.v[4 * g + r][d] = 0;
+    }
+#pragma unroll
+    for (int d = 0; d < W; ++d) {
+      const uint32_t lo[4] = {s.v[0][d], s.v[1][d], s.v[2][d], s.v[3][d]};
+      const uint32_t hi[4] = {s.v[4][d], s.v[5][d], s.v[6][d], s.v[7][d]};
+      uint32_t tl[4], th[4];
+      transpose4(lo, tl);
+      transpose4(hi, th);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const v8h vf = codes_f16(tl[i], th[i]);
+#pragma unroll
+        for (int t = 0; t < NR; ++t) o[t][4 * d + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[t], o[t][4 * d + i], 0, 0, 0);
+      }
+    }
+  };
+
+  int key = k0 + 32 * w;
+  if (key < k1) {
+    FewStep<D> s[2];
+    int pid[2];
+    pages(key, pid);
+    load(key, pid, s[0]);
+    pages(key + FEW_UNIT, pid);
+    for (;;) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (key + FEW_UNIT < k1) load(key + FEW_UNIT, pid, s[1 - u]);
+        pages(key + 2 * FEW_UNIT, pid);
+        compute(key, s[u]);
+        key += FEW_UNIT;
+        if (key >= k1) goto done;
+      }
     }
   }
-  l = wave_sum(l);
-  const float r = l == 0.0f ? 0.0f : 1.0f / l;
-  T* out = static_cast<T*>(a.o) + b * a.os[0] + h * a.os[1] + row * a.os[2];
-  for (int i = 0; i < D / 64; ++i) out[lane + 64 * i] = (T)cvt_pk_16<DT>(o[i] * r, 0.0f);
+done:
+#pragma unroll
+  for (int t = 0; t < NR; ++t) {
+    l[t] = row_reduce<16>(l[t], sum_of);
+    if (q == 0) ml[w][0][16 * t + c] = m[t], ml[w][1][16 * t + c] = l[t];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < NR; ++t) {
+    const int rt = 16 * t + c;
+    const float top = fmaxf(fmaxf(ml[0][0][rt], ml[1][0][rt]), fmaxf(ml[2][0][rt], ml[3][0][rt]));
+    const float f = __builtin_amdgcn_exp2f(m[t] - top);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int i = 0; i < DI; i += 4)  // channel DI (4 q + r) + i
+        *reinterpret_cast<v4f*>(&om[w][c][DI * (4 * q + r) + i]) =
+            v4f{o[t][i][r] * f, o[t][i + 1][r] * f, o[t][i + 2][r] * f, o[t][i + 3][r] * f};
+    __syncthreads();
+    const int rr = threadIdx.x >> 4, row = 16 * t + rr, ch = (threadIdx.x & 15) * DI;
+    if (row < a.R) {
+      float sum[DI], mm[4], ll = 0.0f;
+#pragma unroll
+      for (int i = 0; i < DI; ++i) sum[i] = (om[0][rr][ch + i] + om[1][rr][ch + i]) + (om[2][rr][ch + i] + om[3][rr][ch + i]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) mm[u] = ml[u][0][row];
+      const float top4 = fmaxf(fmaxf(mm[0], mm[1]), fmaxf(mm[2], mm[3]));
+#pragma unroll
+      for (int u = 0; u < 4; ++u) ll = __builtin_fmaf(ml[u][1][row], __builtin_amdgcn_exp2f(mm[u] - top4), ll);
+      if (a.splits == 1) {
+        const float inv = ll == 0.0f ? 0.0f : __fdiv_rn(1.0f, ll);
+#pragma unroll
+        for (int i = 0; i < DI; ++i) sum[i] *= inv;
+        store_row<DT, DI>(a.o, out_row(a, b, hk, row) + ch, sum);
+      } else {
+        const int64_t at = (((int64_t)b * a.c.H + hk) * a.splits + split) * a.R + row;
+#pragma unroll
+        for (int i = 0; i < DI; i += 4)
+          *reinterpret_cast<v4f*>(a.part + at * D + ch + i) = v4f{sum[i], sum[i + 1], sum[i + 2], sum[i + 3]};
+        if (ch == 0) *reinterpret_cast<v2f*>(a.stat + at * 2) = v2f{top4, ll};
+      }
+    }
+    if (t + 1 < NR) __syncthreads();
+  }
+}
+
+// ---- many rows -------------------------------------------------------------------------
+// A workgroup of eight waves takes 256 rows of a key head, 32 a wave, and goes through its keys in tiles of 64.  The
+// codes of a tile are converted once, into LDS as fp16, keys by rows and values transposed, while the tile before is
+// computed; two buffers, one barrier a tile.
+constexpr int MANY_ROWS = 256, MANY_KEYS = 64;
+
+// LDS of one tile: keys [64][D] and values [D][64] in fp16, in 16-byte chunks with a swizzle, and the scales of its four
+// granules of 16 keys.
+template <int D>
+struct ManyTile {
+  v4i k[MANY_KEYS * D / 8];
+  v4i v[D * MANY_KEYS / 8];
+  float ks[4], ev[4], iv[4];
+  int there[4];
+};
+template <int D>
+__device__ __forceinline__ int many_k(int key, int chunk) {
+  return key * (D / 8) + (chunk ^ (D == 128 ? key & 15 : (key >> 1) & 7));
+}
+__device__ __forceinline__ int many_v(int ch, int chunk) { return ch * 8 + (chunk ^ ((ch >> 1 ^ ch >> 4) & 7)); }
+
+template <int DT, int D>
+__global__ __launch_bounds__(512, 2) void kv_attend_many_kernel(const AttendArgs a) {
+  constexpr int KK = D / 16, DT32 = D / 32, KB = D / 8;  // products a score tile; output tiles; K bytes a thread
+  __shared__ ManyTile<D> tile[2];
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r0 = (gridDim.x / a.splits - 1 - blockIdx.x / a.splits) * MANY_ROWS, split = blockIdx.x % a.splits;
+  const int hk = blockIdx.y, b = blockIdx.z;
+  const KvSeq seq = kv_seq(a, b);
+  const int end = kv_end(a, seq, r0, r0 + MANY_ROWS), chunk = kv_chunk(a, end, MANY_KEYS);
+  const int k0 = split * chunk, k1 = min(k0 + chunk, end);
+  if (a.splits > 1 && k0 >= k1) return;
+
+  const int row = r0 + 32 * w + c;
+  const int limit = row < a.R ? kv_limit(a, seq, row) : 0;
+  int low = row < a.R ? limit : INT32_MAX, high = limit;
+#pragma unroll
+  for (int off = 16; off; off >>= 1) low = min(low, __shfl_xor(low, off, 64)), high = max(high, __shfl_xor(high, off, 64));
+  low = __builtin_amdgcn_readfirstlane(low), high = __builtin_amdgcn_readfirstlane(high);
+  v8h qf[KK];
+  const float factor = load_query<DT, 32>(a, b, hk, min(row, a.R - 1), limit > 0, qf, [&](int j) { return 16 * j + 8 * h; });
+
+  float m = KV_NONE, l = 0.0f;
+  v16f o[DT32];
+#pragma unroll
+  for (int i = 0; i < DT32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[i][r] = 0.0f;
+
+  // this thread's part of a tile: KB bytes of key tid / 8, and of 4 keys from 4 (tid / 32) on (D = 128; twice as many keys
+  // a wave for D = 64) four channels' bytes
+  constexpr int VT = D / 4;  // threads a row of values
+  const bool has_v = threadIdx.x < 16 * VT;
+  const int kkey = threadIdx.x >> 3, kch = (threadIdx.x & 7) * KB, vkey = (threadIdx.x / VT & 15) * 4, vch = threadIdx.x % VT * 4;
+  const int mask = (1 << a.c.shift) - 1;
+  auto page_of = [&](int key) { return key < k1 ? kv_page(a.c, b, key >> a.c.shift) : -1; };
+  uint32_t kreg[KB / 4], vreg[4];
+  uint32_t ksb = 127, vsb = 127;
+  int kp, vp, gp;  // pages of the next tile's keys: this thread's key, its values, its granule (threads 0 .. 3)
+  auto find = [&](int key0) {
+    kp = page_of(key0 + kkey), vp = page_of(key0 + vkey);
+    gp = threadIdx.x < 4 ? page_of(key0 + 16 * (int)threadIdx.x) : -1;
+  };
+  int gthere = 0;
+  auto load = [&](int key0) {
+    const int64_t kph = (int64_t)max(kp, 0) * a.c.H + hk, vph = (int64_t)max(vp, 0) * a.c.H + hk;
+    const uint8_t* k = a.c.k + ((kph << a.c.shift) + ((key0 + kkey) & mask)) * D + kch;
+    const uint8_t* v = a.c.v + ((vph << a.c.shift) + ((key0 + vkey) & mask)) * D + vch;
+    if constexpr (KB == 16) {
+      const v4i x = *reinterpret_cast<const v4i*>(k);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) kreg[j] = x[j];
+    } else {
+      const v2i x = *reinterpret_cast<const v2i*>(k);
+      kreg[0] = x[0], kreg[1] = x[1];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      vreg[j] = 0;  // what is not there may be NaN, which a probability of 0 does not cancel
+      if (has_v && vp >= 0 && key0 + vkey + j < k1) vreg[j] = *reinterpret_cast<const uint32_t*>(v + j * D);
+    }
+    if (threadIdx.x < 4) {
+      const int64_t ph = (int64_t)max(gp, 0) * a.c.H + hk;
+      ksb = a.c.ks[ph], vsb = a.c.vs[ph];
+      gthere = gp >= 0;
+    }
+  };
+  auto put = [&](ManyTile<D>& t) {
+#pragma unroll
+    for (int j = 0; j < KB / 8; ++j)
+      t.k[many_k<D>(kkey, kch / 8 + j)] = __builtin_bit_cast(v4i, codes_f16(kreg[2 * j], kreg[2 * j + 1]));
+    if (has_v) {
+      uint32_t x[4];
+      transpose4(vreg, x);
+      // keys 16 t + 4 h + 0 .. 3 and 16 t + 8 + 4 h + 0 .. 3 are the chunk that half h of a wave reads for step t
+      const int u = vkey >> 2, chunk16 = (u >> 2) * 2 + (u & 1), part = (u >> 1) & 1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const v2h lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)x[j], 1.0f, false);
+        const v2h hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)x[j], 1.0f, true);
+        reinterpret_cast<v2i*>(&t.v[many_v(vch + j, chunk16)])[part] =
+            v2i{__builtin_bit_cast(int, lo), __builtin_bit_cast(int, hi)};
+      }
+    }
+    if (threadIdx.x < 4) {
+      t.ks[threadIdx.x] = kv_scale(ksb);
+      t.ev[threadIdx.x] = (float)((int)vsb - 127), t.iv[threadIdx.x] = __uint_as_float((254 - vsb) << 23);
+      t.there[threadIdx.x] = gthere;
+    }
+  };
+
+  if (k0 < k1) {
+    find(k0);
+    load(k0);
+    find(k0 + MANY_KEYS);
+    put(tile[0]);
+  }
+  for (int key0 = k0, u = 0; key0 < k1; key0 += MANY_KEYS, u ^= 1) {
+    __syncthreads();
+    const ManyTile<D>& t = tile[u];
+    const bool more = key0 + MANY_KEYS < k1;
+    if (more) {
+      load(key0 + MANY_KEYS);
+      find(key0 + 2 * MANY_KEYS);
+    }
+    if (key0 < high) {
+      v16f x[2];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[g][r] = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+          x[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, t.k[many_k<D>(32 * g + c, 2 * kk + h)]), qf[kk],
+                                                        x[g], 0, 0, 0);
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float f = factor * t.ks[g], e = t.ev[g];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) x[g >> 1][(g & 1) * 8 + r] = __builtin_fmaf(x[g >> 1][(g & 1) * 8 + r], f, e);
+      }
+      const bool whole = key0 + MANY_KEYS <= low && (t.there[0] & t.there[1] & t.there[2] & t.there[3]);
+      if (!whole) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            x[g][r] = key0 + 32 * g + 8 * (r >> 2) + 4 * h + (r & 3) < limit && t.there[2 * g + (r >> 3)] ? x[g][r] : -INFINITY;
+      }
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, x[g][r]);
+      if (__ballot(top > m + KV_SLACK)) {
+        const float next = fmaxf(m, row_reduce<32>(top, max_of)), alpha = __builtin_amdgcn_exp2f(m - next);
+        m = next;
+        l *= alpha;
+#pragma unroll
+        for (int i = 0; i < DT32; ++i) o[i] *= alpha;
+      }
+      v8h pf[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float p[8], sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) p[r] = __builtin_amdgcn_exp2f(x[g >> 1][(g & 1) * 8 + r] - m), sum += p[r];
+        l = __builtin_fmaf(sum, t.iv[g], l);
+        pf[g] = __builtin_bit_cast(v8h, v4i{(int)pack_f16(p[0], p[1]), (int)pack_f16(p[2], p[3]), (int)pack_f16(p[4], p[5]),
+                                            (int)pack_f16(p[6], p[7])});
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int i = 0; i < DT32; ++i)
+          o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, t.v[many_v(32 * i + c, 2 * g + h)]), pf[g], o[i],
+                                                        0, 0, 0);
+    }
+    if (more) put(tile[u ^ 1]);
+  }
+  l = row_reduce<32>(l, sum_of);
+  if (row >= a.R) return;
+  if (a.splits == 1) {
+    const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+    const int64_t at = out_row(a, b, hk, row) + 4 * h;
+#pragma unroll
+    for (int i = 0; i < DT32; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float f[4] = {o[i][4 * g] * inv, o[i][4 * g + 1] * inv, o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv};
+        store_row<DT, 4>(a.o, at + 32 * i + 8 * g, f);
+      }
+  } else {
+    const int64_t at = (((int64_t)b * a.c.H + hk) * a.splits + split) * a.R + row;
+#pragma unroll
+    for (int i = 0; i < DT32; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<v4f*>(a.part + at * D + 32 * i + 8 * g + 4 * h) =
+            v4f{o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]};
+    if (h == 0) *reinterpret_cast<v2f*>(a.stat + at * 2) = v2f{m, l};
+  }
+}
+
+// ---- splits joined ---------------------------------------------------------------------
+constexpr int KV_MAX_SPLITS = 64;
+
+// One wave a row: the splits' maxima and sums in a lane each, then their outputs, D / 64 channels a lane.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void kv_attend_join_kernel(const AttendArgs a, int rows, int unit) {
+  constexpr int W = D / 64;
+  typedef float vf __attribute__((ext_vector_type(W)));
+  const int lane = threadIdx.x & 63, hk = blockIdx.y, b = blockIdx.z;
+  const int row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (row >= a.R) return;
+  const int r0 = row / rows * rows, end = kv_end(a, kv_seq(a, b), r0, r0 + rows);
+  const int chunk = kv_chunk(a, end, unit), n = end ? (end + chunk - 1) / chunk : 0;
+  const int64_t at = (((int64_t)b * a.c.H + hk) * a.splits) * a.R + row;
+  float m = KV_NONE, l = 0.0f;
+  if (lane < n) {
+    const v2f s = *reinterpret_cast<const v2f*>(a.stat + (at + (int64_t)lane * a.R) * 2);
+    m = s[0], l = s[1];
+  }
+  const float f = __builtin_amdgcn_exp2f(m - lanes_max<64>(m));
+  const float sum = lanes_sum<64>(l * f);
+  float o[W] = {};
+  const float* part = a.part + at * D + lane * W;
+#pragma unroll 8
+  for (int s = 0; s < n; ++s) {
+    const vf x = *reinterpret_cast<const vf*>(part + (int64_t)s * a.R * D);
+    const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s));
+#pragma unroll
+    for (int i = 0; i < W; ++i) o[i] = __builtin_fmaf(((const float*)&x)[i], fs, o[i]);
+  }
+  const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+  const int64_t to = out_row(a, b, hk, row) + lane * W;
+#pragma unroll
+  for (int i = 0; i < W; ++i) store1<DT>(a.o, to + i, o[i] * inv);
+}
+
+// ---- plan ------------------------------------------------------------------------------
+struct AttendPlan {
+  bool few;
+  int splits;
+  int64_t rows, tiles;  // rows a key head, row tiles of them
+};
+static AttendPlan plan_attend(int64_t B, int64_t H, int64_t Hk, int64_t S, int64_t width, int64_t page) {
+  AttendPlan p{};
+  p.rows = S * (H / Hk);
+  p.few = p.rows <= FEW_ROWS;
+  p.tiles = p.few ? 1 : cdiv(p.rows, MANY_ROWS);
+  const int64_t groups = B * Hk * p.tiles, unit = p.few ? FEW_UNIT : 4 * MANY_KEYS;
+  const int64_t want = cdiv(p.few ? 1024 : 512, groups), most = cdiv(width * page, unit);
+  p.splits = (int)(want < 1 ? 1 : want > most ? most : want);
+  if (p.splits > KV_MAX_SPLITS) p.splits = KV_MAX_SPLITS;
+  if (p.splits < 1) p.splits = 1;
+  return p;
+}
+
+template <int DT, int D>
+static int launch_attend(AttendArgs& a, const AttendPlan& p, int B, hipStream_t st) {
+  const char* what = "kv_attend";
+  const int Hk = a.c.H;
+  if (p.few) {
+    const dim3 grid(p.splits, Hk, B);
+    if (a.R <= 16)
+      kv_attend_few_kernel<DT, D, 1><<<grid, 256, 0, st>>>(a);
+    else if (a.R <= 32)
+      kv_attend_few_kernel<DT, D, 2><<<grid, 256, 0, st>>>(a);
+    else
+      kv_attend_few_kernel<DT, D, 4><<<grid, 256, 0, st>>>(a);
+  } else {
+    if (!grid_fits(p.tiles * p.splits, 512)) return set_error(MXF8_EINVAL, "%s: shape too large", what);
+    const dim3 grid((unsigned)(p.tiles * p.splits), Hk, B);
+    kv_attend_many_kernel<DT, D><<<grid, 512, 0, st>>>(a);
+  }
+  if (const int rc = check_launch(what)) return rc;
+  if (p.splits == 1) return MXF8_OK;
+  kv_attend_join_kernel<DT, D><<<dim3((unsigned)cdiv(a.R, 4), Hk, B), 256, 0, st>>>(a, p.few ? FEW_ROWS : MANY_ROWS,
+                                                                                     p.few ? FEW_UNIT : MANY_KEYS);
+  return check_launch(what);
 }
 
 }  // namespace mxf8
@@ -77,7 +659,9 @@ using namespace mxf8;
 
 extern "C" int64_t mxf8_kv_attend_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t S, int64_t D,
                                                   int64_t table_width, int64_t page_size) {
-  return 0;
+  if (B <= 0 || H <= 0 || Hk <= 0 || H % Hk || S <= 0 || D <= 0 || table_width <= 0 || page_size <= 0) return 0;
+  const AttendPlan p = plan_attend(B, H, Hk, S, table_width, page_size);
+  return p.splits == 1 ? 0 : B * Hk * p.splits * p.rows * (D + 2) * 4;
 }
 
 extern "C" int mxf8_kv_attend(const void* q, const int64_t q_strides[4], int dtype, int64_t B, int64_t H, int64_t S,
@@ -91,7 +675,7 @@ extern "C" int mxf8_kv_attend(const void* q, const int64_t q_strides[4], int dty
   if (const int rc = kv_check_pages(what, k_codes, v_codes, k_scale, v_scale, pages, Hk, page_size, D, page_table,
                                     table_stride, table_width, B, &a.c))
     return rc;
-  if (H < 0 || H > 65535 || S < 0 || S > (1 << 30)) return set_error(MXF8_EINVAL, "%s: bad shape", what);
+  if (H < 0 || H > 65535 || S < 0) return set_error(MXF8_EINVAL, "%s: bad shape", what);
   if (H && (Hk == 0 || H % Hk))
     return set_error(MXF8_EINVAL, "%s: %lld heads over %lld key heads", what, (long long)H, (long long)Hk);
   if (dtype != MXF8_BF16 && dtype != MXF8_F16) return set_error(MXF8_EINVAL, "%s: bad dtype %d", what, dtype);
@@ -100,20 +684,22 @@ extern "C" int mxf8_kv_attend(const void* q, const int64_t q_strides[4], int dty
   if (!q || !out || !q_strides || !out_strides || !lengths) return set_error(MXF8_EINVAL, "%s: null pointer", what);
   if (q_strides[3] != 1 || out_strides[3] != 1)
     return set_error(MXF8_EINVAL, "%s: channels must be contiguous", what);
+  if (S > (1 << 28) || S * (H / Hk) > (1 << 28)) return set_error(MXF8_EINVAL, "%s: shape too large", what);
+  const AttendPlan p = plan_attend(B, H, Hk, S, table_width, page_size);
+  if (p.splits > 1 && (!workspace || (uintptr_t)workspace % 16))
+    return set_error(MXF8_EINVAL, "%s: a 16-byte aligned workspace is needed", what);
+  if (pages == 0) a.c.width = 0;  // no keys
   a.q = q, a.o = out;
   for (int i = 0; i < 3; ++i) a.qs[i] = q_strides[i], a.os[i] = out_strides[i];
   a.lengths = lengths, a.q_lengths = q_lengths;
-  a.B = (int)B, a.H = (int)H, a.S = (int)S, a.causal = causal != 0;
+  a.H = (int)H, a.S = (int)S, a.G = (int)(H / Hk), a.R = (int)p.rows, a.causal = causal != 0;
   a.scale = scale * 1.4426950408889634f;
-  if (!grid_fits(cdiv(S, 4), 256)) return set_error(MXF8_EINVAL, "%s: shape too large", what);
-  const dim3 grid((unsigned)cdiv(S, 4), (unsigned)H, (unsigned)B);
+  a.splits = p.splits;
+  a.part = static_cast<float*>(workspace);
+  a.stat = a.part + B * Hk * p.splits * p.rows * D;
   auto launch = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    if (D == 128)
-      kv_attend_row_kernel<DT, 128><<<grid, 256, 0, stream>>>(a);
-    else
-      kv_attend_row_kernel<DT, 64><<<grid, 256, 0, stream>>>(a);
-    return check_launch(what);
+    return D == 128 ? launch_attend<DT, 128>(a, p, (int)B, stream) : launch_attend<DT, 64>(a, p, (int)B, stream);
   };
   return dtype == MXF8_BF16 ? launch(std::integral_constant<int, MXF8_BF16>{})
                             : launch(std::integral_constant<int, MXF8_F16>{});

@@ -20,7 +20,7 @@ int kv_check_pages(const char* what, const void* k, const void* v, const void* k
   if (page != 16 && page != 32 && page != 64 && page != 128)
     return set_error(MXF8_EINVAL, "%s: a page holds 16, 32, 64 or 128 tokens, got %lld", what, (long long)page);
   if (pages < 0 || pages > INT32_MAX || H < 0 || H > 65535 || B < 0 || B > 65535 || width < 0 ||
-      width > INT32_MAX / page)
+      width > (1 << 30) / page)
     return set_error(MXF8_EINVAL, "%s: bad shape", what);
   if (width && B > 1 && table_stride < width)
     return set_error(MXF8_EINVAL, "%s: page table rows overlap", what);
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
   const float* turns = a.turns + b * a.turns_batch;
   float wk[8], wp[8];
   // half-split partner: channel c +- P, in lane l +- P / 8 of the token where P % 8 == 0
-  const int plane = (lane - l % 64) + min(max(c0 < a.P ? l + a.P / 8 : l - a.P / 8, 0), L - 1);
+  const int plane = (lane - l) + min(max(c0 < a.P ? l + a.P / 8 : l - a.P / 8, 0), L - 1);
   if (a.w) {
     Raw8<DT> w;
     w.load(a.w, c0);
@@ -191,7 +191,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
           k[i][j] = k[i][j] == k[i][j] ? k[i][j] : 0.0f;
           v[j] = v[j] == v[j] ? v[j] : 0.0f;
         }
-        nan_key = l == 0 && (any_bad >> (lane - l % 64) & ((1ull << L) - 1)) ? 0x7fu : 0u;
+        nan_key = l == 0 && (any_bad >> (lane - l) & ((1ull << L) - 1)) ? 0x7fu : 0u;
       }
       if (first + i * T < page && pos >= lo && pos < hi) {
         uint32_t w[4];
