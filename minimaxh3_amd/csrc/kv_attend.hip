@@ -127,8 +127,13 @@ __device__ __forceinline__ float load_query(const AttendArgs& a, int b, int hk, 
     e = min(max((int)(__float_as_uint(top) >> 23) - 127, -126), 126);
   }
 #pragma unroll
-  for (int j = 0; j < N; ++j) f[j] = query_f16<DT>(r[j], __uint_as_float((uint32_t)(127 - e) << 23));
-  return a.scale * __uint_as_float((uint32_t)(127 + e) << 23);
+  for (int j = 0; j < N; ++j) {
+    f[j] = query_f16<DT>(r[j], __uint_as_float((uint32_t)(127 - e) << 23));
+    if (a.scale < 0.0f) f[j] = -f[j];  // so that the factor of the scores is not negative, and their largest its own
+  }
+  // (at least 2^-90: times a page's 2^-32 or more it is still no 0, which would make NaN of a score that is hidden as -inf;
+  // scores under so small a factor are 0 for all that matters)
+  return fmaxf(fabsf(a.scale) * __uint_as_float((uint32_t)(127 + e) << 23), 0x1p-90f);
 }
 
 // N consecutive channels of an output row.
@@ -233,8 +238,10 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(const AttendArgs a) 
     float ks[2], ev[2], iv[2];
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-      ks[g] = kv_scale(__builtin_amdgcn_readfirstlane(s.ks[g]));
-      const int e = (int)__builtin_amdgcn_readfirstlane(s.vs[g]) - 127;
+      const uint32_t kb = s.pid[g] < 0 ? 127 : __builtin_amdgcn_readfirstlane(s.ks[g]);
+      const uint32_t vb = s.pid[g] < 0 ? 127 : __builtin_amdgcn_readfirstlane(s.vs[g]);
+      ks[g] = kv_scale(kb);
+      const int e = (int)vb - 127;
       ev[g] = (float)e, iv[g] = __uint_as_float((uint32_t)(127 - e) << 23);
     }
     v8h pf[NR];
@@ -369,32 +376,34 @@ done:
 }
 
 // ---- many rows -------------------------------------------------------------------------
-// A workgroup of eight waves takes 256 rows of a key head, 32 a wave, and goes through its keys in tiles of 64.  The
-// codes of a tile are converted once, into LDS as fp16, keys by rows and values transposed, while the tile before is
-// computed; two buffers, one barrier a tile.
+// A workgroup of eight waves takes 256 rows of a key head, 32 a wave, and goes through its keys in tiles of 64.  A tile's
+// codes go into LDS once, the keys as they are, the values transposed and converted to fp16; a wave converts the keys'
+// fragments as it reads them.
+// The two waves of a SIMD (of the groups w < 4 and w >= 4) take turns with the matrix unit: between two barriers, group 0
+// first makes the scores of its next tile and the value product of this one and then takes the next one's exponentials, group
+// 1 first takes exponentials and then multiplies.  Fragments are read from LDS well before their products, and each wave
+// stages its share of the keys of tile j + 3 and the values of j + 1 among them.
 constexpr int MANY_ROWS = 256, MANY_KEYS = 64;
 
-// LDS of one tile: keys [64][D] and values [D][64] in fp16, in 16-byte chunks with a swizzle, and the scales of its four
-// granules of 16 keys.
+// LDS, in 16-byte chunks with a swizzle: keys [64][D] and values [D][64] in fp16; of each granule of 16 keys, the keys'
+// scale, the values' exponent and 2^-that, and whether it is there.
 template <int D>
-struct ManyTile {
-  v4i k[MANY_KEYS * D / 8];
-  v4i v[D * MANY_KEYS / 8];
-  float ks[4], ev[4], iv[4];
-  int there[4];
+struct ManyLds {
+  v4i k[4][MANY_KEYS * D / 8];
+  v4i v[2][D * MANY_KEYS / 8];
+  v4f scale[4][4];
+  v4f unused[64];  // where the other lanes of a wave write when one writes a scale
 };
 template <int D>
-__device__ __forceinline__ int many_k(int key, int chunk) {
-  return key * (D / 8) + (chunk ^ (D == 128 ? key & 15 : (key >> 1) & 7));
-}
+__device__ __forceinline__ int many_k(int key, int chunk) { return key * (D / 8) + (chunk ^ lds_swz<2 * D>(key)); }
 __device__ __forceinline__ int many_v(int ch, int chunk) { return ch * 8 + (chunk ^ ((ch >> 1 ^ ch >> 4) & 7)); }
 
 template <int DT, int D>
 __global__ __launch_bounds__(512, 2) void kv_attend_many_kernel(const AttendArgs a) {
-  constexpr int KK = D / 16, DT32 = D / 32, KB = D / 8;  // products a score tile; output tiles; K bytes a thread
-  __shared__ ManyTile<D> tile[2];
+  constexpr int KK = D / 16, OT = D / 32;  // products a score tile; output tiles
+  __shared__ ManyLds<D> lds;
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = w >> 2;
   const int r0 = (gridDim.x / a.splits - 1 - blockIdx.x / a.splits) * MANY_ROWS, split = blockIdx.x % a.splits;
   const int hk = blockIdx.y, b = blockIdx.z;
   const KvSeq seq = kv_seq(a, b);
@@ -402,153 +411,260 @@ __global__ __launch_bounds__(512, 2) void kv_attend_many_kernel(const AttendArgs
   const int k0 = split * chunk, k1 = min(k0 + chunk, end);
   if (a.splits > 1 && k0 >= k1) return;
 
-  const int row = r0 + 32 * w + c;
-  const int limit = row < a.R ? kv_limit(a, seq, row) : 0;
+  const int row = r0 + 32 * w + c, limit = row < a.R ? kv_limit(a, seq, row) : 0;
   int low = row < a.R ? limit : INT32_MAX, high = limit;
-#pragma unroll
-  for (int off = 16; off; off >>= 1) low = min(low, __shfl_xor(low, off, 64)), high = max(high, __shfl_xor(high, off, 64));
-  low = __builtin_amdgcn_readfirstlane(low), high = __builtin_amdgcn_readfirstlane(high);
   v8h qf[KK];
   const float factor = load_query<DT, 32>(a, b, hk, min(row, a.R - 1), limit > 0, qf, [&](int j) { return 16 * j + 8 * h; });
-
   float m = KV_NONE, l = 0.0f;
-  v16f o[DT32];
+  v16f o[OT];
 #pragma unroll
-  for (int i = 0; i < DT32; ++i)
+  for (int i = 0; i < OT; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[i][r] = 0.0f;
+#pragma unroll
+  for (int off = 16; off; off >>= 1) low = min(low, __shfl_xor(low, off, 64)), high = max(high, __shfl_xor(high, off, 64));
+  // every row of the wave sees the keys before `low`, none those from `high` on
+  low = __builtin_amdgcn_readfirstlane(low), high = __builtin_amdgcn_readfirstlane(high);
 
-  // this thread's part of a tile: KB bytes of key tid / 8, and of 4 keys from 4 (tid / 32) on (D = 128; twice as many keys
-  // a wave for D = 64) four channels' bytes
-  constexpr int VT = D / 4;  // threads a row of values
-  const bool has_v = threadIdx.x < 16 * VT;
-  const int kkey = threadIdx.x >> 3, kch = (threadIdx.x & 7) * KB, vkey = (threadIdx.x / VT & 15) * 4, vch = threadIdx.x % VT * 4;
+  // Each wave stages 16 bytes a lane of one granule of 16 keys.  D = 128: half of granule w / 2, 8 of its keys and two times
+  // 4 of its values' keys; D = 64: waves 0 to 3 the keys of granule w, waves 4 to 7 the values of granule w - 4.
   const int mask = (1 << a.c.shift) - 1;
-  auto page_of = [&](int key) { return key < k1 ? kv_page(a.c, b, key >> a.c.shift) : -1; };
-  uint32_t kreg[KB / 4], vreg[4];
-  uint32_t ksb = 127, vsb = 127;
-  int kp, vp, gp;  // pages of the next tile's keys: this thread's key, its values, its granule (threads 0 .. 3)
-  auto find = [&](int key0) {
-    kp = page_of(key0 + kkey), vp = page_of(key0 + vkey);
-    gp = threadIdx.x < 4 ? page_of(key0 + 16 * (int)threadIdx.x) : -1;
+  const int gran = D == 128 ? w >> 1 : w & 3;
+  const bool has_k = D == 128 || w < 4, has_v = D == 128 || w >= 4;
+  const int skey = D == 128 ? (w & 1) * 8 + (lane >> 3) : lane >> 2, sch = D == 128 ? lane & 7 : lane & 3;
+  const int vu = D == 128 ? (w & 1) * 2 + (lane >> 5) : lane >> 4, vch = lane % (D / 4) * 4;  // values 4 vu + j, 4 channels
+  v4i kreg;
+  uint32_t vreg[4], ksb = 127, vsb = 127;
+  bool kthere = false, vthere = false;
+  auto index = [&](int j) { return min(k0 + j * MANY_KEYS + 16 * gran, k1 - 1) >> a.c.shift; };  // (behind the end: the last)
+  auto entry = [&](int j) { return kv_entry(a.c, b, index(j)); };
+  // (the same as a vector load: a scalar one would make every wait for LDS a wait for it)
+  const int zero = __builtin_amdgcn_mbcnt_lo(0, 0);
+  auto entry_ahead = [&](int j) { return a.c.table[b * a.c.table_stride + index(j) + zero]; };
+  auto place = [&](int j, int page, bool& there) {  // (no page: page 0 is read and not used)
+    there = k0 + j * MANY_KEYS + 16 * gran < k1 && kv_valid(a.c, page);
+    return (int64_t)(there ? page : 0) * a.c.H + hk;
   };
-  int gthere = 0;
-  auto load = [&](int key0) {
-    const int64_t kph = (int64_t)max(kp, 0) * a.c.H + hk, vph = (int64_t)max(vp, 0) * a.c.H + hk;
-    const uint8_t* k = a.c.k + ((kph << a.c.shift) + ((key0 + kkey) & mask)) * D + kch;
-    const uint8_t* v = a.c.v + ((vph << a.c.shift) + ((key0 + vkey) & mask)) * D + vch;
-    if constexpr (KB == 16) {
-      const v4i x = *reinterpret_cast<const v4i*>(k);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) kreg[j] = x[j];
-    } else {
-      const v2i x = *reinterpret_cast<const v2i*>(k);
-      kreg[0] = x[0], kreg[1] = x[1];
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      vreg[j] = 0;  // what is not there may be NaN, which a probability of 0 does not cancel
-      if (has_v && vp >= 0 && key0 + vkey + j < k1) vreg[j] = *reinterpret_cast<const uint32_t*>(v + j * D);
-    }
-    if (threadIdx.x < 4) {
-      const int64_t ph = (int64_t)max(gp, 0) * a.c.H + hk;
-      ksb = a.c.ks[ph], vsb = a.c.vs[ph];
-      gthere = gp >= 0;
-    }
+  auto load_k = [&](int j, int page) {  // of tile j of this split
+    if (!has_k) return;
+    const int64_t ph = place(j, page, kthere);
+    const uint8_t* p = a.c.k + ((ph << a.c.shift) + ((k0 + j * MANY_KEYS + 16 * gran) & mask)) * D;
+    kreg = *reinterpret_cast<const v4i*>(p + skey * D + 16 * sch);
+    ksb = a.c.ks[ph], vsb = a.c.vs[ph];
   };
-  auto put = [&](ManyTile<D>& t) {
+  auto load_v = [&](int j, int page) {
+    if (!has_v) return;
+    const int64_t ph = place(j, page, vthere);
+    const uint8_t* p = a.c.v + ((ph << a.c.shift) + ((k0 + j * MANY_KEYS + 16 * gran) & mask)) * D;
 #pragma unroll
-    for (int j = 0; j < KB / 8; ++j)
-      t.k[many_k<D>(kkey, kch / 8 + j)] = __builtin_bit_cast(v4i, codes_f16(kreg[2 * j], kreg[2 * j + 1]));
-    if (has_v) {
-      uint32_t x[4];
-      transpose4(vreg, x);
-      // keys 16 t + 4 h + 0 .. 3 and 16 t + 8 + 4 h + 0 .. 3 are the chunk that half h of a wave reads for step t
-      const int u = vkey >> 2, chunk16 = (u >> 2) * 2 + (u & 1), part = (u >> 1) & 1;
+    for (int i = 0; i < 4; ++i) vreg[i] = *reinterpret_cast<const uint32_t*>(p + (4 * vu + i) * D + vch);
+  };
+  const int put_k_at[2] = {many_k<D>(16 * gran + skey, 2 * sch), many_k<D>(16 * gran + skey, 2 * sch + 1)};
+  int put_v_at[4];  // in halves of chunks
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const v2h lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)x[j], 1.0f, false);
-        const v2h hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)x[j], 1.0f, true);
-        reinterpret_cast<v2i*>(&t.v[many_v(vch + j, chunk16)])[part] =
-            v2i{__builtin_bit_cast(int, lo), __builtin_bit_cast(int, hi)};
-      }
-    }
-    if (threadIdx.x < 4) {
-      t.ks[threadIdx.x] = kv_scale(ksb);
-      t.ev[threadIdx.x] = (float)((int)vsb - 127), t.iv[threadIdx.x] = __uint_as_float((254 - vsb) << 23);
-      t.there[threadIdx.x] = gthere;
+  for (int i = 0; i < 4; ++i) put_v_at[i] = 2 * many_v(vch + i, 2 * gran + (vu & 1)) + (vu >> 1);
+  v4f* const scale_at = skey == 0 && sch == 0 ? &lds.scale[0][gran] : &lds.unused[lane];
+  auto put_k = [&](int j) {
+    if (!has_k) return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      lds.k[j & 3][put_k_at[i]] = __builtin_bit_cast(v4i, codes_f16((uint32_t)kreg[2 * i], (uint32_t)kreg[2 * i + 1]));
+    const uint32_t kb = kthere ? ksb : 127, vb = kthere ? vsb : 127;
+    scale_at[skey == 0 && sch == 0 ? (j & 3) * 4 : 0] =
+        v4f{kv_scale(kb), (float)((int)vb - 127), __uint_as_float((254 - vb) << 23), kthere ? 1.0f : 0.0f};
+  };
+  auto put_v = [&](int j) {
+    if (!has_v) return;
+    // what is not there may be NaN, which a probability of 0 does not cancel
+    const int there = vthere ? k1 - (k0 + j * MANY_KEYS + 16 * gran + 4 * vu) : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) vreg[i] = i < there ? vreg[i] : 0;
+    // keys 16 t + 4 h + 0 .. 3 and 16 t + 8 + 4 h + 0 .. 3 are the chunk that half h of a wave reads for step t
+    uint32_t x[4];
+    transpose4(vreg, x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const v2h lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)x[i], 1.0f, false);
+      const v2h hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)x[i], 1.0f, true);
+      reinterpret_cast<v2i*>(lds.v[j & 1])[put_v_at[i]] = v2i{__builtin_bit_cast(int, lo), __builtin_bit_cast(int, hi)};
     }
   };
 
-  if (k0 < k1) {
-    find(k0);
-    load(k0);
-    find(k0 + MANY_KEYS);
-    put(tile[0]);
-  }
-  for (int key0 = k0, u = 0; key0 < k1; key0 += MANY_KEYS, u ^= 1) {
-    __syncthreads();
-    const ManyTile<D>& t = tile[u];
-    const bool more = key0 + MANY_KEYS < k1;
-    if (more) {
-      load(key0 + MANY_KEYS);
-      find(key0 + 2 * MANY_KEYS);
-    }
-    if (key0 < high) {
-      v16f x[2];
+  int kat[KK], vat[4];  // chunks of this lane's fragments in a buffer
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
+  for (int i = 0; i < KK; ++i) kat[i] = many_k<D>(c, 2 * i + h);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[g][r] = 0.0f;
+  for (int g = 0; g < 4; ++g) vat[g] = many_v(c, 2 * g + h);  // channel 32 i + c, chunk 2 g + h: vat[g ^ i], 256 i further
+
+  v16f x[2];
+  v8h pf[4];
+  v4i kf[KK][2], vf[4][OT];
+  auto read_k = [&](int j, int part) {  // half of a tile's fragments, by channels
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk)
-          x[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, t.k[many_k<D>(32 * g + c, 2 * kk + h)]), qf[kk],
-                                                        x[g], 0, 0, 0);
-      }
-      float top = -INFINITY;
+    for (int i = part * KK / 2; i < (part + 1) * KK / 2; ++i)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const float f = factor * t.ks[g], e = t.ev[g];
+      for (int g = 0; g < 2; ++g) kf[i][g] = lds.k[j & 3][kat[i] + g * 32 * (D / 8)];
+  };
+  auto read_v = [&](int j, int g) {
 #pragma unroll
-        for (int r = 0; r < 8; ++r) x[g >> 1][(g & 1) * 8 + r] = __builtin_fmaf(x[g >> 1][(g & 1) * 8 + r], f, e);
-      }
-      const bool whole = key0 + MANY_KEYS <= low && (t.there[0] & t.there[1] & t.there[2] & t.there[3]);
-      if (!whole) {
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            x[g][r] = key0 + 32 * g + 8 * (r >> 2) + 4 * h + (r & 3) < limit && t.there[2 * g + (r >> 3)] ? x[g][r] : -INFINITY;
-      }
+    for (int i = 0; i < OT; ++i) vf[g][i] = lds.v[j & 1][vat[g ^ i] + 256 * i];
+  };
+  auto scores = [&](int part) {
+    if (part == 0) {
 #pragma unroll
       for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, x[g][r]);
-      if (__ballot(top > m + KV_SLACK)) {
-        const float next = fmaxf(m, row_reduce<32>(top, max_of)), alpha = __builtin_amdgcn_exp2f(m - next);
-        m = next;
-        l *= alpha;
+        for (int r = 0; r < 16; ++r) x[g][r] = 0.0f;
+    }
 #pragma unroll
-        for (int i = 0; i < DT32; ++i) o[i] *= alpha;
-      }
-      v8h pf[4];
+    for (int i = part * KK / 2; i < (part + 1) * KK / 2; ++i)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) x[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, kf[i][g]), qf[i], x[g], 0, 0, 0);
+  };
+  auto values = [&](int g) {
+#pragma unroll
+    for (int i = 0; i < OT; ++i)
+      o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, vf[g][i]), pf[g], o[i], 0, 0, 0);
+  };
+  auto exponentials = [&](int j) {
+    const int key0 = k0 + j * MANY_KEYS;
+    float f[4], e[4], iv[4], y[4];
+    v4f s[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) s[g] = lds.scale[j & 3][g];
+    auto tops = [&]() {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        float p[8], sum = 0.0f;
+        y[g] = x[g >> 1][(g & 1) * 8];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) p[r] = __builtin_amdgcn_exp2f(x[g >> 1][(g & 1) * 8 + r] - m), sum += p[r];
-        l = __builtin_fmaf(sum, t.iv[g], l);
-        pf[g] = __builtin_bit_cast(v8h, v4i{(int)pack_f16(p[0], p[1]), (int)pack_f16(p[2], p[3]), (int)pack_f16(p[4], p[5]),
-                                            (int)pack_f16(p[6], p[7])});
+        for (int r = 1; r < 8; ++r) y[g] = fmaxf(y[g], x[g >> 1][(g & 1) * 8 + r]);
       }
+    };
+    tops();
+    bool all = key0 + MANY_KEYS <= low;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      f[g] = factor * s[g][0], e[g] = s[g][1], iv[g] = s[g][2];
+      all = all & (__builtin_amdgcn_readfirstlane(__float_as_uint(s[g][3])) != 0);
+    }
+    if (!all) {
 #pragma unroll
       for (int g = 0; g < 4; ++g)
 #pragma unroll
-        for (int i = 0; i < DT32; ++i)
-          o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, t.v[many_v(32 * i + c, 2 * g + h)]), pf[g], o[i],
-                                                        0, 0, 0);
+        for (int r = 0; r < 8; ++r)
+          x[g >> 1][(g & 1) * 8 + r] = key0 + 16 * g + 8 * (r >> 2) + 4 * h + (r & 3) < limit && s[g][3] != 0.0f
+                                           ? x[g >> 1][(g & 1) * 8 + r]
+                                           : -INFINITY;
+      tops();
     }
-    if (more) put(tile[u ^ 1]);
+    float top = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) top = fmaxf(top, __builtin_fmaf(y[g], f[g], e[g]));
+    if (__ballot(top > m + KV_SLACK)) {
+      const float next = fmaxf(m, row_reduce<32>(top, max_of)), alpha = __builtin_amdgcn_exp2f(m - next);
+      m = next;
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < OT; ++i) o[i] *= alpha;
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float n = e[g] - m;
+      float sum = 0.0f;
+      v4i words;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[g >> 1][(g & 1) * 8 + 2 * r], f[g], n));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[g >> 1][(g & 1) * 8 + 2 * r + 1], f[g], n));
+        words[r] = (int)pack_f16(p0, p1);
+        sum += p0 + p1;
+      }
+      l = __builtin_fmaf(sum, iv[g], l);
+      pf[g] = __builtin_bit_cast(v8h, words);
+    }
+  };
+  // (a phase's products and exponentials stay in it)
+  auto change = [&]() {
+    __builtin_amdgcn_sched_barrier(0);
+    __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  const int n = (k1 - k0 + MANY_KEYS - 1) / MANY_KEYS;  // tiles
+  if (n > 0) {
+    int page[3] = {entry(0), entry(1), entry(2)};
+    load_v(0, page[0]);
+    v4i first_k[3];
+    uint32_t first_s[3][2];
+    bool first_there[3];
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+      load_k(j, page[j]);
+      first_k[j] = kreg, first_s[j][0] = ksb, first_s[j][1] = vsb, first_there[j] = kthere;
+    }
+    put_v(0);
+    load_v(1, page[1]);
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+      kreg = first_k[j], ksb = first_s[j][0], vsb = first_s[j][1], kthere = first_there[j];
+      put_k(j);
+    }
+    page[0] = page[2], page[1] = entry(3), page[2] = entry(4);  // of tiles j + 2, j + 3, j + 4
+    load_k(3, page[1]);
+    int ahead = entry_ahead(5);
+    change();
+    read_k(0, 0);
+    read_k(0, 1);
+    scores(0);
+    scores(1);
+    auto fetch = [&](int j) {
+      load_v(j + 2, page[0]);
+      load_k(j + 4, page[2]);
+      page[0] = page[1], page[1] = page[2], page[2] = __builtin_amdgcn_readfirstlane(ahead);
+      ahead = entry_ahead(j + 6);
+    };
+    // a wave whose rows see nothing of a tile, or that has none, only stages
+    auto sees = [&](int j) { return k0 + j * MANY_KEYS < high; };
+    if (!group && sees(0)) exponentials(0);
+    read_k(1, 0);
+    for (int j = 0; j + 1 < n; ++j) {
+      if (sees(j)) {
+        if (group) exponentials(j);
+        __builtin_amdgcn_s_setprio(1);
+        read_k(j + 1, 1);
+        scores(0);
+        put_k(j + 3);
+        __builtin_amdgcn_sched_barrier(0);
+        read_v(j, 0);
+        read_v(j, 1);
+        scores(1);
+        put_v(j + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        read_v(j, 2);
+        read_v(j, 3);
+        values(0);
+        values(1);
+        fetch(j);
+        values(2);
+        values(3);
+        __builtin_amdgcn_s_setprio(0);
+        if (!group) exponentials(j + 1);
+        read_k(j + 2, 0);
+      } else {
+        put_k(j + 3);
+        put_v(j + 1);
+        fetch(j);
+      }
+      change();
+    }
+    if (sees(n - 1)) {
+      if (group) exponentials(n - 1);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        read_v(n - 1, g);
+        values(g);
+      }
+    }
   }
   l = row_reduce<32>(l, sum_of);
   if (row >= a.R) return;
@@ -556,16 +672,16 @@ __global__ __launch_bounds__(512, 2) void kv_attend_many_kernel(const AttendArgs
     const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
     const int64_t at = out_row(a, b, hk, row) + 4 * h;
 #pragma unroll
-    for (int i = 0; i < DT32; ++i)
+    for (int i = 0; i < OT; ++i)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const float f[4] = {o[i][4 * g] * inv, o[i][4 * g + 1] * inv, o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv};
-        store_row<DT, 4>(a.o, at + 32 * i + 8 * g, f);
+        const float z[4] = {o[i][4 * g] * inv, o[i][4 * g + 1] * inv, o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv};
+        store_row<DT, 4>(a.o, at + 32 * i + 8 * g, z);
       }
   } else {
     const int64_t at = (((int64_t)b * a.c.H + hk) * a.splits + split) * a.R + row;
 #pragma unroll
-    for (int i = 0; i < DT32; ++i)
+    for (int i = 0; i < OT; ++i)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         *reinterpret_cast<v4f*>(a.part + at * D + 32 * i + 8 * g + 4 * h) =
@@ -616,14 +732,26 @@ struct AttendPlan {
   int splits;
   int64_t rows, tiles;  // rows a key head, row tiles of them
 };
-static AttendPlan plan_attend(int64_t B, int64_t H, int64_t Hk, int64_t S, int64_t width, int64_t page) {
+static AttendPlan plan_attend(int64_t B, int64_t H, int64_t Hk, int64_t S, int64_t D, int64_t width, int64_t page) {
   AttendPlan p{};
   p.rows = S * (H / Hk);
   p.few = p.rows <= FEW_ROWS;
   p.tiles = p.few ? 1 : cdiv(p.rows, MANY_ROWS);
-  const int64_t groups = B * Hk * p.tiles, unit = p.few ? FEW_UNIT : 4 * MANY_KEYS;
-  const int64_t want = cdiv(p.few ? 1024 : 512, groups), most = cdiv(width * page, unit);
-  p.splits = (int)(want < 1 ? 1 : want > most ? most : want);
+  const int64_t groups = B * Hk * p.tiles, keys = width * page;
+  p.splits = 1;
+  if (p.few) {
+    const int64_t want = cdiv(1024, groups), most = cdiv(keys, FEW_UNIT);
+    p.splits = (int)(want > most ? most : want);
+  } else {
+    // The rounds that the workgroups make over the compute units, of so many tiles each and some three tiles' time to begin
+    // and end, and joining: about five tiles' time, and two passes over the sums at 5 TB/s.
+    double best = 0.0;
+    for (int n = 1; n <= KV_MAX_SPLITS && (n == 1 || n * 4 * MANY_KEYS <= keys); ++n) {
+      const double rounds = (double)cdiv(groups * n, 256), each = (double)cdiv(cdiv(keys, n), MANY_KEYS) + 3.0;
+      const double join = n == 1 ? 0.0 : 5.0 + (double)groups * n * MANY_ROWS * D * 8.0 / 5.0e6;
+      if (n == 1 || rounds * each + join < best) best = rounds * each + join, p.splits = n;
+    }
+  }
   if (p.splits > KV_MAX_SPLITS) p.splits = KV_MAX_SPLITS;
   if (p.splits < 1) p.splits = 1;
   return p;
@@ -660,7 +788,7 @@ using namespace mxf8;
 extern "C" int64_t mxf8_kv_attend_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t S, int64_t D,
                                                   int64_t table_width, int64_t page_size) {
   if (B <= 0 || H <= 0 || Hk <= 0 || H % Hk || S <= 0 || D <= 0 || table_width <= 0 || page_size <= 0) return 0;
-  const AttendPlan p = plan_attend(B, H, Hk, S, table_width, page_size);
+  const AttendPlan p = plan_attend(B, H, Hk, S, D, table_width, page_size);
   return p.splits == 1 ? 0 : B * Hk * p.splits * p.rows * (D + 2) * 4;
 }
 
@@ -685,7 +813,7 @@ extern "C" int mxf8_kv_attend(const void* q, const int64_t q_strides[4], int dty
   if (q_strides[3] != 1 || out_strides[3] != 1)
     return set_error(MXF8_EINVAL, "%s: channels must be contiguous", what);
   if (S > (1 << 28) || S * (H / Hk) > (1 << 28)) return set_error(MXF8_EINVAL, "%s: shape too large", what);
-  const AttendPlan p = plan_attend(B, H, Hk, S, table_width, page_size);
+  const AttendPlan p = plan_attend(B, H, Hk, S, D, table_width, page_size);
   if (p.splits > 1 && (!workspace || (uintptr_t)workspace % 16))
     return set_error(MXF8_EINVAL, "%s: a 16-byte aligned workspace is needed", what);
   if (pages == 0) a.c.width = 0;  // no keys

@@ -17,10 +17,17 @@ struct KvPages {
   int H, width, shift;  // page = 1 << shift tokens
 };
 
+// Entry i of sequence b, for an i that is the same for the whole wave: read through the scalar cache.
+__device__ __forceinline__ int kv_entry(const KvPages& c, int b, int i) {
+  typedef const __attribute__((address_space(4))) int32_t* consts;
+  return ((consts)(uintptr_t)c.table)[b * c.table_stride + __builtin_amdgcn_readfirstlane(i)];
+}
+__device__ __forceinline__ bool kv_valid(const KvPages& c, int p) { return (uint32_t)p < (uint64_t)c.pages; }
+
 // Page `i` of sequence b, or -1 where there is none (an entry that names no page of the pool counts as none).
 __device__ __forceinline__ int kv_page(const KvPages& c, int b, int i) {
   const int p = c.table[b * c.table_stride + i];
-  return (uint32_t)p < (uint64_t)c.pages ? p : -1;
+  return kv_valid(c, p) ? p : -1;
 }
 
 // Tokens of sequence b that can be there: lengths beyond the table's pages, and negative ones, are cut.
