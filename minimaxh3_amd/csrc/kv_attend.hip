@@ -110,9 +110,11 @@ __device__ __forceinline__ float load_query(const AttendArgs& a, int b, int hk, 
   Raw8<DT> r[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    r[j].zero();
-    if (there) r[j].load(a.q, at + channel(j));
+    r[j].load(a.q, at + channel(j));  // (before it is known whether the row is there: the load need not wait for the lengths)
   }
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (!there) r[j].zero();
   int e = 0;
   if constexpr (DT == MXF8_BF16) {
     float top = 0.0f;
@@ -166,7 +168,7 @@ struct FewStep {
 };
 
 template <int DT, int D, int NR>
-__global__ __launch_bounds__(256) void kv_attend_few_kernel(const AttendArgs a) {
+__global__ __launch_bounds__(256, (D == 64 ? (NR == 1 ? 4 : NR == 2 ? 3 : 2) : NR == 1 ? 3 : 4 / NR)) void kv_attend_few_kernel(const AttendArgs a) {
   constexpr int KK = D / 32, DI = D / 16, W = D / 64;
   __shared__ float om[4][16][D + 4];
   __shared__ float ml[4][2][16 * NR];
@@ -203,12 +205,16 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(const AttendArgs a) 
   }
 
   const int mask = (1 << a.c.shift) - 1;
+  const uint32_t k_lane = c * D + 16 * q, v_lane = 4 * q * D + c * DI;
   auto pages = [&](int key0, int (&pid)[2]) {
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       const int key = key0 + 16 * g;
       pid[g] = -1;
-      if (key < k1) pid[g] = __builtin_amdgcn_readfirstlane(kv_page(a.c, b, key >> a.c.shift));
+      if (key < k1) {
+        const int p = kv_entry(a.c, b, key >> a.c.shift);
+        pid[g] = kv_valid(a.c, p) ? p : -1;
+      }
     }
   };
   auto load = [&](int key0, const int (&pid)[2], FewStep<D>& s) {
@@ -219,17 +225,17 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(const AttendArgs a) 
       const int64_t at = ((ph << a.c.shift) + ((key0 + 16 * g) & mask)) * D;
       s.pid[g] = pid[g];
       s.ks[g] = a.c.ks[ph], s.vs[g] = a.c.vs[ph];
-      const uint8_t* k = a.c.k + at + c * D + 16 * q;
-      const uint8_t* v = a.c.v + at + 4 * q * D + c * DI;
+      // (addresses: a base that the wave shares and 32 bits of a lane's own)
+      const gbytes k = (gbytes)(a.c.k + at), v = (gbytes)(a.c.v + at);
 #pragma unroll
-      for (int j = 0; j < W; ++j) s.k[g][j] = *reinterpret_cast<const v4i*>(k + 64 * j);
+      for (int j = 0; j < W; ++j) s.k[g][j] = *(const __attribute__((address_space(1))) v4i*)(k + (k_lane + 64 * j));
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if constexpr (W == 2) {
-          const v2i x = *reinterpret_cast<const v2i*>(v + j * D);
+          const v2i x = *(const __attribute__((address_space(1))) v2i*)(v + (v_lane + j * D));
           s.v[4 * g + j][0] = x[0], s.v[4 * g + j][W - 1] = x[1];
         } else {
-          s.v[4 * g + j][0] = *reinterpret_cast<const uint32_t*>(v + j * D);
+          s.v[4 * g + j][0] = *(const __attribute__((address_space(1))) uint32_t*)(v + (v_lane + j * D));
         }
     }
   };
@@ -693,37 +699,59 @@ __global__ __launch_bounds__(512, 2) void kv_attend_many_kernel(const AttendArgs
 // ---- splits joined ---------------------------------------------------------------------
 constexpr int KV_MAX_SPLITS = 64;
 
-// One wave a row: the splits' maxima and sums in a lane each, then their outputs, D / 64 channels a lane.
-template <int DT, int D>
+// One row to WAVES waves: the splits' maxima and sums in a lane each, then their outputs, four channels a lane and 256 / D
+// splits at once.  The first loads do not wait to know how many splits there are.
+template <int DT, int D, int WAVES>
 __global__ __launch_bounds__(256) void kv_attend_join_kernel(const AttendArgs a, int rows, int unit) {
-  constexpr int W = D / 64;
-  typedef float vf __attribute__((ext_vector_type(W)));
+  constexpr int L = D / 4, P = 64 / L, U = 8;  // lanes of a split, splits at once, loads in flight
+  __shared__ v4f sums[4][64];
   const int lane = threadIdx.x & 63, hk = blockIdx.y, b = blockIdx.z;
-  const int row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (row >= a.R) return;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = blockIdx.x * (4 / WAVES) + w / WAVES;
+  if (WAVES == 1 && row >= a.R) return;
+  const int64_t at = (((int64_t)b * a.c.H + hk) * a.splits) * a.R + row;
+  const float* part = a.part + at * D + lane % L * 4;
+  const int first = w % WAVES * P + lane / L;  // this lane's splits: first, first + P WAVES, ...
+  auto load = [&](int s) { return *reinterpret_cast<const v4f*>(part + (int64_t)s * a.R * D); };
+  v4f x[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) x[i] = load(min(first + i * P * WAVES, a.splits - 1));
+  float m = KV_NONE, l = 0.0f;
+  const v2f st = *reinterpret_cast<const v2f*>(a.stat + (at + (int64_t)min(lane, a.splits - 1) * a.R) * 2);
   const int r0 = row / rows * rows, end = kv_end(a, kv_seq(a, b), r0, r0 + rows);
   const int chunk = kv_chunk(a, end, unit), n = end ? (end + chunk - 1) / chunk : 0;
-  const int64_t at = (((int64_t)b * a.c.H + hk) * a.splits) * a.R + row;
-  float m = KV_NONE, l = 0.0f;
-  if (lane < n) {
-    const v2f s = *reinterpret_cast<const v2f*>(a.stat + (at + (int64_t)lane * a.R) * 2);
-    m = s[0], l = s[1];
-  }
+  if (lane < n) m = st[0], l = st[1];
   const float f = __builtin_amdgcn_exp2f(m - lanes_max<64>(m));
   const float sum = lanes_sum<64>(l * f);
-  float o[W] = {};
-  const float* part = a.part + at * D + lane * W;
-#pragma unroll 8
-  for (int s = 0; s < n; ++s) {
-    const vf x = *reinterpret_cast<const vf*>(part + (int64_t)s * a.R * D);
-    const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s));
+  v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s0 = first;; s0 += U * P * WAVES) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) o[i] = __builtin_fmaf(((const float*)&x)[i], fs, o[i]);
+    for (int i = 0; i < U; ++i) {
+      const int s = s0 + i * P * WAVES;
+      const float fs = __shfl(f, s & 63, 64);
+      if (s < n) o += x[i] * fs;
+    }
+    if (s0 - lane / L + U * P * WAVES >= n) break;
+#pragma unroll
+    for (int i = 0; i < U; ++i) x[i] = load(min(s0 + (U + i) * P * WAVES, a.splits - 1));
   }
-  const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
-  const int64_t to = out_row(a, b, hk, row) + lane * W;
+  if constexpr (P == 2 || P == 4) {
 #pragma unroll
-  for (int i = 0; i < W; ++i) store1<DT>(a.o, to + i, o[i] * inv);
+    for (int off = L; off < 64; off *= 2)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], off, 64);
+  }
+  if constexpr (WAVES > 1) {
+    sums[w][lane] = o;
+    __syncthreads();
+    if (w % WAVES) return;
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) o += sums[w + i][lane];
+  }
+  if (lane >= L || row >= a.R) return;
+  const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+  const float z[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+  store_row<DT, 4>(a.o, out_row(a, b, hk, row) + lane * 4, z);
 }
 
 // ---- plan ------------------------------------------------------------------------------
@@ -776,8 +804,11 @@ static int launch_attend(AttendArgs& a, const AttendPlan& p, int B, hipStream_t 
   }
   if (const int rc = check_launch(what)) return rc;
   if (p.splits == 1) return MXF8_OK;
-  kv_attend_join_kernel<DT, D><<<dim3((unsigned)cdiv(a.R, 4), Hk, B), 256, 0, st>>>(a, p.few ? FEW_ROWS : MANY_ROWS,
-                                                                                     p.few ? FEW_UNIT : MANY_KEYS);
+  const int rows = p.few ? FEW_ROWS : MANY_ROWS, unit = p.few ? FEW_UNIT : MANY_KEYS;
+  if (p.few)
+    kv_attend_join_kernel<DT, D, 4><<<dim3((unsigned)a.R, Hk, B), 256, 0, st>>>(a, rows, unit);
+  else
+    kv_attend_join_kernel<DT, D, 1><<<dim3((unsigned)cdiv(a.R, 4), Hk, B), 256, 0, st>>>(a, rows, unit);
   return check_launch(what);
 }
 

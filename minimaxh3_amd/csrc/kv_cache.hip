@@ -40,7 +40,9 @@ __device__ __forceinline__ int kv_exponent(float amax) {
 }
 __device__ __forceinline__ float kv_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-enum { TURN_NONE, TURN_INTERLEAVED, TURN_HALF, TURN_HALF_ANY };
+// What happens to a key on the way: nothing; the norm or the rotation of neighbouring channels, or both; with half-split pairs,
+// whose partners are at the same place of another lane's eight (P % 8 == 0), or anywhere.
+enum { KEY_PLAIN, KEY_PAIRS, KEY_HALF, KEY_HALF_ANY };
 
 struct AppendArgs {
   KvPages c;
@@ -49,17 +51,125 @@ struct AppendArgs {
   const float* turns;     // cos / sin [.., S, P, 2]
   int64_t turns_batch;
   const int32_t *starts, *counts;
-  int S, P, mode, heads;  // heads: of one workgroup
+  int S, P;
   float eps;
 };
 
-// A workgroup writes one page of one sequence, head after head: D / 8 lanes hold a token's eight channels each, so the
-// page's maximum is one reduction over values that stay in registers until they are rounded.
-template <int DT, int D, int N>
-__global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
-  constexpr int L = D / 8, T = 256 / L;  // lanes a token, tokens a step
-  __shared__ float red[2][2][4];
-  __shared__ float exchange[256 * 8];
+// f over the L (8 or 16) neighbouring lanes that hold a token.
+template <int L>
+__device__ __forceinline__ double lanes_sum64(double v) {
+#define MXF8_STEP(CTRL)                                                                                            \
+  {                                                                                                                \
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);                                                            \
+    const uint32_t lo = __builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xf, 0xf, true);                          \
+    const uint32_t hi = __builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, true);                  \
+    v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);                                                      \
+  }
+  MXF8_STEP(0xb1)
+  MXF8_STEP(0x4e)
+  MXF8_STEP(0x141)
+  if constexpr (L == 16) MXF8_STEP(0x140)
+#undef MXF8_STEP
+  return v;
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, off, 64));
+  return v;
+}
+
+template <int N>
+__device__ __forceinline__ uint32_t block_max(const uint32_t (&waves)[N]) {
+  uint32_t v = waves[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) v = max(v, waves[i]);
+  return v;
+}
+
+// The largest |x| of eight as stored: of 16 bits in both halves, of fp32 as it is; infinities and NaN come last.
+template <int DT>
+__device__ __forceinline__ uint32_t raw_max(const Raw8<DT>& r, uint32_t top) {
+  if constexpr (DT == MXF8_F32) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(r.w[j]) & 0x7fffffffu);
+  } else {
+    typedef unsigned short v2u __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(v2u, top),
+                                                                   __builtin_bit_cast(v2u, r.w[j] & 0x7fff7fffu)));
+  }
+  return top;
+}
+// raw_max's result as fp32 bits
+template <int DT>
+__device__ __forceinline__ uint32_t raw_max_f32(uint32_t top) {
+  if constexpr (DT == MXF8_F32) return top;
+  const uint32_t t = max(top & 0xffffu, top >> 16);
+  return DT == MXF8_BF16 ? t << 16 : __float_as_uint(f16_bits_to_f32(t));
+}
+
+// Eight values to codes under 2^e; none is larger than 448 2^e.
+typedef short v2s __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ v2i codes_of(const float (&f)[8], float scale) {
+  v2s w[2] = {};
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    w[j] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w[j], f[4 * j], f[4 * j + 1], scale, false);
+    w[j] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w[j], f[4 * j + 2], f[4 * j + 3], scale, true);
+  }
+  return v2i{__builtin_bit_cast(int, w[0]), __builtin_bit_cast(int, w[1])};
+}
+template <int DT>
+__device__ __forceinline__ v2i codes_of(const Raw8<DT>& r, float scale) {
+  if constexpr (DT == MXF8_F32) {
+    float f[8];
+    r.get(f);
+    return codes_of(f, scale);
+  } else {
+    v2s w[2] = {};
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if constexpr (DT == MXF8_BF16) {
+        w[j] = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w[j], __builtin_bit_cast(v2bf, r.w[2 * j]), scale, false);
+        w[j] = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w[j], __builtin_bit_cast(v2bf, r.w[2 * j + 1]), scale, true);
+      } else {
+        w[j] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w[j], __builtin_bit_cast(v2h, r.w[2 * j]), scale, false);
+        w[j] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w[j], __builtin_bit_cast(v2h, r.w[2 * j + 1]), scale, true);
+      }
+    return v2i{__builtin_bit_cast(int, w[0]), __builtin_bit_cast(int, w[1])};
+  }
+}
+
+constexpr uint32_t INF_BITS = 0x7f800000u, LARGEST_BITS = 0x63600000u;  // of 448 2^63
+
+// fp64 to fp32 on the way to a code: rounded to nearest, but off a tie between two codes that the value is not on.  (So
+// the code is the one nearest to the value in 64 bits, down to 2^-6 of the scale.)
+__device__ __forceinline__ void round_keys(const double (&y)[8], float (&f)[8]) {
+  bool tie = false;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    f[j] = (float)y[j];
+    tie |= __float_as_uint(f[j]) << 12 == 0x80000000u;
+  }
+  if (__ballot(tie)) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const double d = y[j] - (double)f[j];
+      if (__float_as_uint(f[j]) << 12 == 0x80000000u && d != 0.0)
+        f[j] = __uint_as_float(__float_as_uint(f[j]) + ((d > 0.0) == (f[j] > 0.0f) ? 1 : -1));
+    }
+  }
+}
+
+// A workgroup writes one page and head of one sequence: D / 8 lanes hold a token's eight channels each, so the
+// page's maximum is one reduction over values that stay in registers until they are rounded.  Keys are normed and turned in
+// fp64, which costs less than the memory takes and leaves no key on the wrong side of a border between two codes.
+template <int DT, int D, int MODE, int THREADS, int N>
+__global__ __launch_bounds__(THREADS, MODE == KEY_HALF_ANY || (N == 4 && THREADS == 512) ? 2 : 4) void kv_append_kernel(const AppendArgs a) {
+  constexpr int L = D / 8, T = THREADS / L, WAVES = THREADS / 64;  // lanes a token, tokens a step
+  __shared__ uint32_t red[2][WAVES];
+  __shared__ float exchange[MODE == KEY_HALF_ANY ? THREADS * 8 : 1];
   const int b = blockIdx.z, lane = threadIdx.x & 63, l = threadIdx.x % L, c0 = 8 * l;
   const int page = 1 << a.c.shift;
   const int64_t start = a.starts[b];
@@ -71,218 +181,318 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
   if (pid < 0) return;
   const bool any_old = start > base;
   const int first = threadIdx.x / L;  // this thread's tokens of the page: first, first + T, ...
+  bool there[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) there[i] = first + i * T < page && base + first + i * T >= lo && base + first + i * T < hi;
+  const int64_t s0 = base + first - start;  // of the call's tokens, this thread's first
   const float* turns = a.turns + b * a.turns_batch;
-  float wk[8], wp[8];
-  // half-split partner: channel c +- P, in lane l +- P / 8 of the token where P % 8 == 0
-  const int plane = (lane - l) + min(max(c0 < a.P ? l + a.P / 8 : l - a.P / 8, 0), L - 1);
-  if (a.w) {
-    Raw8<DT> w;
-    w.load(a.w, c0);
-    w.get(wk);
-    if (a.mode == TURN_HALF) w.from_lane(plane);
-    w.get(wp);
+  // half-split: the channel that each of this lane's turns with, and the norm's weights of both
+  auto partner = [&](int j) {
+    if (MODE == KEY_HALF) return (c0 < a.P ? c0 + a.P : c0 < 2 * a.P ? c0 - a.P : c0) + j;
+    const int c = c0 + j;
+    return c < a.P ? c + a.P : c < 2 * a.P ? c - a.P : c;
+  };
+  Raw8<DT> wk, wp;
+  wk.fill(1.0f), wp.fill(1.0f);
+  if (MODE != KEY_PLAIN && a.w) {
+    wk.load(a.w, c0);
+    if (MODE == KEY_HALF) wp.load(a.w, partner(0));
   }
-  for (int h = blockIdx.y * a.heads, last = min(h + a.heads, a.c.H), turn = 0; h < last; ++h, turn ^= 1) {
-    Raw8<DT> kr[N], vr[N];
+  const int plane = (lane - l) + partner(0) / 8;  // the lane that holds all eight
+  const int h = blockIdx.y;
+  Raw8<DT> kr[N], vr[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int64_t pos = base + first + i * T;
-      kr[i].zero(), vr[i].zero();
-      if (first + i * T < page && pos >= lo && pos < hi) {
-        const int64_t s = pos - start;
-        kr[i].load_stream(a.x[0], b * a.xs[0][0] + h * a.xs[0][1] + s * a.xs[0][2] + c0);
-        vr[i].load_stream(a.x[1], b * a.xs[1][0] + h * a.xs[1][1] + s * a.xs[1][2] + c0);
-      }
+  for (int i = 0; i < N; ++i) {
+    kr[i].zero(), vr[i].zero();
+    if (there[i]) {
+      kr[i].load_stream(a.x[0], b * a.xs[0][0] + h * a.xs[0][1] + (s0 + i * T) * a.xs[0][2] + c0);
+      vr[i].load_stream(a.x[1], b * a.xs[1][0] + h * a.xs[1][1] + (s0 + i * T) * a.xs[1][2] + c0);
     }
-    const int64_t ph = (int64_t)pid * a.c.H + h;
-    const int ek_old = (int)a.c.ks[ph] - 127, ev_old = (int)a.c.vs[ph] - 127;
-    float k[N][8], amax[2] = {0.0f, 0.0f};
-    bool bad[N];
+  }
+  // interleaved: a lane's four pairs of a token, neighbours in memory
+  auto load_turns = [&](int i, float (&cs)[8]) {
+    if (MODE != KEY_PAIRS) return;
+    // (a token that is not there has zeros, and any angles)
+    const float* t = turns + ((there[i] ? s0 + i * T : 0) * a.P + c0 / 2) * 2;
+    if (c0 / 2 + 4 <= a.P) {
+      const floats4 t0 = *(gfloats4)(gbytes)t, t1 = *(gfloats4)(gbytes)(t + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) cs[j] = t0[j], cs[4 + j] = t1[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) cs[j] = c0 / 2 + j / 2 < a.P ? t[j] : 0.0f;
+    }
+  };
+  float cs[2][8];
+  load_turns(0, cs[0]);
+  const int64_t ph = (int64_t)pid * a.c.H + h;
+  const int old[2] = {(int)a.c.ks[ph] - 127, (int)a.c.vs[ph] - 127};
+  float k[N][8];
+  uint32_t raw[2] = {0, 0}, top[2];
+#pragma unroll
+  for (int i = 0; i < N; ++i) raw[0] = raw_max(kr[i], raw[0]), raw[1] = raw_max(vr[i], raw[1]);
+  top[0] = raw_max_f32<DT>(raw[0]), top[1] = raw_max_f32<DT>(raw[1]);
+  if constexpr (MODE == KEY_PLAIN) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) kr[i].get(k[i]);
+  } else {
+    float size = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int64_t pos = base + first + i * T;
-      const bool there = first + i * T < page && pos >= lo && pos < hi;
-      float f[8], q[8];
-      kr[i].get(f);
-      if (a.mode == TURN_HALF) kr[i].from_lane(plane);
-      kr[i].get(q);
+      __builtin_amdgcn_sched_barrier(0);  // (one token's 64-bit values at a time)
+      if (i + 1 < N) load_turns(i + 1, cs[(i + 1) & 1]);
+      float x[8], w[8];
+      kr[i].get(x);
+      wk.get(w);
+      double y[8], g = 1.0;
       if (a.w) {
-        float ss = 0.0f;
+        double ss = 0.0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(f[j], f[j], ss);
-        const float r = rsqrtf(__builtin_fmaf(lanes_sum<L>(ss), 1.0f / D, a.eps));
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] *= r * wk[j], q[j] *= r * wp[j];
+        for (int j = 0; j < 8; ++j) ss = __builtin_fma((double)x[j], (double)x[j], ss);
+        g = rsqrt(__builtin_fma(lanes_sum64<L>(ss), 1.0 / D, (double)a.eps));
       }
-      const float2* t = reinterpret_cast<const float2*>(turns) + (there ? pos - start : 0) * a.P;
-      if (a.mode == TURN_INTERLEAVED) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float x = f[2 * j], y = f[2 * j + 1];
+      for (int j = 0; j < 8; ++j) y[j] = (double)x[j] * (g * (double)w[j]);
+      if constexpr (MODE == KEY_PAIRS) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
           if (c0 / 2 + j < a.P) {
-            const float2 cs = t[c0 / 2 + j];
-            f[2 * j] = __builtin_fmaf(x, cs.x, -(y * cs.y));
-            f[2 * j + 1] = __builtin_fmaf(x, cs.y, y * cs.x);
+            const double u = y[2 * j], v = y[2 * j + 1], co = cs[i & 1][2 * j], si = cs[i & 1][2 * j + 1];
+            y[2 * j] = __builtin_fma(u, co, -(v * si));
+            y[2 * j + 1] = __builtin_fma(u, si, v * co);
           }
-        }
-      } else if (a.mode != TURN_NONE) {
-        if (a.mode == TURN_HALF_ANY) {
+      } else {
+        float q[8];
+        const float* t = turns + (there[i] ? s0 + i * T : 0) * a.P * 2;
+        if constexpr (MODE == KEY_HALF) {
+          Raw8<DT> r = kr[i];
+          r.from_lane(plane);
+          r.get(q);
+          wp.get(w);
+        } else {
           // (this wave's part of the exchange alone: LDS operations of a wave complete in order)
           float* mine = exchange + (threadIdx.x & ~63) * 8;
-          *reinterpret_cast<v4f*>(mine + lane * 8) = v4f{f[0], f[1], f[2], f[3]};
-          *reinterpret_cast<v4f*>(mine + lane * 8 + 4) = v4f{f[4], f[5], f[6], f[7]};
+          *reinterpret_cast<v4f*>(mine + lane * 8) = v4f{x[0], x[1], x[2], x[3]};
+          *reinterpret_cast<v4f*>(mine + lane * 8 + 4) = v4f{x[4], x[5], x[6], x[7]};
           __builtin_amdgcn_wave_barrier();
-          const float* head = mine + (lane - l) * 8;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int c = c0 + j;
-            q[j] = head[c < a.P ? c + a.P : c < 2 * a.P ? c - a.P : c];
-          }
+          for (int j = 0; j < 8; ++j) q[j] = mine[(lane - l) * 8 + partner(j)];
           __builtin_amdgcn_wave_barrier();
+          typedef typename Elem<DT>::T E;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (a.w) w[j] = Elem<DT>::to_f32(static_cast<const E*>(a.w)[partner(j)]);
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int c = c0 + j;
-          if (c < 2 * a.P) {
-            const float2 cs = t[c < a.P ? c : c - a.P];
-            f[j] = __builtin_fmaf(f[j], cs.x, q[j] * (c < a.P ? -cs.y : cs.y));
+        for (int j4 = 0; j4 < 8; j4 += 2) {
+          float co[2], si[2];
+          if (MODE == KEY_HALF && c0 < 2 * a.P) {  // this lane's pairs are neighbours
+            const floats4 v = *(gfloats4)(gbytes)(t + (min(c0, partner(0)) + j4) * 2);
+            co[0] = v[0], si[0] = v[1], co[1] = v[2], si[1] = v[3];
+          } else {
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+              const int pair = min(c0 + j4 + m, partner(j4 + m));
+              co[m] = pair < a.P ? t[2 * pair] : 1.0f, si[m] = pair < a.P ? t[2 * pair + 1] : 0.0f;
+            }
+          }
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            const int j = j4 + m;
+            if (c0 + j < 2 * a.P)
+              y[j] = __builtin_fma(y[j], (double)co[m], (double)q[j] * (g * (double)w[j]) * (double)(c0 + j < a.P ? -si[m] : si[m]));
           }
         }
       }
-      bad[i] = false;
+      round_keys(y, k[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) size = fmaxf(size, fabsf(k[i][j]));
+    }
+    // (what is not finite before the turn stays so, but a maximum leaves NaN out)
+    top[0] = max(__float_as_uint(size), top[0] >= INF_BITS ? top[0] : 0);
+  }
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    top[p] = wave_max_u32(top[p]);
+    if (lane == 0) red[p][threadIdx.x >> 6] = top[p];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+    top[p] = block_max(red[p]);
+  uint8_t* code[2] = {const_cast<uint8_t*>(a.c.k) + (ph << a.c.shift) * D, const_cast<uint8_t*>(a.c.v) + (ph << a.c.shift) * D};
+  int e[2];
+  if (max(top[0], top[1]) <= LARGEST_BITS) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      e[p] = kv_exponent(__uint_as_float(top[p]));
+      if (any_old) e[p] = max(e[p], old[p]);
+    }
+    const float sk = kv_pow2(e[0]), sv = kv_pow2(e[1]);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (there[i]) {
+        const int64_t o = (int64_t)(first + i * T) * D + c0;
+        *reinterpret_cast<v2i*>(code[0] + o) = codes_of(k[i], sk);
+        *reinterpret_cast<v2i*>(code[1] + o) = codes_of<DT>(vr[i], sv);
+      }
+  } else {
+    // Something is not finite, or past the scales' range: the largest finite size, infinities as the largest code.  A NaN
+    // anywhere in a token stays as one in its key, which reaches the rows that attend to it and no others; a NaN among
+    // the values would reach every row of a product, also those whose mask leaves it out.
+    float size[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
       float v[8];
       vr[i].get(v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        k[i][j] = f[j];
-        const float x = fabsf(f[j]), y = fabsf(v[j]);
-        amax[0] = fmaxf(amax[0], x < INFINITY ? x : 0.0f);
-        amax[1] = fmaxf(amax[1], y < INFINITY ? y : 0.0f);
-        bad[i] |= !(x <= INFINITY) || !(y <= INFINITY);
+        const float x = fabsf(k[i][j]), y = fabsf(v[j]);
+        size[0] = fmaxf(size[0], x < INFINITY ? x : 0.0f), size[1] = fmaxf(size[1], y < INFINITY ? y : 0.0f);
       }
     }
+    __syncthreads();
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      amax[p] = lanes_max<64>(amax[p]);
-      if (lane == 0) red[turn][p][threadIdx.x >> 6] = amax[p];
+      top[p] = wave_max_u32(__float_as_uint(size[p]));
+      if (lane == 0) red[p][threadIdx.x >> 6] = top[p];
     }
-    __syncthreads();  // (the two halves of `red` in turn: the next head's writes pass this one's reads by a barrier)
-    int e[2];
+    __syncthreads();
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      e[p] = kv_exponent(fmaxf(fmaxf(red[turn][p][0], red[turn][p][1]), fmaxf(red[turn][p][2], red[turn][p][3])));
-      if (any_old) e[p] = max(e[p], p ? ev_old : ek_old);
+      e[p] = kv_exponent(__uint_as_float(block_max(red[p])));
+      if (any_old) e[p] = max(e[p], old[p]);
     }
     const float ik = kv_pow2(-e[0]), iv = kv_pow2(-e[1]);
-    uint8_t* kc = const_cast<uint8_t*>(a.c.k) + (ph << a.c.shift) * D;
-    uint8_t* vc = const_cast<uint8_t*>(a.c.v) + (ph << a.c.shift) * D;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int64_t pos = base + first + i * T;
       float v[8];
       vr[i].get(v);
-      // A NaN anywhere in the token stays as one in its key, which reaches the rows that attend to it and no others;
-      // a NaN among the values would reach every row of a product, also those whose mask leaves it out.
-      const uint64_t any_bad = __ballot(bad[i]);
-      uint32_t nan_key = 0;
-      if (any_bad) {
+      bool bad = false;
+      uint32_t w[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          k[i][j] = k[i][j] == k[i][j] ? k[i][j] : 0.0f;
-          v[j] = v[j] == v[j] ? v[j] : 0.0f;
+      for (int p = 0; p < 4; ++p) {
+        float x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[j] = p < 2 ? k[i][4 * p + j] : v[4 * (p - 2) + j];
+          bad |= x[j] != x[j];
+          x[j] = x[j] == x[j] ? clamp448(x[j] * (p < 2 ? ik : iv)) : 0.0f;
         }
-        nan_key = l == 0 && (any_bad >> (lane - l) & ((1ull << L) - 1)) ? 0x7fu : 0u;
+        w[p] = cvt4_e4m3(x[0], x[1], x[2], x[3]);
       }
-      if (first + i * T < page && pos >= lo && pos < hi) {
-        uint32_t w[4];
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const float* x = p < 2 ? k[i] + 4 * p : v + 4 * (p - 2);
-          const float s = p < 2 ? ik : iv;
-          w[p] = cvt4_e4m3(clamp448(x[0] * s), clamp448(x[1] * s), clamp448(x[2] * s), clamp448(x[3] * s));
-        }
-        w[0] |= nan_key;
+      const uint64_t any = __ballot(bad);
+      if (l == 0 && (any >> lane & ((1ull << L) - 1))) w[0] |= 0x7fu;
+      if (there[i]) {
         const int64_t o = (int64_t)(first + i * T) * D + c0;
-        *reinterpret_cast<v2i*>(kc + o) = v2i{(int)w[0], (int)w[1]};
-        *reinterpret_cast<v2i*>(vc + o) = v2i{(int)w[2], (int)w[3]};
+        *reinterpret_cast<v2i*>(code[0] + o) = v2i{(int)w[0], (int)w[1]};
+        *reinterpret_cast<v2i*>(code[1] + o) = v2i{(int)w[2], (int)w[3]};
       }
     }
-    if (threadIdx.x == 0) {
-      const_cast<uint8_t*>(a.c.ks)[ph] = (uint8_t)(e[0] + 127);
-      const_cast<uint8_t*>(a.c.vs)[ph] = (uint8_t)(e[1] + 127);
-    }
+  }
+  if (threadIdx.x == 0) {
+    const_cast<uint8_t*>(a.c.ks)[ph] = (uint8_t)(e[0] + 127);
+    const_cast<uint8_t*>(a.c.vs)[ph] = (uint8_t)(e[1] + 127);
+  }
+  if (any_old)
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const int d = (p ? ev_old : ek_old) - e[p];
-      if (!any_old || d >= 0) continue;
+      const int d = old[p] - e[p];
+      if (d >= 0) continue;
       const float s = kv_pow2(max(d, -126));
-      uint8_t* c = p ? vc : kc;
-      for (int64_t o = threadIdx.x * 8; o < (start - base) * D; o += 256 * 8) {
-        v2i w = *reinterpret_cast<const v2i*>(c + o);
+      for (int64_t o = threadIdx.x * 8; o < (start - base) * D; o += THREADS * 8) {
+        v2i w = *reinterpret_cast<const v2i*>(code[p] + o);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const v2f x = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], false), y = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], true);
           w[j] = (int)cvt4_e4m3(x[0] * s, x[1] * s, y[0] * s, y[1] * s);
         }
-        *reinterpret_cast<v2i*>(c + o) = w;
+        *reinterpret_cast<v2i*>(code[p] + o) = w;
       }
     }
-  }
 }
 
-template <int DT, int D>
-static int launch_append(AppendArgs& a, dim3 grid, hipStream_t st) {
-  const int steps = (D << a.c.shift) / 2048;
-  if (steps <= 1)
-    kv_append_kernel<DT, D, 1><<<grid, 256, 0, st>>>(a);
-  else if (steps == 2)
-    kv_append_kernel<DT, D, 2><<<grid, 256, 0, st>>>(a);
-  else if (steps == 4)
-    kv_append_kernel<DT, D, 4><<<grid, 256, 0, st>>>(a);
+template <int DT, int D, int MODE>
+static int launch_append(const AppendArgs& a, dim3 grid, hipStream_t st) {
+  // Up to four tokens a lane in workgroups of 256; two in 512 where half-split pairs cost more registers.
+  const int chunks = (D << a.c.shift) / 8;  // of eight channels
+  constexpr int BIG = MODE <= KEY_PAIRS ? 256 : 512;
+  if (chunks <= 256)
+    kv_append_kernel<DT, D, MODE, 256, 1><<<grid, 256, 0, st>>>(a);
+  else if (chunks == 512)
+    kv_append_kernel<DT, D, MODE, 256, 2><<<grid, 256, 0, st>>>(a);
+  else if (chunks == 1024)
+    kv_append_kernel<DT, D, MODE, BIG, 1024 / BIG><<<grid, BIG, 0, st>>>(a);
   else if constexpr (D == 128)
-    kv_append_kernel<DT, D, 8><<<grid, 256, 0, st>>>(a);
+    kv_append_kernel<DT, D, MODE, 512, 4><<<grid, 512, 0, st>>>(a);
   return check_launch("kv_append");
+}
+template <int DT, int D>
+static int launch_append(const AppendArgs& a, int mode, dim3 grid, hipStream_t st) {
+  switch (mode) {
+    case KEY_PLAIN: return launch_append<DT, D, KEY_PLAIN>(a, grid, st);
+    case KEY_PAIRS: return launch_append<DT, D, KEY_PAIRS>(a, grid, st);
+    case KEY_HALF: return launch_append<DT, D, KEY_HALF>(a, grid, st);
+    default: return launch_append<DT, D, KEY_HALF_ANY>(a, grid, st);
+  }
 }
 
 struct ReadArgs {
   KvPages c;
   const int32_t *starts, *lengths;
   void *k, *v;
-  int64_t T, chunks;  // tokens of a sequence, and its chunks of 16 channels
+  int64_t T, pages;  // tokens of a sequence, and the pages that they may touch
 };
 
-// 16 channels of a token, of keys and of values, per thread.
-template <int DT, int D>
+// Eight channels a lane, so that a wave stores a row of memory at once; a page and head is 128 such chunks or a multiple, and
+// each wave reads chunks of one page, of keys and of values, I times.
+template <int DT, int D, int I>
 __global__ __launch_bounds__(256) void kv_read_kernel(const ReadArgs a) {
-  constexpr int L = D / 16;
-  const int b = blockIdx.z, h = blockIdx.y;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= a.chunks) return;
-  const int64_t t = i / L, c = i % L * 16, pos = a.starts[b] + t;
-  int pid = -1;
-  if (pos >= 0 && pos < kv_length(a.c, a.lengths ? (int64_t)a.lengths[b] : INT64_MAX))
-    pid = kv_page(a.c, b, (int)(pos >> a.c.shift));
-  const int64_t ph = (int64_t)max(pid, 0) * a.c.H + h, o = ((int64_t)b * a.c.H + h) * a.T * D + t * D + c;
+  constexpr int L = D / 8;
+  const int b = blockIdx.z, h = blockIdx.y, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int per = a.c.shift + (D == 128 ? 4 : 3) - 6;  // log2 of the waves' turns that a page takes
+  const int64_t start = a.starts[b], first = start >> a.c.shift;
+  const int64_t end = min(start + a.T, (int64_t)kv_length(a.c, a.lengths ? (int64_t)a.lengths[b] : INT64_MAX));
+  v2i x[I][2];
+  float s[I][2];
+  int64_t at[I];
 #pragma unroll
-  for (int p = 0; p < 2; ++p) {
-    v4i w = {0, 0, 0, 0};
-    float s = 0.0f;
-    if (pid >= 0) {
-      w = *reinterpret_cast<const v4i*>((p ? a.c.v : a.c.k) + ((ph << a.c.shift) + (pos & ((1 << a.c.shift) - 1))) * D + c);
-      s = kv_scale((p ? a.c.vs : a.c.ks)[ph]);
+  for (int i = 0; i < I; ++i) {
+    const int64_t turn = (int64_t)(blockIdx.x * I + i) * 4 + w, index = first + (turn >> per);
+    const int slot = ((int)(turn & ((1 << per) - 1)) * 64 + lane) / L;
+    const int64_t pos = (index << a.c.shift) + slot;
+    at[i] = (turn >> per) < a.pages && pos >= start && pos < start + a.T ? pos - start : -1;
+    int pid = -1;
+    if ((index << a.c.shift) < end && index >= 0) {
+      pid = kv_entry(a.c, b, (int)index);
+      pid = kv_valid(a.c, pid) ? pid : -1;
     }
+    const int64_t ph = (int64_t)max(pid, 0) * a.c.H + h;
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
+    for (int p = 0; p < 2; ++p) {
+      x[i][p] = v2i{0, 0}, s[i][p] = 0.0f;
+      if (pid >= 0) {
+        s[i][p] = kv_scale((p ? a.c.vs : a.c.ks)[ph]);
+        if (at[i] >= 0 && pos < end)
+          x[i][p] = *reinterpret_cast<const v2i*>((p ? a.c.v : a.c.k) + ((ph << a.c.shift) + slot) * D + lane % L * 8);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    if (at[i] < 0) continue;
+    const int64_t o = (((int64_t)b * a.c.H + h) * a.T + at[i]) * D + lane % L * 8;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
       float f[8];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const v2f x = __builtin_amdgcn_cvt_pk_f32_fp8(w[2 * g + j], false);
-        const v2f y = __builtin_amdgcn_cvt_pk_f32_fp8(w[2 * g + j], true);
-        f[4 * j] = x[0] * s, f[4 * j + 1] = x[1] * s, f[4 * j + 2] = y[0] * s, f[4 * j + 3] = y[1] * s;
+        const v2f u = __builtin_amdgcn_cvt_pk_f32_fp8(x[i][p][j], false), v = __builtin_amdgcn_cvt_pk_f32_fp8(x[i][p][j], true);
+        f[4 * j] = u[0] * s[i][p], f[4 * j + 1] = u[1] * s[i][p], f[4 * j + 2] = v[0] * s[i][p], f[4 * j + 3] = v[1] * s[i][p];
       }
       Raw8<DT> r;
       r.set(f);
-      r.stream(p ? a.v : a.k, o + 8 * g);
+      r.stream(p ? a.v : a.k, o);
     }
   }
 }
@@ -320,15 +530,14 @@ extern "C" int mxf8_kv_append(const void* k, const int64_t k_strides[4], const v
   a.turns = turns, a.turns_batch = turns_batch_stride;
   a.starts = starts, a.counts = counts;
   a.S = (int)S, a.P = (int)P, a.eps = eps;
-  a.mode = P == 0 ? TURN_NONE : interleaved ? TURN_INTERLEAVED : P % 8 == 0 ? TURN_HALF : TURN_HALF_ANY;
-  a.heads = 1;
+  const int mode = P == 0 && !k_weight ? KEY_PLAIN : P == 0 || interleaved ? KEY_PAIRS : P % 8 == 0 ? KEY_HALF : KEY_HALF_ANY;
   // a run of S tokens touches up to so many pages, wherever it starts
   const int64_t touched = (S + page_size - 2) / page_size + 1;
-  if (!grid_fits(touched, 256)) return set_error(MXF8_EINVAL, "%s: shape too large", what);
-  const dim3 grid((unsigned)touched, (unsigned)cdiv(H, a.heads), (unsigned)B);
+  if (!grid_fits(touched, 512)) return set_error(MXF8_EINVAL, "%s: shape too large", what);
+  const dim3 grid((unsigned)touched, (unsigned)H, (unsigned)B);
   auto launch = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    return D == 128 ? launch_append<DT, 128>(a, grid, stream) : launch_append<DT, 64>(a, grid, stream);
+    return D == 128 ? launch_append<DT, 128>(a, mode, grid, stream) : launch_append<DT, 64>(a, mode, grid, stream);
   };
   return dtype == MXF8_BF16  ? launch(std::integral_constant<int, MXF8_BF16>{})
          : dtype == MXF8_F16 ? launch(std::integral_constant<int, MXF8_F16>{})
@@ -351,15 +560,19 @@ extern "C" int mxf8_kv_read(const uint8_t* k_codes, const uint8_t* v_codes, cons
   if (B == 0 || H == 0 || T == 0) return MXF8_OK;
   if (!starts || !k || !v) return set_error(MXF8_EINVAL, "%s: null pointer", what);
   a.starts = starts, a.lengths = lengths, a.k = k, a.v = v;
-  a.T = T, a.chunks = T * (D / 16);
-  if (!grid_fits(cdiv(a.chunks, 256), 256)) return set_error(MXF8_EINVAL, "%s: shape too large", what);
-  const dim3 grid((unsigned)cdiv(a.chunks, 256), (unsigned)H, (unsigned)B);
+  a.T = T, a.pages = (T + page_size - 2) / page_size + 1;
+  // four turns of a wave in flight together where there are enough to go round
+  const int64_t turns = a.pages * (page_size * D / 512);
+  const bool many = turns * H * B >= 4 * 4096;
+  const int64_t blocks = cdiv(turns, many ? 16 : 4);
+  if (!grid_fits(blocks, 256)) return set_error(MXF8_EINVAL, "%s: shape too large", what);
+  const dim3 grid((unsigned)blocks, (unsigned)H, (unsigned)B);
   auto launch = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     if (D == 128)
-      kv_read_kernel<DT, 128><<<grid, 256, 0, stream>>>(a);
+      many ? kv_read_kernel<DT, 128, 4><<<grid, 256, 0, stream>>>(a) : kv_read_kernel<DT, 128, 1><<<grid, 256, 0, stream>>>(a);
     else
-      kv_read_kernel<DT, 64><<<grid, 256, 0, stream>>>(a);
+      many ? kv_read_kernel<DT, 64, 4><<<grid, 256, 0, stream>>>(a) : kv_read_kernel<DT, 64, 1><<<grid, 256, 0, stream>>>(a);
     return check_launch(what);
   };
   return dtype == MXF8_BF16  ? launch(std::integral_constant<int, MXF8_BF16>{})

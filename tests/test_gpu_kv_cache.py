@@ -133,6 +133,22 @@ def test_append_one_token_at_a_time(d, page):
         check_append(cache, table, i32(t, max(0, t - 5)), k.bfloat16().cuda(), v.bfloat16().cuda())
 
 
+def test_append_small_halves():
+    """fp16's own subnormals, under exponents that keep them."""
+    cache, table = FP8KVCache(8, 2, 64, 16), pages_for(1, 1, 4)
+    x = torch.randint(-1500, 1500, (1, 2, 40, 64), generator=torch.Generator().manual_seed(1)) * 2.0 ** -24
+    check_append(cache, table, i32(0), x.half().cuda(), (x * 2.0 ** -1).half().cuda())
+
+
+def test_append_far_from_one():
+    """A page's values at both ends of the exponents' range, and past them."""
+    cache, table = FP8KVCache(12, 1, 128, 16), pages_for(1, 1, 8)
+    x = torch.randn((1, 1, 128, 128), generator=torch.Generator().manual_seed(1))
+    size = torch.tensor([2.0 ** -36, 2.0 ** -44, 1e-38, 2.0 ** 60, 2.0 ** 71, 2.0 ** 72, 1e30, 1.0]).repeat_interleave(16)
+    check_append(cache, table, i32(0), (x * size[:, None]).cuda(), (x * size.flip(0)[:, None]).cuda())
+    check_append(cache, table, i32(0), (x * size[:, None]).bfloat16().cuda(), (x * size.flip(0)[:, None]).bfloat16().cuda())
+
+
 def test_append_special_values():
     cache, table = FP8KVCache(8, 1, 64, 16), pages_for(1, 1, 4)
     x = torch.randn((1, 1, 48, 64), generator=torch.Generator().manual_seed(1))
@@ -147,6 +163,29 @@ def test_append_special_values():
     assert torch.isnan(k).sum() == 2 and (k[0, 0, 16:32] == 0).all()
     # a value of the page is the largest, an infinity as large as the scale allows; the other tokens keep theirs
     assert k[0, 0, 3, 7] == k[0, 0, 3, 7].abs() > 2 and (w[0, 0, 0] - v[0, 0, 0].cuda()).abs().max() < 0.2
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_append_special_values_turned(interleaved, dtype):
+    """A NaN, an infinity or an overflow on the way makes its token's keys what they are, and leaves the others alone."""
+    cache, table = FP8KVCache(8, 2, 64, 32), pages_for(1, 1, 3)
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn((1, 2, 70, 64), generator=g).to(DT[dtype])
+    angle = torch.rand((70, 32), generator=g) * 7
+    turns = torch.stack([angle.cos(), angle.sin()], -1).cuda()
+    clean = FP8KVCache(8, 2, 64, 32)
+    append_kv(clean, table, i32(0), x.cuda(), x.cuda(), table=turns, interleaved=interleaved)
+    bad = x.clone()
+    bad[0, 0, 3, 7], bad[0, 0, 40, 5], bad[0, 0, 66, 9] = float("nan"), float("inf"), torch.finfo(DT[dtype]).max
+    append_kv(cache, table, i32(0), bad.cuda(), x.cuda(), table=turns, interleaved=interleaved)
+    k, v = read_kv(cache, table, i32(0), 70, dtype=torch.float32)
+    kc, vc = read_kv(clean, table, i32(0), 70, dtype=torch.float32)
+    assert torch.equal(v, vc) and torch.equal(k[:, 1], kc[:, 1])
+    assert torch.isnan(k[0, 0, 3, 0]) and (torch.isnan(k[0, 0]).any(-1).nonzero()[:, 0].tolist() == [3])
+    same = torch.ones(64, dtype=torch.bool)
+    same[[3, 40]] = False
+    assert torch.equal(k[0, 0, :64][same], kc[0, 0, :64][same]) and k[0, 0, 66].abs().max() > 1e4
 
 
 def test_append_where_there_is_no_page():
@@ -279,6 +318,25 @@ def test_attend_missing_pages(S, H, Hk):
 
 
 @pytest.mark.parametrize("S,H,Hk", [(1, 4, 2), (6, 4, 1), (130, 2, 2)])
+@pytest.mark.parametrize("byte", [0, 255])
+def test_attend_missing_pages_beside_a_page_of_nothing(S, H, Hk, byte):
+    """Pages that nobody names hold NaN codes under any scale, page 0 among them."""
+    table = pages_for(4, 1, 12, extra=0) + 1
+    lengths = i32(16 * 11 + 5)
+    cache = normal_cache(4, 14, Hk, 16, 64, table, lengths)
+    holes = table.clone()
+    holes[0, 3:6], holes[0, 9] = -1, 14
+    q = torch.randn((1, H, S, 64), generator=torch.Generator().manual_seed(4)).bfloat16().cuda()
+    want = [check_attend(q, cache, holes, lengths, c) for c in (False, True)]
+    for t in (cache.k, cache.v):
+        t.view(torch.uint8)[0], t.view(torch.uint8)[13] = 0xFF, 0x7F
+    for t in (cache.k_scale, cache.v_scale):
+        t[0], t[13] = byte, byte
+    for c, w in zip((False, True), want):
+        assert torch.equal(cached_attention(q, cache, holes, lengths, causal=c), w)
+
+
+@pytest.mark.parametrize("S,H,Hk", [(1, 4, 2), (6, 4, 1), (130, 2, 2)])
 @pytest.mark.parametrize("D", [64, 128])
 def test_attend_what_is_not_there_changes_nothing(S, H, Hk, D):
     """NaN codes and any scales behind a sequence's end and in pages that it does not name."""
@@ -335,6 +393,8 @@ def test_attend_any_scales(S, H, Hk, D):
     for size in (2.0 ** -40, 2.0 ** 30):  # queries beyond fp16's range under a scale that brings the scores back
         check_attend((q.float() * size).bfloat16(), cache, table, i32(185), scale=0.1 / size)
     check_attend(torch.zeros_like(q), cache, table, i32(185))
+    for scale in (0.0, -0.1, 1e-30):
+        check_attend(q, cache, table, i32(185), scale=scale)
 
 
 @pytest.mark.parametrize("S,H,Hk", [(1, 2, 2), (4, 8, 2), (70, 2, 1)])
