@@ -26,7 +26,7 @@ struct AttendArgs {
   void* o;
   int64_t qs[3], os[3];  // strides of batch, head, token
   const int32_t *lengths, *q_lengths;
-  int H, S, G, R, causal;  // G heads a key head, R = S G rows of it: row i G + g is query i of head g
+  int B, H, S, G, R, causal;  // G heads a key head, R = S G rows of it: row i G + g is query i of head g
   float scale;             // times log2 e
   int splits;              // parts of the keys
   float *part, *stat;      // with more than one: sums [B, Hk, splits, R, D], and (maximum, sum of p) [.., 2]
@@ -102,16 +102,17 @@ __device__ __forceinline__ v8h query_f16(const Raw8<DT>& r, float s) {
   }
 }
 
-// One row's fragments of a query: N pieces of eight channels at channel(i), and the factor of its scores.
-template <int DT, int LANES, int N, class F>
-__device__ __forceinline__ float load_query(const AttendArgs& a, int b, int hk, int row, bool there, v8h (&f)[N], F channel) {
+// One row's fragments of a query: N pieces of eight channels at channel(i).
+template <int DT, int N, class F>
+__device__ __forceinline__ void load_query(const AttendArgs& a, int b, int hk, int row, Raw8<DT> (&r)[N], F channel) {
   const int i = (uint32_t)row / (uint32_t)a.G, g = row - i * a.G;
   const int64_t at = b * a.qs[0] + (hk * a.G + g) * a.qs[1] + i * a.qs[2];
-  Raw8<DT> r[N];
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    r[j].load(a.q, at + channel(j));  // (before it is known whether the row is there: the load need not wait for the lengths)
-  }
+  for (int j = 0; j < N; ++j) r[j].load(a.q, at + channel(j));
+}
+// The same as fp16 (zeros for a row that is not there), and the factor of its scores.
+template <int DT, int LANES, int N>
+__device__ __forceinline__ float scale_query(const AttendArgs& a, bool there, Raw8<DT> (&r)[N], v8h (&f)[N]) {
 #pragma unroll
   for (int j = 0; j < N; ++j)
     if (!there) r[j].zero();
@@ -156,25 +157,30 @@ __device__ __forceinline__ int64_t out_row(const AttendArgs& a, int b, int hk, i
 // Up to 64 rows a key head (its G heads' S queries): a workgroup takes a part of the keys, its four waves every fourth
 // step of 32 keys each, straight from memory into the layout of 16 x 16 x 32 products, and joins their sums at the end.
 // No LDS on the way: a lane loads 16 channels of its key, and for the values 8 keys' D / 16 channels, which it transposes in
-// registers.  The next step's loads are in flight while a step is computed.
+// registers.  The next steps' loads are in flight while a step is computed.
 constexpr int FEW_ROWS = 64, FEW_UNIT = 128;
 
 template <int D>
 struct FewStep {
   v4i k[2][D / 64];
   uint32_t v[8][D / 64];
-  int pid[2];
+  bool there[2];
   uint32_t ks[2], vs[2];
 };
 
 template <int DT, int D, int NR>
 __global__ __launch_bounds__(256, (D == 64 ? (NR == 1 ? 4 : NR == 2 ? 3 : 2) : NR == 1 ? 3 : 4 / NR)) void kv_attend_few_kernel(const AttendArgs a) {
-  constexpr int KK = D / 32, DI = D / 16, W = D / 64;
+  constexpr int KK = D / 32, DI = D / 16, W = D / 64, STEPS = D == 128 || NR > 1 ? 2 : 3;
   __shared__ float om[4][16][D + 4];
   __shared__ float ml[4][2][16 * NR];
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
+  // (before it is known which rows are there: the loads need not wait for the lengths)
+  Raw8<DT> raw[NR][KK];
+#pragma unroll
+  for (int t = 0; t < NR; ++t)
+    load_query(a, b, hk, min(16 * t + c, a.R - 1), raw[t], [&](int j) { return 64 * (j / 2) + 16 * q + 8 * (j % 2); });
   const KvSeq seq = kv_seq(a, b);
   const int end = kv_end(a, seq, 0, a.R), chunk = kv_chunk(a, end, FEW_UNIT);
   const int k0 = split * chunk, k1 = min(k0 + chunk, end);
@@ -188,8 +194,6 @@ __global__ __launch_bounds__(256, (D == 64 ? (NR == 1 ? 4 : NR == 2 ? 3 : 2) : N
     const int row = 16 * t + c;
     limit[t] = row < a.R ? kv_limit(a, seq, row) : 0;
     low = min(low, row < a.R ? limit[t] : INT32_MAX);
-    factor[t] = load_query<DT, 16>(a, b, hk, min(row, a.R - 1), limit[t] > 0, qf[t],
-                                   [&](int j) { return 64 * (j / 2) + 16 * q + 8 * (j % 2); });
   }
 #pragma unroll
   for (int off = 8; off; off >>= 1) low = min(low, __shfl_xor(low, off, 64));
@@ -206,24 +210,17 @@ __global__ __launch_bounds__(256, (D == 64 ? (NR == 1 ? 4 : NR == 2 ? 3 : 2) : N
 
   const int mask = (1 << a.c.shift) - 1;
   const uint32_t k_lane = c * D + 16 * q, v_lane = 4 * q * D + c * DI;
-  auto pages = [&](int key0, int (&pid)[2]) {
+  auto pages = [&](int key0, int (&entry)[2]) {  // (behind the end: the last again)
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const int key = key0 + 16 * g;
-      pid[g] = -1;
-      if (key < k1) {
-        const int p = kv_entry(a.c, b, key >> a.c.shift);
-        pid[g] = kv_valid(a.c, p) ? p : -1;
-      }
-    }
+    for (int g = 0; g < 2; ++g) entry[g] = kv_entry(a.c, b, min(key0 + 16 * g, k1 - 1) >> a.c.shift);
   };
-  auto load = [&](int key0, const int (&pid)[2], FewStep<D>& s) {
+  auto load = [&](int key0, const int (&entry)[2], FewStep<D>& s) {
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       // (no page: page 0 is read and not used)
-      const int64_t ph = (int64_t)max(pid[g], 0) * a.c.H + hk;
+      s.there[g] = key0 + 16 * g < k1 && kv_valid(a.c, entry[g]);
+      const int64_t ph = (int64_t)(s.there[g] ? entry[g] : 0) * a.c.H + hk;
       const int64_t at = ((ph << a.c.shift) + ((key0 + 16 * g) & mask)) * D;
-      s.pid[g] = pid[g];
       s.ks[g] = a.c.ks[ph], s.vs[g] = a.c.vs[ph];
       // (addresses: a base that the wave shares and 32 bits of a lane's own)
       const gbytes k = (gbytes)(a.c.k + at), v = (gbytes)(a.c.v + at);
@@ -240,12 +237,12 @@ __global__ __launch_bounds__(256, (D == 64 ? (NR == 1 ? 4 : NR == 2 ? 3 : 2) : N
     }
   };
   auto compute = [&](int key0, FewStep<D>& s) {
-    const bool whole = key0 + 32 <= low && s.pid[0] >= 0 && s.pid[1] >= 0;
+    const bool whole = key0 + 32 <= low && s.there[0] && s.there[1];
     float ks[2], ev[2], iv[2];
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-      const uint32_t kb = s.pid[g] < 0 ? 127 : __builtin_amdgcn_readfirstlane(s.ks[g]);
-      const uint32_t vb = s.pid[g] < 0 ? 127 : __builtin_amdgcn_readfirstlane(s.vs[g]);
+      const uint32_t kb = !s.there[g] ? 127 : __builtin_amdgcn_readfirstlane(s.ks[g]);
+      const uint32_t vb = !s.there[g] ? 127 : __builtin_amdgcn_readfirstlane(s.vs[g]);
       ks[g] = kv_scale(kb);
       const int e = (int)vb - 127;
       ev[g] = (float)e, iv[g] = __uint_as_float((uint32_t)(127 - e) << 23);
@@ -271,7 +268,7 @@ __global__ __launch_bounds__(256, (D == 64 ? (NR == 1 ? 4 : NR == 2 ? 3 : 2) : N
         for (int g = 0; g < 2; ++g)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            x[g][r] = key0 + 16 * g + 4 * q + r < limit[t] && s.pid[g] >= 0 ? x[g][r] : -INFINITY;
+            x[g][r] = key0 + 16 * g + 4 * q + r < limit[t] && s.there[g] ? x[g][r] : -INFINITY;
       }
       const float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
                               fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
@@ -297,7 +294,7 @@ __global__ __launch_bounds__(256, (D == 64 ? (NR == 1 ? 4 : NR == 2 ? 3 : 2) : N
       for (int g = 0; g < 2; ++g)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (key0 + 16 * g + 4 * q + r >= k1 || s.pid[g] < 0)
+          if (key0 + 16 * g + 4 * q + r >= k1 || !s.there[g])
 #pragma unroll
             for (int d = 0; d < W; ++d) s.v[4 * g + r][d] = 0;
     }
@@ -317,18 +314,25 @@ __global__ __launch_bounds__(256, (D == 64 ? (NR == 1 ? 4 : NR == 2 ? 3 : 2) : N
     }
   };
 
+  // STEPS - 1 steps' loads are in flight while one is computed, and the page entries of one more
   int key = k0 + 32 * w;
   if (key < k1) {
-    FewStep<D> s[2];
-    int pid[2];
-    pages(key, pid);
-    load(key, pid, s[0]);
-    pages(key + FEW_UNIT, pid);
+    FewStep<D> s[STEPS];
+    int entry[2];
+    pages(key, entry);
+#pragma unroll
+    for (int u = 0; u + 1 < STEPS; ++u) {
+      if (key + u * FEW_UNIT < k1) load(key + u * FEW_UNIT, entry, s[u]);
+      pages(key + (u + 1) * FEW_UNIT, entry);
+    }
+#pragma unroll
+    for (int t = 0; t < NR; ++t) factor[t] = scale_query<DT, 16>(a, limit[t] > 0, raw[t], qf[t]);
     for (;;) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (key + FEW_UNIT < k1) load(key + FEW_UNIT, pid, s[1 - u]);
-        pages(key + 2 * FEW_UNIT, pid);
+      for (int u = 0; u < STEPS; ++u) {
+        const int next = key + (STEPS - 1) * FEW_UNIT;
+        if (next < k1) load(next, entry, s[(u + STEPS - 1) % STEPS]);
+        pages(next + FEW_UNIT, entry);
         compute(key, s[u]);
         key += FEW_UNIT;
         if (key >= k1) goto done;
@@ -410,17 +414,23 @@ __global__ __launch_bounds__(512, 2) void kv_attend_many_kernel(const AttendArgs
   __shared__ ManyLds<D> lds;
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = w >> 2;
-  const int r0 = (gridDim.x / a.splits - 1 - blockIdx.x / a.splits) * MANY_ROWS, split = blockIdx.x % a.splits;
-  const int hk = blockIdx.y, b = blockIdx.z;
+  // Neighbouring workgroups take different key heads: where their number is a multiple of eight, all that read one head's keys
+  // are on one XCD, and its L2 has them.  The last rows come first: under a causal mask they see the most keys.
+  const int groups = a.c.H * a.B, x0 = blockIdx.x / groups, hb = blockIdx.x % groups;
+  const int tiles = (a.R + MANY_ROWS - 1) / MANY_ROWS, split = x0 / tiles, r0 = (tiles - 1 - x0 % tiles) * MANY_ROWS;
+  const int hk = hb % a.c.H, b = hb / a.c.H;
+  const int row = r0 + 32 * w + c;
+  Raw8<DT> raw[KK];
+  load_query(a, b, hk, min(row, a.R - 1), raw, [&](int j) { return 16 * j + 8 * h; });
   const KvSeq seq = kv_seq(a, b);
   const int end = kv_end(a, seq, r0, r0 + MANY_ROWS), chunk = kv_chunk(a, end, MANY_KEYS);
   const int k0 = split * chunk, k1 = min(k0 + chunk, end);
   if (a.splits > 1 && k0 >= k1) return;
 
-  const int row = r0 + 32 * w + c, limit = row < a.R ? kv_limit(a, seq, row) : 0;
+  const int limit = row < a.R ? kv_limit(a, seq, row) : 0;
   int low = row < a.R ? limit : INT32_MAX, high = limit;
   v8h qf[KK];
-  const float factor = load_query<DT, 32>(a, b, hk, min(row, a.R - 1), limit > 0, qf, [&](int j) { return 16 * j + 8 * h; });
+  const float factor = scale_query<DT, 32>(a, limit > 0, raw, qf);
   float m = KV_NONE, l = 0.0f;
   v16f o[OT];
 #pragma unroll
@@ -666,25 +676,37 @@ __global__ __launch_bounds__(512, 2) void kv_attend_many_kernel(const AttendArgs
     if (sees(n - 1)) {
       if (group) exponentials(n - 1);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        read_v(n - 1, g);
-        values(g);
-      }
+      for (int g = 0; g < 4; ++g)
+        if (g == 0 || k0 + (n - 1) * MANY_KEYS + 16 * g < k1) {
+          read_v(n - 1, g);
+          values(g);
+        }
     }
   }
   l = row_reduce<32>(l, sum_of);
-  if (row >= a.R) return;
   if (a.splits == 1) {
+    // rows of the output through LDS, where this wave's keys were, so that a row is stored at once
     const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-    const int64_t at = out_row(a, b, hk, row) + 4 * h;
+    __syncthreads();
+    v2i* mine = reinterpret_cast<v2i*>(lds.k) + w * 32 * (D / 4);
+    auto at = [&](int r, int piece) { return r * (D / 4) + (piece ^ (r & 15)); };  // pieces of four channels
 #pragma unroll
     for (int i = 0; i < OT; ++i)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const float z[4] = {o[i][4 * g] * inv, o[i][4 * g + 1] * inv, o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv};
-        store_row<DT, 4>(a.o, at + 32 * i + 8 * g, z);
-      }
-  } else {
+      for (int g = 0; g < 4; ++g)
+        mine[at(c, 8 * i + 2 * g + h)] = v2i{(int)cvt_pk_16<DT>(o[i][4 * g] * inv, o[i][4 * g + 1] * inv),
+                                             (int)cvt_pk_16<DT>(o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv)};
+    __builtin_amdgcn_wave_barrier();  // (LDS operations of a wave complete in order)
+    constexpr int L = D / 8;          // lanes of a row
+#pragma unroll
+    for (int i = 0; i < 32 * L / 64; ++i) {
+      const int r = i * (64 / L) + lane / L, to = r0 + 32 * w + r;
+      const v2i u = mine[at(r, lane % L * 2)], v = mine[at(r, lane % L * 2 + 1)];
+      if (to < a.R)
+        *reinterpret_cast<words4*>(static_cast<uint16_t*>(a.o) + out_row(a, b, hk, to) + lane % L * 8) =
+            words4{(uint32_t)u[0], (uint32_t)u[1], (uint32_t)v[0], (uint32_t)v[1]};
+    }
+  } else if (row < a.R) {
     const int64_t at = (((int64_t)b * a.c.H + hk) * a.splits + split) * a.R + row;
 #pragma unroll
     for (int i = 0; i < OT; ++i)
@@ -768,8 +790,11 @@ static AttendPlan plan_attend(int64_t B, int64_t H, int64_t Hk, int64_t S, int64
   const int64_t groups = B * Hk * p.tiles, keys = width * page;
   p.splits = 1;
   if (p.few) {
-    const int64_t want = cdiv(1024, groups), most = cdiv(keys, FEW_UNIT);
-    p.splits = (int)(want > most ? most : want);
+    // Two workgroups a compute unit, however short their parts are; up to eight where each still has 1024 keys, which evens
+    // out sequences of different lengths.
+    const int64_t few = cdiv(512, groups), parts = cdiv(keys, FEW_UNIT), more = cdiv(2048, groups), thousands = keys / 1024;
+    const int64_t n = more < thousands ? more : thousands, m = few < parts ? few : parts;
+    p.splits = (int)(n > m ? n : m);
   } else {
     // The rounds that the workgroups make over the compute units, of so many tiles each and some three tiles' time to begin
     // and end, and joining: about five tiles' time, and two passes over the sums at 5 TB/s.
@@ -798,14 +823,14 @@ static int launch_attend(AttendArgs& a, const AttendPlan& p, int B, hipStream_t 
     else
       kv_attend_few_kernel<DT, D, 4><<<grid, 256, 0, st>>>(a);
   } else {
-    if (!grid_fits(p.tiles * p.splits, 512)) return set_error(MXF8_EINVAL, "%s: shape too large", what);
-    const dim3 grid((unsigned)(p.tiles * p.splits), Hk, B);
-    kv_attend_many_kernel<DT, D><<<grid, 512, 0, st>>>(a);
+    const int64_t blocks = p.tiles * p.splits * Hk * B;
+    if (!grid_fits(blocks, 512)) return set_error(MXF8_EINVAL, "%s: shape too large", what);
+    kv_attend_many_kernel<DT, D><<<dim3((unsigned)blocks), 512, 0, st>>>(a);
   }
   if (const int rc = check_launch(what)) return rc;
   if (p.splits == 1) return MXF8_OK;
   const int rows = p.few ? FEW_ROWS : MANY_ROWS, unit = p.few ? FEW_UNIT : MANY_KEYS;
-  if (p.few)
+  if (p.splits > 16)  // (more than a wave reads at once, D = 128)
     kv_attend_join_kernel<DT, D, 4><<<dim3((unsigned)a.R, Hk, B), 256, 0, st>>>(a, rows, unit);
   else
     kv_attend_join_kernel<DT, D, 1><<<dim3((unsigned)cdiv(a.R, 4), Hk, B), 256, 0, st>>>(a, rows, unit);
@@ -851,7 +876,7 @@ extern "C" int mxf8_kv_attend(const void* q, const int64_t q_strides[4], int dty
   a.q = q, a.o = out;
   for (int i = 0; i < 3; ++i) a.qs[i] = q_strides[i], a.os[i] = out_strides[i];
   a.lengths = lengths, a.q_lengths = q_lengths;
-  a.H = (int)H, a.S = (int)S, a.G = (int)(H / Hk), a.R = (int)p.rows, a.causal = causal != 0;
+  a.B = (int)B, a.H = (int)H, a.S = (int)S, a.G = (int)(H / Hk), a.R = (int)p.rows, a.causal = causal != 0;
   a.scale = scale * 1.4426950408889634f;
   a.splits = p.splits;
   a.part = static_cast<float*>(workspace);
