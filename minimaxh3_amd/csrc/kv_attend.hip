@@ -722,10 +722,10 @@ __global__ __launch_bounds__(512, 2) void kv_attend_many_kernel(const AttendArgs
 constexpr int KV_MAX_SPLITS = 64;
 
 // One row to WAVES waves: the splits' maxima and sums in a lane each, then their outputs, four channels a lane and 256 / D
-// splits at once.  The first loads do not wait to know how many splits there are.
-template <int DT, int D, int WAVES>
+// splits at once, U times in flight together.  The first loads do not wait to know how many splits there are.
+template <int DT, int D, int WAVES, int U>
 __global__ __launch_bounds__(256) void kv_attend_join_kernel(const AttendArgs a, int rows, int unit) {
-  constexpr int L = D / 4, P = 64 / L, U = 8;  // lanes of a split, splits at once, loads in flight
+  constexpr int L = D / 4, P = 64 / L;  // lanes of a split, splits at once
   __shared__ v4f sums[4][64];
   const int lane = threadIdx.x & 63, hk = blockIdx.y, b = blockIdx.z;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -831,9 +831,11 @@ static int launch_attend(AttendArgs& a, const AttendPlan& p, int B, hipStream_t 
   if (p.splits == 1) return MXF8_OK;
   const int rows = p.few ? FEW_ROWS : MANY_ROWS, unit = p.few ? FEW_UNIT : MANY_KEYS;
   if (p.splits > 16)  // (more than a wave reads at once, D = 128)
-    kv_attend_join_kernel<DT, D, 4><<<dim3((unsigned)a.R, Hk, B), 256, 0, st>>>(a, rows, unit);
+    kv_attend_join_kernel<DT, D, 4, 8><<<dim3((unsigned)a.R, Hk, B), 256, 0, st>>>(a, rows, unit);
+  else if (p.splits > 4)
+    kv_attend_join_kernel<DT, D, 1, 8><<<dim3((unsigned)cdiv(a.R, 4), Hk, B), 256, 0, st>>>(a, rows, unit);
   else
-    kv_attend_join_kernel<DT, D, 1><<<dim3((unsigned)cdiv(a.R, 4), Hk, B), 256, 0, st>>>(a, rows, unit);
+    kv_attend_join_kernel<DT, D, 1, 2><<<dim3((unsigned)cdiv(a.R, 4), Hk, B), 256, 0, st>>>(a, rows, unit);
   return check_launch(what);
 }
 
