@@ -67,7 +67,7 @@ def test_kv_read(lib):
         refused(lib, call(**bad), text)
     refused(lib, call(t=-1), "shape")
     refused(lib, call(t=(1 << 30) + 1), "shape")
-    refused(lib, call(t=1 << 30), "too large")
+    refused(lib, call(t=1 << 30, page=128, d=128), "too large")
     refused(lib, call(dtype=4), "dtype")
     for null in ("starts", "k", "v"):
         refused(lib, call(**{null: None}), "null")
