@@ -664,6 +664,7 @@ __global__ __launch_bounds__(512, 2) void kv_attend_many_kernel(const AttendArgs
         values(2);
         values(3);
         __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
         if (!group) exponentials(j + 1);
         read_k(j + 2, 0);
       } else {
@@ -799,7 +800,7 @@ static AttendPlan plan_attend(int64_t B, int64_t H, int64_t Hk, int64_t S, int64
     // The rounds that the workgroups make over the compute units, of so many tiles each and some three tiles' time to begin
     // and end, and joining: about five tiles' time, and two passes over the sums at 5 TB/s.
     double best = 0.0;
-    for (int n = 1; n <= KV_MAX_SPLITS && (n == 1 || n * 4 * MANY_KEYS <= keys); ++n) {
+    for (int n = 1; n <= KV_MAX_SPLITS && (n == 1 || (n * 4 * MANY_KEYS <= keys && groups * n <= 2048)); ++n) {
       const double rounds = (double)cdiv(groups * n, 256), each = (double)cdiv(cdiv(keys, n), MANY_KEYS) + 3.0;
       const double join = n == 1 ? 0.0 : 5.0 + (double)groups * n * MANY_ROWS * D * 8.0 / 5.0e6;
       if (n == 1 || rounds * each + join < best) best = rounds * each + join, p.splits = n;
