@@ -383,7 +383,8 @@ int mxf8_mxfp4_linear(const void* x, int dtype, int64_t ldx, const uint8_t* w4, 
  * Paged e4m3 cache of keys and values (no counterpart in the reference).  A pool of `pages` pages holds
  * page_size (16, 32, 64 or 128) tokens of H heads each:
  *   k_codes, v_codes [pages, H, page_size, D] e4m3, 16-byte aligned, D 64 or 128
- *   k_scale, v_scale [pages, H] uint8: exponent + 127 of the power of two that the page's codes are times
+ *   k_scale, v_scale [pages, H] uint8: exponent + 127, 95 to 190, of the power of two that the page's codes are times
+ *   values hold no NaN codes (mxf8_kv_append writes none): one would reach every row of a tile
  * Sequence b's tokens t are in page page_table[b, t / page_size] (int32, row stride table_stride, table_width
  * entries a row) at t % page_size.  An entry outside [0, pages) names no page: nothing is written there,
  * it reads as zeros, and no query sees it; nor do tokens behind the table's last entry exist.
@@ -399,7 +400,7 @@ int mxf8_mxfp4_linear(const void* x, int dtype, int64_t ldx, const uint8_t* w4, 
  *   or the one it has where that is larger and the page holds tokens before starts[b]; their codes are then
  *   rounded again where e grew.  A code is the e4m3 number nearest to x * 2^-e, ties to even, an infinity the
  *   largest.  A NaN in a token's key or value makes its key NaN (in its first channel) and is held as 0
- * A page may be in one sequence of a call only, as far as tokens are written to it.
+ * No page may be written to through two entries of a call's page table.
  */
 int mxf8_kv_append(const void* k, const int64_t k_strides[4], const void* v, const int64_t v_strides[4], int dtype,
                    int64_t B, int64_t H, int64_t S, int64_t D, const float* turns, int64_t turns_batch_stride,

@@ -158,6 +158,12 @@ __device__ __forceinline__ int64_t out_row(const AttendArgs& a, int b, int hk, i
 // step of 32 keys each, straight from memory into the layout of 16 x 16 x 32 products, and joins their sums at the end.
 // No LDS on the way: a lane loads 16 channels of its key, and for the values 8 keys' D / 16 channels, which it transposes in
 // registers.  The next steps' loads are in flight while a step is computed.
+//
+// Bound by memory where the parts are long: 8 key heads x 131149 keys x 128, one query of 32 heads, 268 MB in 43 us (6.2
+// TB/s, a part from the last cache); 64 sequences of 129 to 8192 tokens 113 us (4.7), of 4600 each 109 (5.5).  Short parts are bound by
+// the chain of lengths, page entries, codes and join, some 4 us, and by a lone wave's issue (a step of D = 128 takes
+// it 0.8 us).  Three or four steps ahead are no faster, with fewer waves; more than two workgroups a compute unit only
+// even out lengths.
 constexpr int FEW_ROWS = 64, FEW_UNIT = 128;
 
 template <int D>
@@ -393,6 +399,13 @@ done:
 // first makes the scores of its next tile and the value product of this one and then takes the next one's exponentials, group
 // 1 first takes exponentials and then multiplies.  Fragments are read from LDS well before their products, and each wave
 // stages its share of the keys of tile j + 3 and the values of j + 1 among them.
+//
+// A tile's 2048 cycles of products take some 4000 (over the whole launch the matrix unit is 42% busy, the vector unit 52%, LDS
+// 37%), at a clock under the power limit: 2.0 of 2.4 GHz.  1560 queries x 24 heads of 128 over 21840 keys: 450-470 us with the join's 18, 900-930 TFLOP/s
+// (a library product of 8192^3 in fp16 reaches 1147 here).  What the parts bring there: both groups in the same order 492, without
+// the wave priorities 470, a barrier between the two phases as well 518, key codes converted at each read instead of once
+// 517, fragments read as they are needed 560-590.  One wave a SIMD with 64 rows and 512 registers would read LDS half as often,
+// but the compiler then keeps the scores in accumulation registers and spills.
 constexpr int MANY_ROWS = 256, MANY_KEYS = 64;
 
 // LDS, in 16-byte chunks with a swizzle: keys [64][D] and values [D][64] in fp16; of each granule of 16 keys, the keys'

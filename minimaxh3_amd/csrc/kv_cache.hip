@@ -164,7 +164,11 @@ __device__ __forceinline__ void round_keys(const double (&y)[8], float (&f)[8]) 
 
 // A workgroup writes one page and head of one sequence: D / 8 lanes hold a token's eight channels each, so the
 // page's maximum is one reduction over values that stay in registers until they are rounded.  Keys are normed and turned in
-// fp64, which costs less than the memory takes and leaves no key on the wrong side of a border between two codes.
+// fp64, which leaves no key on the wrong side of a border between two codes (fp32 has two or three of a million there).
+//
+// Bound by memory where keys stay as they are: 20280 tokens x 24 heads x 128 in bf16, 374 MB, 65 us (5.7 TB/s).  Normed 78,
+// turned by neighbouring pairs or both 95, half-split 129: the cos / sin of a token come from L2 again for each head, as many
+// bytes as its keys and values, and the fp64 takes some 40 us of the vector units beside the loads.
 template <int DT, int D, int MODE, int THREADS, int N>
 __global__ __launch_bounds__(THREADS, MODE == KEY_HALF_ANY || (N == 4 && THREADS == 512) ? 2 : 4) void kv_append_kernel(const AppendArgs a) {
   constexpr int L = D / 8, T = THREADS / L, WAVES = THREADS / 64;  // lanes a token, tokens a step
@@ -241,6 +245,11 @@ __global__ __launch_bounds__(THREADS, MODE == KEY_HALF_ANY || (N == 4 && THREADS
     for (int i = 0; i < N; ++i) {
       __builtin_amdgcn_sched_barrier(0);  // (one token's 64-bit values at a time)
       if (i + 1 < N) load_turns(i + 1, cs[(i + 1) & 1]);
+      if (!__ballot(there[i])) {  // none of this wave's tokens
+#pragma unroll
+        for (int j = 0; j < 8; ++j) k[i][j] = 0.0f;
+        continue;
+      }
       float x[8], w[8];
       kr[i].get(x);
       wk.get(w);
@@ -414,17 +423,25 @@ __global__ __launch_bounds__(THREADS, MODE == KEY_HALF_ANY || (N == 4 && THREADS
 
 template <int DT, int D, int MODE>
 static int launch_append(const AppendArgs& a, dim3 grid, hipStream_t st) {
-  // Up to four tokens a lane in workgroups of 256; two in 512 where half-split pairs cost more registers.
+  // Pages of 1024 chunks: four tokens a lane in workgroups of 256, or, where these do not go round or half-split pairs cost more
+  // registers, two in 512 (1560 tokens x 24 heads, turned: 17.5 / 15.4 us; 20280: 95 / 98).
   const int chunks = (D << a.c.shift) / 8;  // of eight channels
-  constexpr int BIG = MODE <= KEY_PAIRS ? 256 : 512;
-  if (chunks <= 256)
+  const int64_t blocks = (int64_t)grid.x * grid.y * grid.z;
+  if (chunks <= 256) {
     kv_append_kernel<DT, D, MODE, 256, 1><<<grid, 256, 0, st>>>(a);
-  else if (chunks == 512)
+  } else if (chunks == 512) {
     kv_append_kernel<DT, D, MODE, 256, 2><<<grid, 256, 0, st>>>(a);
-  else if (chunks == 1024)
-    kv_append_kernel<DT, D, MODE, BIG, 1024 / BIG><<<grid, BIG, 0, st>>>(a);
-  else if constexpr (D == 128)
+  } else if (chunks == 1024) {
+    if constexpr (MODE <= KEY_PAIRS) {
+      if (blocks >= 1024) {
+        kv_append_kernel<DT, D, MODE, 256, 4><<<grid, 256, 0, st>>>(a);
+        return check_launch("kv_append");
+      }
+    }
+    kv_append_kernel<DT, D, MODE, 512, 2><<<grid, 512, 0, st>>>(a);
+  } else if constexpr (D == 128) {
     kv_append_kernel<DT, D, MODE, 512, 4><<<grid, 512, 0, st>>>(a);
+  }
   return check_launch("kv_append");
 }
 template <int DT, int D>
@@ -445,7 +462,8 @@ struct ReadArgs {
 };
 
 // Eight channels a lane, so that a wave stores a row of memory at once; a page and head is 128 such chunks or a multiple, and
-// each wave reads chunks of one page, of keys and of values, I times.
+// each wave reads chunks of one page, of keys and of values, I times.  Bound by memory: 20280 tokens x 24 heads x 128, 374 MB,
+// 54 us (a part of it from the last cache; 16 channels a lane, two stores of half a row, 133).
 template <int DT, int D, int I>
 __global__ __launch_bounds__(256) void kv_read_kernel(const ReadArgs a) {
   constexpr int L = D / 8;

@@ -42,7 +42,8 @@ class FP8KVCache:
 
     @classmethod
     def from_tensors(cls, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> FP8KVCache:
-        """A cache on these tensors themselves (codes as e4m3 or their bytes)."""
+        """A cache on these tensors themselves (codes as e4m3 or their bytes).  Scale bytes of pages in use are 95
+        to 190, as ``append_kv`` writes them, and their values hold no NaN."""
         cache = cls.__new__(cls)
         cache._set(k, v, k_scale, v_scale)
         return cache
@@ -89,7 +90,7 @@ def append_kv(cache: FP8KVCache, page_table: torch.Tensor, starts: torch.Tensor,
 
     An infinity is held as the largest number.  A NaN in a token's key or value makes the rows that attend
     to that token (and head) NaN, and no others.  Tokens behind the page table's last entry, or where
-    it names no page, are dropped.
+    it names no page, are dropped.  A page may not be written to through two entries of the table.
     """
     ops.kv_append(*cache.tensors(), page_table, starts, k, v, counts, table, k_weight, float(eps), bool(interleaved))
 
