@@ -5,8 +5,9 @@
 // Keys and values are codes times a power of two for each page.  Codes become fp16 exactly and go into the fp16 matrix
 // instructions; a key's power of two multiplies the score, and a value's, 2^e_j, goes into the exponent:
 //   p'_ij = 2^(x_ij + e_j - m_i),  o_i = sum_j p'_ij code_j / sum_j p'_ij 2^-e_j
-// with m_i a running maximum of x_ij + e_j.  So p' is at most about 1 however the pages' sizes differ, and its half step
-// in fp16, 2^-11 of it, is all that the value product rounds; bf16 queries are exact in fp16 under a power of two per row.
+// with m_i a running maximum of x_ij + e_j.  So p' is at most 2^8 however the pages' sizes differ, and its half step
+// in fp16, 2^-11 of it or 2^-25, is all that the value product rounds; bf16 queries are exact in fp16 under a power of two
+// per row, down to 2^-17 of the row's largest (the half step below is 2^-25 of it).
 // (e4m3 probabilities would run twice as fast and be off by 2^-4, bf16 ones by 2^-8.)
 //
 // The products are made transposed, S' = K Q' and O' = V' P': then a lane holds one row's scores and outputs, the maximum

@@ -52,6 +52,7 @@ struct AppendArgs {
   int64_t turns_batch;
   const int32_t *starts, *counts;
   int S, P;
+  int eights;  // groups of eight pages that go through their heads together
   float eps;
 };
 
@@ -176,9 +177,17 @@ __global__ __launch_bounds__(THREADS, MODE == KEY_HALF_ANY || (N == 4 && THREADS
   __shared__ float exchange[MODE == KEY_HALF_ANY ? THREADS * 8 : 1];
   const int b = blockIdx.z, lane = threadIdx.x & 63, l = threadIdx.x % L, c0 = 8 * l;
   const int page = 1 << a.c.shift;
+  // Every eighth page to one XCD with all its heads, so that its L2 holds the page's cos / sin for them
+  uint32_t p = blockIdx.x, h = blockIdx.y;
+  if (a.eights) {
+    const uint32_t id = blockIdx.y * gridDim.x + blockIdx.x, H = a.c.H, group = id / (8 * H), r = id - group * 8 * H;
+    const bool whole = group < (uint32_t)a.eights;
+    h = whole ? r / 8 : r % H;
+    p = 8 * group + (whole ? r % 8 : r / H);
+  }
   const int64_t start = a.starts[b];
   const int64_t count = a.counts ? min(max(a.counts[b], 0), a.S) : a.S;
-  const int64_t index = (start >> a.c.shift) + blockIdx.x, base = index << a.c.shift;
+  const int64_t index = (start >> a.c.shift) + p, base = index << a.c.shift;
   const int64_t lo = max(max(start, base), (int64_t)0), hi = min(start + count, base + page);
   if (lo >= hi || index >= a.c.width) return;
   const int pid = kv_page(a.c, b, (int)index);
@@ -203,7 +212,6 @@ __global__ __launch_bounds__(THREADS, MODE == KEY_HALF_ANY || (N == 4 && THREADS
     if (MODE == KEY_HALF) wp.load(a.w, partner(0));
   }
   const int plane = (lane - l) + partner(0) / 8;  // the lane that holds all eight
-  const int h = blockIdx.y;
   Raw8<DT> kr[N], vr[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -552,6 +560,7 @@ extern "C" int mxf8_kv_append(const void* k, const int64_t k_strides[4], const v
   // a run of S tokens touches up to so many pages, wherever it starts
   const int64_t touched = (S + page_size - 2) / page_size + 1;
   if (!grid_fits(touched, 512)) return set_error(MXF8_EINVAL, "%s: shape too large", what);
+  a.eights = touched * H < (1 << 30) ? (int)(touched / 8) : 0;
   const dim3 grid((unsigned)touched, (unsigned)H, (unsigned)B);
   auto launch = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;

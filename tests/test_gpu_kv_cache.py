@@ -123,6 +123,21 @@ def test_append_turned(interleaved, weighted, d, p, dtype):
     check_append(cache, table, i32(0, 40), k, v, turns=turns, weight=w, interleaved=interleaved)
 
 
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("d,page,dtype", [(128, 64, "bf16"), (64, 128, "fp32")])
+def test_append_many_workgroups(d, page, dtype, turned):
+    """More than a thousand pages and heads in a call."""
+    g = torch.Generator().manual_seed(7)
+    b, h, s = 8, 9, 15 * page - 3
+    cache, table = random_cache(8, b * 17 + 3, h, page, d), pages_for(9, b, 17)
+    k, v = (torch.randn((b, h, s, d), generator=g).to(DT[dtype]).cuda() for _ in range(2))
+    angle = torch.rand((s, d // 2 - 3), generator=g) * 7
+    turns = torch.stack([angle.cos(), angle.sin()], -1).cuda() if turned else None
+    w = (1 + 0.2 * torch.randn(d, generator=g)).to(DT[dtype]).cuda() if turned else None
+    starts = i32(*[i * page // 5 for i in range(b)])
+    check_append(cache, table, starts, k, v, counts=i32(*[s - 11 * i for i in range(b)]), turns=turns, weight=w)
+
+
 @pytest.mark.parametrize("d,page", [(128, 64), (64, 16), (128, 128)])
 def test_append_one_token_at_a_time(d, page):
     """Sizes that grow and fall: pages whose exponent rises under what they hold."""
