@@ -144,35 +144,31 @@ __device__ __forceinline__ v2i codes_of(const Raw8<DT>& r, float scale) {
 
 constexpr uint32_t INF_BITS = 0x7f800000u, LARGEST_BITS = 0x63600000u;  // of 448 2^63
 
-// fp64 to fp32 on the way to a code: rounded to nearest, but off a tie between two codes that the value is not on.  (So
-// the code is the one nearest to the value in 64 bits, down to 2^-6 of the scale.)
+// fp64 to fp32 on the way to a code: rounded to nearest, but off a border (of two codes, or of 448 2^e: a fp32 number whose last
+// 19 bits are 0) that the value is not on.  So the code is the one nearest to the value in 64 bits.
 __device__ __forceinline__ void round_keys(const double (&y)[8], float (&f)[8]) {
-  bool tie = false;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    f[j] = (float)y[j];
-    tie |= __float_as_uint(f[j]) << 12 == 0x80000000u;
-  }
-  if (__ballot(tie)) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const double d = y[j] - (double)f[j];
-      if (__float_as_uint(f[j]) << 12 == 0x80000000u && d != 0.0)
-        f[j] = __uint_as_float(__float_as_uint(f[j]) + ((d > 0.0) == (f[j] > 0.0f) ? 1 : -1));
-    }
+    const float r = (float)y[j];
+    const double d = y[j] - (double)r;
+    const bool border = __float_as_uint(r) << 13 == 0 && r != 0.0f && fabsf(r) < INFINITY && d != 0.0;
+    f[j] = border ? __uint_as_float(__float_as_uint(r) + ((d > 0.0) == (r > 0.0f) ? 1 : -1)) : r;
   }
 }
 
 // A workgroup writes one page and head of one sequence: D / 8 lanes hold a token's eight channels each, so the
-// page's maximum is one reduction over values that stay in registers until they are rounded.  Keys are normed and turned in
-// fp64, which leaves no key on the wrong side of a border between two codes (fp32 has two or three of a million there).
+// page's maximum is one reduction over values that stay in registers until they are rounded.  A key's code is the one that its
+// norm and turn in fp64 give (fp32 would put two or three of a million on the wrong side of a border between two codes).  Keys of
+// 16 bits are computed in fp32 whose error is known, and again in fp64 only by the waves, some 3% of them, that have a
+// channel so near to a border that the error might decide; fp32 keys, and pairs that no lane holds whole, in fp64 alone.
 //
-// Bound by memory where keys stay as they are: 20280 tokens x 24 heads x 128 in bf16, 374 MB, 65 us (5.7 TB/s).  Normed 78,
-// turned by neighbouring pairs or both 95, half-split 129: the cos / sin of a token come from L2 again for each head, as many
-// bytes as its keys and values, and the fp64 takes some 40 us of the vector units beside the loads.
+// Bound by memory where keys stay as they are: 20280 tokens x 24 heads x 128 in bf16, 374 MB, 65 us (5.7 TB/s).  Normed and
+// turned by neighbouring pairs 83 (the vector unit 59% busy; all in fp64 93 and 84%), half-split 104 (127).  With a head's pages after
+// each other instead of a page's heads 99, and 500 MB read for 261: the table, 10 MB, outgrew the L2s between two heads.
 template <int DT, int D, int MODE, int THREADS, int N>
 __global__ __launch_bounds__(THREADS, MODE == KEY_HALF_ANY || (N == 4 && THREADS == 512) ? 2 : 4) void kv_append_kernel(const AppendArgs a) {
   constexpr int L = D / 8, T = THREADS / L, WAVES = THREADS / 64;  // lanes a token, tokens a step
+  constexpr bool QUICK = DT != MXF8_F32 && (MODE == KEY_PAIRS || MODE == KEY_HALF);
   __shared__ uint32_t red[2][WAVES];
   __shared__ float exchange[MODE == KEY_HALF_ANY ? THREADS * 8 : 1];
   const int b = blockIdx.z, lane = threadIdx.x & 63, l = threadIdx.x % L, c0 = 8 * l;
@@ -239,6 +235,57 @@ __global__ __launch_bounds__(THREADS, MODE == KEY_HALF_ANY || (N == 4 && THREADS
   load_turns(0, cs[0]);
   const int64_t ph = (int64_t)pid * a.c.H + h;
   const int old[2] = {(int)a.c.ks[ph] - 127, (int)a.c.vs[ph] - 127};
+  // One token's eight channels in fp32, within 13 units of their last place: x w is exact, the turn's second product keeps
+  // its rounding error (so that what cancels leaves no more than three half units), and the norm's factor comes last: 14 halves of
+  // 2^-23 in its sum, half of that in the root, two for itself, one for the last product.  False where this may
+  // decide a code or a scale, within 16 units of a border (see round_keys), or where something over- or underflows.
+  auto quick_key = [&](int i, const float (&x)[8], const float (&w)[8], float (&f)[8]) {
+    float g = 1.0f, u[8];
+    if (a.w) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(x[j], x[j], ss);
+      g = __builtin_amdgcn_rsqf(__builtin_fmaf(lanes_sum<L>(ss), 1.0f / D, a.eps));
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = u[j] = x[j] * w[j];
+    // a co + b si
+    auto turn = [](float a, float co, float b, float si) {
+      const float p = b * si;
+      return __builtin_fmaf(a, co, p) + __builtin_fmaf(b, si, -p);
+    };
+    if constexpr (MODE == KEY_PAIRS) {
+#pragma unroll
+      for (int j = 0; j < 8; j += 2)
+        if (c0 / 2 + j / 2 < a.P) {
+          f[j] = turn(u[j], cs[i & 1][j], -u[j + 1], cs[i & 1][j + 1]);
+          f[j + 1] = turn(u[j + 1], cs[i & 1][j], u[j], cs[i & 1][j + 1]);
+        }
+    } else {
+      Raw8<DT> r = kr[i];
+      r.from_lane(plane);
+      float q[8], wq[8];
+      r.get(q);
+      wp.get(wq);
+      if (c0 < 2 * a.P) {
+        const float* t = turns + ((there[i] ? s0 + i * T : 0) * a.P + min(c0, partner(0))) * 2;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          const floats4 v = *(gfloats4)(gbytes)(t + 2 * j);
+          f[j] = turn(u[j], v[0], q[j] * wq[j], c0 < a.P ? -v[1] : v[1]);
+          f[j + 1] = turn(u[j + 1], v[2], q[j + 1] * wq[j + 1], c0 < a.P ? -v[3] : v[3]);
+        }
+      }
+    }
+    uint32_t near = ~0u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      f[j] *= g;
+      near = min(near, (__float_as_uint(f[j]) + 16) << 13);
+    }
+    // (what is neither normed nor turned is exact)
+    return (near > 32u << 13 && g >= 0x1p-40f && g <= 0x1p40f) || (!a.w && c0 >= 2 * a.P);
+  };
   float k[N][8];
   uint32_t raw[2] = {0, 0}, top[2];
 #pragma unroll
@@ -251,7 +298,7 @@ __global__ __launch_bounds__(THREADS, MODE == KEY_HALF_ANY || (N == 4 && THREADS
     float size = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      __builtin_amdgcn_sched_barrier(0);  // (one token's 64-bit values at a time)
+      __builtin_amdgcn_sched_barrier(0);  // (one token's values at a time)
       if (i + 1 < N) load_turns(i + 1, cs[(i + 1) & 1]);
       if (!__ballot(there[i])) {  // none of this wave's tokens
 #pragma unroll
@@ -261,6 +308,15 @@ __global__ __launch_bounds__(THREADS, MODE == KEY_HALF_ANY || (N == 4 && THREADS
       float x[8], w[8];
       kr[i].get(x);
       wk.get(w);
+      if constexpr (QUICK) {
+        const bool sure = quick_key(i, x, w, k[i]);
+        if (!__ballot(there[i] && !sure)) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) size = fmaxf(size, fabsf(k[i][j]));
+          continue;
+        }
+      }
+      // the same in 64 bits, rounded once
       double y[8], g = 1.0;
       if (a.w) {
         double ss = 0.0;
@@ -432,7 +488,7 @@ __global__ __launch_bounds__(THREADS, MODE == KEY_HALF_ANY || (N == 4 && THREADS
 template <int DT, int D, int MODE>
 static int launch_append(const AppendArgs& a, dim3 grid, hipStream_t st) {
   // Pages of 1024 chunks: four tokens a lane in workgroups of 256, or, where these do not go round or half-split pairs cost more
-  // registers, two in 512 (1560 tokens x 24 heads, turned: 17.5 / 15.4 us; 20280: 95 / 98).
+  // registers (fp32 turned, half-split), two in 512 (1560 tokens x 24 heads, turned in fp64: 17.5 / 15.4 us; 20280: 95 / 98).
   const int chunks = (D << a.c.shift) / 8;  // of eight channels
   const int64_t blocks = (int64_t)grid.x * grid.y * grid.z;
   if (chunks <= 256) {
@@ -440,7 +496,7 @@ static int launch_append(const AppendArgs& a, dim3 grid, hipStream_t st) {
   } else if (chunks == 512) {
     kv_append_kernel<DT, D, MODE, 256, 2><<<grid, 256, 0, st>>>(a);
   } else if (chunks == 1024) {
-    if constexpr (MODE <= KEY_PAIRS) {
+    if constexpr (MODE == KEY_PLAIN || (MODE == KEY_PAIRS && DT != MXF8_F32)) {
       if (blocks >= 1024) {
         kv_append_kernel<DT, D, MODE, 256, 4><<<grid, 256, 0, st>>>(a);
         return check_launch("kv_append");

@@ -123,19 +123,46 @@ def test_append_turned(interleaved, weighted, d, p, dtype):
     check_append(cache, table, i32(0, 40), k, v, turns=turns, weight=w, interleaved=interleaved)
 
 
-@pytest.mark.parametrize("turned", [False, True])
-@pytest.mark.parametrize("d,page,dtype", [(128, 64, "bf16"), (64, 128, "fp32")])
-def test_append_many_workgroups(d, page, dtype, turned):
+@pytest.mark.parametrize("turned,interleaved", [(False, True), (True, True), (True, False)])
+@pytest.mark.parametrize("d,page,dtype", [(128, 64, "bf16"), (64, 128, "fp32"), (128, 64, "fp16")])
+def test_append_many_workgroups(d, page, dtype, turned, interleaved):
     """More than a thousand pages and heads in a call."""
     g = torch.Generator().manual_seed(7)
     b, h, s = 8, 9, 15 * page - 3
     cache, table = random_cache(8, b * 17 + 3, h, page, d), pages_for(9, b, 17)
     k, v = (torch.randn((b, h, s, d), generator=g).to(DT[dtype]).cuda() for _ in range(2))
-    angle = torch.rand((s, d // 2 - 3), generator=g) * 7
+    angle = torch.rand((s, d // 2 - (3 if interleaved else 8)), generator=g) * 7
     turns = torch.stack([angle.cos(), angle.sin()], -1).cuda() if turned else None
     w = (1 + 0.2 * torch.randn(d, generator=g)).to(DT[dtype]).cuda() if turned else None
     starts = i32(*[i * page // 5 for i in range(b)])
-    check_append(cache, table, starts, k, v, counts=i32(*[s - 11 * i for i in range(b)]), turns=turns, weight=w)
+    check_append(cache, table, starts, k, v, counts=i32(*[s - 11 * i for i in range(b)]), turns=turns, weight=w,
+                 interleaved=interleaved)
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("weighted", [True, False])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_append_any_sizes(interleaved, weighted, dtype):
+    """Tokens and weights of any size in one page, exact zeros, ties between codes, turns by whole quarters."""
+    g = torch.Generator().manual_seed(11)
+    s, d, page = 150, 128, 32
+    cache, table = FP8KVCache(8, 2, d, page), pages_for(1, 1, 6)
+    x = torch.randn((1, 2, s, d), generator=g)
+    top = 38 if dtype == "bf16" else 4
+    x[0, 0] *= 10.0 ** (torch.rand((s, 1), generator=g) * 2 * top - top)
+    x[0, 1, ::3, ::5], x[0, 1, 7] = 0.0, 0.0
+    x[0, 1, 64:] = (torch.randint(-31, 32, (s - 64, d), generator=g) * 2.0 ** -3)  # codes and the ties between them
+    angle = torch.rand((s, 64), generator=g) * 7
+    angle[70:90] = torch.pi / 2 * torch.arange(20)[:, None]
+    turns = torch.stack([angle.cos(), angle.sin()], -1)
+    turns[70:90] = turns[70:90].round()
+    w = None
+    if weighted:
+        w = torch.randn(d, generator=g) * 10.0 ** (torch.rand(d, generator=g) * top - top / 2)
+        w = w.to(DT[dtype]).cuda()
+    for n in (64, 24):
+        check_append(cache, table, i32(0), x.to(DT[dtype]).cuda(), x.to(DT[dtype]).cuda(), weight=w,
+                     turns=turns[:, :n].contiguous().cuda(), interleaved=interleaved)
 
 
 @pytest.mark.parametrize("d,page", [(128, 64), (64, 16), (128, 128)])
