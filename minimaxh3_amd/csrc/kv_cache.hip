@@ -163,8 +163,8 @@ __device__ __forceinline__ void round_keys(const double (&y)[8], float (&f)[8]) 
 // channel so near to a border that the error might decide; fp32 keys, and pairs that no lane holds whole, in fp64 alone.
 //
 // Bound by memory where keys stay as they are: 20280 tokens x 24 heads x 128 in bf16, 374 MB, 65 us (5.7 TB/s).  Normed and
-// turned by neighbouring pairs 83 (the vector unit 59% busy; all in fp64 93 and 84%), half-split 104 (127).  With a head's pages after
-// each other instead of a page's heads 99, and 500 MB read for 261: the table, 10 MB, outgrew the L2s between two heads.
+// turned by neighbouring pairs 83 (the vector unit 59% busy; all in fp64 93 and 84%), half-split 91.  With a head's pages after each other
+// instead of a page's heads that was 99, and 500 MB read for 261: the table, 10 MB, outgrew the L2s between two heads.
 template <int DT, int D, int MODE, int THREADS, int N>
 __global__ __launch_bounds__(THREADS, MODE == KEY_HALF_ANY || (N == 4 && THREADS == 512) ? 2 : 4) void kv_append_kernel(const AppendArgs a) {
   constexpr int L = D / 8, T = THREADS / L, WAVES = THREADS / 64;  // lanes a token, tokens a step
@@ -487,8 +487,8 @@ __global__ __launch_bounds__(THREADS, MODE == KEY_HALF_ANY || (N == 4 && THREADS
 
 template <int DT, int D, int MODE>
 static int launch_append(const AppendArgs& a, dim3 grid, hipStream_t st) {
-  // Pages of 1024 chunks: four tokens a lane in workgroups of 256, or, where these do not go round or half-split pairs cost more
-  // registers (fp32 turned, half-split), two in 512 (1560 tokens x 24 heads, turned in fp64: 17.5 / 15.4 us; 20280: 95 / 98).
+  // Pages of 1024 chunks: four tokens a lane in workgroups of 256, or, where these do not go round or the registers do not
+  // hold them, two in 512 (1560 tokens x 24 heads, turned in fp64: 17.5 / 15.4 us; 20280 turned 82 / 92, half-split 91 / 104).
   const int chunks = (D << a.c.shift) / 8;  // of eight channels
   const int64_t blocks = (int64_t)grid.x * grid.y * grid.z;
   if (chunks <= 256) {
@@ -496,7 +496,7 @@ static int launch_append(const AppendArgs& a, dim3 grid, hipStream_t st) {
   } else if (chunks == 512) {
     kv_append_kernel<DT, D, MODE, 256, 2><<<grid, 256, 0, st>>>(a);
   } else if (chunks == 1024) {
-    if constexpr (MODE == KEY_PLAIN || (MODE == KEY_PAIRS && DT != MXF8_F32)) {
+    if constexpr (MODE == KEY_PLAIN || (MODE != KEY_HALF_ANY && DT != MXF8_F32)) {
       if (blocks >= 1024) {
         kv_append_kernel<DT, D, MODE, 256, 4><<<grid, 256, 0, st>>>(a);
         return check_launch("kv_append");
