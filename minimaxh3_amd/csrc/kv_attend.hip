@@ -401,8 +401,8 @@ done:
 // 1 first takes exponentials and then multiplies.  Fragments are read from LDS well before their products, and each wave
 // stages its share of the keys of tile j + 3 and the values of j + 1 among them.
 //
-// A tile's 2048 cycles of products take some 4000 (over the whole launch the matrix unit is 42% busy, the vector unit 52%, LDS
-// 37%), at a clock under the power limit: 2.0 of 2.4 GHz.  1560 queries x 24 heads of 128 over 21840 keys: 450-470 us with the join's 18, 900-930 TFLOP/s
+// A tile's 2048 cycles of products take some 4000 (over the whole launch the matrix unit is 45% busy, the vector unit 56%, LDS
+// 40%), at a clock under the power limit: 2.0 of 2.4 GHz.  1560 queries x 24 heads of 128 over 21840 keys: 457-476 us with the join's 18, 880-915 TFLOP/s
 // (a library product of 8192^3 in fp16 reaches 1147 here).  What the parts bring there: both groups in the same order 492, without
 // the wave priorities 470, a barrier between the two phases as well 518, key codes converted at each read instead of once
 // 517, fragments read as they are needed 560-590.  One wave a SIMD with 64 rows and 512 registers would read LDS half as often,
