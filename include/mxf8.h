@@ -395,7 +395,8 @@ int mxf8_mxfp4_linear(const void* x, int dtype, int64_t ldx, const uint8_t* w4, 
  * to each sequence, from its token starts[b] (int32) on; counts NULL, or only the first counts[b] of them.
  * Tokens from there on are taken as not there before; other tokens and pages stay as they are.
  *   keys are normed per head with k_weight [D] (or NULL) and turned by turns [S, P, 2] fp32 (cos, sin) with
- *   batch stride turns_batch_stride (0: one for all; P = 0: none), as in mxf8_rotate_qk, in fp32
+ *   batch stride turns_batch_stride (0: one for all; P = 0: none), as in mxf8_rotate_qk but unrounded: the codes are
+ *   those of the keys in fp64
  *   a page and head's exponent e is the smallest in [-32, 63] with max |x| <= 448 * 2^e over the new tokens in it,
  *   or the one it has where that is larger and the page holds tokens before starts[b]; their codes are then
  *   rounded again where e grew.  A code is the e4m3 number nearest to x * 2^-e, ties to even, an infinity the
