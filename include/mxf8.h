@@ -430,8 +430,9 @@ int64_t mxf8_kv_attend_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t
  *   out [B, H, S, D] of q's dtype, any strides with contiguous channels
  *   workspace: mxf8_kv_attend_workspace_bytes(...) bytes, 16-byte aligned (NULL where that is 0)
  * Products of 16-bit floating point numbers (q and the probabilities in fp16 under scales of their own, codes
- * exactly), sums and softmax statistics in fp32.  The same call gives the same bits; how keys are split, and with
- * it the order of the sums, depends on the shapes of the call and on lengths[b].
+ * exactly), scores, sums and softmax statistics in fp32 (a row with a score past 3.4e38 in size may be NaN).  The same
+ * call gives the same bits; how keys are split, and with it the order of the sums, depends on the shapes of the call and
+ * on lengths[b].
  */
 int mxf8_kv_attend(const void* q, const int64_t q_strides[4], int dtype, int64_t B, int64_t H, int64_t S, int64_t D,
                    const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_scale, const uint8_t* v_scale,

@@ -33,8 +33,9 @@ struct AttendArgs {
   float *part, *stat;      // with more than one: sums [B, Hk, splits, R, D], and (maximum, sum of p) [.., 2]
 };
 
-constexpr float KV_NONE = -1.0e30f;  // a maximum of no scores
-constexpr float KV_SLACK = 8.0f;     // p' may grow to 2^8 before the running maximum follows
+constexpr float KV_LARGEST = 3.40282347e38f;
+constexpr float KV_NONE = -KV_LARGEST;  // a maximum of no scores: none is below it
+constexpr float KV_SLACK = 8.0f;        // p' may grow to 2^8 before the running maximum follows
 
 // ---- rows and splits -------------------------------------------------------------------
 struct KvSeq {
@@ -135,10 +136,12 @@ __device__ __forceinline__ float scale_query(const AttendArgs& a, bool there, Ra
     f[j] = query_f16<DT>(r[j], __uint_as_float((uint32_t)(127 - e) << 23));
     if (a.scale < 0.0f) f[j] = -f[j];  // so that the factor of the scores is not negative, and their largest its own
   }
-  // (at least 2^-90: times a page's 2^-32 or more it is still no 0, which would make NaN of a score that is hidden as -inf;
-  // scores under so small a factor are 0 for all that matters)
-  return fmaxf(fabsf(a.scale) * __uint_as_float((uint32_t)(127 + e) << 23), 0x1p-90f);
+  // (at least 2^-117: times a page's 2^-32 or more it is still no 0, which would make NaN of a score that is hidden as -inf;
+  // scores under so small a factor, of products below 2^32 and pages up to 2^63, are below 2^-22)
+  return fmaxf(fabsf(a.scale) * __uint_as_float((uint32_t)(127 + e) << 23), 0x1p-117f);
 }
+// The factor of a page's scores.  (Never infinite: products of 0 have a score of 0.)
+__device__ __forceinline__ float page_factor(float factor, float scale) { return fminf(factor * scale, KV_LARGEST); }
 
 // N consecutive channels of an output row.
 template <int DT, int N>
@@ -266,7 +269,7 @@ __global__ __launch_bounds__(256, (D == 64 ? (NR == 1 ? 4 : NR == 2 ? 3 : 2) : N
           acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
               codes_f16((uint32_t)s.k[g][kk / 2][2 * (kk % 2)], (uint32_t)s.k[g][kk / 2][2 * (kk % 2) + 1]), qf[t][kk], acc,
               0, 0, 0);
-        const float f = factor[t] * ks[g];
+        const float f = page_factor(factor[t], ks[g]);
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[g][r] = __builtin_fmaf(acc[r], f, ev[g]);
       }
@@ -279,7 +282,7 @@ __global__ __launch_bounds__(256, (D == 64 ? (NR == 1 ? 4 : NR == 2 ? 3 : 2) : N
       }
       const float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
                               fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-      if (__ballot(top > m[t] + KV_SLACK)) {
+      if (__ballot(top - m[t] > KV_SLACK)) {
         const float next = fmaxf(m[t], row_reduce<16>(top, max_of)), alpha = __builtin_amdgcn_exp2f(m[t] - next);
         m[t] = next;
         l[t] *= alpha;
@@ -445,6 +448,10 @@ __global__ __launch_bounds__(512, 2) void kv_attend_many_kernel(const AttendArgs
   int low = row < a.R ? limit : INT32_MAX, high = limit;
   v8h qf[KK];
   const float factor = scale_query<DT, 32>(a, limit > 0, raw, qf);
+  // One fma makes a probability's exponent, whose product is unrounded and whose sum e - m is not: with scores of 2^20 it is off
+  // by up to 2^-3, with larger ones it would leave fp16's range.  A wave that has such rows, or rows whose factor
+  // may overflow, rounds the scores first, as their maximum was.
+  bool far = __ballot(factor >= 0x1p64f) != 0;
   float m = KV_NONE, l = 0.0f;
   v16f o[OT];
 #pragma unroll
@@ -558,7 +565,7 @@ __global__ __launch_bounds__(512, 2) void kv_attend_many_kernel(const AttendArgs
   };
   auto exponentials = [&](int j) {
     const int key0 = k0 + j * MANY_KEYS;
-    float f[4], e[4], iv[4], y[4];
+    float f[4], e[4], iv[4], n[4], y[4];
     v4f s[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) s[g] = lds.scale[j & 3][g];
@@ -577,6 +584,10 @@ __global__ __launch_bounds__(512, 2) void kv_attend_many_kernel(const AttendArgs
       f[g] = factor * s[g][0], e[g] = s[g][1], iv[g] = s[g][2];
       all = all & (__builtin_amdgcn_readfirstlane(__float_as_uint(s[g][3])) != 0);
     }
+    if (far) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) f[g] = page_factor(factor, s[g][0]);
+    }
     if (!all) {
 #pragma unroll
       for (int g = 0; g < 4; ++g)
@@ -590,22 +601,33 @@ __global__ __launch_bounds__(512, 2) void kv_attend_many_kernel(const AttendArgs
     float top = -INFINITY;
 #pragma unroll
     for (int g = 0; g < 4; ++g) top = fmaxf(top, __builtin_fmaf(y[g], f[g], e[g]));
-    if (__ballot(top > m + KV_SLACK)) {
+    if (__ballot(top - m > KV_SLACK)) {
       const float next = fmaxf(m, row_reduce<32>(top, max_of)), alpha = __builtin_amdgcn_exp2f(m - next);
       m = next;
       l *= alpha;
 #pragma unroll
       for (int i = 0; i < OT; ++i) o[i] *= alpha;
+      far |= __ballot(fabsf(m) >= 0x1p20f && m != KV_NONE) != 0;
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) n[g] = e[g] - m;
+    if (far) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          x[g >> 1][(g & 1) * 8 + r] = __builtin_fmaf(x[g >> 1][(g & 1) * 8 + r], f[g], e[g]) - m;
+        f[g] = 1.0f, n[g] = 0.0f;
+      }
     }
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const float n = e[g] - m;
       float sum = 0.0f;
       v4i words;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[g >> 1][(g & 1) * 8 + 2 * r], f[g], n));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[g >> 1][(g & 1) * 8 + 2 * r + 1], f[g], n));
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[g >> 1][(g & 1) * 8 + 2 * r], f[g], n[g]));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[g >> 1][(g & 1) * 8 + 2 * r + 1], f[g], n[g]));
         words[r] = (int)pack_f16(p0, p1);
         sum += p0 + p1;
       }

@@ -107,8 +107,9 @@ def cached_attention(q: torch.Tensor, cache: FP8KVCache, page_table: torch.Tenso
     own (without it all see all: a frame's tokens among each other, or text).  A row that sees no key
     is 0.  lengths, q_lengths: int32 [B].  scale defaults to 1 / sqrt(D).
 
-    Codes are used as they are, q and the probabilities in fp16 under scales of their own, and sums are
-    fp32.  The same call gives the same bits; a row's last bit may differ between calls of different shapes.
+    Codes are used as they are, q and the probabilities in fp16 under scales of their own, and scores and sums are
+    fp32 (a row with a score past 3.4e38 in size may be NaN).  The same call gives the same bits; a row's last bit may
+    differ between calls of different shapes.
     """
     return ops.kv_attend(q, *cache.tensors(), page_table, lengths, q_lengths, bool(causal),
                          1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale))

@@ -733,3 +733,57 @@ def test_refusals():
     bad.k_scale = bad.k_scale[:, :1]
     with pytest.raises(ValueError):
         attend(cache=bad)
+
+
+# ---------------------------------------------------------------------------------------
+# scores of any size, probabilities far below the largest, lengths past the table
+# ---------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("S,H,Hk", [(1, 4, 2), (4, 8, 1), (40, 1, 1), (70, 2, 2), (130, 1, 1)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attend_scores_of_any_size(S, H, Hk, D):
+    """Scores up to the largest fp32 number, of either sign.  Keys are one row times 1, 2 or 4: a row's weight is spread
+    evenly over those of the largest score."""
+    page, n = 16, 300
+    table = pages_for(D, 1, 20)
+    g = torch.Generator().manual_seed(D)
+    factor = 2.0 ** torch.randint(0, 3, (n,), generator=g)
+    v = torch.randn((1, Hk, n, D), generator=g).clamp(-4, 4)
+    v[..., 0] = 4.0  # (one exponent for all pages: it is added to scores whose last bits are larger)
+    for key, query, size in ((3.0, 5.0, 2.0 ** 15), (3.0, 5.0, 2.0 ** 20), (1.0, 7.0, 2.0 ** 25), (3.0, 5.0, 2.0 ** 40), (3.0, 3.0, 2.0 ** 70),
+                             (1.0, 1.0, 2.0 ** 110)):
+        k = (key * 2.0 ** 20 * factor)[None, None, :, None].expand(1, Hk, n, D)
+        cache = FP8KVCache(23, Hk, D, page)
+        append_kv(cache, table, i32(0), k.cuda(), v.cuda())
+        _, w = read_kv(cache, table, i32(0), n, dtype=torch.float32)
+        for sign in (1, -1):
+            q = torch.full((1, H, S, D), sign * query * size / 2 ** 20).bfloat16().cuda()
+            best = (factor == (4 if sign > 0 else 1)).cuda()
+            want = w[:, :, best].double().mean(2).repeat_interleave(H // Hk, 1)[:, :, None]
+            tol = 2.0 ** -10 * w[:, :, best].double().abs().mean(2).repeat_interleave(H // Hk, 1)[:, :, None]
+            got = cached_attention(q, cache, table, i32(n), scale=0.11).double()
+            tol = tol + (want.abs() + tol) * 2.0 ** -8
+            assert ((got - want).abs() <= tol).all(), (size, sign, ((got - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("S,H,Hk", [(1, 4, 2), (40, 1, 1), (70, 2, 2)])
+def test_attend_no_scores(S, H, Hk):
+    """A scale of 0, and rows that are large only where all keys are 0: every key weighs the same."""
+    table = pages_for(1, 1, 20)
+    g = torch.Generator().manual_seed(1)
+    for dtype in (torch.float16, torch.bfloat16):
+        k, v = (torch.randn((1, Hk, 300, 128), generator=g) for _ in range(2))
+        k[:, :, :, :8] = 0.0
+        cache = FP8KVCache(23, Hk, 128, 16)
+        append_kv(cache, table, i32(0), k.cuda() * 2.0 ** 70, v.cuda())
+        _, w = read_kv(cache, table, i32(0), 300, dtype=torch.float32)
+        want, a = (t.double().mean(2, keepdim=True).repeat_interleave(H // Hk, 1) for t in (w, w.abs()))
+        full = torch.full((1, H, S, 128), torch.finfo(dtype).max, dtype=dtype, device="cuda")
+        part = torch.zeros_like(full)
+        part[..., :8] = full[..., :8]
+        for q, scale in ((full, 0.0), (part, 1.0), (part, -3.0)):
+            got = cached_attention(q, cache, table, i32(300), scale=scale).double()
+            tol = 2.0 ** -10 * a
+            tol = tol + (want.abs() + tol) * torch.finfo(dtype).eps / 2
+            assert ((got - want).abs() <= tol).all(), (dtype, scale, ((got - want).abs() / tol).max())
