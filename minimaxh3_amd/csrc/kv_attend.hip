@@ -5,9 +5,12 @@
 // Keys and values are codes times a power of two for each page.  Codes become fp16 exactly and go into the fp16 matrix
 // instructions; a key's power of two multiplies the score, and a value's, 2^e_j, goes into the exponent:
 //   p'_ij = 2^(x_ij + e_j - m_i),  o_i = sum_j p'_ij code_j / sum_j p'_ij 2^-e_j
-// with m_i a running maximum of x_ij + e_j.  So p' is at most 2^8 however the pages' sizes differ, and its half step
-// in fp16, 2^-11 of it or 2^-25, is all that the value product rounds; bf16 queries are exact in fp16 under a power of two
-// per row, down to 2^-17 of the row's largest (the half step below is 2^-25 of it).
+// with m_i 7 below a running maximum of x_ij + e_j, or up to 15 below the maximum that is to come.  So the row's largest p' is
+// from 2^7 to 2^15 (fp16 ends at 65504) however the pages' sizes differ, and p' half step in fp16, 2^-11 of it or 2^-25, is
+// all that the value product rounds.  What this comes to in an output: 2^-11 of sum p |v| / sum p, and where p 2^e is far
+// below the row's largest, 2^-32 max(p 2^e) |code_j| / sum p for each such key j.  (With the largest at 1 to 2^8 it was 2^-25: of 20280
+// keys 2^-22 as likely as one whose value is 0, it lost up to 18%, and 2^-26 all.)  bf16 queries are exact in fp16
+// under a power of two per row, down to 2^-17 of the row's largest (the half step below is 2^-25 of it).
 // (e4m3 probabilities would run twice as fast and be off by 2^-4, bf16 ones by 2^-8.)
 //
 // The products are made transposed, S' = K Q' and O' = V' P': then a lane holds one row's scores and outputs, the maximum
@@ -35,7 +38,8 @@ struct AttendArgs {
 
 constexpr float KV_LARGEST = 3.40282347e38f;
 constexpr float KV_NONE = -KV_LARGEST;  // a maximum of no scores: none is below it
-constexpr float KV_SLACK = 8.0f;        // p' may grow to 2^8 before the running maximum follows
+// p' of a row's largest so far is 2^7 when m follows it, and may grow to 2^15 before m follows again.
+constexpr float KV_UP = 7.0f, KV_SLACK = 8.0f;
 
 // ---- rows and splits -------------------------------------------------------------------
 struct KvSeq {
@@ -88,6 +92,8 @@ __device__ __forceinline__ float row_reduce(float v, F f) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return f(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
+// m for a largest x + e of `top`.  (Beside scores of 2^20 KV_UP would be rounded, up to 16 where their steps are 16.)
+__device__ __forceinline__ float up_of(float top) { return top - (fabsf(top) < 0x1p20f ? KV_UP : 0.0f); }
 __device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ float sum_of(float a, float b) { return a + b; }
 
@@ -282,8 +288,8 @@ __global__ __launch_bounds__(256, (D == 64 ? (NR == 1 ? 4 : NR == 2 ? 3 : 2) : N
       }
       const float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
                               fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-      if (__ballot(top - m[t] > KV_SLACK)) {
-        const float next = fmaxf(m[t], row_reduce<16>(top, max_of)), alpha = __builtin_amdgcn_exp2f(m[t] - next);
+      if (__ballot(top - m[t] > KV_UP + KV_SLACK)) {
+        const float next = fmaxf(m[t], up_of(row_reduce<16>(top, max_of))), alpha = __builtin_amdgcn_exp2f(m[t] - next);
         m[t] = next;
         l[t] *= alpha;
 #pragma unroll
@@ -601,8 +607,8 @@ __global__ __launch_bounds__(512, 2) void kv_attend_many_kernel(const AttendArgs
     float top = -INFINITY;
 #pragma unroll
     for (int g = 0; g < 4; ++g) top = fmaxf(top, __builtin_fmaf(y[g], f[g], e[g]));
-    if (__ballot(top - m > KV_SLACK)) {
-      const float next = fmaxf(m, row_reduce<32>(top, max_of)), alpha = __builtin_amdgcn_exp2f(m - next);
+    if (__ballot(top - m > KV_UP + KV_SLACK)) {
+      const float next = fmaxf(m, up_of(row_reduce<32>(top, max_of))), alpha = __builtin_amdgcn_exp2f(m - next);
       m = next;
       l *= alpha;
 #pragma unroll

@@ -124,3 +124,25 @@ def attend(q, k, v, there, lengths, scale: float, causal: bool = False, q_length
                 p = np.exp(x - x.max())
                 o[b, h, i], a[b, h, i] = p @ vv / p.sum(), p @ np.abs(vv) / p.sum()
     return o, a
+
+
+def attend_small(q, k, v, e, lengths, scale: float, causal: bool = False):
+    """As `attend`, all tokens there; e [B, Hk, T]: the exponents of the values' pages.  Returns (o, a, small).
+
+    The kernels round p 2^e to fp16 with the row's largest so far at 2^7 or above: half a step of the smallest numbers,
+    2^-25, is 2^-32 of that largest.  `small` is this for each key, times the value's code, over sum p."""
+    B, H, S, D = q.shape
+    T, G = k.shape[2], H // k.shape[1]
+    o, a, small = np.zeros((3, B, H, S, D))
+    for b in range(B):
+        for h in range(H):
+            kk, vv, ee = k[b, h // G], v[b, h // G], np.exp2(e[b, h // G].astype(np.float64))
+            codes = np.abs(vv) / ee[:, None]
+            x = q[b, h] @ kk.T * scale
+            seen = np.arange(T) < (lengths[b] - S + np.arange(S)[:, None] + 1 if causal else lengths[b])
+            x = np.where(seen, x, -np.inf)
+            p = np.exp(x - x.max(-1, keepdims=True))
+            total = p.sum(-1, keepdims=True)
+            o[b, h], a[b, h] = p @ vv / total, p @ np.abs(vv) / total
+            small[b, h] = 2.0 ** -32 * (p * ee).max(-1, keepdims=True) * (seen @ codes) / total
+    return o, a, small

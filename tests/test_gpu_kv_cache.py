@@ -3,8 +3,9 @@
 Codes are exact but where the unrounded key lies within its 32-bit evaluation's bound of a border between two.
 The attention's outputs: half a step of the output type, and 2^-10 of sum p |v| / sum p.  Of that half are the
 probabilities' own half steps in fp16 (2^-11 each); the scores' fp32 sums over D products (D 2^-24 of
-sum |q k| scale, under 2^-13 for scores of size 10), exp2, the row sum and probabilities below fp16's normal range (2^-25
-of the largest each) share the other half."""
+sum |q k| scale, under 2^-13 for scores of size 10), exp2 and the row sum share the other half.  Probabilities below fp16's
+normal range add 2^-32 of the row's largest p 2^e each, times their code (`oracle.kv_cache.attend_small`): with the values
+and scores of most tests here too little to count."""
 import math
 
 import numpy as np
@@ -787,3 +788,53 @@ def test_attend_no_scores(S, H, Hk):
             tol = 2.0 ** -10 * a
             tol = tol + (want.abs() + tol) * torch.finfo(dtype).eps / 2
             assert ((got - want).abs() <= tol).all(), (dtype, scale, ((got - want).abs() / tol).max())
+
+
+def check_attend_small(q, cache, table, lengths, causal=False, scale=None):
+    """As check_attend, with what the oracle says that probabilities below fp16's normal numbers may add."""
+    got = cached_attention(q, cache, table, lengths, causal=causal, scale=scale)
+    pool = ok.Pool(*raw(cache))
+    tb = table.cpu().numpy()
+    T, c = tb.shape[1] * cache.page_size, q.shape[-1] ** -0.5 if scale is None else scale
+    k, v = ok.read(pool, tb, np.zeros(len(tb), int), T)
+    e = np.repeat(pool.scales[1][tb].astype(int) - 127, cache.page_size, 1).transpose(0, 2, 1)  # [B, Hk, T]
+    o, a, small = ok.attend_small(f64(q), k, v, e, lengths.cpu().numpy(), c, causal)
+    tol = 2.0 ** -10 * a + small
+    err = np.abs(f64(got) - o)
+    tol = tol + ob.half_step(np.abs(o) + tol, "bf16" if q.dtype == torch.bfloat16 else "fp16")
+    assert (err <= tol).all(), ((err / tol).max(), (err / np.abs(o).mean()).max())
+
+
+@pytest.mark.parametrize("below", [18, 22, 26])
+@pytest.mark.parametrize("S,H,Hk,D,n", [(1, 4, 2, 64, 20280), (3, 8, 1, 128, 3001), (33, 1, 1, 64, 9001), (70, 1, 1, 64, 20280),
+                                        (66, 2, 2, 128, 4099)])
+def test_attend_many_keys_far_below_the_largest(S, H, Hk, D, n, below):
+    """Keys with all the weight and values of 0 among thousands that are 2^18 to 2^26 times less likely: the output is
+    the sum of these."""
+    g = torch.Generator().manual_seed(below)
+    table = pages_for(below, 1, -(-n // 64))
+    k = torch.randn((1, Hk, n, D), generator=g)
+    v = 1 + 0.25 * torch.randn((1, Hk, n, D), generator=g)
+    k[..., 0], k[..., ::32, 0], v[..., ::32, :] = 0.0, float(below), 0.0
+    q = torch.randn((1, H, S, D), generator=g) * 8 / math.sqrt(D)  # scores of the other channels: 1 in powers of two
+    q[..., 0] = 8.0
+    cache = FP8KVCache(table.numel() + 3, Hk, D, 64)
+    append_kv(cache, table, i32(0), k.cuda(), v.cuda())
+    check_attend_small(q.bfloat16().cuda(), cache, table, i32(n), scale=math.log(2) / 8)
+
+
+@pytest.mark.parametrize("spread", [16, 24])
+@pytest.mark.parametrize("S,H,Hk,D", [(1, 4, 2, 64), (5, 8, 1, 128), (40, 1, 1, 64), (70, 2, 2, 64), (130, 1, 1, 128)])
+def test_attend_pages_large_in_one_channel(S, H, Hk, D, spread):
+    """Every other page has values 2^16 or 2^24 times the rest, in one channel, and zeros in the others."""
+    g = torch.Generator().manual_seed(spread)
+    n, table = 16 * 40 - 3, pages_for(spread, 1, 40)
+    k, v = (torch.randn((1, Hk, n, D), generator=g) for _ in range(2))
+    big = torch.arange(n) // 16 % 2 == 1
+    v[:, :, big] = 0.0
+    v[:, :, big, 5] = 1.5 * 2.0 ** spread
+    q = torch.randn((1, H, S, D), generator=g).bfloat16().cuda()
+    cache = FP8KVCache(table.numel() + 3, Hk, D, 16)
+    append_kv(cache, table, i32(0), k.cuda(), v.cuda())
+    check_attend_small(q, cache, table, i32(n))
+    check_attend_small(q, cache, table, i32(n), causal=True)
