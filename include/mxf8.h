@@ -426,7 +426,7 @@ int64_t mxf8_kv_attend_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t
  * (int32) tokens of each sequence; head h reads key head h / (H / Hk), H a multiple of Hk.
  *   q_lengths NULL, or only the first q_lengths[b] (int32) queries of item b are there; the others' outputs are 0
  *   causal: query i of n sees the keys up to lengths[b] - n + i (its own token, where the queries are the last
- *   tokens of the cache); a query that sees no key gives 0
+ *   tokens of the cache), also where lengths[b] is past the table's tokens; a query that sees no key gives 0
  *   out [B, H, S, D] of q's dtype, any strides with contiguous channels
  *   workspace: mxf8_kv_attend_workspace_bytes(...) bytes, 16-byte aligned (NULL where that is 0)
  * Products of 16-bit floating point numbers (q and the probabilities in fp16 under scales of their own, codes

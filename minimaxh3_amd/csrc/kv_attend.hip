@@ -44,22 +44,26 @@ constexpr float KV_UP = 7.0f, KV_SLACK = 8.0f;
 // ---- rows and splits -------------------------------------------------------------------
 struct KvSeq {
   int len, n;  // keys and queries that are there
+  int diag;    // keys that the last query sees under a causal mask: tokens that the table has no entries for count here
 };
 __device__ __forceinline__ KvSeq kv_seq(const AttendArgs& a, int b) {
   KvSeq s;
-  s.len = kv_length(a.c, a.lengths[b]);
+  s.diag = max(a.lengths[b], 0);
+  s.len = kv_length(a.c, s.diag);
   s.n = a.q_lengths ? min(max(a.q_lengths[b], 0), a.S) : a.S;
   return s;
 }
+// How many keys query i of s.n sees under a causal mask.
+__device__ __forceinline__ int kv_seen(KvSeq s, int i) { return min(max(s.diag - (s.n - 1 - i), 0), s.len); }
 // How many keys row `row` sees, from the first on.
 __device__ __forceinline__ int kv_limit(const AttendArgs& a, KvSeq s, int row) {
   const int i = (uint32_t)row / (uint32_t)a.G;
-  return i >= s.n ? 0 : a.causal ? max(s.len - s.n + i + 1, 0) : s.len;
+  return i >= s.n ? 0 : a.causal ? kv_seen(s, i) : s.len;
 }
 // How many keys the rows [r0, r1) of a tile see, and how many of them one split takes (a multiple of `unit`).
 __device__ __forceinline__ int kv_end(const AttendArgs& a, KvSeq s, int r0, int r1) {
   const int i1 = min((int)((uint32_t)(min(r1, a.R) - 1) / (uint32_t)a.G), s.n - 1);
-  return (int)((uint32_t)r0 / (uint32_t)a.G) >= s.n ? 0 : a.causal ? max(s.len - s.n + i1 + 1, 0) : s.len;
+  return (int)((uint32_t)r0 / (uint32_t)a.G) >= s.n ? 0 : a.causal ? kv_seen(s, i1) : s.len;
 }
 __device__ __forceinline__ int kv_chunk(const AttendArgs& a, int end, int unit) {
   return ((end + a.splits - 1) / a.splits + unit - 1) / unit * unit;

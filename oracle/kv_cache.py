@@ -112,7 +112,7 @@ def attend(q, k, v, there, lengths, scale: float, causal: bool = False, q_length
     T, G = k.shape[2], H // k.shape[1]
     o, a = np.zeros((B, H, S, D)), np.zeros((B, H, S, D))
     for b in range(B):
-        length = min(max(int(lengths[b]), 0), T)
+        length = int(lengths[b])  # (past the table's end there are no tokens, but the diagonal counts from it)
         n = S if q_lengths is None else min(max(int(q_lengths[b]), 0), S)
         for i in range(n):
             seen = there[b] & (np.arange(T) < (length - n + i + 1 if causal else length))

@@ -838,3 +838,24 @@ def test_attend_pages_large_in_one_channel(S, H, Hk, D, spread):
     append_kv(cache, table, i32(0), k.cuda(), v.cuda())
     check_attend_small(q, cache, table, i32(n))
     check_attend_small(q, cache, table, i32(n), causal=True)
+
+
+@pytest.mark.parametrize("S,H,Hk", [(1, 4, 2), (12, 2, 1), (80, 2, 2), (150, 1, 1)])
+@pytest.mark.parametrize("past", [1, 7, 100])
+def test_attend_causal_past_the_table(S, H, Hk, past):
+    """Tokens behind the table's last page are dropped, and the other tokens' queries see what they would with more
+    entries that name no page."""
+    page, width = 16, 12
+    length = page * width + past
+    table = pages_for(past, 1, width)
+    g = torch.Generator().manual_seed(past)
+    k, v = (torch.randn((1, Hk, length, 64), generator=g).bfloat16().cuda() for _ in range(2))
+    cache = FP8KVCache(width + 3, Hk, 64, page)
+    append_kv(cache, table, i32(0), k, v)
+    q = torch.randn((1, H, S, 64), generator=g).bfloat16().cuda()
+    wide = torch.cat([table, torch.full((1, 8), -1, dtype=torch.int32, device="cuda")], 1)
+    check_attend(q, cache, wide, i32(length), causal=True)
+    got = check_attend(q, cache, table, i32(length), causal=True)
+    # the last query sees all that is there
+    want = cached_attention(q[:, :, -1:], cache, table, i32(length))
+    assert (got[:, :, -1:] - want).abs().max() <= 2.0 ** -7 * want.abs().max()
