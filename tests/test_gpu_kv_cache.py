@@ -859,3 +859,83 @@ def test_attend_causal_past_the_table(S, H, Hk, past):
     # the last query sees all that is there
     want = cached_attention(q[:, :, -1:], cache, table, i32(length))
     assert (got[:, :, -1:] - want).abs().max() <= 2.0 ** -7 * want.abs().max()
+
+
+# ---------------------------------------------------------------------------------------
+# key codes of the keys in 64 bits
+# ---------------------------------------------------------------------------------------
+
+def fp32_keys(k, turns, weight, eps, interleaved):
+    """The keys [1, H, S, D] in 32 bits."""
+    x = k.float().cpu()
+    if weight is not None:
+        x = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + eps) * weight.float().cpu()
+    p, t = turns.shape[-2], turns.cpu()
+    a, b = (slice(0, 2 * p, 2), slice(1, 2 * p, 2)) if interleaved else (slice(0, p), slice(p, 2 * p))
+    u, v, y = x[..., a], x[..., b], x.clone()
+    y[..., a], y[..., b] = u * t[..., 0] - v * t[..., 1], u * t[..., 1] + v * t[..., 0]
+    return f64(y)
+
+
+def check_codes_of_64_bits(k, turns, weight, interleaved, page, eps, undecided):
+    """Codes and scales of k [1, H, S, D] in an empty cache: those of the key in 64 bits, exactly where all of its
+    arithmetic is that of the oracle, else but where `undecided` of its size changes the oracle's code.  The key in 32
+    bits has another code somewhere, or the inputs would not test this."""
+    _, H, S, D = k.shape
+    table = pages_for(S, 1, -(-S // page))
+    cache = FP8KVCache(table.numel() + 3, H, D, page)
+    append_kv(cache, table, i32(0), k, k, table=turns, k_weight=weight, eps=eps, interleaved=interleaved)
+    codes, scales = raw(cache)
+    key, _ = ob.rotate(f64(k), f64(turns), None if weight is None else f64(weight), eps, interleaved)
+    single = fp32_keys(k, turns, weight, eps, interleaved)
+    others = 0
+    for i, p in enumerate(table[0].tolist()):
+        for h in range(H):
+            x = key[0, h, i * page: (i + 1) * page]
+            e = ok.exponent(np.abs(x).max())
+            assert int(scales[0][p, h]) - 127 == e, (i, h)
+            got = codes[0][p, h, : len(x)]
+            near = [ok.round_codes(x * (1 + d), e) for d in (-undecided, undecided)]
+            assert ((got == near[0]) | (got == near[1])).all(), (i, h, np.argwhere((got != near[0]) & (got != near[1]))[:5])
+            y = single[0, h, i * page: (i + 1) * page]
+            others += int((ok.round_codes(y, ok.exponent(np.abs(y).max())) != got).sum())
+    assert others
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("weighted", [True, False])
+@pytest.mark.parametrize("d,p", [(128, 64), (128, 56), (128, 21), (64, 32)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_append_keys_beside_borders(interleaved, weighted, d, p, dtype):
+    """Keys 2^-26 of their size above or below a border of two codes, normal and subnormal, or of two scales."""
+    g = torch.Generator().manual_seed(d + p)
+    h, page, s = 2, 32, 32 * 6 - 5
+    rnd = lambda n, *shape: torch.randint(0, n, shape, generator=g)  # noqa: E731
+    mids = torch.from_numpy((e4m3_decode(np.arange(126, dtype=np.uint8)).astype(np.float64)
+                             + e4m3_decode(np.arange(1, 127, dtype=np.uint8))) / 2)
+    c = mids[rnd(126, s, p)]
+    c[:: page, 0] = 448.0  # each page's largest, on a scale's border or beside it
+    c = c * torch.exp2(torch.tensor([-8.0, 0.0, 5.0])[torch.arange(s) // page % 3])[:, None]
+    side = rnd(2, s, p) * 2 - 1
+    side[:: page, 0] = rnd(3, len(range(0, s, page))) - 1
+    turns = torch.stack([c * (rnd(2, s, p) * 2 - 1), c * side * 2.0 ** -16], -1).float().cuda()
+    # one of a pair's two is 1 and the other 2^-10, times cos and 2^-16 of it
+    small = rnd(2, p).bool()
+    size = torch.ones(d)
+    size[slice(0, 2 * p, 2) if interleaved else slice(0, p)] = torch.where(small, 2.0 ** -10, 1.0)
+    size[slice(1, 2 * p, 2) if interleaved else slice(p, 2 * p)] = torch.where(small, 1.0, 2.0 ** -10)
+    x = (rnd(2, 1, h, s, d) * 2 - 1) * (1.0 if weighted else size)
+    weight = size.to(DT[dtype]).cuda() if weighted else None
+    check_codes_of_64_bits(x.to(DT[dtype]).cuda(), turns, weight, interleaved, page, 0.0, 0.0)
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("dtype,weighted", [("bf16", True), ("fp16", True), ("bf16", False), ("fp16", False)])
+def test_append_codes_of_many_keys(interleaved, dtype, weighted):
+    """Two or three keys of a million are in 32 bits on the other side of a border."""
+    g = torch.Generator().manual_seed(21)
+    s, h, d = 8192, 4, 128
+    k = torch.randn((1, h, s, d), generator=g).to(DT[dtype]).cuda()
+    angle = torch.rand((s, d // 2), generator=g) * 7
+    w = (1 + 0.2 * torch.randn(d, generator=g)).to(DT[dtype]).cuda() if weighted else None
+    check_codes_of_64_bits(k, torch.stack([angle.cos(), angle.sin()], -1).cuda(), w, interleaved, 64, 1e-6, 2.0 ** -45 if weighted else 0.0)
