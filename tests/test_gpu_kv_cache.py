@@ -939,3 +939,26 @@ def test_append_codes_of_many_keys(interleaved, dtype, weighted):
     angle = torch.rand((s, d // 2), generator=g) * 7
     w = (1 + 0.2 * torch.randn(d, generator=g)).to(DT[dtype]).cuda() if weighted else None
     check_codes_of_64_bits(k, torch.stack([angle.cos(), angle.sin()], -1).cuda(), w, interleaved, 64, 1e-6, 2.0 ** -45 if weighted else 0.0)
+
+
+@torch.no_grad()
+def test_compiled_step_keeps_its_writes():
+    """Through the shape kernels, with the writes in place taken out of the graph and put back after it: later
+    steps see them, in the tensors that the cache was made of too."""
+    torch._dynamo.reset()
+    try:
+        clip, ref = Clip(), Clip()
+        g = torch.Generator().manual_seed(16)
+        pos = torch.stack([torch.zeros(FRAME), torch.arange(FRAME) // 10, torch.arange(FRAME) % 10], -1)
+        clip.turns = ref.turns = [rotary_table(pos.cuda(), (44, 42, 42))]
+        codes = [t.view(torch.uint8) for t in (clip.cache.k, clip.cache.v)]
+        run = torch.compile(lambda x, start, length: clip.step(x, 0, start, length)[0], backend="aot_eager", fullgraph=True)
+        for i in range(3):
+            x = torch.randn((1, FRAME, 3, H, D), generator=g).bfloat16().cuda()
+            start, length = i32(i * FRAME), i32((i + 1) * FRAME)
+            assert torch.equal(run(x, start, length), ref.step(x, 0, start, length)[0]), i
+            for a, b, c in zip(clip.cache.tensors(), ref.cache.tensors(), codes + [None] * 2):
+                assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+                assert c is None or c.data_ptr() == a.data_ptr()
+    finally:
+        torch._dynamo.reset()
