@@ -30,7 +30,7 @@ struct AttendArgs {
   void* o;
   int64_t qs[3], os[3];  // strides of batch, head, token
   const int32_t *lengths, *q_lengths;
-  int B, H, S, G, R, causal;  // G heads a key head, R = S G rows of it: row i G + g is query i of head g
+  int B, S, G, R, causal;  // G heads a key head, R = S G rows of it: row i G + g is query i of head g
   float scale;             // times log2 e
   int splits;              // parts of the keys
   float *part, *stat;      // with more than one: sums [B, Hk, splits, R, D], and (maximum, sum of p) [.., 2]
@@ -804,12 +804,10 @@ __global__ __launch_bounds__(256) void kv_attend_join_kernel(const AttendArgs a,
 #pragma unroll
     for (int i = 0; i < U; ++i) x[i] = load(min(s0 + (U + i) * P * WAVES, a.splits - 1));
   }
-  if constexpr (P == 2 || P == 4) {
 #pragma unroll
-    for (int off = L; off < 64; off *= 2)
+  for (int off = L; off < 64; off *= 2)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], off, 64);
-  }
+    for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], off, 64);
   if constexpr (WAVES > 1) {
     sums[w][lane] = o;
     __syncthreads();
@@ -925,7 +923,7 @@ extern "C" int mxf8_kv_attend(const void* q, const int64_t q_strides[4], int dty
   a.q = q, a.o = out;
   for (int i = 0; i < 3; ++i) a.qs[i] = q_strides[i], a.os[i] = out_strides[i];
   a.lengths = lengths, a.q_lengths = q_lengths;
-  a.B = (int)B, a.H = (int)H, a.S = (int)S, a.G = (int)(H / Hk), a.R = (int)p.rows, a.causal = causal != 0;
+  a.B = (int)B, a.S = (int)S, a.G = (int)(H / Hk), a.R = (int)p.rows, a.causal = causal != 0;
   a.scale = scale * 1.4426950408889634f;
   a.splits = p.splits;
   a.part = static_cast<float*>(workspace);

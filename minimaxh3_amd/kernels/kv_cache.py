@@ -104,8 +104,9 @@ def cached_attention(q: torch.Tensor, cache: FP8KVCache, page_table: torch.Tenso
     H is a multiple of the cache's heads, and head h attends to key head h // (H / Hk).  With ``q_lengths``
     [B] only the first q_lengths[b] queries of a sequence are there, and the others' rows are 0.
     ``causal``: the queries are the sequence's last tokens, already appended, and each sees the keys up to its
-    own (also where ``lengths`` is past the table, and the last tokens were dropped; without it all see all: a frame's tokens among each other, or text).  A row that sees no key
-    is 0.  lengths, q_lengths: int32 [B].  scale defaults to 1 / sqrt(D).
+    own (also where ``lengths`` is past the table, and the last tokens were dropped; without it all see all: a
+    frame's tokens among each other, or text).  A row that sees no key is 0.  lengths, q_lengths: int32 [B].  scale
+    defaults to 1 / sqrt(D).
 
     Codes are used as they are, q and the probabilities in fp16 under scales of their own, and scores and sums are
     fp32 (a row with a score past 3.4e38 in size may be NaN).  The same call gives the same bits; a row's last bit may
