@@ -174,10 +174,20 @@ __device__ __forceinline__ int64_t out_row(const AttendArgs& a, int b, int hk, i
 // registers.  The next steps' loads are in flight while a step is computed.
 //
 // Bound by memory where the parts are long: 8 key heads x 131149 keys x 128, one query of 32 heads, 268 MB in 43 us (6.2
-// TB/s, a part from the last cache); 64 sequences of 129 to 8192 tokens 113 us (4.7), of 4600 each 109 (5.5).  Short parts are bound by
+// TB/s, a part from the last cache); 64 sequences of 129 to 8192 tokens 104 us (5.2), of 4600 each 110 (5.5).  Short parts are bound by
 // the chain of lengths, page entries, codes and join, some 4 us, and by a lone wave's issue (a step of D = 128 takes
 // it 0.8 us).  Three or four steps ahead are no faster, with fewer waves; more than two workgroups a compute unit only
 // even out lengths.
+//
+// Against the kernel for many rows, 8 key heads, us here / there with the joins:
+//   rows                            17           32           33           48           64
+//   D = 64, 16 x 4096 keys          20.5 / 46.5  21.4 / 47.0  27.0 / 48.9  27.8 / 49.5  29.3 / 50.5
+//   D = 64, 64 x 4096               56 / 166     61 / 171     91 / 178     94 / 182     101 / 184
+//   D = 64, 1 x 32768               14.3 / 27.3  15.4 / 27.6  19.7 / 28.8  20.6 / 29.2  21.5 / 29.2
+//   D = 128, 16 x 4096              29.7 / 53.0  31.4 / 53.5  53.9 / 55.9  54.7 / 57.1  57.0 / 58.2
+//   D = 128, 64 x 4096              110 / 187    116 / 189    208 / 193    210 / 195    219 / 195
+//   D = 128, 1 x 32768              20.5 / 31.7  21.3 / 32.1  38.4 / 33.3  39.3 / 34.1  41.5 / 35.0
+// (33 rows of 128 channels and more hold one wave a SIMD: from 4% faster to 19% slower there.)
 constexpr int FEW_ROWS = 64, FEW_UNIT = 128;
 
 template <int D>
@@ -415,7 +425,7 @@ done:
 // stages its share of the keys of tile j + 3 and the values of j + 1 among them.
 //
 // A tile's 2048 cycles of products take some 4000 (over the whole launch the matrix unit is 45% busy, the vector unit 56%, LDS
-// 40%), at a clock under the power limit: 2.0 of 2.4 GHz.  1560 queries x 24 heads of 128 over 21840 keys: 457-476 us with the join's 18, 880-915 TFLOP/s
+// 40%), at a clock under the power limit: 1.8-2.0 of 2.4 GHz.  1560 queries x 24 heads of 128 over 21840 keys: 457-476 us with the join's 18, 880-915 TFLOP/s
 // (a library product of 8192^3 in fp16 reaches 1147 here).  What the parts bring there: both groups in the same order 492, without
 // the wave priorities 470, a barrier between the two phases as well 518, key codes converted at each read instead of once
 // 517, fragments read as they are needed 560-590.  One wave a SIMD with 64 rows and 512 registers would read LDS half as often,
@@ -836,7 +846,8 @@ static AttendPlan plan_attend(int64_t B, int64_t H, int64_t Hk, int64_t S, int64
   p.splits = 1;
   if (p.few) {
     // Two workgroups a compute unit, however short their parts are; up to eight where each still has 1024 keys, which evens
-    // out sequences of different lengths.
+    // out sequences of different lengths.  KV_MAX_SPLITS, as many as a wave of the join has lanes, ends both: one sequence's
+    // 131072 keys of one head are read by 64 workgroups, 1.6 TB/s (22 us; of two heads 22, of four 26, of eight 45).
     const int64_t few = cdiv(512, groups), parts = cdiv(keys, FEW_UNIT), more = cdiv(2048, groups), thousands = keys / 1024;
     const int64_t n = more < thousands ? more : thousands, m = few < parts ? few : parts;
     p.splits = (int)(n > m ? n : m);

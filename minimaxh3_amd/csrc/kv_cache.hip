@@ -165,6 +165,8 @@ __device__ __forceinline__ void round_keys(const double (&y)[8], float (&f)[8]) 
 // Bound by memory where keys stay as they are: 20280 tokens x 24 heads x 128 in bf16, 374 MB, 65 us (5.7 TB/s).  Normed and
 // turned by neighbouring pairs 83 (the vector unit 59% busy; all in fp64 93 and 84%), half-split 91.  With a head's pages after each other
 // instead of a page's heads that was 99, and 500 MB read for 261: the table, 10 MB, outgrew the L2s between two heads.
+// In fp64 alone: fp32 keys, 633 MB with the table, 149 by neighbouring pairs and 181 half-split (128 as they are, 4.9 TB/s); half-split
+// pairs through LDS, 60 of them, 203 in bf16 and 290 in fp32.
 template <int DT, int D, int MODE, int THREADS, int N>
 __global__ __launch_bounds__(THREADS, MODE == KEY_HALF_ANY || (N == 4 && THREADS == 512) ? 2 : 4) void kv_append_kernel(const AppendArgs a) {
   constexpr int L = D / 8, T = THREADS / L, WAVES = THREADS / 64;  // lanes a token, tokens a step
@@ -487,8 +489,14 @@ __global__ __launch_bounds__(THREADS, MODE == KEY_HALF_ANY || (N == 4 && THREADS
 
 template <int DT, int D, int MODE>
 static int launch_append(const AppendArgs& a, dim3 grid, hipStream_t st) {
-  // Pages of 1024 chunks: four tokens a lane in workgroups of 256, or, where these do not go round or the registers do not
-  // hold them, two in 512 (1560 tokens x 24 heads, turned in fp64: 17.5 / 15.4 us; 20280 turned 82 / 92, half-split 91 / 104).
+  // Pages of 1024 chunks: four tokens a lane in workgroups of 256, or, where these are few or the registers do not hold
+  // them, two in 512.  us of four / two, 24 heads of 128 in bf16, pages of 64 tokens:
+  //   workgroups        120        408         624          792          1056         2088         7632
+  //   plain keys        4.8 / 4.5  5.6 / 5.7   7.1 / 7.1    8.3 / 8.2    11.4 / 11.5  21.4 / 22.9  65 / 70
+  //   normed, pairs     7.3 / 6.1  8.7 / 8.1   10.4 / 11.4  11.8 / 13.6  15.6 / 16.1  26.8 / 28.5  79 / 82
+  //   normed, halves    9.2 / 7.1  10.0 / 9.7  11.5 / 12.9  13.5 / 15.8  17.6 / 19.4  30.2 / 33.8  91 / 102
+  // Turned keys take 86 or 102 registers with two tokens a lane, so that 512 workgroups are a round; from there to 1024 four
+  // are 9-15% faster, and of 64 channels 4-14% slower at 624.
   const int chunks = (D << a.c.shift) / 8;  // of eight channels
   const int64_t blocks = (int64_t)grid.x * grid.y * grid.z;
   if (chunks <= 256) {
